@@ -76,6 +76,17 @@ SIGNATURES = {
     "clef_attention_gated_qnorm": (_i, [_p, _l, _l, _p, _f, _p, _p, _l, _p, _l, _i, _i, _i, _i, _i, _p, _l, _l,
                                         _p, _l, _p]),
     "clef_rotary_table": (_i, [_i, _i, _d, _i, _p, _p]),
+    "clef_linear_scan_workspace": (_z, [_i] * 7),
+    "clef_linear_scan": (_i, [_p, _p, _p, _l, _l, _i, _p, _i, _i, _i, _i, _i, _f, _p, _p, _l, _i, _p, _p, _z, _p]),
+    "clef_linear_scan_varlen": (_i, [_p, _p, _p, _l, _l, _i, _p, _p, _i, _i, _i, _i, _i, _i, _f, _p, _l, _p, _l, _i,
+                                     _p, _p, _z, _p]),
+    "clef_linear_step": (_i, [_p, _p, _p, _l, _l, _i, _p, _p, _i, _i, _i, _i, _i, _f, _p, _l, _p, _i, _p, _l, _i,
+                              _p]),
+    "clef_delta_step": (_i, [_p, _p, _p, _l, _l, _i, _p, _p, _l, _i, _p, _i, _i, _i, _i, _i, _p, _l, _p, _i, _p, _l,
+                             _i, _p]),
+    "clef_attention_shared_workspace": (_z, [_i] * 8),
+    "clef_attention_gated_shared": (_i, [_p, _l, _p, _l, _p, _l, _i, _p, _l, _p, _l, _p, _p, _p, _i, _i, _i, _i, _i,
+                                         _i, _i, _p, _l, _l, _p, _l, _p, _z, _p]),
     "clef_embed": (_i, [_p, _i, _p, _i, _i, _i, _p, _p]),
     "clef_head_logits": (_i, [_p, _i, _p, _i, _p, _p]),
 }
@@ -138,6 +149,72 @@ def _token_view(t, name, rows_last2):
     if not t.is_cuda:
         raise ClefError(-1, f"{name} must be a device tensor")
     return t.stride(0)
+
+
+def _here(*tensors):
+    """Refuses tensors that are not on the current device (the launch goes to its stream)."""
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.get_device() != torch.cuda.current_device()):
+            raise ClefError(-1, "every tensor must be on the current device")
+
+
+def _token_stride(t, name):
+    """_token_view's stride as the C ABI takes it: 0 (contiguous) for a single row, whose
+    stride means nothing; rows that overlap (a broadcast token axis) are refused."""
+    stride = _token_view(t, name, 2)
+    if t.shape[0] == 1:
+        return 0
+    if stride < t.shape[1] * t.shape[2]:
+        raise ClefError(-1, f"{name} must have a token stride of at least a token row")
+    return stride
+
+
+def _scratch(n, device):
+    """A 256-byte aligned workspace of this call's own (the caching allocator's
+    order on the current stream keeps it until the launch has run)."""
+    ws = torch.empty(n + 256, dtype=torch.uint8, device=device)
+    off = (-ws.data_ptr()) % 256
+    return ws[off:off + n]
+
+
+def _index(t, n, name):
+    if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise ClefError(-1, f"{name} must be a contiguous int32 device tensor [{n}]")
+
+
+def _step_args(q, k, v, states, slots, new_states, out_dtype, out):
+    """Checks and defaults that the two single-token steps share: (B, Hk, Hv, dk,
+    dv, state stride, states, new_states, out)."""
+    if q.dim() != 3 or v.dim() != 3:
+        raise ClefError(-1, "q, k, v must be [rows, heads, width]")
+    B, Hk, dk = q.shape
+    Hv, dv = v.shape[1], v.shape[2]
+    if k.shape != q.shape or v.shape[0] != B:
+        raise ClefError(-1, "step tensor shapes")
+    if q.dtype != k.dtype or q.dtype != v.dtype or q.stride(0) != k.stride(0):
+        raise ClefError(-1, "q, k, v must share a dtype; q and k a token stride")
+    if new_states is None:
+        new_states = states
+    if new_states is None or new_states.dim() != 4 or new_states.shape[1:] != (Hv, dk, dv):
+        raise ClefError(-1, "new_states must be [slots, Hv, dk, dv]")
+    nslots = new_states.shape[0]
+    stride = Hv * dk * dv
+    for x in (states, new_states):
+        if x is not None and (x.dtype != torch.float32 or not x.is_contiguous()):
+            raise ClefError(-1, "states must be contiguous f32")
+    if states is not None:
+        if states.shape == (Hv, dk, dv):
+            stride = 0
+        elif states.shape != new_states.shape:
+            raise ClefError(-1, "states must be [Hv, dk, dv] (one for all) or the shape of new_states")
+    if slots is not None:
+        _index(slots, B, "slots")
+    if out is None:
+        out = torch.empty((B, Hv, dv), dtype=out_dtype, device=q.device)
+    if out.shape != (B, Hv, dv):
+        raise ClefError(-1, "out must be [rows, Hv, dv]")
+    _here(q, k, v, states, slots, new_states, out)
+    return B, Hk, Hv, dk, dv, stride, new_states, nslots, out
 
 
 class DeltaScan:
@@ -241,6 +318,128 @@ class DeltaScan:
             _ptr(cu_seqlens), nseq, T, Hk, Hv, dk, dv, self.chunk, self.precision, _ptr(initial), stride,
             _ptr(out), so, _dt(out), _ptr(final), _ptr(ws), ws.numel(), _stream()))
         return out, final
+
+    def step(self, q, k, v, g, beta, states, slots=None, new_states=None, out_dtype=torch.float32, out=None):
+        """One token of each row b (q, k [B, Hk, dk], v [B, Hv, dv], g, beta [B, Hv]):
+        state slots[b] (row b's own if slots is None) is read from `states` and its
+        successor written to `new_states` (default: in place), both [slots, Hv, dk, dv]
+        f32; `states` may be None (zeros) or one [Hv, dk, dv] state for all.  Rows of
+        one slot are tokens of one request in row order; slots out of range are rows
+        without a request.  Returns out [B, Hv, dv].  f32 in both profiles."""
+        B, Hk, Hv, dk, dv, stride, new_states, nslots, out = _step_args(q, k, v, states, slots, new_states, out_dtype,
+                                                                        out)
+        if dk != self.key_dim or dv != self.value_dim:
+            raise ClefError(-1, "DeltaNet tensor shapes")
+        if g.shape != (B, Hv) or beta.shape != (B, Hv) or g.dtype != beta.dtype:
+            raise ClefError(-1, "DeltaNet gate shapes")
+        if g.stride(1) != 1 or beta.stride(1) != 1 or (B > 1 and (g.stride(0) != beta.stride(0) or g.stride(0) < Hv)):
+            raise ClefError(-1, "g and beta must share a token stride with contiguous heads")
+        _here(g, beta)
+        sqk, sv, so = _token_stride(q, "q"), _token_stride(v, "v"), _token_stride(out, "out")
+        _token_stride(k, "k")
+        _check(lib().clef_delta_step(
+            _ptr(q), _ptr(k), _ptr(v), sqk, sv, _dt(q), _ptr(g), _ptr(beta), g.stride(0) if B > 1 else 0, _dt(g), _ptr(slots), B, Hk,
+            Hv, dk, dv, _ptr(states), stride, _ptr(new_states), nslots, _ptr(out), so, _dt(out), _stream()))
+        return out
+
+
+class LinearScan:
+    """Linear attention with one decay per head, S <- e^g S + k v^T, o = scale S^T q
+    (`scale` defaults to 1 / sqrt(key_dim)): prompts, ragged batches of prompts and
+    single tokens.  The inputs' dtype sets the arithmetic: f32 (f32 products) or f16
+    (f16 MFMA, f32 accumulation and states)."""
+
+    def __init__(self, key_dim: int, value_dim: int, scale: float = None):
+        self.key_dim, self.value_dim = key_dim, value_dim
+        self.scale = float(key_dim) ** -0.5 if scale is None else float(scale)
+
+    def _inputs(self, q, k, v, g, out_dtype, out):
+        if q.dim() != 3 or v.dim() != 3:
+            raise ClefError(-1, "q, k, v must be [tokens, heads, width]")
+        T, _, dk = q.shape
+        Hv, dv = v.shape[1], v.shape[2]
+        if k.shape != q.shape or v.shape[0] != T or dk != self.key_dim or dv != self.value_dim:
+            raise ClefError(-1, "linear attention tensor shapes")
+        if q.dtype != k.dtype or q.dtype != v.dtype or q.stride(0) != k.stride(0):
+            raise ClefError(-1, "q, k, v must share a dtype; q and k a token stride")
+        self._decays(g, Hv)
+        if out is None:
+            out = torch.empty((T, Hv, dv), dtype=out_dtype, device=q.device)
+        if out.shape != (T, Hv, dv):
+            raise ClefError(-1, "out must be [tokens, Hv, dv]")
+        _here(q, k, v, g, out)
+        _token_stride(k, "k")
+        return out, _token_stride(q, "q"), _token_stride(v, "v"), _token_stride(out, "out")
+
+    @staticmethod
+    def _decays(g, Hv):
+        if g.shape != (Hv,) or g.dtype != torch.float32 or not g.is_contiguous():
+            raise ClefError(-1, "g must be a contiguous f32 tensor [Hv] of log-decays")
+
+    def _workspace(self, T, nseq, Hk, Hv, q):
+        n = lib().clef_linear_scan_workspace(T, nseq, Hk, Hv, self.key_dim, self.value_dim, _dt(q))
+        if n == 0:
+            raise ClefError(-1, last_error())
+        return _scratch(n, q.device)
+
+    def prefill(self, q, k, v, g, initial=None, out_dtype=torch.float32, want_final=True, out=None):
+        """q, k [T, Hk, dk], v [T, Hv, dv], g [Hv]; initial None or [Hv, dk, dv] f32.
+        Returns (out [T, Hv, dv], final [Hv, dk, dv] or None)."""
+        out, sqk, sv, so = self._inputs(q, k, v, g, out_dtype, out)
+        T, Hk, dk = q.shape
+        Hv, dv = v.shape[1], v.shape[2]
+        if initial is not None and (initial.shape != (Hv, dk, dv) or initial.dtype != torch.float32 or
+                                    not initial.is_contiguous()):
+            raise ClefError(-1, "initial state must be contiguous f32 [Hv, dk, dv]")
+        _here(initial)
+        final = torch.empty((Hv, dk, dv), dtype=torch.float32, device=q.device) if want_final else None
+        ws = self._workspace(T, 1, Hk, Hv, q)
+        _check(lib().clef_linear_scan(
+            _ptr(q), _ptr(k), _ptr(v), sqk, sv, _dt(q), _ptr(g), T, Hk, Hv, dk, dv, self.scale, _ptr(initial),
+            _ptr(out), so, _dt(out), _ptr(final), _ptr(ws), ws.numel(), _stream()))
+        return out, final
+
+    def prefill_varlen(self, q, k, v, g, cu_seqlens, initial=None, out_dtype=torch.float32, want_final=True,
+                       out=None):
+        """Ragged batch: tokens cu_seqlens[s]..cu_seqlens[s+1]-1 form sequence s (int32
+        device tensor [nseq + 1]).  initial: None, one shared [Hv, dk, dv] state, or
+        [nseq, Hv, dk, dv].  Returns (out [T, Hv, dv], final [nseq, Hv, dk, dv] or None)."""
+        out, sqk, sv, so = self._inputs(q, k, v, g, out_dtype, out)
+        T, Hk, dk = q.shape
+        Hv, dv = v.shape[1], v.shape[2]
+        nseq = cu_seqlens.numel() - 1
+        _index(cu_seqlens, nseq + 1, "cu_seqlens")
+        stride = 0
+        if initial is not None:
+            if initial.dtype != torch.float32 or not initial.is_contiguous():
+                raise ClefError(-1, "initial states must be contiguous f32")
+            if initial.shape == (nseq, Hv, dk, dv):
+                stride = Hv * dk * dv
+            elif initial.shape != (Hv, dk, dv):
+                raise ClefError(-1, "initial state must be [Hv, dk, dv] or [nseq, Hv, dk, dv]")
+        _here(cu_seqlens, initial)
+        ws = self._workspace(T, nseq, Hk, Hv, q)
+        final = torch.empty((nseq, Hv, dk, dv), dtype=torch.float32, device=q.device) if want_final else None
+        _check(lib().clef_linear_scan_varlen(
+            _ptr(q), _ptr(k), _ptr(v), sqk, sv, _dt(q), _ptr(g), _ptr(cu_seqlens), nseq, T, Hk, Hv, dk, dv,
+            self.scale, _ptr(initial), stride, _ptr(out), so, _dt(out), _ptr(final), _ptr(ws), ws.numel(), _stream()))
+        return out, final
+
+    def step(self, q, k, v, g, states, slots=None, new_states=None, out_dtype=torch.float32, out=None):
+        """One token of each row (q, k [B, Hk, dk], v [B, Hv, dv], g [Hv]); states, slots
+        and new_states as in DeltaScan.step.  Returns out [B, Hv, dv]."""
+        B, Hk, Hv, dk, dv, stride, new_states, nslots, out = _step_args(q, k, v, states, slots, new_states, out_dtype,
+                                                                        out)
+        if dk != self.key_dim or dv != self.value_dim:
+            raise ClefError(-1, "linear attention tensor shapes")
+        self._decays(g, Hv)
+        _here(g)
+        sqk, sv, so = _token_stride(q, "q"), _token_stride(v, "v"), _token_stride(out, "out")
+        _token_stride(k, "k")
+        _check(lib().clef_linear_step(
+            _ptr(q), _ptr(k), _ptr(v), sqk, sv, _dt(q), _ptr(g), _ptr(slots), B, Hk, Hv, dk, dv, self.scale,
+            _ptr(states), stride, _ptr(new_states), nslots, _ptr(out), so, _dt(out), _stream()))
+        return out
 
 
 def ragged_plan(cu_seqlens, T, unit):
@@ -472,6 +671,59 @@ def attention_gated_varlen(q, k, vt, gate, cu_seqlens, prefix_k=None, prefix_vt=
         heads, kvh, d, _ptr(gate), gate.stride(0), gate.stride(1), _ptr(y), heads * d, _ptr(ws), ws.numel(),
         _stream()))
     return y
+
+
+def attention_gated_shared(q, k, vt, gate, cu_seqlens, key_starts, key_lens, prefix_k=None, prefix_vt=None,
+                           max_keys=None, out=None):
+    """Requests of one to a few tokens behind one shared prefix, which is read once for
+    all: q [heads, T, d] packed by cu_seqlens; prefix_k [kvh, np, d], prefix_vt
+    [kvh, d, >= np] (or None); own keys in a cache k [kvh, rows, d], vt [kvh, d, ldv],
+    sequence s's at rows key_starts[s] .. + key_lens[s] - 1 (its queries are the last
+    of them), at most max_keys (default: all rows) each; k and vt None: only the prefix.
+    gate [T, heads, *] view.  Returns y [T, heads * d]."""
+    if q.dim() != 3 or not q.is_contiguous():
+        raise ClefError(-1, "q must be contiguous [heads, T, d]")
+    heads, T, d = q.shape
+    nseq = cu_seqlens.numel() - 1
+    _index(cu_seqlens, nseq + 1, "cu_seqlens")
+    if (prefix_k is None) != (prefix_vt is None) or (k is None) != (vt is None):
+        raise ClefError(-1, "keys and values come together")
+    if k is None and prefix_k is None:
+        raise ClefError(-1, "no keys: neither a prefix nor own keys")
+    kvh = (prefix_k if k is None else k).shape[0]
+    for name, a, b in (("prefix", prefix_k, prefix_vt), ("own", k, vt)):
+        if a is None:
+            continue
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != kvh or a.shape[2] != d or b.shape[:2] != (kvh, d):
+            raise ClefError(-1, f"{name} keys must be [kv_heads, keys, d] and values [kv_heads, d, keys]")
+        if a.dtype != q.dtype or b.dtype != q.dtype or not a.is_contiguous() or not b.is_contiguous():
+            raise ClefError(-1, f"{name} keys and values must be contiguous and of q's dtype")
+    np_ = 0 if prefix_k is None else prefix_k.shape[1]
+    rows, ldv = (0, 0) if k is None else (k.shape[1], vt.shape[2])
+    if k is not None:
+        _index(key_starts, nseq, "key_starts")
+        _index(key_lens, nseq, "key_lens")
+    max_keys = rows if max_keys is None else min(int(max_keys), rows)
+    if gate.dim() != 3 or gate.shape[:2] != (T, heads) or gate.shape[2] < d or gate.stride(2) != 1 or \
+            gate.dtype != q.dtype:
+        raise ClefError(-1, "gate must be a [T, heads, d] view of q's dtype")
+    if out is None:
+        out = torch.empty((T, heads * d), dtype=q.dtype, device=q.device)
+    if out.shape != (T, heads * d) or out.stride(1) != 1 or out.dtype != q.dtype:
+        raise ClefError(-1, "out must be [T, heads * d] rows of q's dtype")
+    _here(q, k, vt, gate, cu_seqlens, prefix_k, prefix_vt, out)
+    if k is not None:
+        _here(key_starts, key_lens)
+    n = lib().clef_attention_shared_workspace(T, nseq, np_, max_keys, _dt(q), heads, kvh, d)
+    if n == 0:
+        raise ClefError(-1, last_error())
+    ws = _scratch(n, q.device)
+    _check(lib().clef_attention_gated_shared(
+        _ptr(q), T, _ptr(prefix_k), np_, _ptr(prefix_vt), 0 if prefix_vt is None else prefix_vt.shape[2], np_,
+        _ptr(k), rows, _ptr(vt), ldv, _ptr(cu_seqlens), None if k is None else _ptr(key_starts),
+        None if k is None else _ptr(key_lens), nseq, T, max_keys, _dt(q), heads, kvh, d, _ptr(gate), gate.stride(0),
+        gate.stride(1), _ptr(out), out.stride(0), _ptr(ws), ws.numel(), _stream()))
+    return out
 
 
 # ---------------------------------------------------------------------------

@@ -134,6 +134,72 @@ int clef_delta_scan_varlen(const void* q, const void* k, const void* v, int64_t 
                            size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------- */
+/* Linear attention with one decay per head, and single-token steps         */
+/* ---------------------------------------------------------------------- */
+/*
+ * Linear attention: per token and v-head h
+ *   S <- S*exp(g[h]) + k v^T; o = scale * S^T q
+ * with v-head i reading k-head i/(Hv/Hk) as in clef_delta_scan; q and k are
+ * taken as they are (no normalisation).  No counterpart in the reference,
+ * whose linear layers are gated DeltaNet.
+ * q, k: [T, Hk, dk] (token strides sqk, dtype_qkv); v: [T, Hv, dv] (token
+ * stride sv, dtype_qkv); g: [Hv] f32 log-decays (<= 0; -infinity forgets all);
+ * out: [T, Hv, dv] (token stride so, dtype_out).  initial: [Hv, dk, dv] f32 or
+ * NULL (zero state); final_state [Hv, dk, dv] f32 or NULL receives the state
+ * after token T; the two may not overlap.
+ * CLEF_F32 inputs are multiplied in f32 (f32 MFMA).  CLEF_F16 inputs are
+ * multiplied on f16 MFMA with f32 accumulation; there the scores (scale q.k
+ * exp(g n)) and a scaled copy of the state are rounded to f16 as factors of
+ * an output, the f32 states themselves are not (their factors keep 22 bits),
+ * and scores beyond 65504 overflow.
+ * Limits: 1 <= T <= 1048576; 1 <= Hk <= Hv <= 256; Hv % Hk == 0;
+ * 1 <= dk <= 128; 1 <= dv <= 128.  workspace: clef_linear_scan_workspace
+ * (nseq 1 for a single sequence) bytes, 256-byte aligned.
+ */
+size_t clef_linear_scan_workspace(int T, int nseq, int Hk, int Hv, int dk, int dv, int dtype_qkv);
+int clef_linear_scan(const void* q, const void* k, const void* v, int64_t sqk, int64_t sv, int dtype_qkv,
+                     const float* g, int T, int Hk, int Hv, int dk, int dv, float scale, const float* initial,
+                     void* out, int64_t so, int dtype_out, float* final_state, void* workspace,
+                     size_t workspace_bytes, void* stream);
+/*
+ * Ragged batch of nseq sequences packed by cu_seqlens (device int32, nseq + 1
+ * offsets, 1 <= nseq <= 4096; sequences may be empty, and rows behind the last
+ * one are left as they were).  initial: as in clef_delta_scan_varlen (stride
+ * initial_stride floats, 0 = one state shared by all); final_states
+ * [nseq, Hv, dk, dv] or NULL (an empty sequence's is its initial state).  A
+ * malformed table gives unspecified values, never an access out of bounds.
+ */
+int clef_linear_scan_varlen(const void* q, const void* k, const void* v, int64_t sqk, int64_t sv, int dtype_qkv,
+                            const float* g, const int32_t* cu_seqlens, int nseq, int T, int Hk, int Hv, int dk,
+                            int dv, float scale, const float* initial, int64_t initial_stride, void* out, int64_t so,
+                            int dtype_out, float* final_states, void* workspace, size_t workspace_bytes,
+                            void* stream);
+/*
+ * One token of each of B rows (1 <= B <= 4096) by the recurrences of
+ * clef_linear_scan and clef_delta_scan (there with the L2 norms of q and k),
+ * in f32 whatever the inputs' dtype, over a pool of nslots states:
+ * row b reads state slots[b] at states + slots[b] * state_stride floats
+ * ([Hv, dk, dv] f32) and writes its successor to new_states + slots[b] * Hv *
+ * dk * dv.  slots: device int32 [B], or NULL (row b is slot b, B <= nslots).
+ *  - states may be new_states (in place, state_stride Hv * dk * dv); else the
+ *    two may not overlap, and slots that no row names are not written.
+ *    states NULL: zero states; state_stride 0: one state shared by all slots
+ *    (requests forked from one prefix).
+ *  - Rows that name one slot are tokens of one request, taken in row order.
+ *  - A slot outside 0 .. nslots - 1 marks a row without a request: nothing of
+ *    it is read or written, and its row of out is left as it was.
+ * q, k, v, g, beta and out as in the scans, with B rows for T.
+ */
+int clef_linear_step(const void* q, const void* k, const void* v, int64_t sqk, int64_t sv, int dtype_qkv,
+                     const float* g, const int32_t* slots, int B, int Hk, int Hv, int dk, int dv, float scale,
+                     const float* states, int64_t state_stride, float* new_states, int nslots, void* out, int64_t so,
+                     int dtype_out, void* stream);
+int clef_delta_step(const void* q, const void* k, const void* v, int64_t sqk, int64_t sv, int dtype_qkv,
+                    const void* g, const void* beta, int64_t sgb, int dtype_gb, const int32_t* slots, int B, int Hk,
+                    int Hv, int dk, int dv, const float* states, int64_t state_stride, float* new_states, int nslots,
+                    void* out, int64_t so, int dtype_out, void* stream);
+
+/* ---------------------------------------------------------------------- */
 /* Projections                                                             */
 /* ---------------------------------------------------------------------- */
 /*
@@ -328,6 +394,40 @@ int clef_attention_gated_varlen(const void* q, int64_t ldq_tok, const void* k, i
                                 const void* prefix_k, int64_t ldpk_tok, const void* prefix_vt,
                                 int64_t ldpv_tok, int np, int dtype, int heads, int kv_heads, int d,
                                 const void* gate, int64_t ldg, int64_t hsg, void* y, int64_t ldy,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Gated attention of a batch of requests, one to a few tokens each, behind one
+ * shared prefix, which is read once for all of them (clef_attention_gated_varlen
+ * walks it once per sequence and query tile; it is the form for prompts, this
+ * one the form for answers).  Sequence s has the n query rows cu_seqlens[s] ..
+ * cu_seqlens[s+1]-1, which are the last n of its own len = key_lens[s] tokens:
+ * query i sees the np prefix keys and the sequence's own keys 0 .. len - n + i,
+ *   y[t, h*d + e] = attn(...)[h, t, e] * sigmoid(gate[t, h, e]).
+ * Own keys live in a cache with room: key j of sequence s is row key_starts[s]
+ * + j of k [kv_heads, ldk_tok, d] and vt [kv_heads, d, ldv_tok] (any start).
+ * max_keys bounds len (longer ones are cut to it), so that cu_seqlens,
+ * key_starts and key_lens, all device int32, may change under a captured
+ * launch.  A query that sees no key gives zeros; keys that no query of its
+ * sequence sees, and rows of the caches between the sequences, may hold
+ * anything.  Query rows behind the last sequence leave y as it was.
+ * q [heads, ldq_tok, d] (rows 0..T-1); prefix_k [kv_heads, ldpk_tok, d],
+ * prefix_vt [kv_heads, d, ldpv_tok]; dtype CLEF_F16 or CLEF_F32 for q, keys,
+ * values, gate and y, with f32 sums and softmax.  1 <= T <= 65536, 1 <= nseq
+ * <= 4096, heads <= 256, heads % kv_heads == 0, d a multiple of 8 up to 256;
+ * np and max_keys up to 2^24, not both 0 (0: the buffers may be NULL); q, keys
+ * and values 16-byte aligned, ldpv_tok and ldv_tok multiples of 8.  A table
+ * that does not fit gives unspecified values, never an access out of bounds.
+ * workspace: clef_attention_shared_workspace bytes, 256-byte aligned.  No
+ * counterpart in the reference (one request per flash-attention call there).
+ */
+size_t clef_attention_shared_workspace(int T, int nseq, int np, int max_keys, int dtype, int heads, int kv_heads,
+                                       int d);
+int clef_attention_gated_shared(const void* q, int64_t ldq_tok, const void* prefix_k, int64_t ldpk_tok,
+                                const void* prefix_vt, int64_t ldpv_tok, int np, const void* k, int64_t ldk_tok,
+                                const void* vt, int64_t ldv_tok, const int32_t* cu_seqlens, const int32_t* key_starts,
+                                const int32_t* key_lens, int nseq, int T, int max_keys, int dtype, int heads,
+                                int kv_heads, int d, const void* gate, int64_t ldg, int64_t hsg, void* y, int64_t ldy,
                                 void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------- */
