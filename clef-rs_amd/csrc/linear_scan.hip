@@ -3,8 +3,38 @@
 //   S_t = e^{g_h} S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t
 // with v-head i reading k-head i / (Hv / Hk), from each sequence's own initial
 // state.
+//
+// Chunked form.  Over a chunk of n <= 64 tokens that starts from state S, with
+// local i, j = 0 .. n - 1 and l = e^g,
+//   o_i = scale (l^{i+1} S^T q_i + sum_{j<=i} l^{i-j} (q_i.k_j) v_j)
+//   S  <- l^n S + sum_j k_j (l^{n-1-j} v_j)^T
+// are matrix products (4 dk dv + 128 (dk + dv) flops per token against the
+// recurrence's 4 dk dv, but on MFMA).  Chunks are sequential, so a sequence
+// is cut into units of whole chunks: one launch forms what each unit adds to
+// a zero state, a second joins these into the state that each unit starts
+// from, a third walks the units side by side.  Prompts of one unit take the
+// third alone.
+//
+// A work-group owns one unit of one k-head for NH of its v-heads (the scores
+// q.k serve them all) and holds their states in the f32 accumulators of its
+// waves, 32 value columns to a wave.  Products are laid out so that every
+// accumulator is the next product's operand as it stands: the scores are
+// formed transposed (K Q^T: a lane has one query and 4 keys of a tile), the
+// state as S[dk][dv] and the output transposed (o^T = S^T q^T + V^T P^T: a
+// lane has one query and 8 value columns, one 16-byte store).  For f16,
+// whose operands hold 8 consecutive k-indices a lane, the tiles' rows are
+// taken in the order 8 (r / 4) + 4 t + r % 4 (two tiles t to a block of 32), and
+// then a lane's accumulators of both tiles are exactly its operand.  V^T and
+// K^T come out of LDS transposed (ds_read_b64_tr_b16).
+//
+// Precision.  The states, their sums and the scores are f32.  Rounded once, to
+// f16, because the f16 matrix product takes no other factor: the decayed
+// scores, and a copy of the state scaled by a power of two (so that no state
+// overflows) for S^T q.  The decayed values of the state update are split into
+// two f16 factors (22 bits), since the f32 states are results themselves.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "../../include/clef_hip.h"
@@ -15,6 +45,7 @@ namespace {
 
 constexpr int kMaxSeq = 4096;
 constexpr int kMaxWidth = 128;
+constexpr int C = 64;  // tokens of a chunk
 
 struct LinearParams {
   const void *q, *k, *v;
@@ -22,11 +53,50 @@ struct LinearParams {
   const int* cu;         // [nseq + 1] or null (one sequence of T tokens)
   const float* initial;  // sequence s at initial + s * init_stride; null: zeros
   float* final_state;    // [nseq][Hv][dk][dv] or null
+  float* enter;          // [units][Hv][DK * DV]: unit states in register order
   void* out;
   int64_t sqk, sv, so, init_stride;
   int T, nseq, Hk, Hv, dk, dv;
+  int unit;              // tokens of a unit, a multiple of C
+  int nunits;            // at most T / unit + nseq
+  int vec_qk, vec_v, vec_out;  // 16-byte accesses allowed
   float scale;
 };
+
+typedef short short4_t __attribute__((ext_vector_type(4)));
+
+// Matrix fragments of the two dtypes.  KB: k-indices of a fragment (EL per
+// lane, 4 lane groups); TPB: 16-row accumulator tiles of KB rows.
+template <class T> struct Ops;
+template <> struct Ops<half_t> {
+  typedef half8 frag;
+  static constexpr int KB = 32, EL = 8, TPB = 2;
+  // row of the KB-block that row r of its tile t is
+  static __device__ __forceinline__ int row(int t, int r) { return 8 * (r >> 2) + 4 * t + (r & 3); }
+};
+template <> struct Ops<float> {
+  typedef float4_t frag;
+  static constexpr int KB = 16, EL = 4, TPB = 1;
+  static __device__ __forceinline__ int row(int, int r) { return r; }
+};
+
+// Fragment of the transpose of a [token][pitch] LDS tile: operand row (or
+// column) r = lane % 16 is tile column c0 + row(t, r), its k-indices are
+// tokens t0 + EL (lane / 16) + 0 .. EL - 1.
+__device__ __forceinline__ half8 load_t(const half_t* tile, int pitch, int t0, int c0, int t, int lane) {
+  // within 16 lanes, lane 4 a + b names 4 columns of token a, and lane r gets
+  // column r of the 16 named ones for 4 tokens
+  const half_t* p = tile + (t0 + 8 * (lane >> 4) + (lane >> 2 & 3)) * pitch + c0 + 8 * (lane & 3) + 4 * t;
+  typedef __attribute__((address_space(3))) short4_t lds4;
+  union { short4_t s[2]; half8 h; } x;
+  x.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p));
+  x.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * pitch));
+  return x.h;
+}
+__device__ __forceinline__ float4_t load_t(const float* tile, int pitch, int t0, int c0, int, int lane) {
+  const float* p = tile + (t0 + 4 * (lane >> 4)) * pitch + c0 + (lane & 15);
+  return float4_t{p[0], p[pitch], p[2 * pitch], p[3 * pitch]};
+}
 
 // Tokens [t0, t1) of sequence s, inside [0, T] whatever the table holds.
 __device__ __forceinline__ void span_of(const LinearParams& p, int s, int& t0, int& t1) {
@@ -38,59 +108,433 @@ __device__ __forceinline__ void span_of(const LinearParams& p, int s, int& t0, i
   }
 }
 
-// One wave per (sequence, value head, 8 value columns): lane l holds rows l and
-// l + 64 of the state, token after token.
-template <class T, class O>
-__global__ __launch_bounds__(64) void linear_walk(LinearParams p) {
-  constexpr int NC = 8;
-  const int lane = threadIdx.x;
-  const int cols = (p.dv + NC - 1) / NC;
-  const int c0 = blockIdx.x % cols * NC, h = blockIdx.x / cols % p.Hv, s = blockIdx.x / cols / p.Hv;
-  const int hk = h / (p.Hv / p.Hk);
-  int t0, t1;
-  span_of(p, s, t0, t1);
-  const float decay = expf(p.g[h]);
-  float S[2][NC];
-  for (int i = 0; i < 2; ++i)
-    for (int j = 0; j < NC; ++j) {
-      const int r = lane + 64 * i;
-      S[i][j] = p.initial && r < p.dk && c0 + j < p.dv
-                    ? p.initial[s * p.init_stride + ((int64_t)h * p.dk + r) * p.dv + c0 + j]
-                    : 0.0f;
-    }
-  for (int t = t0; t < t1; ++t) {
-    float q[2], k[2];
-    for (int i = 0; i < 2; ++i) {
-      const int r = lane + 64 * i;
-      q[i] = r < p.dk ? to_f32(static_cast<const T*>(p.q)[t * p.sqk + (int64_t)hk * p.dk + r]) : 0.0f;
-      k[i] = r < p.dk ? to_f32(static_cast<const T*>(p.k)[t * p.sqk + (int64_t)hk * p.dk + r]) : 0.0f;
-    }
-    for (int j = 0; j < NC; ++j) {
-      if (c0 + j >= p.dv) break;
-      const float v = to_f32(static_cast<const T*>(p.v)[t * p.sv + (int64_t)h * p.dv + c0 + j]);
-      float o = 0.0f;
-      for (int i = 0; i < 2; ++i) {
-        S[i][j] = fmaf(k[i], v, S[i][j] * decay);
-        o = fmaf(q[i], S[i][j], o);
-      }
-      o = warp_sum(o);
-      if (lane == 0) static_cast<O*>(p.out)[t * p.so + (int64_t)h * p.dv + c0 + j] = cvt_out<O>(o * p.scale);
-    }
+// Units are numbered without a table: sequence s's first is cu[s] / unit + s,
+// so that the ceil(len / unit) of one never reach the next one's first.
+// Numbers that no sequence uses are idle.
+__device__ __forceinline__ int first_unit(const LinearParams& p, int s) {
+  return p.cu ? min(max(p.cu[s], 0), p.T) / p.unit + s : 0;
+}
+// The sequence of unit u: the last one whose first unit is at most u, by 64-way
+// steps (every lane of a wave probes one sequence).
+__device__ __forceinline__ int unit_seq(const LinearParams& p, int u, int lane) {
+  int lo = 0, width = p.nseq;
+  while (width > 1) {
+    const int step = (width + 63) / 64;
+    const int s = lo + lane * step;
+    const uint64_t at = __ballot(lane * step < width && first_unit(p, s) <= u);
+    const int n = at ? 63 - __clzll(at) : 0;
+    lo += n * step;
+    width = min(step, width - n * step);
   }
-  if (!p.final_state) return;
-  for (int i = 0; i < 2; ++i)
-    for (int j = 0; j < NC; ++j) {
-      const int r = lane + 64 * i;
-      if (r < p.dk && c0 + j < p.dv)
-        p.final_state[(((int64_t)s * p.Hv + h) * p.dk + r) * p.dv + c0 + j] = S[i][j];
-    }
+  return lo;
 }
 
-template <class T, class O>
-int launch_walk(const LinearParams& p, hipStream_t st) {
-  const unsigned grid = (unsigned)p.nseq * p.Hv * ((p.dv + 7) / 8);
-  hipLaunchKernelGGL((linear_walk<T, O>), dim3(grid), dim3(64), 0, st, p);
-  return check_launch("linear attention scan");
+// e^g as a power of two per token: l^n = 2^{lg n}; an infinite decay stays
+// finite, so that l^0 = 1.
+__device__ __forceinline__ float log2_decay(float g) {
+  const float x = g * 1.44269504088896341f;
+  return x < -1e30f ? -1e30f : x;
+}
+
+// 64 rows of a [rows][W] tile in registers, 16 bytes at a time, zeros behind
+// `rows` and `width`.
+template <class T, int W, int THREADS>
+struct Staged {
+  static constexpr int EL = 16 / sizeof(T), VPR = W / EL, N = C * VPR / THREADS;
+  static constexpr int PITCH = W + EL;  // LDS rows 16 bytes apart in their banks
+  static_assert(C * VPR % THREADS == 0, "whole vectors per thread");
+  typedef typename Ops<T>::frag vec;
+  static_assert(sizeof(vec) == 16, "16-byte vectors");
+  vec x[N];
+
+  __device__ __forceinline__ void load(const T* src, int64_t stride, int rows, int width, bool wide, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = tid + i * THREADS, r = at / VPR, c = at % VPR * EL;
+      vec y = {};
+      if (r < rows) {
+        if (wide) {
+          if (c < width) y = *reinterpret_cast<const vec*>(src + r * stride + c);
+        } else {
+#pragma unroll
+          for (int e = 0; e < EL; ++e)
+            if (c + e < width) y[e] = src[r * stride + c + e];
+        }
+      }
+      x[i] = y;
+    }
+  }
+  __device__ __forceinline__ void store(T* tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = tid + i * THREADS;
+      *reinterpret_cast<vec*>(tile + at / VPR * PITCH + at % VPR * EL) = x[i];
+    }
+  }
+};
+
+template <class T>
+__device__ __forceinline__ typename Ops<T>::frag frag_at(const T* p) {
+  return *reinterpret_cast<const typename Ops<T>::frag*>(p);
+}
+
+// LDS of a work-group (elements of T): q, k, NH tiles of v, NH blocks of scores.
+template <class T, int DK, int DV, int NH, bool OUT>
+struct Shared {
+  static constexpr int EL = 16 / sizeof(T);
+  static constexpr int K = 0, V = K + C * (DK + EL), Q = V + NH * C * (DV + EL);
+  static constexpr int P = Q + (OUT ? C * (DK + EL) : 0);
+  static constexpr int ALL = P + (OUT ? NH * C * C : 0);
+};
+
+// One unit of NH v-heads.  OUT: walk it from its entering state and write the
+// outputs (and the final state behind a sequence's last unit); else: what it
+// adds to a zero state.
+template <class T, class O, int DK, int DV, int NH, bool OUT>
+__global__ __launch_bounds__(DV * 2, 1) void linear_chunks(LinearParams p) {
+  constexpr int NW = DV / 32, THREADS = 64 * NW;  // a wave for 32 value columns
+  constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL, TPB = Ops<T>::TPB;
+  constexpr int NKB = DK / KB;   // k-blocks of a key row
+  constexpr int NCB = C / KB;    // k-blocks of a chunk
+  constexpr int QT = C / 16;     // query tiles of a chunk
+  constexpr int VB = 32 / KB;    // KB-blocks of a wave's value columns
+  constexpr int VT = 2;          // 16-column tiles of them
+  constexpr int PK = DK + EL, PV = DV + EL;
+  typedef typename Ops<T>::frag frag;
+  typedef Shared<T, DK, DV, NH, OUT> Lds;
+  __shared__ __attribute__((aligned(16))) char smem[Lds::ALL * sizeof(T)];
+  T* const sK = reinterpret_cast<T*>(smem) + Lds::K;
+  T* const sV = reinterpret_cast<T*>(smem) + Lds::V;
+  T* const sQ = reinterpret_cast<T*>(smem) + Lds::Q;
+  T* const sP = reinterpret_cast<T*>(smem) + Lds::P;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, grp = lane >> 4;
+  const int groups = p.Hv / NH;
+  const int h0 = blockIdx.x % groups * NH, u = blockIdx.x / groups;
+  const int hk = h0 / (p.Hv / p.Hk);
+  const int s = p.nseq > 1 ? __builtin_amdgcn_readfirstlane(unit_seq(p, u, lane)) : 0;
+  int t0, t1;
+  span_of(p, s, t0, t1);
+  const int index = u - first_unit(p, s);
+  const int begin = t0 + index * p.unit, end = min(begin + p.unit, t1);
+  if (index < 0 || (index > 0 && begin >= t1)) return;
+  const bool last = end == t1;
+  if (!OUT && last) return;  // what follows a sequence's last unit is the walk's to write
+
+  float lg[NH];
+#pragma unroll
+  for (int n = 0; n < NH; ++n) lg[n] = log2_decay(p.g[h0 + n]);
+
+  const T* q = static_cast<const T*>(p.q) + (int64_t)hk * p.dk;
+  const T* k = static_cast<const T*>(p.k) + (int64_t)hk * p.dk;
+  const T* v = static_cast<const T*>(p.v) + (int64_t)h0 * p.dv;
+  Staged<T, DK, THREADS> rq, rk;
+  Staged<T, DV, THREADS> rv[NH];
+  auto fetch = [&](int t) {
+    const int rows = min(C, end - t);
+    if (OUT) rq.load(q + t * p.sqk, p.sqk, rows, p.dk, p.vec_qk, tid);
+    rk.load(k + t * p.sqk, p.sqk, rows, p.dk, p.vec_qk, tid);
+#pragma unroll
+    for (int n = 0; n < NH; ++n) rv[n].load(v + t * p.sv + n * p.dv, p.sv, rows, p.dv, p.vec_v, tid);
+  };
+  if (begin < end) fetch(begin);
+
+  // ---- the entering state: tile (b, t, x) of S has rows KB b + row(t, .) and
+  // columns 32 wave + column(x)
+  const int c0 = wave * 32;
+  auto column = [&](int x, int i) { return c0 + (x / TPB) * KB + Ops<T>::row(x % TPB, i); };
+  float4_t S[NH][NKB * TPB][VT];
+#pragma unroll
+  for (int n = 0; n < NH; ++n) {
+    const int h = h0 + n;
+    if (OUT && index > 0) {
+      const float* src = p.enter + ((int64_t)u * p.Hv + h) * (DK * DV) + wave * (DK * 32);
+#pragma unroll
+      for (int a = 0; a < NKB * TPB; ++a)
+#pragma unroll
+        for (int x = 0; x < VT; ++x) S[n][a][x] = *reinterpret_cast<const float4_t*>(src + ((a * VT + x) * 64 + lane) * 4);
+    } else {
+      const float* src = OUT && p.initial ? p.initial + s * p.init_stride + (int64_t)h * p.dk * p.dv : nullptr;
+#pragma unroll
+      for (int a = 0; a < NKB * TPB; ++a)
+#pragma unroll
+        for (int x = 0; x < VT; ++x)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = a / TPB * KB + Ops<T>::row(a % TPB, 4 * grp + i), col = column(x, r);
+            S[n][a][x][i] = src && row < p.dk && col < p.dv ? src[row * p.dv + col] : 0.0f;
+          }
+    }
+  }
+
+  for (int t = begin; t < end; t += C) {
+    const int rows = min(C, end - t);
+    if (OUT) rq.store(sQ, tid);
+    rk.store(sK, tid);
+#pragma unroll
+    for (int n = 0; n < NH; ++n) rv[n].store(sV + n * C * PV, tid);
+    lds_barrier();
+    if (t + C < end) fetch(t + C);
+
+    if constexpr (OUT) {
+      // ---- scores, transposed: keys of block b x queries of tile qt
+#pragma unroll
+      for (int qt = wave; qt < QT; qt += NW) {
+        frag fq[NKB];
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) fq[kb] = frag_at(sQ + (qt * 16 + r) * PK + kb * KB + grp * EL);
+#pragma unroll
+        for (int b = 0; b < NCB; ++b) {
+          if (b * KB > qt * 16 + 15) continue;  // keys behind every query of the tile
+          float4_t acc[TPB] = {};
+#pragma unroll
+          for (int x = 0; x < TPB; ++x)
+#pragma unroll
+            for (int kb = 0; kb < NKB; ++kb)
+              Mma<T>::mma(acc[x], frag_at(sK + (b * KB + Ops<T>::row(x, r)) * PK + kb * KB + grp * EL), fq[kb]);
+          const int i = qt * 16 + r;  // query
+#pragma unroll
+          for (int n = 0; n < NH; ++n) {
+            frag f;
+#pragma unroll
+            for (int x = 0; x < TPB; ++x)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int j = b * KB + Ops<T>::row(x, 4 * grp + e);  // key
+                const float w = acc[x][e] * p.scale * __builtin_amdgcn_exp2f(lg[n] * (float)max(i - j, 0));
+                f[x * 4 + e] = static_cast<T>(j <= i ? w : 0.0f);
+              }
+            *reinterpret_cast<frag*>(sP + n * C * C + ((qt * NCB + b) * 64 + lane) * EL) = f;
+          }
+        }
+      }
+      lds_barrier();
+
+      // ---- outputs, transposed: value columns x queries
+#pragma unroll
+      for (int n = 0; n < NH; ++n) {
+        // f16: the state's copy scaled to at most 2^14 by a power of two
+        float up = 1.0f, down = 1.0f;
+        if constexpr (sizeof(T) == 2) {
+          float big = 0.0f;
+#pragma unroll
+          for (int a = 0; a < NKB * TPB; ++a)
+#pragma unroll
+            for (int x = 0; x < VT; ++x)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(S[n][a][x][i]));
+          big = lane_max<16>(big);
+          big = fmaxf(big, __shfl_xor(big, 16, 64));
+          big = fmaxf(big, __shfl_xor(big, 32, 64));
+          const uint32_t ex = max(__float_as_uint(big) >> 23, 14u);  // sign clear
+          up = __uint_as_float((267u - ex) << 23);    // 2^(13 - exponent)
+          down = __uint_as_float((ex - 13u) << 23);
+        }
+        auto state_part = [&](float4_t (&o)[VT][QT]) {
+#pragma unroll
+          for (int x = 0; x < VT; ++x)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) o[x][qt] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kb = 0; kb < NKB; ++kb) {
+            frag fs[VT];
+#pragma unroll
+            for (int x = 0; x < VT; ++x)
+#pragma unroll
+              for (int y = 0; y < TPB; ++y)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) fs[x][y * 4 + e] = static_cast<T>(S[n][kb * TPB + y][x][e] * up);
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+              const frag fq = frag_at(sQ + (qt * 16 + r) * PK + kb * KB + grp * EL);
+#pragma unroll
+              for (int x = 0; x < VT; ++x) Mma<T>::mma(o[x][qt], fs[x], fq);
+            }
+          }
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) {
+            const float w = p.scale * down * __builtin_amdgcn_exp2f(lg[n] * (float)(qt * 16 + r + 1));
+#pragma unroll
+            for (int x = 0; x < VT; ++x) o[x][qt] *= w;
+          }
+        };
+        float4_t o[VT][QT];
+        state_part(o);
+#pragma unroll
+        for (int b = 0; b < NCB; ++b) {
+          frag fv[VT];
+#pragma unroll
+          for (int x = 0; x < VT; ++x) fv[x] = load_t(sV + n * C * PV, PV, b * KB, c0 + x / TPB * KB, x % TPB, lane);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) {
+            if (b * KB > qt * 16 + 15) continue;
+            const frag fp = frag_at(sP + n * C * C + ((qt * NCB + b) * 64 + lane) * EL);
+#pragma unroll
+            for (int x = 0; x < VT; ++x) Mma<T>::mma(o[x][qt], fv[x], fp);
+          }
+        }
+        // An infinite or NaN value times a masked score of 0 is NaN: where an
+        // output is not finite, the products are formed again one by one, over
+        // the keys that its query sees.
+        float test = 0.0f;
+#pragma unroll
+        for (int x = 0; x < VT; ++x)
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) test = fmaf(o[x][qt][i], 0.0f, test);
+        if (__any(test != 0.0f)) {
+          state_part(o);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int x = 0; x < VT; ++x)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int col = column(x, 4 * grp + e), i = qt * 16 + r;
+                float sum = o[x][qt][e];
+                for (int j = 0; j <= i; ++j) {
+                  // score (i, j) in its fragment's place
+                  const int jj = j % KB, gj = jj / EL;
+                  const float w = to_f32(sP[n * C * C + ((qt * NCB + j / KB) * 64 + gj * 16 + r) * EL + jj % EL]);
+                  sum = fmaf(w, to_f32(sV[n * C * PV + j * PV + col]), sum);
+                }
+                o[x][qt][e] = sum;
+              }
+        }
+        O* out = static_cast<O*>(p.out) + t * p.so + (int64_t)(h0 + n) * p.dv;
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          const int i = qt * 16 + r;
+          if (i >= rows) continue;
+#pragma unroll
+          for (int y = 0; y < VB; ++y) {  // EL consecutive columns
+            const int col = c0 + y * KB + grp * EL;
+            O* dst = out + i * p.so + col;
+            if (p.vec_out && col < p.dv) {
+              if constexpr (sizeof(O) == 2) {
+                typedef O vecn __attribute__((ext_vector_type(EL)));
+                vecn w;
+#pragma unroll
+                for (int e = 0; e < EL; ++e) w[e] = cvt_out<O>(o[y * TPB + e / 4][qt][e % 4]);
+                *reinterpret_cast<vecn*>(dst) = w;
+              } else {
+#pragma unroll
+                for (int x = 0; x < TPB; ++x) *reinterpret_cast<float4_t*>(dst + x * 4) = o[y * TPB + x][qt];
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < EL; ++e)
+                if (col + e < p.dv) dst[e] = cvt_out<O>(o[y * TPB + e / 4][qt][e % 4]);
+            }
+          }
+        }
+      }
+    }
+
+    // ---- S <- l^rows S + K^T (l^{rows-1-j} V)
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      const float w = __builtin_amdgcn_exp2f(lg[n] * (float)rows);
+#pragma unroll
+      for (int a = 0; a < NKB * TPB; ++a)
+#pragma unroll
+        for (int x = 0; x < VT; ++x) S[n][a][x] *= w;
+    }
+#pragma unroll
+    for (int b = 0; b < NCB; ++b) {
+      frag hi[NH][VT], lo[NH][VT];
+#pragma unroll
+      for (int n = 0; n < NH; ++n) {
+        float w[EL];
+#pragma unroll
+        for (int e = 0; e < EL; ++e)
+          w[e] = __builtin_amdgcn_exp2f(lg[n] * (float)max(rows - 1 - (b * KB + grp * EL + e), 0));
+#pragma unroll
+        for (int x = 0; x < VT; ++x) {
+          const frag f = load_t(sV + n * C * PV, PV, b * KB, c0 + x / TPB * KB, x % TPB, lane);
+#pragma unroll
+          for (int e = 0; e < EL; ++e) {
+            const float y = to_f32(f[e]) * w[e];
+            hi[n][x][e] = cvt_out<T>(y);  // of the rounded product, as the next line takes it
+            if constexpr (sizeof(T) == 2) lo[n][x][e] = static_cast<T>(y - to_f32(hi[n][x][e]));
+          }
+        }
+      }
+#pragma unroll
+      for (int a = 0; a < NKB * TPB; ++a) {
+        const frag fk = load_t(sK, PK, b * KB, a / TPB * KB, a % TPB, lane);
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int x = 0; x < VT; ++x) {
+            Mma<T>::mma(S[n][a][x], fk, hi[n][x]);
+            if constexpr (sizeof(T) == 2) Mma<T>::mma(S[n][a][x], fk, lo[n][x]);
+          }
+      }
+    }
+    lds_barrier();  // everyone is done with the tiles
+  }
+
+#pragma unroll
+  for (int n = 0; n < NH; ++n) {
+    const int h = h0 + n;
+    if constexpr (!OUT) {
+      float* dst = p.enter + ((int64_t)u * p.Hv + h) * (DK * DV) + wave * (DK * 32);
+#pragma unroll
+      for (int a = 0; a < NKB * TPB; ++a)
+#pragma unroll
+        for (int x = 0; x < VT; ++x) *reinterpret_cast<float4_t*>(dst + ((a * VT + x) * 64 + lane) * 4) = S[n][a][x];
+    } else if (p.final_state && last) {
+      float* dst = p.final_state + ((int64_t)s * p.Hv + h) * p.dk * p.dv;
+#pragma unroll
+      for (int a = 0; a < NKB * TPB; ++a)
+#pragma unroll
+        for (int x = 0; x < VT; ++x)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = a / TPB * KB + Ops<T>::row(a % TPB, 4 * grp + i), col = column(x, r);
+            if (row < p.dk && col < p.dv) dst[row * p.dv + col] = S[n][a][x][i];
+          }
+    }
+  }
+}
+
+// The state that each unit starts from: enter[u] holds what unit u adds, and
+// becomes what it starts with (units behind a sequence's first).  A thread owns
+// 4 elements of one (sequence, head).
+template <class T, int DK, int DV>
+__global__ __launch_bounds__(256) void linear_join(LinearParams p) {
+  constexpr int KB = Ops<T>::KB, TPB = Ops<T>::TPB;
+  const int per = DK * DV / 4 / 256;  // work-groups of a state
+  const int part = blockIdx.x % per, h = blockIdx.x / per % p.Hv, s = blockIdx.x / per / p.Hv;
+  int t0, t1;
+  span_of(p, s, t0, t1);
+  const int n = (t1 - t0 + p.unit - 1) / p.unit;
+  if (n < 2) return;
+  const int e = (part * 256 + threadIdx.x) * 4;  // wave * DK * 32 + ((a * 2 + x) * 64 + lane) * 4
+  float4_t run = {0.f, 0.f, 0.f, 0.f};
+  if (p.initial) {
+    const int lane = e / 4 % 64, x = e / 256 % 2, a = e / 512 % (DK / 16), wave = e / (DK * 32);
+    const float* src = p.initial + s * p.init_stride + (int64_t)h * p.dk * p.dv;
+    const int col = wave * 32 + x / TPB * KB + Ops<T>::row(x % TPB, lane & 15);
+    for (int i = 0; i < 4; ++i) {
+      const int row = a / TPB * KB + Ops<T>::row(a % TPB, 4 * (lane >> 4) + i);
+      if (row < p.dk && col < p.dv) run[i] = src[row * p.dv + col];
+    }
+  }
+  const float w = __builtin_amdgcn_exp2f(log2_decay(p.g[h]) * (float)p.unit);
+  const int64_t step = (int64_t)p.Hv * (DK * DV);
+  float* at = p.enter + (first_unit(p, s) * (int64_t)p.Hv + h) * (DK * DV) + e;
+  float4_t next = *reinterpret_cast<const float4_t*>(at);
+  for (int u = 1; u < n; ++u) {
+    const float4_t add = next;
+    at += step;
+    if (u + 1 < n) next = *reinterpret_cast<const float4_t*>(at);
+    run = run * w + add;
+    *reinterpret_cast<float4_t*>(at) = run;
+  }
 }
 
 bool valid_dtype(int d) { return d == CLEF_F32 || d == CLEF_F16; }
@@ -106,7 +550,48 @@ int linear_dims(int T, int nseq, int Hk, int Hv, int dk, int dv, int dtype_qkv) 
   return 0;
 }
 
-size_t workspace_bytes(int T, int nseq, int Hk, int Hv, int dk, int dv, int dtype_qkv) { return 256; }
+// Tokens of a unit: enough units that the work-groups fill the chip once, and
+// none shorter than 4 chunks, since a cut costs two launches and two passes
+// over a state.
+int unit_tokens(int T, int groups) {
+  const int64_t want = ((int64_t)T * groups + device_cus() - 1) / device_cus();
+  return static_cast<int>((std::max<int64_t>(want, 256) + C - 1) / C * C);
+}
+int padded(int d) { return d <= 64 ? 64 : 128; }
+// v-heads of a work-group: two of one k-head share their scores (f16; in f32
+// two would not fit the LDS)
+int paired(int Hk, int Hv, int dtype) { return dtype == CLEF_F16 && Hv / Hk % 2 == 0 ? 2 : 1; }
+
+size_t workspace_bytes(int T, int nseq, int Hk, int Hv, int dk, int dv, int dtype) {
+  const int unit = unit_tokens(T, Hv / paired(Hk, Hv, dtype));
+  if (T <= unit) return 256;  // every sequence is one unit
+  return ((size_t)T / unit + nseq) * Hv * padded(dk) * padded(dv) * 4;
+}
+
+template <class T, class O, int DK, int DV, int NH>
+int launch(const LinearParams& p, hipStream_t st) {
+  const dim3 grid((unsigned)p.nunits * (p.Hv / NH)), block(DV * 2);
+  if (p.unit < p.T) {
+    hipLaunchKernelGGL((linear_chunks<T, T, DK, DV, NH, false>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((linear_join<T, DK, DV>), dim3((unsigned)p.nseq * p.Hv * (DK * DV / 1024)), dim3(256), 0, st, p);
+  }
+  hipLaunchKernelGGL((linear_chunks<T, O, DK, DV, NH, true>), grid, block, 0, st, p);
+  return check_launch("linear attention scan");
+}
+
+template <class T, class O, int DK, int DV>
+int launch_heads(const LinearParams& p, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (paired(p.Hk, p.Hv, CLEF_F16) == 2) return launch<T, O, DK, DV, 2>(p, st);
+  }
+  return launch<T, O, DK, DV, 1>(p, st);
+}
+
+template <class T, class O>
+int launch_widths(const LinearParams& p, hipStream_t st) {
+  if (padded(p.dk) == 64) return padded(p.dv) == 64 ? launch_heads<T, O, 64, 64>(p, st) : launch_heads<T, O, 64, 128>(p, st);
+  return padded(p.dv) == 64 ? launch_heads<T, O, 128, 64>(p, st) : launch_heads<T, O, 128, 128>(p, st);
+}
 
 int linear_scan(const void* q, const void* k, const void* v, int64_t sqk, int64_t sv, int dtype_qkv, const float* g,
                 const int32_t* cu_seqlens, int nseq, int T, int Hk, int Hv, int dk, int dv, float scale,
@@ -139,9 +624,19 @@ int linear_scan(const void* q, const void* k, const void* v, int64_t sqk, int64_
   p.sqk = sqk; p.sv = sv; p.so = so; p.init_stride = initial_stride;
   p.T = T; p.nseq = nseq; p.Hk = Hk; p.Hv = Hv; p.dk = dk; p.dv = dv;
   p.scale = scale;
+  p.unit = unit_tokens(T, Hv / paired(Hk, Hv, dtype_qkv));
+  p.nunits = (cu_seqlens ? T / p.unit : (T + p.unit - 1) / p.unit - 1) + nseq;
+  p.enter = static_cast<float*>(workspace);
+  auto wide = [](const void* x, int64_t stride, int width, int dtype) {
+    const int el = dtype == CLEF_F16 ? 8 : 4;
+    return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && stride % el == 0 && width % el == 0;
+  };
+  p.vec_qk = wide(q, sqk, dk, dtype_qkv) && wide(k, sqk, dk, dtype_qkv);
+  p.vec_v = wide(v, sv, dv, dtype_qkv);
+  p.vec_out = wide(out, so, dv, CLEF_F16) && dv % 8 == 0;
   if (dtype_qkv == CLEF_F16)
-    return dtype_out == CLEF_F16 ? launch_walk<half_t, half_t>(p, st) : launch_walk<half_t, float>(p, st);
-  return dtype_out == CLEF_F16 ? launch_walk<float, half_t>(p, st) : launch_walk<float, float>(p, st);
+    return dtype_out == CLEF_F16 ? launch_widths<half_t, half_t>(p, st) : launch_widths<half_t, float>(p, st);
+  return dtype_out == CLEF_F16 ? launch_widths<float, half_t>(p, st) : launch_widths<float, float>(p, st);
 }
 
 }  // namespace
