@@ -35,6 +35,7 @@ namespace {
 
 constexpr int kMaxSeq = 4096;
 constexpr int kMaxKeys = 1 << 24;
+constexpr int kMaxParts = 128;  // of a row, prefix and own
 
 struct SharedParams {
   const void* q;           // [heads][ldq][d]
@@ -72,16 +73,19 @@ __device__ __forceinline__ typename Ops<T>::frag frag_at(const T* p) {
   return *reinterpret_cast<const typename Ops<T>::frag*>(p);
 }
 
-// The sequence that token t belongs to, or -1 (rows behind the last one).
-__device__ __forceinline__ int seq_of(const SharedParams& p, int t) {
-  int lo = 0, hi = p.nseq;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu[mid + 1] <= t) lo = mid + 1;
-    else hi = mid;
+// The sequence that token t belongs to, or -1 (rows behind the last one): the
+// first one that ends behind t, by 64-way steps (a lane of the wave for each probe).
+__device__ __forceinline__ int seq_of(const SharedParams& p, int t, int lane) {
+  int lo = 0, width = p.nseq;  // it is among [lo, lo + width], if any
+  while (width > 0) {
+    const int step = (width + 63) / 64;
+    const int i = lane * step + step - 1;  // the last of the lane's step sequences
+    const uint64_t ends = __ballot(i < width && p.cu[lo + i + 1] <= t);
+    const int n = __popcll(ends);  // whole steps that end before
+    lo += n * step;
+    width = min(step - 1, width - n * step);
   }
-  if (lo >= p.nseq || p.cu[lo] > t) return -1;
-  return lo;
+  return lo < p.nseq && p.cu[lo] <= t ? lo : -1;
 }
 
 // First cache row and count of the own keys that token t of sequence s sees,
@@ -297,106 +301,219 @@ __global__ __launch_bounds__(256) void shared_few_rows(SharedParams p) {
   }
 }
 
-// Part of the prefix for 128 stacked rows (f16): wave w has rows 32 w + (0..31),
-// tiles of 64 keys pass through LDS, double-buffered, the next tile's loads in
-// flight during a tile's products.
+// Part of the prefix for 128 stacked rows (f16, d = D): wave w has rows 32 w +
+// (0..31), one per lane of a half wave, on 32 x 32 x 16 products.  Tiles of 64
+// keys pass through LDS by DMA, double-buffered; the scores of tile j + 1 are
+// formed while tile j's exponentials run on the vector ALU, and the products
+// with V under the next scores' maximum.  Its LDS reads (64 KiB a wave and tile)
+// and its products take the same time at their peak rates, which bounds it.
+//
+// LDS layout: key row x of a tile holds key x with bits 2 and 3 exchanged, so that
+// the 16 weights a lane forms of a 32-key half are its operands in key order;
+// 16-byte slots are permuted by their row (XOR), against bank conflicts.
+__device__ __forceinline__ void dma16s(const void* base, uint32_t off, void* lds_block) {
+  // global_load_lds_dwordx4: lane l writes 16 bytes at M0 + 16 l, awaited by
+  // vm_wait_all; the wait states cover M0 and the readfirstlane before it
+  const uint32_t m0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_block));
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(b >> 32)));
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(b)));
+  const uint64_t sb = (static_cast<uint64_t>(hi) << 32) | lo;
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(sb), "{m0}"(m0) : "memory");
+}
+__device__ __forceinline__ void vm_wait_all() { __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8)); }
+__device__ __forceinline__ float halves_max(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
+
 template <int D>
 __global__ __launch_bounds__(256, 1) void shared_many_rows(SharedParams p) {
-  typedef half_t T;
-  constexpr int RT = 2, KB = 32, EL = 8, BK = 64;
-  constexpr int PK = D + EL, PV = BK + EL;      // pitches that spread 16 rows over the banks
-  constexpr int NK = BK * D / EL / 256, NV = D * BK / EL / 256;  // vectors a thread moves
-  __shared__ __attribute__((aligned(16))) T sK[2][BK * PK];
-  __shared__ __attribute__((aligned(16))) T sV[2][D * PV];
+  constexpr int BK = 64, NKB = D / 16, NDT = D / 32, KS = D / 8;
+  constexpr int NDMA = D / 32;     // DMA instructions per wave, operand and tile
+  constexpr int KROWS = 512 / D;   // key rows of one
+  constexpr int PD = 8;            // operand reads in flight
+  constexpr int NS1 = 2 * NKB, NS2 = 4 * NDT, EPS1 = 32 / NS1, EPS2 = 32 / NS2;
+  __shared__ __attribute__((aligned(1024))) half_t sK[2][BK * D];
+  __shared__ __attribute__((aligned(1024))) half_t sV[2][D * BK];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = lane & 15, grp = lane >> 4;
+  const int n = lane & 31, g = lane >> 5;
   const int G = p.heads / p.kvh, rows = p.T * G;
   const int split = blockIdx.x % p.psplits, kv = blockIdx.x / p.psplits % p.kvh;
-  const int row0 = blockIdx.x / p.psplits / p.kvh * 128 + wave * 32;
+  const int at = blockIdx.x / p.psplits / p.kvh * 128 + 32 * wave + n;  // the lane's row
   const int k0 = split * p.pkeys, k1 = min(k0 + p.pkeys, p.np);
-  const T* k = static_cast<const T*>(p.pk) + (int64_t)kv * p.ldpk * p.d;
-  const T* vt = static_cast<const T*>(p.pvt) + (int64_t)kv * p.d * p.ldpv;
+  const half_t* K = static_cast<const half_t*>(p.pk) + (int64_t)kv * p.ldpk * D;
+  const half_t* V = static_cast<const half_t*>(p.pvt) + (int64_t)kv * D * p.ldpv;
 
-  half8 rk[NK], rv[NV];
-  auto fetch = [&](int j0) {
+  half8 qf[NKB];  // features 16 kb + 8 g .. + 7 of the lane's row
+  {
+    const int row = min(at, rows - 1);
+    const half_t* q = static_cast<const half_t*>(p.q) + ((int64_t)(kv * G + row % G) * p.ldq + row / G) * D;
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      const int at = tid + i * 256, j = at / (D / EL), e = at % (D / EL) * EL;
-      rk[i] = j0 + j < k1 && e < p.d ? frag_at(k + (int64_t)(j0 + j) * p.d + e) : half8{};
-    }
+    for (int kb = 0; kb < NKB; ++kb) qf[kb] = frag_at(q + 16 * kb + 8 * g);
+  }
+
+  // DMA instruction wave * NDMA + x writes 1 KiB: KROWS key rows, or 8 feature rows
+  auto key_of = [](int r) { return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1); };
+  auto swizzle = [](int r) { return D >= 128 ? (r & 15) : ((r >> 1) & 7); };
+  uint32_t ko[NDMA], vo[NDMA];
+  int kr[NDMA];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int at = tid + i * 256, e = at / (BK / EL), j = at % (BK / EL) * EL;
-      rv[i] = e < p.d ? run_at<T, false>(vt + e * p.ldpv + j0 + j, k1 - j0 - j) : half8{};
+  for (int x = 0; x < NDMA; ++x) {
+    const int row = (wave * NDMA + x) * KROWS + lane / KS;
+    kr[x] = key_of(row);
+    ko[x] = 16u * ((lane % KS) ^ swizzle(row));
+    const int e = (wave * NDMA + x) * 8 + (lane >> 3);
+    vo[x] = 2u * ((uint32_t)e * (uint32_t)p.ldpv + 8 * ((lane & 7) ^ ((e >> 1) & 7)));
+  }
+  auto issue_k = [&](int buf, int j0) {  // keys behind the last: the last again (masked)
+    const half_t* base = K + (int64_t)j0 * D;
+    const int left = p.np - 1 - j0;
+#pragma unroll
+    for (int x = 0; x < NDMA; ++x)
+      dma16s(base, ko[x] + 2u * D * min(kr[x], left), &sK[buf][(wave * NDMA + x) * 512]);
+  };
+  const int vlast = (int)(p.ldpv - 8);
+  auto issue_v = [&](int buf, int j0) {  // columns behind the row: its last 8 (zeroed below)
+    const int over = max(0, j0 + 56 - vlast);
+    const half_t* base = V + j0;
+#pragma unroll
+    for (int x = 0; x < NDMA; ++x) {
+      const int e = (wave * NDMA + x) * 8 + (lane >> 3);
+      const int c = 8 * ((lane & 7) ^ ((e >> 1) & 7));
+      dma16s(base, over ? vo[x] - 2u * max(0, j0 + c - vlast) : vo[x], &sV[buf][(wave * NDMA + x) * 512]);
     }
   };
-  auto stage = [&](int b) {
+
+  constexpr int KPER = D >= 128 ? 8 : 4;
+  int koff[KPER], voff[4];
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      const int at = tid + i * 256;
-      *reinterpret_cast<half8*>(sK[b] + at / (D / EL) * PK + at % (D / EL) * EL) = rk[i];
-    }
+  for (int x = 0; x < KPER; ++x) koff[x] = n * 2 * D + 16 * ((2 * x + g) ^ swizzle(n));
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int at = tid + i * 256;
-      *reinterpret_cast<half8*>(sV[b] + at / (BK / EL) * PV + at % (BK / EL) * EL) = rv[i];
-    }
+  for (int x = 0; x < 4; ++x) voff[x] = n * 128 + 16 * ((2 * x + g) ^ ((n >> 1) & 7));
+  auto operand = [&](const char* kbase, const char* vbase, int i) {
+    if (i < NS1)  // k-block i / 2, key half i % 2
+      return *reinterpret_cast<const half8*>(kbase + koff[(i >> 1) % KPER] + (i & 1) * 64 * D +
+                                             ((i >> 1) / KPER) * 32 * KPER);
+    i -= NS1;  // 16-key block i / NDT, feature tile i % NDT
+    return *reinterpret_cast<const half8*>(vbase + voff[i / NDT] + (i % NDT) * 32 * 128);
   };
-  fetch(k0);
-  half8 fq[D / KB][RT];
-  load_queries<T, D, RT>(p, fq, kv, row0, rows, lane);
-  Soft<T, D, RT> st;
-  st.clear();
-  stage(0);
-  if (k0 + BK < k1) fetch(k0 + BK);
+  // accumulator x = 16 half + e of a lane is this key of the tile (and 8 g more)
+  auto key_in_tile = [](int x) { return 32 * (x >> 4) + 16 * ((x >> 3) & 1) + (x & 7); };
+
+  float16_t O[NDT] = {}, Sc[2] = {}, Sn[2];
+  float l = 0.0f, m = -INFINITY;
+  half8 fb[PD];
+  const int ntiles = (k1 - k0 + BK - 1) / BK;
+  issue_k(0, k0);
+  issue_v(0, k0);
+  if (ntiles > 1) issue_k(1, k0 + BK);
+  vm_wait_all();
   lds_barrier();
-  int b = 0;
-  for (int j0 = k0; j0 < k1; j0 += BK, b ^= 1) {
-    if (j0 + BK < k1) {
-      stage(b ^ 1);
-      if (j0 + 2 * BK < k1) fetch(j0 + 2 * BK);
+  {
+    const char* kbase = reinterpret_cast<const char*>(sK[0]);
+#pragma unroll
+    for (int i = 0; i < PD; ++i) fb[i] = operand(kbase, kbase, i);
+#pragma unroll
+    for (int i = 0; i < NS1; ++i) {
+      Sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[i % PD], qf[i >> 1], Sc[i & 1], 0, 0, 0);
+      if (i + PD < NS1) fb[i % PD] = operand(kbase, kbase, i + PD);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    float4_t S[4][RT] = {};
+    const int thr = k1 - k0 - 8 * g;
 #pragma unroll
-    for (int kb = 0; kb < D / KB; ++kb)
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const half8 fk = frag_at(sK[b] + (a / 2 * KB + Ops<T>::row(a % 2, r)) * PK + kb * KB + grp * EL);
-#pragma unroll
-        for (int y = 0; y < RT; ++y) Mma<T>::mma(S[a][y], fk, fq[kb][y]);
-      }
-    if (j0 + BK > k1) {
-#pragma unroll
-      for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (j0 + a / 2 * KB + Ops<T>::row(a % 2, 4 * grp + i) >= k1) {
-#pragma unroll
-            for (int y = 0; y < RT; ++y) S[a][y][i] = -INFINITY;
-          }
+    for (int x = 0; x < 32; ++x) {
+      const float y = key_in_tile(x) >= thr ? -INFINITY : Sc[x >> 4][x & 15];
+      Sc[x >> 4][x & 15] = y;
+      m = fmaxf(m, y);
     }
-    half8 w[2][RT];
-    st.template weights<2>(S, w, p.c);
+    m = halves_max(m);
+  }
+  lds_barrier();  // all waves are done with K(0) before K(2) replaces it
+
+  // iteration j: K(j + 1), V(j) resident, masked scores of tile j in Sc
+  for (int j = 0; j < ntiles; ++j) {
+    const int j0 = k0 + j * BK;
+    if (j + 2 < ntiles) issue_k(j & 1, j0 + 2 * BK);
+    if (j + 1 < ntiles) issue_v((j + 1) & 1, j0 + BK);
+    if (j0 + BK > k1) {  // zero the values behind the last key
+      half_t* v = sV[j & 1];
+      for (int x = tid; x < D * 8; x += 256) {
+        const int e = x >> 3, slot = x & 7, c = j0 + 8 * (slot ^ ((e >> 1) & 7));
+        if (c + 8 > k1) {
+          half8 y = frag_at(v + e * 64 + slot * 8);
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const half8 fv = frag_at(sV[b] + (e * 16 + r) * PV + x * KB + grp * EL);
-#pragma unroll
-        for (int y = 0; y < RT; ++y) Mma<T>::mma(st.o[e][y], fv, w[x][y]);
+          for (int i = 0; i < 8; ++i)
+            if (c + i >= k1) y[i] = half_t(0);
+          *reinterpret_cast<half8*>(v + e * 64 + slot * 8) = y;
+        }
       }
-    lds_barrier();  // this tile is read, the next one written
-  }
+      lds_barrier();
+    }
+    const char* kbase = reinterpret_cast<const char*>(sK[(j + 1) & 1]);
+    const char* vbase = reinterpret_cast<const char*>(sV[j & 1]);
+    const float ref = m == -INFINITY ? 0.0f : m * p.c;
+    const int thr = k1 - (j0 + BK) - 8 * g;
 #pragma unroll
-  for (int y = 0; y < RT; ++y) {
-    const int at = row0 + y * 16 + r;
-    const float l = sum4(st.l[y]);
-    if (at >= rows) continue;
-    const int64_t to = (int64_t)split * p.T * p.heads + (int64_t)(at / G) * p.heads + kv * G + at % G;
-    if (grp == 0) p.ml[to] = float2{st.m[y], l};
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e) *reinterpret_cast<float4_t*>(p.part + to * D + e * 16 + grp * 4) = st.o[e][y];
+      for (int e = 0; e < 16; ++e) Sn[h][e] = 0.0f;
+    half8 w[4];
+    float sum = 0.0f, top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PD; ++i) fb[i] = operand(kbase, vbase, i);
+    // scores of the next tile (in the last iteration of stale keys, not used) beside this one's weights
+#pragma unroll
+    for (int i = 0; i < NS1; ++i) {
+      Sn[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[i % PD], qf[i >> 1], Sn[i & 1], 0, 0, 0);
+      fb[i % PD] = operand(kbase, vbase, i + PD);
+#pragma unroll
+      for (int u = 0; u < EPS1; ++u) {
+        const int x = i * EPS1 + u;
+        const float y = __builtin_amdgcn_exp2f(fmaf(Sc[x >> 4][x & 15], p.c, -ref));
+        sum += y;
+        w[x >> 3][x & 7] = static_cast<half_t>(y);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    auto mask_max = [&](int x) {
+      const float y = key_in_tile(x) >= thr ? -INFINITY : Sn[x >> 4][x & 15];
+      Sc[x >> 4][x & 15] = y;
+      top = fmaxf(top, y);
+    };
+#pragma unroll
+    for (int i = 0; i < NS2; ++i) {
+      O[i % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[(NS1 + i) % PD], w[i / NDT], O[i % NDT], 0, 0, 0);
+      if (i + PD < NS2) fb[(NS1 + i) % PD] = operand(kbase, vbase, NS1 + i + PD);
+      if (i >= 2) {
+#pragma unroll
+        for (int u = 0; u < EPS2; ++u) mask_max((i - 2) * EPS2 + u);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int x = 32 - 2 * EPS2; x < 32; ++x) mask_max(x);
+    l += sum;
+    if (j + 1 < ntiles) {
+      const float to = fmaxf(m, halves_max(top));
+      if (__any((to - m) * p.c > 8.0f)) {
+        const float f = m == to ? 1.0f : __builtin_amdgcn_exp2f((m - to) * p.c);
+#pragma unroll
+        for (int t = 0; t < NDT; ++t) O[t] *= f;
+        l *= f;
+        m = to;
+      }
+    }
+    vm_wait_all();
+    lds_barrier();
   }
+  l += __shfl_xor(l, 32, 64);
+  if (at >= rows) return;
+  const int64_t to = (int64_t)split * p.T * p.heads + (int64_t)(at / G) * p.heads + kv * G + at % G;
+  if (g == 0) p.ml[to] = float2{m * p.c, l};
+#pragma unroll
+  for (int t = 0; t < NDT; ++t)
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      *reinterpret_cast<float4_t*>(p.part + to * D + 32 * t + 8 * x + 4 * g) =
+          float4_t{O[t][4 * x], O[t][4 * x + 1], O[t][4 * x + 2], O[t][4 * x + 3]};
 }
 
 // Own keys of one token's rows of one key head (16 of them at a time), the
@@ -408,13 +525,14 @@ __global__ __launch_bounds__(256) void shared_own(SharedParams p) {
   __shared__ __attribute__((aligned(16))) float sum[16 * P];
   __shared__ float2 stat[16];
   __shared__ float tops[4][16];
+  __shared__ float2 pml[JOIN ? kMaxParts : 1][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.heads / p.kvh, tiles = (G + 15) / 16;
   int at = blockIdx.x;
   const int split = JOIN ? 0 : at % p.osplits;
   if (!JOIN) at /= p.osplits;
   const int g0 = at % tiles * 16, kv = at / tiles % p.kvh, t = at / tiles / p.kvh;
-  const int s = seq_of(p, t);
+  const int s = __builtin_amdgcn_readfirstlane(seq_of(p, t, lane));
   if (s < 0) return;
   int first, count;
   own_span(p, s, t, first, count);
@@ -426,6 +544,12 @@ __global__ __launch_bounds__(256) void shared_own(SharedParams p) {
     count = 0;  // they are among the parts
   }
   const int rows = min(16, G - g0);
+  const int parts = p.psplits + p.osplits;
+  const int64_t step = (int64_t)p.T * p.heads, row = (int64_t)t * p.heads + kv * G + g0;
+  if constexpr (JOIN) {
+    for (int i = tid; i < parts * 16; i += 256)
+      pml[i / 16][i % 16] = i % 16 < rows ? p.ml[i / 16 * step + row + i % 16] : float2{-INFINITY, 0.0f};
+  }
   typename Ops<T>::frag fq[D / KB][1];
   load_queries<T, D, 1>(p, fq, kv, t * G + g0, t * G + g0 + rows, lane);
   Soft<T, D, 1> st;
@@ -435,38 +559,50 @@ __global__ __launch_bounds__(256) void shared_own(SharedParams p) {
   for (int j = k0 + wave * KB; j < count; j += 4 * KB)
     take_block<T, D, 1, true>(st, fq, k, vt, p.ldv, first + j, count - j, p.d, p.c, lane);
   join_waves<T, D, 1>(st, sum, stat, tops, wave, lane);
-  const int64_t row = (int64_t)t * p.heads + kv * G + g0;
   if constexpr (!JOIN) {
-    const int64_t to = (int64_t)(p.psplits + split) * p.T * p.heads + row;
+    const int64_t to = (p.psplits + split) * step + row;
     for (int i = tid; i < rows * (D / 4); i += 256) {
       const int x = i / (D / 4), e = i % (D / 4) * 4;
       *reinterpret_cast<float4_t*>(p.part + (to + x) * D + e) = *reinterpret_cast<const float4_t*>(sum + x * P + e);
       if (e == 0) p.ml[to + x] = stat[x];
     }
   } else {
-    const int parts = p.psplits + p.osplits;
-    const int64_t step = (int64_t)p.T * p.heads;
-    for (int i = tid; i < rows * (D / 4); i += 256) {
-      const int x = i / (D / 4), e = i % (D / 4) * 4;
+    // the parts' weights, a row to 16 lanes
+    {
+      const int x = tid / 16, n0 = tid % 16;
       float m = stat[x].x;
-      for (int n = 0; n < parts; ++n) m = fmaxf(m, p.ml[n * step + row + x].x);
+      for (int n = n0; n < parts; n += 16) m = fmaxf(m, pml[n][x].x);
+      m = lane_max<16>(m);
       const float ref = m == -INFINITY ? 0.0f : m;
-      float f = __builtin_amdgcn_exp2f(stat[x].x - ref);
-      float l = stat[x].y * f;
-      float4_t o = *reinterpret_cast<const float4_t*>(sum + x * P + e) * f;
-      for (int n = 0; n < parts; ++n) {
-        const float2 a = p.ml[n * step + row + x];
-        f = __builtin_amdgcn_exp2f(a.x - ref);
-        l = fmaf(a.y, f, l);
-        o += *reinterpret_cast<const float4_t*>(p.part + (n * step + row + x) * D + e) * f;
+      float l = 0.0f;
+      for (int n = n0; n < parts; n += 16) {
+        const float f = __builtin_amdgcn_exp2f(pml[n][x].x - ref);
+        l = fmaf(pml[n][x].y, f, l);
+        pml[n][x].x = f;
       }
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
-      const int h = kv * G + g0 + x;
-      for (int j = 0; j < 4; ++j) {
-        if (e + j >= p.d) break;
-        const float gate = to_f32(static_cast<const T*>(p.gate)[t * p.ldg + h * p.hsg + e + j]);
-        static_cast<T*>(p.y)[t * p.ldy + (int64_t)h * p.d + e + j] = cvt_out<T>(o[j] * inv * sigmoid(gate));
+      l = sum16(l);
+      if (n0 == 0) {
+        const float f = __builtin_amdgcn_exp2f(stat[x].x - ref);
+        l = fmaf(stat[x].y, f, l);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+        stat[x] = float2{f, inv};
       }
+    }
+    lds_barrier();
+    for (int i = tid; i < rows * (D / 4); i += 256) {
+      const int x = i / (D / 4), e = i % (D / 4) * 4, h = kv * G + g0 + x;
+      if (e >= p.d) continue;
+      const T* gp = static_cast<const T*>(p.gate) + t * p.ldg + h * p.hsg + e;
+      T gate[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) gate[j] = gp[j];
+      float4_t o = *reinterpret_cast<const float4_t*>(sum + x * P + e) * stat[x].x;
+      const float* src = p.part + (row + x) * D + e;
+#pragma unroll 8
+      for (int n = 0; n < parts; ++n) o += *reinterpret_cast<const float4_t*>(src + n * step * D) * pml[n][x].x;
+      T* y = static_cast<T*>(p.y) + t * p.ldy + (int64_t)h * p.d + e;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = cvt_out<T>(o[j] * stat[x].y * sigmoid(to_f32(gate[j])));
     }
   }
 }
@@ -475,42 +611,46 @@ int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 // How the work is split, from the shapes alone (the workspace follows from it).
 struct Plan {
-  bool many;            // 128 rows to a work-group
-  int tile, row_tiles;  // rows of a work-group; their count over T * G rows
+  bool many;  // 128 rows to a work-group
+  int tile;   // rows of a work-group otherwise
   int psplits, pkeys, osplits, okeys;
 };
-Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh) {
+Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) {
   Plan x{};
   const int64_t rows = (int64_t)T * (heads / kvh);
   const int cus = device_cus();
-  x.many = dtype == CLEF_F16 && rows > 32;
-  x.tile = x.many ? 128 : rows > 16 ? 32 : 16;
-  x.row_tiles = static_cast<int>((rows + x.tile - 1) / x.tile);
-  if (np) {
-    const int64_t groups = (int64_t)x.row_tiles * kvh;
-    const int64_t want = std::max<int64_t>(1, (x.many ? cus : 2 * cus) / groups);
-    x.pkeys = static_cast<int>(((np + want - 1) / want + 127) / 128 * 128);
-    x.psplits = (np + x.pkeys - 1) / x.pkeys;
-  }
-  if (max_keys > 1024) {
-    const int64_t groups = (int64_t)T * kvh;
-    const int64_t want = std::max<int64_t>(1, 2 * cus / groups);
-    x.okeys = static_cast<int>(((max_keys + want - 1) / want + 511) / 512 * 512);
-    x.osplits = (max_keys + x.okeys - 1) / x.okeys;
-  }
+  x.many = dtype == CLEF_F16 && rows > 32 && d == padded(d);
+  x.tile = rows > 16 ? 32 : 16;
+  // splits until the chip is full (many rows: one work-group to a CU), but no
+  // shorter than two tiles of keys
+  auto split = [&](int keys, int64_t groups, int fill, int least, int most, int& parts, int& each) {
+    const int64_t want = std::min<int64_t>(std::max<int64_t>(1, fill / groups), most);
+    each = static_cast<int>(((keys + want - 1) / want + least - 1) / least * least);
+    parts = (keys + each - 1) / each;
+  };
+  const int tile = x.many ? 128 : x.tile;
+  if (np) split(np, (rows + tile - 1) / tile * kvh, x.many ? cus : 2 * cus, 128, kMaxParts / 2, x.psplits, x.pkeys);
+  if (max_keys > 1024) split(max_keys, (int64_t)T * kvh, 2 * cus, 512, kMaxParts / 2, x.osplits, x.okeys);
   return x;
 }
 
 template <class T, int D>
 int launch(const SharedParams& p, const Plan& x, hipStream_t st) {
-  const int G = p.heads / p.kvh, tiles = (G + 15) / 16;
+  const int G = p.heads / p.kvh, tiles = (G + 15) / 16, rows = p.T * G;
   if (x.psplits) {
-    const dim3 grid((unsigned)x.row_tiles * p.kvh * x.psplits);
+    const unsigned each = (unsigned)p.kvh * x.psplits;
+    bool done = false;
     if constexpr (sizeof(T) == 2) {
-      if (x.many) hipLaunchKernelGGL((shared_many_rows<D>), grid, dim3(256), 0, st, p);
+      // its loads address a key head's values with 32 bits
+      if (x.many && p.ldpv * D * 2 < (int64_t(1) << 32)) {
+        hipLaunchKernelGGL((shared_many_rows<D>), dim3((rows + 127) / 128 * each), dim3(256), 0, st, p);
+        done = true;
+      }
     }
-    if (x.tile == 32) hipLaunchKernelGGL((shared_few_rows<T, D, 2>), grid, dim3(256), 0, st, p);
-    if (x.tile == 16) hipLaunchKernelGGL((shared_few_rows<T, D, 1>), grid, dim3(256), 0, st, p);
+    if (!done && x.tile == 32)
+      hipLaunchKernelGGL((shared_few_rows<T, D, 2>), dim3((rows + 31) / 32 * each), dim3(256), 0, st, p);
+    if (!done && x.tile == 16)
+      hipLaunchKernelGGL((shared_few_rows<T, D, 1>), dim3((rows + 15) / 16 * each), dim3(256), 0, st, p);
   }
   const unsigned own = (unsigned)p.T * p.kvh * tiles;
   if (x.osplits) hipLaunchKernelGGL((shared_own<T, D, false>), dim3(own * x.osplits), dim3(256), 0, st, p);
@@ -539,7 +679,7 @@ int shared_dims(int T, int nseq, int np, int max_keys, int dtype, int heads, int
 }
 
 size_t workspace_bytes(int T, int nseq, int np, int max_keys, int dtype, int heads, int kv_heads, int d) {
-  const Plan x = plan_of(T, np, max_keys, dtype, heads, kv_heads);
+  const Plan x = plan_of(T, np, max_keys, dtype, heads, kv_heads, d);
   const size_t rows = (size_t)(x.psplits + x.osplits) * T * heads;
   return rows * padded(d) * 4 + rows * sizeof(float2) + 256;
 }
@@ -588,7 +728,7 @@ extern "C" int clef_attention_gated_shared(
   p.nkeys = static_cast<int>(ldk_tok < ldv_tok ? ldk_tok : ldv_tok);
   p.heads = heads; p.kvh = kv_heads; p.d = d;
   p.c = static_cast<float>(1.44269504088896340736 / std::sqrt(static_cast<double>(d)));
-  const clef::Plan x = clef::plan_of(T, np, max_keys, dtype, heads, kv_heads);
+  const clef::Plan x = clef::plan_of(T, np, max_keys, dtype, heads, kv_heads, d);
   p.psplits = x.psplits; p.pkeys = x.pkeys; p.osplits = x.osplits; p.okeys = x.okeys;
   p.part = static_cast<float*>(workspace);
   p.ml = reinterpret_cast<float2*>(p.part + (size_t)(x.psplits + x.osplits) * T * heads * clef::padded(d));
