@@ -163,23 +163,11 @@ struct Soft {
 // straight into operands.  For few rows, where no other wave would use the
 // same keys.
 
-// 8 (4) consecutive values from any address, zeros from `left` on
-template <class T, bool ANY>
-__device__ __forceinline__ typename Ops<T>::frag run_at(const T* p, int left) {
-  typename Ops<T>::frag x = {};
-  if (left >= Ops<T>::EL) {
-    if (ANY) __builtin_memcpy(&x, p, 16);
-    else x = frag_at(p);
-  } else {
-#pragma unroll
-    for (int e = 0; e < Ops<T>::EL; ++e)
-      if (e < left) x[e] = p[e];
-  }
-  return x;
-}
-
 // One block: keys row0 .. + KB - 1 of k [.][d] and vt [d][ldv], those from
-// `left` on masked (left >= 1).  ANY: value rows at any alignment.
+// `left` on masked (left >= 1): their scores are -inf and their values 0, whatever
+// the buffers hold there.  A lane's 16 bytes of a value row that would end behind
+// the row are taken from its end, and shifted where they reach keys (ANY: row0 at
+// any alignment; otherwise they hold masked keys alone).
 template <class T, int D, int RT, bool ANY>
 __device__ __forceinline__ void take_block(Soft<T, D, RT>& st, const typename Ops<T>::frag (&fq)[D / Ops<T>::KB][RT],
                                            const T* k, const T* vt, int64_t ldv, int64_t row0, int left, int d, float c,
@@ -188,9 +176,16 @@ __device__ __forceinline__ void take_block(Soft<T, D, RT>& st, const typename Op
   typedef typename Ops<T>::frag frag;
   const int r = lane & 15, grp = lane >> 4;
   frag fv[D / 16];
+  const int64_t col = row0 + grp * EL, col_in = min(col, ldv - EL);
+  const T* vr = vt + r * ldv + col_in;
 #pragma unroll
-  for (int e = 0; e < D / 16; ++e)
-    fv[e] = e * 16 + r < d ? run_at<T, ANY>(vt + (e * 16 + r) * ldv + row0 + grp * EL, left - grp * EL) : frag{};
+  for (int e = 0; e < D / 16; ++e) {
+    fv[e] = frag{};
+    if (e * 16 + r < d) {
+      if (ANY) __builtin_memcpy(&fv[e], vr + e * 16 * ldv, 16);
+      else fv[e] = frag_at(vr + e * 16 * ldv);
+    }
+  }
   float4_t S[TPB][RT] = {};
 #pragma unroll
   for (int x = 0; x < TPB; ++x) {
@@ -211,6 +206,16 @@ __device__ __forceinline__ void take_block(Soft<T, D, RT>& st, const typename Op
 #pragma unroll
           for (int y = 0; y < RT; ++y) S[x][y][i] = -INFINITY;
         }
+    typedef unsigned __int128 bits;
+    constexpr int W = 8 * sizeof(T);
+    const int keep = min(max(left - grp * EL, 0), EL), off = (int)min(col - col_in, (int64_t)EL);
+    const bits mask = keep == 0 ? 0 : ~bits(0) >> (EL - keep) * W;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) {
+      bits x = __builtin_bit_cast(bits, fv[e]);
+      if (ANY && off) x = off < EL ? x >> off * W : 0;
+      fv[e] = __builtin_bit_cast(frag, x & mask);
+    }
   }
   frag w[1][RT];
   st.template weights<1>(S, w, c);
