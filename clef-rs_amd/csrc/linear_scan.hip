@@ -17,11 +17,11 @@
 //
 // A work-group owns one unit of one k-head for NH of its v-heads (the scores
 // q.k serve them all) and holds their states in the f32 accumulators of its
-// waves, 32 value columns to a wave.  Products are laid out so that every
+// waves, 16 value columns to a wave.  Products are laid out so that every
 // accumulator is the next product's operand as it stands: the scores are
 // formed transposed (K Q^T: a lane has one query and 4 keys of a tile), the
 // state as S[dk][dv] and the output transposed (o^T = S^T q^T + V^T P^T: a
-// lane has one query and 8 value columns, one 16-byte store).  For f16,
+// lane has one query and 4 value columns).  For f16,
 // whose operands hold 8 consecutive k-indices a lane, the tiles' rows are
 // taken in the order 8 (r / 4) + 4 t + r % 4 (two tiles t to a block of 32), and
 // then a lane's accumulators of both tiles are exactly its operand.  V^T and
@@ -80,23 +80,46 @@ template <> struct Ops<float> {
   static __device__ __forceinline__ int row(int, int r) { return r; }
 };
 
-// Fragment of the transpose of a [token][pitch] LDS tile: operand row (or
-// column) r = lane % 16 is tile column c0 + row(t, r), its k-indices are
-// tokens t0 + EL (lane / 16) + 0 .. EL - 1.
-__device__ __forceinline__ half8 load_t(const half_t* tile, int pitch, int t0, int c0, int t, int lane) {
-  // within 16 lanes, lane 4 a + b names 4 columns of token a, and lane r gets
-  // column r of the 16 named ones for 4 tokens
-  const half_t* p = tile + (t0 + 8 * (lane >> 4) + (lane >> 2 & 3)) * pitch + c0 + 8 * (lane & 3) + 4 * t;
+// Fragments of a transposed LDS tile: operand row (or column) r = lane % 16 is
+// one tile column, its k-indices are EL tokens.  f16: within 16 lanes, lane 4 a
+// + b names 4 columns of token a, and lane r receives column r of the 16 named
+// ones for 4 tokens (p: what the lane names; p + step: 4 tokens on).
+__device__ __forceinline__ half8 transposed(const half_t* p, int step) {
   typedef __attribute__((address_space(3))) short4_t lds4;
   union { short4_t s[2]; half8 h; } x;
   x.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p));
-  x.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * pitch));
+  x.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + step));
   return x.h;
 }
-__device__ __forceinline__ float4_t load_t(const float* tile, int pitch, int t0, int c0, int, int lane) {
-  const float* p = tile + (t0 + 4 * (lane >> 4)) * pitch + c0 + (lane & 15);
+__device__ __forceinline__ float4_t transposed(const float* p, int pitch) {
   return float4_t{p[0], p[pitch], p[2 * pitch], p[3 * pitch]};
 }
+
+// The LDS tiles.  Keys are read along their rows (scores) and transposed (state),
+// values transposed only, queries along their rows.  f16, 128-wide keys: 16-byte
+// columns exchanged by a function of the row (XOR) that spreads both the 16 rows
+// of a score operand (8 (r / 4) + 4 t + r % 4) and the 4 tokens x 4 columns of a
+// transposed read over the banks.  Elsewhere rows are padded: by 16 bytes, which
+// spreads consecutive rows, and value rows of f16 by 64, for the transposed reads.
+template <class T, int DK, int DV>
+struct Tiles {
+  static constexpr int EL = Ops<T>::EL;
+  static constexpr bool XOR = sizeof(T) == 2 && DK == 128;
+  static constexpr int PQ = DK + EL, PK = XOR ? DK : DK + EL, PV = sizeof(T) == 2 ? DV + 32 : DV + EL;
+  static __device__ __forceinline__ int key(int row, int col) {  // col a multiple of EL
+    return XOR ? row * DK + (((col >> 3) ^ ((row & 3) << 2 | (row >> 3 & 3))) << 3) : row * PK + col;
+  }
+  // what lane names for key columns c0 + row(t, .) of tokens t0 + EL (lane / 16) ..
+  static __device__ __forceinline__ int key_t(int t0, int c0, int t, int lane) {
+    if constexpr (sizeof(T) == 2) return key(t0 + 8 * (lane >> 4) + (lane >> 2 & 3), c0 + 8 * (lane & 3)) + 4 * t;
+    else return (t0 + 4 * (lane >> 4)) * PK + c0 + (lane & 15);
+  }
+  static __device__ __forceinline__ int value_t(int t0, int c0, int t, int lane) {
+    if constexpr (sizeof(T) == 2) return (t0 + 8 * (lane >> 4) + (lane >> 2 & 3)) * PV + c0 + 8 * (lane & 3) + 4 * t;
+    else return (t0 + 4 * (lane >> 4)) * PV + c0 + (lane & 15);
+  }
+  static constexpr int KSTEP = sizeof(T) == 2 ? 4 * PK : PK, VSTEP = sizeof(T) == 2 ? 4 * PV : PV;
+};
 
 // Tokens [t0, t1) of sequence s, inside [0, T] whatever the table holds.
 __device__ __forceinline__ void span_of(const LinearParams& p, int s, int& t0, int& t1) {
@@ -129,6 +152,8 @@ __device__ __forceinline__ int unit_seq(const LinearParams& p, int u, int lane) 
   return lo;
 }
 
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
 // e^g as a power of two per token: l^n = 2^{lg n}; an infinite decay stays
 // finite, so that l^0 = 1.
 __device__ __forceinline__ float log2_decay(float g) {
@@ -141,7 +166,6 @@ __device__ __forceinline__ float log2_decay(float g) {
 template <class T, int W, int THREADS>
 struct Staged {
   static constexpr int EL = 16 / sizeof(T), VPR = W / EL, N = C * VPR / THREADS;
-  static constexpr int PITCH = W + EL;  // LDS rows 16 bytes apart in their banks
   static_assert(C * VPR % THREADS == 0, "whole vectors per thread");
   typedef typename Ops<T>::frag vec;
   static_assert(sizeof(vec) == 16, "16-byte vectors");
@@ -164,11 +188,12 @@ struct Staged {
       x[i] = y;
     }
   }
-  __device__ __forceinline__ void store(T* tile, int tid) const {
+  template <class At>  // at(row, column): the vector's place in the tile
+  __device__ __forceinline__ void store(T* tile, int tid, At place) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int at = tid + i * THREADS;
-      *reinterpret_cast<vec*>(tile + at / VPR * PITCH + at % VPR * EL) = x[i];
+      *reinterpret_cast<vec*>(tile + place(at / VPR, at % VPR * EL)) = x[i];
     }
   }
 };
@@ -178,12 +203,12 @@ __device__ __forceinline__ typename Ops<T>::frag frag_at(const T* p) {
   return *reinterpret_cast<const typename Ops<T>::frag*>(p);
 }
 
-// LDS of a work-group (elements of T): q, k, NH tiles of v, NH blocks of scores.
+// LDS of a work-group (elements of T): k, NH tiles of v, q, NH blocks of scores.
 template <class T, int DK, int DV, int NH, bool OUT>
 struct Shared {
-  static constexpr int EL = 16 / sizeof(T);
-  static constexpr int K = 0, V = K + C * (DK + EL), Q = V + NH * C * (DV + EL);
-  static constexpr int P = Q + (OUT ? C * (DK + EL) : 0);
+  typedef Tiles<T, DK, DV> Tile;
+  static constexpr int K = 0, V = K + C * Tile::PK, Q = V + NH * C * Tile::PV;
+  static constexpr int P = Q + (OUT ? C * Tile::PQ : 0);
   static constexpr int ALL = P + (OUT ? NH * C * C : 0);
 };
 
@@ -191,15 +216,14 @@ struct Shared {
 // outputs (and the final state behind a sequence's last unit); else: what it
 // adds to a zero state.
 template <class T, class O, int DK, int DV, int NH, bool OUT>
-__global__ __launch_bounds__(DV * 2, 1) void linear_chunks(LinearParams p) {
-  constexpr int NW = DV / 32, THREADS = 64 * NW;  // a wave for 32 value columns
+__global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
+  constexpr int NW = DV / 16, THREADS = 64 * NW;  // a wave for 16 value columns
   constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL, TPB = Ops<T>::TPB;
   constexpr int NKB = DK / KB;   // k-blocks of a key row
   constexpr int NCB = C / KB;    // k-blocks of a chunk
   constexpr int QT = C / 16;     // query tiles of a chunk
-  constexpr int VB = 32 / KB;    // KB-blocks of a wave's value columns
-  constexpr int VT = 2;          // 16-column tiles of them
-  constexpr int PK = DK + EL, PV = DV + EL;
+  typedef Tiles<T, DK, DV> Tile;
+  constexpr int PQ = Tile::PQ, PV = Tile::PV;
   typedef typename Ops<T>::frag frag;
   typedef Shared<T, DK, DV, NH, OUT> Lds;
   __shared__ __attribute__((aligned(16))) char smem[Lds::ALL * sizeof(T)];
@@ -240,73 +264,66 @@ __global__ __launch_bounds__(DV * 2, 1) void linear_chunks(LinearParams p) {
   };
   if (begin < end) fetch(begin);
 
-  // ---- the entering state: tile (b, t, x) of S has rows KB b + row(t, .) and
-  // columns 32 wave + column(x)
-  const int c0 = wave * 32;
-  auto column = [&](int x, int i) { return c0 + (x / TPB) * KB + Ops<T>::row(x % TPB, i); };
-  float4_t S[NH][NKB * TPB][VT];
+  // ---- the entering state: tile a of S has rows KB (a / TPB) + row(a % TPB, .)
+  // and the wave's columns cb + row(ct, .)
+  const int cb = wave / TPB * KB, ct = wave % TPB;
+  float4_t S[NH][NKB * TPB];
 #pragma unroll
   for (int n = 0; n < NH; ++n) {
     const int h = h0 + n;
     if (OUT && index > 0) {
-      const float* src = p.enter + ((int64_t)u * p.Hv + h) * (DK * DV) + wave * (DK * 32);
+      const float* src = p.enter + ((int64_t)u * p.Hv + h) * (DK * DV) + wave * (DK * 16);
 #pragma unroll
-      for (int a = 0; a < NKB * TPB; ++a)
-#pragma unroll
-        for (int x = 0; x < VT; ++x) S[n][a][x] = *reinterpret_cast<const float4_t*>(src + ((a * VT + x) * 64 + lane) * 4);
+      for (int a = 0; a < NKB * TPB; ++a) S[n][a] = *reinterpret_cast<const float4_t*>(src + (a * 64 + lane) * 4);
     } else {
       const float* src = OUT && p.initial ? p.initial + s * p.init_stride + (int64_t)h * p.dk * p.dv : nullptr;
+      const int col = cb + Ops<T>::row(ct, r);
 #pragma unroll
       for (int a = 0; a < NKB * TPB; ++a)
 #pragma unroll
-        for (int x = 0; x < VT; ++x)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = a / TPB * KB + Ops<T>::row(a % TPB, 4 * grp + i), col = column(x, r);
-            S[n][a][x][i] = src && row < p.dk && col < p.dv ? src[row * p.dv + col] : 0.0f;
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int row = a / TPB * KB + Ops<T>::row(a % TPB, 4 * grp + i);
+          S[n][a][i] = src && row < p.dk && col < p.dv ? src[row * p.dv + col] : 0.0f;
+        }
     }
   }
 
   for (int t = begin; t < end; t += C) {
     const int rows = min(C, end - t);
-    if (OUT) rq.store(sQ, tid);
-    rk.store(sK, tid);
+    if (OUT) rq.store(sQ, tid, [](int row, int col) { return row * PQ + col; });
+    rk.store(sK, tid, [](int row, int col) { return Tile::key(row, col); });
 #pragma unroll
-    for (int n = 0; n < NH; ++n) rv[n].store(sV + n * C * PV, tid);
+    for (int n = 0; n < NH; ++n) rv[n].store(sV + n * C * PV, tid, [](int row, int col) { return row * PV + col; });
     lds_barrier();
     if (t + C < end) fetch(t + C);
 
     if constexpr (OUT) {
       // ---- scores, transposed: keys of block b x queries of tile qt
 #pragma unroll
-      for (int qt = wave; qt < QT; qt += NW) {
-        frag fq[NKB];
+      for (int job = wave; job < QT * NCB; job += NW) {
+        const int qt = job / NCB, b = job % NCB;
+        if (b * KB > qt * 16 + 15) continue;  // keys behind every query of the tile
+        float4_t acc[TPB] = {};
 #pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) fq[kb] = frag_at(sQ + (qt * 16 + r) * PK + kb * KB + grp * EL);
+        for (int kb = 0; kb < NKB; ++kb) {
+          const frag fq = frag_at(sQ + (qt * 16 + r) * PQ + kb * KB + grp * EL);
 #pragma unroll
-        for (int b = 0; b < NCB; ++b) {
-          if (b * KB > qt * 16 + 15) continue;  // keys behind every query of the tile
-          float4_t acc[TPB] = {};
+          for (int x = 0; x < TPB; ++x)
+            Mma<T>::mma(acc[x], frag_at(sK + Tile::key(b * KB + Ops<T>::row(x, r), kb * KB + grp * EL)), fq);
+        }
+        const int i = qt * 16 + r;  // query
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+          frag f;
 #pragma unroll
           for (int x = 0; x < TPB; ++x)
 #pragma unroll
-            for (int kb = 0; kb < NKB; ++kb)
-              Mma<T>::mma(acc[x], frag_at(sK + (b * KB + Ops<T>::row(x, r)) * PK + kb * KB + grp * EL), fq[kb]);
-          const int i = qt * 16 + r;  // query
-#pragma unroll
-          for (int n = 0; n < NH; ++n) {
-            frag f;
-#pragma unroll
-            for (int x = 0; x < TPB; ++x)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int j = b * KB + Ops<T>::row(x, 4 * grp + e);  // key
-                const float w = acc[x][e] * p.scale * __builtin_amdgcn_exp2f(lg[n] * (float)max(i - j, 0));
-                f[x * 4 + e] = static_cast<T>(j <= i ? w : 0.0f);
-              }
-            *reinterpret_cast<frag*>(sP + n * C * C + ((qt * NCB + b) * 64 + lane) * EL) = f;
-          }
+            for (int e = 0; e < 4; ++e) {
+              const int j = b * KB + Ops<T>::row(x, 4 * grp + e);  // key
+              const float w = acc[x][e] * p.scale * __builtin_amdgcn_exp2f(lg[n] * (float)max(i - j, 0));
+              f[x * 4 + e] = static_cast<T>(j <= i ? w : 0.0f);
+            }
+          *reinterpret_cast<frag*>(sP + n * C * C + (job * 64 + lane) * EL) = f;
         }
       }
       lds_barrier();
@@ -321,113 +338,90 @@ __global__ __launch_bounds__(DV * 2, 1) void linear_chunks(LinearParams p) {
 #pragma unroll
           for (int a = 0; a < NKB * TPB; ++a)
 #pragma unroll
-            for (int x = 0; x < VT; ++x)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(S[n][a][x][i]));
+            for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(S[n][a][i]));
           big = lane_max<16>(big);
           big = fmaxf(big, __shfl_xor(big, 16, 64));
           big = fmaxf(big, __shfl_xor(big, 32, 64));
           const uint32_t ex = max(__float_as_uint(big) >> 23, 14u);  // sign clear
-          up = __uint_as_float((267u - ex) << 23);    // 2^(13 - exponent)
+          up = __uint_as_float((267u - ex) << 23);                   // 2^(13 - exponent)
           down = __uint_as_float((ex - 13u) << 23);
         }
-        auto state_part = [&](float4_t (&o)[VT][QT]) {
+        // An infinite or NaN value times a masked score of 0 is NaN: such values
+        // are left out of the product, and added key by key where a query sees them.
+        frag fv[NCB];
+        float test = 0.0f;
 #pragma unroll
-          for (int x = 0; x < VT; ++x)
+        for (int b = 0; b < NCB; ++b) fv[b] = transposed(sV + n * C * PV + Tile::value_t(b * KB, cb, ct, lane), Tile::VSTEP);
+        {
+          frag zero = {};
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) o[x][qt] = float4_t{0.f, 0.f, 0.f, 0.f};
+          for (int b = 0; b < NCB; ++b) zero += fv[b] * T(0);
 #pragma unroll
-          for (int kb = 0; kb < NKB; ++kb) {
-            frag fs[VT];
+          for (int e = 0; e < EL; ++e) test += to_f32(zero[e]);
+        }
+        const bool odd = __any(test != 0.0f);
+        if (odd) {
 #pragma unroll
-            for (int x = 0; x < VT; ++x)
+          for (int b = 0; b < NCB; ++b)
 #pragma unroll
-              for (int y = 0; y < TPB; ++y)
+            for (int e = 0; e < EL; ++e)
+              if (!finite(to_f32(fv[b][e]))) fv[b][e] = T(0);
+        }
+        float4_t o[QT] = {};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) fs[x][y * 4 + e] = static_cast<T>(S[n][kb * TPB + y][x][e] * up);
+        for (int kb = 0; kb < NKB; ++kb) {
+          frag fs;
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-              const frag fq = frag_at(sQ + (qt * 16 + r) * PK + kb * KB + grp * EL);
+          for (int y = 0; y < TPB; ++y)
 #pragma unroll
-              for (int x = 0; x < VT; ++x) Mma<T>::mma(o[x][qt], fs[x], fq);
-            }
-          }
+            for (int e = 0; e < 4; ++e) fs[y * 4 + e] = static_cast<T>(S[n][kb * TPB + y][e] * up);
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt) {
-            const float w = p.scale * down * __builtin_amdgcn_exp2f(lg[n] * (float)(qt * 16 + r + 1));
+          for (int qt = 0; qt < QT; ++qt)
+            Mma<T>::mma(o[qt], fs, frag_at(sQ + (qt * 16 + r) * PQ + kb * KB + grp * EL));
+        }
 #pragma unroll
-            for (int x = 0; x < VT; ++x) o[x][qt] *= w;
-          }
-        };
-        float4_t o[VT][QT];
-        state_part(o);
+        for (int qt = 0; qt < QT; ++qt)
+          o[qt] *= p.scale * down * __builtin_amdgcn_exp2f(lg[n] * (float)(qt * 16 + r + 1));
 #pragma unroll
-        for (int b = 0; b < NCB; ++b) {
-          frag fv[VT];
-#pragma unroll
-          for (int x = 0; x < VT; ++x) fv[x] = load_t(sV + n * C * PV, PV, b * KB, c0 + x / TPB * KB, x % TPB, lane);
+        for (int b = 0; b < NCB; ++b)
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) {
             if (b * KB > qt * 16 + 15) continue;
-            const frag fp = frag_at(sP + n * C * C + ((qt * NCB + b) * 64 + lane) * EL);
+            Mma<T>::mma(o[qt], fv[b], frag_at(sP + n * C * C + ((qt * NCB + b) * 64 + lane) * EL));
+          }
+        if (odd) {
+#pragma unroll 1
+          for (int j = 0; j < rows; ++j) {
+            const T* vj = sV + n * C * PV + j * PV + cb + Ops<T>::row(ct, 4 * grp);
+            // the scores of key j lie EL apart in their fragments
+            const T* pj = sP + n * C * C + (j / KB * 64 + j % KB / EL * 16 + r) * EL + j % EL;
 #pragma unroll
-            for (int x = 0; x < VT; ++x) Mma<T>::mma(o[x][qt], fv[x], fp);
+            for (int e = 0; e < 4; ++e) {
+              const float v = to_f32(vj[e]);
+              if (finite(v)) continue;
+#pragma unroll
+              for (int qt = 0; qt < QT; ++qt)
+                if (j <= qt * 16 + r) o[qt][e] = fmaf(to_f32(pj[qt * NCB * 64 * EL]), v, o[qt][e]);
+            }
           }
         }
-        // An infinite or NaN value times a masked score of 0 is NaN: where an
-        // output is not finite, the products are formed again one by one, over
-        // the keys that its query sees.
-        float test = 0.0f;
-#pragma unroll
-        for (int x = 0; x < VT; ++x)
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) test = fmaf(o[x][qt][i], 0.0f, test);
-        if (__any(test != 0.0f)) {
-          state_part(o);
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-            for (int x = 0; x < VT; ++x)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int col = column(x, 4 * grp + e), i = qt * 16 + r;
-                float sum = o[x][qt][e];
-                for (int j = 0; j <= i; ++j) {
-                  // score (i, j) in its fragment's place
-                  const int jj = j % KB, gj = jj / EL;
-                  const float w = to_f32(sP[n * C * C + ((qt * NCB + j / KB) * 64 + gj * 16 + r) * EL + jj % EL]);
-                  sum = fmaf(w, to_f32(sV[n * C * PV + j * PV + col]), sum);
-                }
-                o[x][qt][e] = sum;
-              }
-        }
         O* out = static_cast<O*>(p.out) + t * p.so + (int64_t)(h0 + n) * p.dv;
+        const int col = cb + Ops<T>::row(ct, 4 * grp);  // 4 consecutive columns
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
           const int i = qt * 16 + r;
           if (i >= rows) continue;
+          O* dst = out + i * p.so + col;
+          typedef O vec __attribute__((ext_vector_type(4)));
+          vec w;
 #pragma unroll
-          for (int y = 0; y < VB; ++y) {  // EL consecutive columns
-            const int col = c0 + y * KB + grp * EL;
-            O* dst = out + i * p.so + col;
-            if (p.vec_out && col < p.dv) {
-              if constexpr (sizeof(O) == 2) {
-                typedef O vecn __attribute__((ext_vector_type(EL)));
-                vecn w;
+          for (int e = 0; e < 4; ++e) w[e] = cvt_out<O>(o[qt][e]);
+          if (p.vec_out) {
+            if (col < p.dv) *reinterpret_cast<vec*>(dst) = w;
+          } else {
 #pragma unroll
-                for (int e = 0; e < EL; ++e) w[e] = cvt_out<O>(o[y * TPB + e / 4][qt][e % 4]);
-                *reinterpret_cast<vecn*>(dst) = w;
-              } else {
-#pragma unroll
-                for (int x = 0; x < TPB; ++x) *reinterpret_cast<float4_t*>(dst + x * 4) = o[y * TPB + x][qt];
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < EL; ++e)
-                if (col + e < p.dv) dst[e] = cvt_out<O>(o[y * TPB + e / 4][qt][e % 4]);
-            }
+            for (int e = 0; e < 4; ++e)
+              if (col + e < p.dv) dst[e] = w[e];
           }
         }
       }
@@ -438,40 +432,30 @@ __global__ __launch_bounds__(DV * 2, 1) void linear_chunks(LinearParams p) {
     for (int n = 0; n < NH; ++n) {
       const float w = __builtin_amdgcn_exp2f(lg[n] * (float)rows);
 #pragma unroll
-      for (int a = 0; a < NKB * TPB; ++a)
-#pragma unroll
-        for (int x = 0; x < VT; ++x) S[n][a][x] *= w;
+      for (int a = 0; a < NKB * TPB; ++a) S[n][a] *= w;
     }
 #pragma unroll
     for (int b = 0; b < NCB; ++b) {
-      frag hi[NH][VT], lo[NH][VT];
+      frag hi[NH], lo[NH];
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
-        float w[EL];
+        const frag f = transposed(sV + n * C * PV + Tile::value_t(b * KB, cb, ct, lane), Tile::VSTEP);
 #pragma unroll
-        for (int e = 0; e < EL; ++e)
-          w[e] = __builtin_amdgcn_exp2f(lg[n] * (float)max(rows - 1 - (b * KB + grp * EL + e), 0));
-#pragma unroll
-        for (int x = 0; x < VT; ++x) {
-          const frag f = load_t(sV + n * C * PV, PV, b * KB, c0 + x / TPB * KB, x % TPB, lane);
-#pragma unroll
-          for (int e = 0; e < EL; ++e) {
-            const float y = to_f32(f[e]) * w[e];
-            hi[n][x][e] = cvt_out<T>(y);  // of the rounded product, as the next line takes it
-            if constexpr (sizeof(T) == 2) lo[n][x][e] = static_cast<T>(y - to_f32(hi[n][x][e]));
-          }
+        for (int e = 0; e < EL; ++e) {
+          const float w = __builtin_amdgcn_exp2f(lg[n] * (float)max(rows - 1 - (b * KB + grp * EL + e), 0));
+          const float y = to_f32(f[e]) * w;
+          hi[n][e] = cvt_out<T>(y);  // of the rounded product, as the next line takes it
+          if constexpr (sizeof(T) == 2) lo[n][e] = static_cast<T>(y - to_f32(hi[n][e]));
         }
       }
 #pragma unroll
       for (int a = 0; a < NKB * TPB; ++a) {
-        const frag fk = load_t(sK, PK, b * KB, a / TPB * KB, a % TPB, lane);
+        const frag fk = transposed(sK + Tile::key_t(b * KB, a / TPB * KB, a % TPB, lane), Tile::KSTEP);
 #pragma unroll
-        for (int n = 0; n < NH; ++n)
-#pragma unroll
-          for (int x = 0; x < VT; ++x) {
-            Mma<T>::mma(S[n][a][x], fk, hi[n][x]);
-            if constexpr (sizeof(T) == 2) Mma<T>::mma(S[n][a][x], fk, lo[n][x]);
-          }
+        for (int n = 0; n < NH; ++n) {
+          Mma<T>::mma(S[n][a], fk, hi[n]);
+          if constexpr (sizeof(T) == 2) Mma<T>::mma(S[n][a], fk, lo[n]);
+        }
       }
     }
     lds_barrier();  // everyone is done with the tiles
@@ -481,22 +465,19 @@ __global__ __launch_bounds__(DV * 2, 1) void linear_chunks(LinearParams p) {
   for (int n = 0; n < NH; ++n) {
     const int h = h0 + n;
     if constexpr (!OUT) {
-      float* dst = p.enter + ((int64_t)u * p.Hv + h) * (DK * DV) + wave * (DK * 32);
+      float* dst = p.enter + ((int64_t)u * p.Hv + h) * (DK * DV) + wave * (DK * 16);
 #pragma unroll
-      for (int a = 0; a < NKB * TPB; ++a)
-#pragma unroll
-        for (int x = 0; x < VT; ++x) *reinterpret_cast<float4_t*>(dst + ((a * VT + x) * 64 + lane) * 4) = S[n][a][x];
+      for (int a = 0; a < NKB * TPB; ++a) *reinterpret_cast<float4_t*>(dst + (a * 64 + lane) * 4) = S[n][a];
     } else if (p.final_state && last) {
       float* dst = p.final_state + ((int64_t)s * p.Hv + h) * p.dk * p.dv;
+      const int col = cb + Ops<T>::row(ct, r);
 #pragma unroll
       for (int a = 0; a < NKB * TPB; ++a)
 #pragma unroll
-        for (int x = 0; x < VT; ++x)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = a / TPB * KB + Ops<T>::row(a % TPB, 4 * grp + i), col = column(x, r);
-            if (row < p.dk && col < p.dv) dst[row * p.dv + col] = S[n][a][x][i];
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int row = a / TPB * KB + Ops<T>::row(a % TPB, 4 * grp + i);
+          if (row < p.dk && col < p.dv) dst[row * p.dv + col] = S[n][a][i];
+        }
     }
   }
 }
@@ -513,12 +494,12 @@ __global__ __launch_bounds__(256) void linear_join(LinearParams p) {
   span_of(p, s, t0, t1);
   const int n = (t1 - t0 + p.unit - 1) / p.unit;
   if (n < 2) return;
-  const int e = (part * 256 + threadIdx.x) * 4;  // wave * DK * 32 + ((a * 2 + x) * 64 + lane) * 4
+  const int e = (part * 256 + threadIdx.x) * 4;  // wave * DK * 16 + (a * 64 + lane) * 4
   float4_t run = {0.f, 0.f, 0.f, 0.f};
   if (p.initial) {
-    const int lane = e / 4 % 64, x = e / 256 % 2, a = e / 512 % (DK / 16), wave = e / (DK * 32);
+    const int lane = e / 4 % 64, a = e / 256 % (DK / 16), wave = e / (DK * 16);
     const float* src = p.initial + s * p.init_stride + (int64_t)h * p.dk * p.dv;
-    const int col = wave * 32 + x / TPB * KB + Ops<T>::row(x % TPB, lane & 15);
+    const int col = wave / TPB * KB + Ops<T>::row(wave % TPB, lane & 15);
     for (int i = 0; i < 4; ++i) {
       const int row = a / TPB * KB + Ops<T>::row(a % TPB, 4 * (lane >> 4) + i);
       if (row < p.dk && col < p.dv) run[i] = src[row * p.dv + col];
@@ -570,7 +551,7 @@ size_t workspace_bytes(int T, int nseq, int Hk, int Hv, int dk, int dv, int dtyp
 
 template <class T, class O, int DK, int DV, int NH>
 int launch(const LinearParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)p.nunits * (p.Hv / NH)), block(DV * 2);
+  const dim3 grid((unsigned)p.nunits * (p.Hv / NH)), block(DV * 4);
   if (p.unit < p.T) {
     hipLaunchKernelGGL((linear_chunks<T, T, DK, DV, NH, false>), grid, block, 0, st, p);
     hipLaunchKernelGGL((linear_join<T, DK, DV>), dim3((unsigned)p.nseq * p.Hv * (DK * DV / 1024)), dim3(256), 0, st, p);
@@ -633,7 +614,7 @@ int linear_scan(const void* q, const void* k, const void* v, int64_t sqk, int64_
   };
   p.vec_qk = wide(q, sqk, dk, dtype_qkv) && wide(k, sqk, dk, dtype_qkv);
   p.vec_v = wide(v, sv, dv, dtype_qkv);
-  p.vec_out = wide(out, so, dv, CLEF_F16) && dv % 8 == 0;
+  p.vec_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && so % 4 == 0 && dv % 4 == 0;
   if (dtype_qkv == CLEF_F16)
     return dtype_out == CLEF_F16 ? launch_widths<half_t, half_t>(p, st) : launch_widths<half_t, float>(p, st);
   return dtype_out == CLEF_F16 ? launch_widths<float, half_t>(p, st) : launch_widths<float, float>(p, st);

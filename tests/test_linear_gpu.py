@@ -173,7 +173,7 @@ def test_ragged(clef, lens, initial, dtype):
 
 @gpu
 def test_infinities_stay_with_their_sequence(clef):
-    """What one sequence holds does not reach its neighbours, nor a later token an earlier one."""
+    """What one sequence holds does not reach its neighbours."""
     lens, H, d = [70, 130, 64, 40], 2, 64
     cu = np.concatenate([[0], np.cumsum(lens)])
     q, k, v = _inputs(1, int(cu[-1]), H, H, d, d, F16)
@@ -186,6 +186,30 @@ def test_infinities_stay_with_their_sequence(clef):
         a, b = int(cu[s]), int(cu[s + 1])
         check(out[a:b], final[s], q[a:b], k[a:b], v[a:b], g, d ** -0.5)
     assert not torch.isfinite(final[1]).all() and not torch.isfinite(final[2]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_a_token_reaches_only_later_ones(clef, value, dtype):
+    """An infinite or NaN value (key, query) changes nothing before its token, and is seen from it on."""
+    T, H, d, at = 150, 2, 64, 77
+    q, k, v = _inputs(2, T, H, H, d, d, dtype)
+    g = _slopes(H)
+    scan = clef.LinearScan(d, d)
+    clean, _ = scan.prefill(*_cuda(q, k, v, g))
+    for which in range(3):
+        x = [y.clone() for y in (q, k, v)]
+        x[which][at, 1, 5] = value
+        out, _ = scan.prefill(*_cuda(*x, g))
+        assert torch.equal(out[:, 0], clean[:, 0]) and torch.equal(out[:at, 1], clean[:at, 1])
+        if which == 0:  # a query: its own row only
+            assert torch.equal(out[at + 1:, 1], clean[at + 1:, 1]) and not torch.isfinite(out[at, 1]).any()
+        elif which == 1:
+            assert not torch.isfinite(out[at:, 1]).any()
+        else:  # a value: its own column only
+            rest = torch.arange(d, device="cuda") != 5
+            assert torch.equal(out[:, 1, rest], clean[:, 1, rest]) and not torch.isfinite(out[at:, 1, 5]).any()
 
 
 @gpu
