@@ -15,9 +15,8 @@
 // from, a third walks the units side by side.  Prompts of one unit take the
 // third alone.
 //
-// A work-group owns one unit of one k-head for NH of its v-heads (the scores
-// q.k serve them all) and holds their states in the f32 accumulators of its
-// waves, 16 value columns to a wave.  Products are laid out so that every
+// A work-group owns one unit of one v-head and holds its state in the f32
+// accumulators of its waves, 16 value columns to a wave.  Products are laid out so that every
 // accumulator is the next product's operand as it stands: the scores are
 // formed transposed (K Q^T: a lane has one query and 4 keys of a tile), the
 // state as S[dk][dv] and the output transposed (o^T = S^T q^T + V^T P^T: a
@@ -203,20 +202,24 @@ __device__ __forceinline__ typename Ops<T>::frag frag_at(const T* p) {
   return *reinterpret_cast<const typename Ops<T>::frag*>(p);
 }
 
-// LDS of a work-group (elements of T): k, NH tiles of v, q, NH blocks of scores.
-template <class T, int DK, int DV, int NH, bool OUT>
+// LDS of a work-group (elements of T): k, v, q, scores.
+template <class T, int DK, int DV, bool OUT>
 struct Shared {
   typedef Tiles<T, DK, DV> Tile;
-  static constexpr int K = 0, V = K + C * Tile::PK, Q = V + NH * C * Tile::PV;
+  static constexpr int K = 0, V = K + C * Tile::PK, Q = V + C * Tile::PV;
   static constexpr int P = Q + (OUT ? C * Tile::PQ : 0);
-  static constexpr int ALL = P + (OUT ? NH * C * C : 0);
+  static constexpr int ALL = P + (OUT ? C * C : 0);
 };
 
-// One unit of NH v-heads.  OUT: walk it from its entering state and write the
+// One unit of one v-head.  OUT: walk it from its entering state and write the
 // outputs (and the final state behind a sequence's last unit); else: what it
 // adds to a zero state.
-template <class T, class O, int DK, int DV, int NH, bool OUT>
-__global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
+//
+// f16: at most 128 registers, so that two work-groups share a CU and one's
+// products cover the other's barriers and loads (8 waves with two v-heads each,
+// which share the scores, took 133 us for the walk of 16,384 tokens x 32 heads).
+template <class T, class O, int DK, int DV, bool OUT>
+__global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? 4 : 2) void linear_chunks(LinearParams p) {
   constexpr int NW = DV / 16, THREADS = 64 * NW;  // a wave for 16 value columns
   constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL, TPB = Ops<T>::TPB;
   constexpr int NKB = DK / KB;   // k-blocks of a key row
@@ -225,7 +228,7 @@ __global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
   typedef Tiles<T, DK, DV> Tile;
   constexpr int PQ = Tile::PQ, PV = Tile::PV;
   typedef typename Ops<T>::frag frag;
-  typedef Shared<T, DK, DV, NH, OUT> Lds;
+  typedef Shared<T, DK, DV, OUT> Lds;
   __shared__ __attribute__((aligned(16))) char smem[Lds::ALL * sizeof(T)];
   T* const sK = reinterpret_cast<T*>(smem) + Lds::K;
   T* const sV = reinterpret_cast<T*>(smem) + Lds::V;
@@ -233,10 +236,10 @@ __global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
   T* const sP = reinterpret_cast<T*>(smem) + Lds::P;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = lane & 15, grp = lane >> 4;
-  const int groups = p.Hv / NH;
-  const int h0 = blockIdx.x % groups * NH, u = blockIdx.x / groups;
-  const int hk = h0 / (p.Hv / p.Hk);
+  // heads of one k-head on one XCD (work-groups go round them), to share q and k in its L2
+  const int slot = blockIdx.x % p.Hv, u = blockIdx.x / p.Hv;
+  const int h = p.Hv % 8 == 0 ? slot % 8 * (p.Hv / 8) + slot / 8 : slot;
+  const int hk = h / (p.Hv / p.Hk);
   const int s = p.nseq > 1 ? __builtin_amdgcn_readfirstlane(unit_seq(p, u, lane)) : 0;
   int t0, t1;
   span_of(p, s, t0, t1);
@@ -246,35 +249,31 @@ __global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
   const bool last = end == t1;
   if (!OUT && last) return;  // what follows a sequence's last unit is the walk's to write
 
-  float lg[NH];
-#pragma unroll
-  for (int n = 0; n < NH; ++n) lg[n] = log2_decay(p.g[h0 + n]);
+  float lg = log2_decay(p.g[h]);
 
   const T* q = static_cast<const T*>(p.q) + (int64_t)hk * p.dk;
   const T* k = static_cast<const T*>(p.k) + (int64_t)hk * p.dk;
-  const T* v = static_cast<const T*>(p.v) + (int64_t)h0 * p.dv;
+  const T* v = static_cast<const T*>(p.v) + (int64_t)h * p.dv;
   Staged<T, DK, THREADS> rq, rk;
-  Staged<T, DV, THREADS> rv[NH];
+  Staged<T, DV, THREADS> rv;
   auto fetch = [&](int t) {
     const int rows = min(C, end - t);
     if (OUT) rq.load(q + t * p.sqk, p.sqk, rows, p.dk, p.vec_qk, tid);
     rk.load(k + t * p.sqk, p.sqk, rows, p.dk, p.vec_qk, tid);
-#pragma unroll
-    for (int n = 0; n < NH; ++n) rv[n].load(v + t * p.sv + n * p.dv, p.sv, rows, p.dv, p.vec_v, tid);
+    rv.load(v + t * p.sv, p.sv, rows, p.dv, p.vec_v, tid);
   };
   if (begin < end) fetch(begin);
 
   // ---- the entering state: tile a of S has rows KB (a / TPB) + row(a % TPB, .)
   // and the wave's columns cb + row(ct, .)
   const int cb = wave / TPB * KB, ct = wave % TPB;
-  float4_t S[NH][NKB * TPB];
-#pragma unroll
-  for (int n = 0; n < NH; ++n) {
-    const int h = h0 + n;
+  float4_t S[NKB * TPB];
+  {
+    const int r = lane & 15, grp = lane >> 4;
     if (OUT && index > 0) {
       const float* src = p.enter + ((int64_t)u * p.Hv + h) * (DK * DV) + wave * (DK * 16);
 #pragma unroll
-      for (int a = 0; a < NKB * TPB; ++a) S[n][a] = *reinterpret_cast<const float4_t*>(src + (a * 64 + lane) * 4);
+      for (int a = 0; a < NKB * TPB; ++a) S[a] = *reinterpret_cast<const float4_t*>(src + (a * 64 + lane) * 4);
     } else {
       const float* src = OUT && p.initial ? p.initial + s * p.init_stride + (int64_t)h * p.dk * p.dv : nullptr;
       const int col = cb + Ops<T>::row(ct, r);
@@ -283,17 +282,20 @@ __global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int row = a / TPB * KB + Ops<T>::row(a % TPB, 4 * grp + i);
-          S[n][a][i] = src && row < p.dk && col < p.dv ? src[row * p.dv + col] : 0.0f;
+          S[a][i] = src && row < p.dk && col < p.dv ? src[row * p.dv + col] : 0.0f;
         }
     }
   }
 
   for (int t = begin; t < end; t += C) {
     const int rows = min(C, end - t);
+    // formed anew for each chunk: what the compiler would derive from them once
+    // (powers of the decay, addresses) costs more registers than it saves
+    int r = lane & 15, grp = lane >> 4;
+    asm("" : "+v"(r), "+v"(grp), "+v"(lg));
     if (OUT) rq.store(sQ, tid, [](int row, int col) { return row * PQ + col; });
     rk.store(sK, tid, [](int row, int col) { return Tile::key(row, col); });
-#pragma unroll
-    for (int n = 0; n < NH; ++n) rv[n].store(sV + n * C * PV, tid, [](int row, int col) { return row * PV + col; });
+    rv.store(sV, tid, [](int row, int col) { return row * PV + col; });
     lds_barrier();
     if (t + C < end) fetch(t + C);
 
@@ -312,25 +314,23 @@ __global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
             Mma<T>::mma(acc[x], frag_at(sK + Tile::key(b * KB + Ops<T>::row(x, r), kb * KB + grp * EL)), fq);
         }
         const int i = qt * 16 + r;  // query
-#pragma unroll
-        for (int n = 0; n < NH; ++n) {
+        {
           frag f;
 #pragma unroll
           for (int x = 0; x < TPB; ++x)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int j = b * KB + Ops<T>::row(x, 4 * grp + e);  // key
-              const float w = acc[x][e] * p.scale * __builtin_amdgcn_exp2f(lg[n] * (float)max(i - j, 0));
+              const float w = acc[x][e] * p.scale * __builtin_amdgcn_exp2f(lg * (float)max(i - j, 0));
               f[x * 4 + e] = static_cast<T>(j <= i ? w : 0.0f);
             }
-          *reinterpret_cast<frag*>(sP + n * C * C + (job * 64 + lane) * EL) = f;
+          *reinterpret_cast<frag*>(sP + (job * 64 + lane) * EL) = f;
         }
       }
       lds_barrier();
 
       // ---- outputs, transposed: value columns x queries
-#pragma unroll
-      for (int n = 0; n < NH; ++n) {
+      {
         // f16: the state's copy scaled to at most 2^14 by a power of two
         float up = 1.0f, down = 1.0f;
         if constexpr (sizeof(T) == 2) {
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
 #pragma unroll
           for (int a = 0; a < NKB * TPB; ++a)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(S[n][a][i]));
+            for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(S[a][i]));
           big = lane_max<16>(big);
           big = fmaxf(big, __shfl_xor(big, 16, 64));
           big = fmaxf(big, __shfl_xor(big, 32, 64));
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
         frag fv[NCB];
         float test = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NCB; ++b) fv[b] = transposed(sV + n * C * PV + Tile::value_t(b * KB, cb, ct, lane), Tile::VSTEP);
+        for (int b = 0; b < NCB; ++b) fv[b] = transposed(sV + Tile::value_t(b * KB, cb, ct, lane), Tile::VSTEP);
         {
           frag zero = {};
 #pragma unroll
@@ -374,27 +374,27 @@ __global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
 #pragma unroll
           for (int y = 0; y < TPB; ++y)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) fs[y * 4 + e] = static_cast<T>(S[n][kb * TPB + y][e] * up);
+            for (int e = 0; e < 4; ++e) fs[y * 4 + e] = static_cast<T>(S[kb * TPB + y][e] * up);
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt)
             Mma<T>::mma(o[qt], fs, frag_at(sQ + (qt * 16 + r) * PQ + kb * KB + grp * EL));
         }
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
-          o[qt] *= p.scale * down * __builtin_amdgcn_exp2f(lg[n] * (float)(qt * 16 + r + 1));
+          o[qt] *= p.scale * down * __builtin_amdgcn_exp2f(lg * (float)(qt * 16 + r + 1));
 #pragma unroll
         for (int b = 0; b < NCB; ++b)
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) {
             if (b * KB > qt * 16 + 15) continue;
-            Mma<T>::mma(o[qt], fv[b], frag_at(sP + n * C * C + ((qt * NCB + b) * 64 + lane) * EL));
+            Mma<T>::mma(o[qt], fv[b], frag_at(sP + ((qt * NCB + b) * 64 + lane) * EL));
           }
         if (odd) {
 #pragma unroll 1
           for (int j = 0; j < rows; ++j) {
-            const T* vj = sV + n * C * PV + j * PV + cb + Ops<T>::row(ct, 4 * grp);
+            const T* vj = sV + j * PV + cb + Ops<T>::row(ct, 4 * grp);
             // the scores of key j lie EL apart in their fragments
-            const T* pj = sP + n * C * C + (j / KB * 64 + j % KB / EL * 16 + r) * EL + j % EL;
+            const T* pj = sP + (j / KB * 64 + j % KB / EL * 16 + r) * EL + j % EL;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float v = to_f32(vj[e]);
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
             }
           }
         }
-        O* out = static_cast<O*>(p.out) + t * p.so + (int64_t)(h0 + n) * p.dv;
+        O* out = static_cast<O*>(p.out) + t * p.so + (int64_t)h * p.dv;
         const int col = cb + Ops<T>::row(ct, 4 * grp);  // 4 consecutive columns
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
@@ -415,7 +415,11 @@ __global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
           typedef O vec __attribute__((ext_vector_type(4)));
           vec w;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = cvt_out<O>(o[qt][e]);
+          for (int e = 0; e < 4; ++e) {
+            float y = o[qt][e];
+            asm("" : "+v"(y));  // one value from either side of the branch above (or the stores are formed twice)
+            w[e] = cvt_out<O>(y);
+          }
           if (p.vec_out) {
             if (col < p.dv) *reinterpret_cast<vec*>(dst) = w;
           } else {
@@ -428,46 +432,40 @@ __global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
     }
 
     // ---- S <- l^rows S + K^T (l^{rows-1-j} V)
+    {
+      const float w = __builtin_amdgcn_exp2f(lg * (float)rows);
 #pragma unroll
-    for (int n = 0; n < NH; ++n) {
-      const float w = __builtin_amdgcn_exp2f(lg[n] * (float)rows);
-#pragma unroll
-      for (int a = 0; a < NKB * TPB; ++a) S[n][a] *= w;
+      for (int a = 0; a < NKB * TPB; ++a) S[a] *= w;
     }
 #pragma unroll
     for (int b = 0; b < NCB; ++b) {
-      frag hi[NH], lo[NH];
-#pragma unroll
-      for (int n = 0; n < NH; ++n) {
-        const frag f = transposed(sV + n * C * PV + Tile::value_t(b * KB, cb, ct, lane), Tile::VSTEP);
+      frag hi, lo;
+      {
+        const frag f = transposed(sV + Tile::value_t(b * KB, cb, ct, lane), Tile::VSTEP);
 #pragma unroll
         for (int e = 0; e < EL; ++e) {
-          const float w = __builtin_amdgcn_exp2f(lg[n] * (float)max(rows - 1 - (b * KB + grp * EL + e), 0));
+          const float w = __builtin_amdgcn_exp2f(lg * (float)max(rows - 1 - (b * KB + grp * EL + e), 0));
           const float y = to_f32(f[e]) * w;
-          hi[n][e] = cvt_out<T>(y);  // of the rounded product, as the next line takes it
-          if constexpr (sizeof(T) == 2) lo[n][e] = static_cast<T>(y - to_f32(hi[n][e]));
+          hi[e] = cvt_out<T>(y);  // of the rounded product, as the next line takes it
+          if constexpr (sizeof(T) == 2) lo[e] = static_cast<T>(y - to_f32(hi[e]));
         }
       }
 #pragma unroll
       for (int a = 0; a < NKB * TPB; ++a) {
         const frag fk = transposed(sK + Tile::key_t(b * KB, a / TPB * KB, a % TPB, lane), Tile::KSTEP);
-#pragma unroll
-        for (int n = 0; n < NH; ++n) {
-          Mma<T>::mma(S[n][a], fk, hi[n]);
-          if constexpr (sizeof(T) == 2) Mma<T>::mma(S[n][a], fk, lo[n]);
-        }
+        Mma<T>::mma(S[a], fk, hi);
+        if constexpr (sizeof(T) == 2) Mma<T>::mma(S[a], fk, lo);
       }
     }
     lds_barrier();  // everyone is done with the tiles
   }
 
-#pragma unroll
-  for (int n = 0; n < NH; ++n) {
-    const int h = h0 + n;
+  {
+    const int r = lane & 15, grp = lane >> 4;
     if constexpr (!OUT) {
       float* dst = p.enter + ((int64_t)u * p.Hv + h) * (DK * DV) + wave * (DK * 16);
 #pragma unroll
-      for (int a = 0; a < NKB * TPB; ++a) *reinterpret_cast<float4_t*>(dst + (a * 64 + lane) * 4) = S[n][a];
+      for (int a = 0; a < NKB * TPB; ++a) *reinterpret_cast<float4_t*>(dst + (a * 64 + lane) * 4) = S[a];
     } else if (p.final_state && last) {
       float* dst = p.final_state + ((int64_t)s * p.Hv + h) * p.dk * p.dv;
       const int col = cb + Ops<T>::row(ct, r);
@@ -476,7 +474,7 @@ __global__ __launch_bounds__(DV * 4) void linear_chunks(LinearParams p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int row = a / TPB * KB + Ops<T>::row(a % TPB, 4 * grp + i);
-          if (row < p.dk && col < p.dv) dst[row * p.dv + col] = S[n][a][i];
+          if (row < p.dk && col < p.dv) dst[row * p.dv + col] = S[a][i];
         }
     }
   }
@@ -532,46 +530,36 @@ int linear_dims(int T, int nseq, int Hk, int Hv, int dk, int dv, int dtype_qkv) 
 }
 
 // Tokens of a unit: enough units that the work-groups fill the chip once, and
-// none shorter than 4 chunks, since a cut costs two launches and two passes
-// over a state.
-int unit_tokens(int T, int groups) {
-  const int64_t want = ((int64_t)T * groups + device_cus() - 1) / device_cus();
-  return static_cast<int>((std::max<int64_t>(want, 256) + C - 1) / C * C);
+// none shorter than 2 chunks, since a cut costs two launches and passes over a
+// state.
+int unit_tokens(int T, int Hv, int dtype) {
+  const int64_t fill = (int64_t)device_cus() * (dtype == CLEF_F16 ? 2 : 1);
+  const int64_t want = ((int64_t)T * Hv + fill - 1) / fill;
+  return static_cast<int>((std::max<int64_t>(want, 2 * C) + C - 1) / C * C);
 }
 int padded(int d) { return d <= 64 ? 64 : 128; }
-// v-heads of a work-group: two of one k-head share their scores (f16; in f32
-// two would not fit the LDS)
-int paired(int Hk, int Hv, int dtype) { return dtype == CLEF_F16 && Hv / Hk % 2 == 0 ? 2 : 1; }
 
 size_t workspace_bytes(int T, int nseq, int Hk, int Hv, int dk, int dv, int dtype) {
-  const int unit = unit_tokens(T, Hv / paired(Hk, Hv, dtype));
+  const int unit = unit_tokens(T, Hv, dtype);
   if (T <= unit) return 256;  // every sequence is one unit
   return ((size_t)T / unit + nseq) * Hv * padded(dk) * padded(dv) * 4;
 }
 
-template <class T, class O, int DK, int DV, int NH>
+template <class T, class O, int DK, int DV>
 int launch(const LinearParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)p.nunits * (p.Hv / NH)), block(DV * 4);
+  const dim3 grid((unsigned)p.nunits * p.Hv), block(DV * 4);
   if (p.unit < p.T) {
-    hipLaunchKernelGGL((linear_chunks<T, T, DK, DV, NH, false>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((linear_chunks<T, T, DK, DV, false>), grid, block, 0, st, p);
     hipLaunchKernelGGL((linear_join<T, DK, DV>), dim3((unsigned)p.nseq * p.Hv * (DK * DV / 1024)), dim3(256), 0, st, p);
   }
-  hipLaunchKernelGGL((linear_chunks<T, O, DK, DV, NH, true>), grid, block, 0, st, p);
+  hipLaunchKernelGGL((linear_chunks<T, O, DK, DV, true>), grid, block, 0, st, p);
   return check_launch("linear attention scan");
-}
-
-template <class T, class O, int DK, int DV>
-int launch_heads(const LinearParams& p, hipStream_t st) {
-  if constexpr (sizeof(T) == 2) {
-    if (paired(p.Hk, p.Hv, CLEF_F16) == 2) return launch<T, O, DK, DV, 2>(p, st);
-  }
-  return launch<T, O, DK, DV, 1>(p, st);
 }
 
 template <class T, class O>
 int launch_widths(const LinearParams& p, hipStream_t st) {
-  if (padded(p.dk) == 64) return padded(p.dv) == 64 ? launch_heads<T, O, 64, 64>(p, st) : launch_heads<T, O, 64, 128>(p, st);
-  return padded(p.dv) == 64 ? launch_heads<T, O, 128, 64>(p, st) : launch_heads<T, O, 128, 128>(p, st);
+  if (padded(p.dk) == 64) return padded(p.dv) == 64 ? launch<T, O, 64, 64>(p, st) : launch<T, O, 64, 128>(p, st);
+  return padded(p.dv) == 64 ? launch<T, O, 128, 64>(p, st) : launch<T, O, 128, 128>(p, st);
 }
 
 int linear_scan(const void* q, const void* k, const void* v, int64_t sqk, int64_t sv, int dtype_qkv, const float* g,
@@ -605,7 +593,7 @@ int linear_scan(const void* q, const void* k, const void* v, int64_t sqk, int64_
   p.sqk = sqk; p.sv = sv; p.so = so; p.init_stride = initial_stride;
   p.T = T; p.nseq = nseq; p.Hk = Hk; p.Hv = Hv; p.dk = dk; p.dv = dv;
   p.scale = scale;
-  p.unit = unit_tokens(T, Hv / paired(Hk, Hv, dtype_qkv));
+  p.unit = unit_tokens(T, Hv, dtype_qkv);
   p.nunits = (cu_seqlens ? T / p.unit : (T + p.unit - 1) / p.unit - 1) + nseq;
   p.enter = static_cast<float*>(workspace);
   auto wide = [](const void* x, int64_t stride, int width, int dtype) {
