@@ -151,16 +151,28 @@ def _token_view(t, name, rows_last2):
     return t.stride(0)
 
 
-def _here(*tensors):
+if hasattr(torch._C, "_cuda_getDevice"):
+    _current_device = torch._C._cuda_getDevice
+else:
+    _current_device = torch.cuda.current_device
+
+
+def _here(first, *tensors):
     """Refuses tensors that are not on the current device (the launch goes to its stream)."""
+    dev = first.get_device()
+    if dev < 0 or dev != _current_device():
+        raise ClefError(-1, "every tensor must be on the current device")
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.get_device() != torch.cuda.current_device()):
+        if t is not None and t.get_device() != dev:
             raise ClefError(-1, "every tensor must be on the current device")
 
 
 def _token_stride(t, name):
-    """_token_view's stride as the C ABI takes it: 0 (contiguous) for a single row, whose
-    stride means nothing; rows that overlap (a broadcast token axis) are refused."""
+    """The token stride of a [T, H, d] view with contiguous (H, d), as the C ABI takes it: 0
+    for contiguous rows and for a single one; rows that overlap (a broadcast token axis)
+    are refused."""
+    if t.is_contiguous():
+        return 0
     stride = _token_view(t, name, 2)
     if t.shape[0] == 1:
         return 0
@@ -170,11 +182,9 @@ def _token_stride(t, name):
 
 
 def _scratch(n, device):
-    """A 256-byte aligned workspace of this call's own (the caching allocator's
-    order on the current stream keeps it until the launch has run)."""
-    ws = torch.empty(n + 256, dtype=torch.uint8, device=device)
-    off = (-ws.data_ptr()) % 256
-    return ws[off:off + n]
+    """A workspace of this call's own: the caching allocator's order on the current stream
+    keeps it until the launch has run, and its blocks are 512-byte aligned."""
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def _index(t, n, name):
@@ -213,7 +223,7 @@ def _step_args(q, k, v, states, slots, new_states, out_dtype, out):
         out = torch.empty((B, Hv, dv), dtype=out_dtype, device=q.device)
     if out.shape != (B, Hv, dv):
         raise ClefError(-1, "out must be [rows, Hv, dv]")
-    _here(q, k, v, states, slots, new_states, out)
+    _here(q, k, v, new_states, out, states, slots)
     return B, Hk, Hv, dk, dv, stride, new_states, nslots, out
 
 
@@ -391,7 +401,8 @@ class LinearScan:
         if initial is not None and (initial.shape != (Hv, dk, dv) or initial.dtype != torch.float32 or
                                     not initial.is_contiguous()):
             raise ClefError(-1, "initial state must be contiguous f32 [Hv, dk, dv]")
-        _here(initial)
+        if initial is not None:
+            _here(initial)
         final = torch.empty((Hv, dk, dv), dtype=torch.float32, device=q.device) if want_final else None
         ws = self._workspace(T, 1, Hk, Hv, q)
         _check(lib().clef_linear_scan(

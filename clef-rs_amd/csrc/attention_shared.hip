@@ -35,7 +35,8 @@ namespace {
 
 constexpr int kMaxSeq = 4096;
 constexpr int kMaxKeys = 1 << 24;
-constexpr int kMaxParts = 128;  // of a row, prefix and own
+constexpr int kMaxParts = 64;  // of a row over the prefix, and over its own keys
+constexpr int kJoinRows = 8;     // rows of a joining work-group
 
 struct SharedParams {
   const void* q;           // [heads][ldq][d]
@@ -98,6 +99,8 @@ __device__ __forceinline__ void own_span(const SharedParams& p, int s, int t, in
   const int left = max(min(p.cu[s + 1], p.T) - 1 - t, 0);  // queries of s behind t
   count = max(len - left, 0);
 }
+
+typedef float float2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float max4(float x) {  // over the 4 lanes of a query
   x = fmaxf(x, __shfl_xor(x, 16, 64));
@@ -242,46 +245,46 @@ __device__ __forceinline__ void load_queries(const SharedParams& p, typename Ops
   }
 }
 
-// Four waves' parts of the same RT * 16 rows into one, in LDS: sum[row][D + 4]
-// and stat[row] = {m, l}; in wave order, so the result does not depend on timing.
-template <class T, int D, int RT>
-__device__ __forceinline__ void join_waves(Soft<T, D, RT>& st, float* sum, float2* stat, float (*tops)[RT * 16],
-                                           int wave, int lane) {
-  constexpr int P = D + 4;
-  const int r = lane & 15, grp = lane >> 4;
+// Parts of up to ROWS rows that a work-group's waves hold, joined in LDS: each wave
+// leaves its sums, and a reader weighs them with weight().
+template <int D, int N, int ROWS>
+struct Joined {
+  static constexpr int P = D + 4;
+  __attribute__((aligned(16))) float o[N][ROWS][P];
+  float2 ml[N][ROWS];
+
+  template <class T, int RT>
+  __device__ __forceinline__ void put(const Soft<T, D, RT>& st, int tile, int n, int lane, int rows) {
+    const int r = lane & 15, grp = lane >> 4;
+    const float l = sum4(st.l[tile]);
+    if (r >= rows) return;
+    if (grp == 0) ml[n][r] = float2{st.m[tile], l};
 #pragma unroll
-  for (int y = 0; y < RT; ++y)
-    if (grp == 0) tops[wave][y * 16 + r] = st.m[y];
-  lds_barrier();
-#pragma unroll
-  for (int y = 0; y < RT; ++y) {
-    const int row = y * 16 + r;
-    float m = tops[0][row];
-    for (int w = 1; w < 4; ++w) m = fmaxf(m, tops[w][row]);
-    const float f = st.m[y] == m ? 1.0f : __builtin_amdgcn_exp2f(st.m[y] - m);
-    const float l = sum4(st.l[y]) * f;
-    for (int w = 0; w < 4; ++w) {
-      if (w == wave) {
-        if (grp == 0) stat[row] = float2{m, w ? stat[row].y + l : l};
-#pragma unroll
-        for (int e = 0; e < D / 16; ++e) {
-          float4_t* at = reinterpret_cast<float4_t*>(sum + row * P + e * 16 + grp * 4);
-          const float4_t x = st.o[e][y] * f;
-          *at = w ? *at + x : x;
-        }
-      }
-      lds_barrier();
-    }
+    for (int e = 0; e < D / 16; ++e) *reinterpret_cast<float4_t*>(&o[n][r][e * 16 + grp * 4]) = st.o[e][tile];
   }
-}
+  // maximum, sum and (unnormalised) four features from e of row x over all parts
+  __device__ __forceinline__ float4_t take(int x, int e, float& m, float& l) const {
+    m = ml[0][x].x;
+#pragma unroll
+    for (int n = 1; n < N; ++n) m = fmaxf(m, ml[n][x].x);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    l = 0.0f;
+    float4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const float f = __builtin_amdgcn_exp2f(ml[n][x].x - ref);
+      l = fmaf(ml[n][x].y, f, l);
+      sum += *reinterpret_cast<const float4_t*>(&o[n][x][e]) * f;
+    }
+    return sum;
+  }
+};
 
 // Part of the prefix for RT * 16 stacked rows: keys split over the four waves.
 template <class T, int D, int RT>
 __global__ __launch_bounds__(256) void shared_few_rows(SharedParams p) {
-  constexpr int KB = Ops<T>::KB, P = D + 4;
-  __shared__ __attribute__((aligned(16))) float sum[RT * 16 * P];
-  __shared__ float2 stat[RT * 16];
-  __shared__ float tops[4][RT * 16];
+  constexpr int KB = Ops<T>::KB;
+  __shared__ Joined<D, 4, 16> part;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.heads / p.kvh, rows = p.T * G;
   const int split = blockIdx.x % p.psplits, kv = blockIdx.x / p.psplits % p.kvh;
@@ -295,14 +298,21 @@ __global__ __launch_bounds__(256) void shared_few_rows(SharedParams p) {
   const T* vt = static_cast<const T*>(p.pvt) + (int64_t)kv * p.d * p.ldpv;
   for (int j = k0 + wave * KB; j < k1; j += 4 * KB)
     take_block<T, D, RT, false>(st, fq, k, vt, p.ldpv, j, k1 - j, p.d, p.c, lane);
-  join_waves<T, D, RT>(st, sum, stat, tops, wave, lane);
   const int64_t base = (int64_t)split * p.T * p.heads;
-  for (int i = tid; i < RT * 16 * (D / 4); i += 256) {
-    const int row = i / (D / 4), e = i % (D / 4) * 4, at = row0 + row;
-    if (at >= rows) break;
-    const int64_t to = base + (int64_t)(at / G) * p.heads + kv * G + at % G;
-    *reinterpret_cast<float4_t*>(p.part + to * D + e) = *reinterpret_cast<const float4_t*>(sum + row * P + e);
-    if (e == 0) p.ml[to] = stat[row];
+#pragma unroll
+  for (int y = 0; y < RT; ++y) {
+    const int here = min(16, rows - row0 - 16 * y);
+    if (y) lds_barrier();
+    part.put(st, y, wave, lane, here);
+    lds_barrier();
+    for (int i = tid; i < here * (D / 4); i += 256) {
+      const int x = i / (D / 4), e = i % (D / 4) * 4, at = row0 + 16 * y + x;
+      float m, l;
+      const float4_t o = part.take(x, e, m, l);
+      const int64_t to = base + (int64_t)(at / G) * p.heads + kv * G + at % G;
+      *reinterpret_cast<float4_t*>(p.part + to * D + e) = o;
+      if (e == 0) p.ml[to] = float2{m, l};
+    }
   }
 }
 
@@ -521,94 +531,117 @@ __global__ __launch_bounds__(256, 1) void shared_many_rows(SharedParams p) {
           float4_t{O[t][4 * x], O[t][4 * x + 1], O[t][4 * x + 2], O[t][4 * x + 3]};
 }
 
-// Own keys of one token's rows of one key head (16 of them at a time), the
-// keys split over the four waves.  JOIN: all of them, joined with the prefix's
-// and the other parts into the output; else part `split` of the own keys.
-template <class T, int D, bool JOIN>
+// Part `split` of the own keys of one token's rows of one key head (16 of them
+// at a time), the keys split over the four waves.
+template <class T, int D>
 __global__ __launch_bounds__(256) void shared_own(SharedParams p) {
-  constexpr int KB = Ops<T>::KB, P = D + 4;
-  __shared__ __attribute__((aligned(16))) float sum[16 * P];
-  __shared__ float2 stat[16];
-  __shared__ float tops[4][16];
-  __shared__ float2 pml[JOIN ? kMaxParts : 1][16];
+  constexpr int KB = Ops<T>::KB;
+  __shared__ Joined<D, 4, 16> part;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.heads / p.kvh, tiles = (G + 15) / 16;
-  int at = blockIdx.x;
-  const int split = JOIN ? 0 : at % p.osplits;
-  if (!JOIN) at /= p.osplits;
+  const int split = blockIdx.x % p.osplits, at = blockIdx.x / p.osplits;
   const int g0 = at % tiles * 16, kv = at / tiles % p.kvh, t = at / tiles / p.kvh;
   const int s = __builtin_amdgcn_readfirstlane(seq_of(p, t, lane));
   if (s < 0) return;
   int first, count;
   own_span(p, s, t, first, count);
-  int k0 = 0;
-  if (!JOIN) {
-    k0 = split * p.okeys;
-    count = min(count, k0 + p.okeys);
-  } else if (p.osplits) {
-    count = 0;  // they are among the parts
-  }
-  const int rows = min(16, G - g0);
-  const int parts = p.psplits + p.osplits;
-  const int64_t step = (int64_t)p.T * p.heads, row = (int64_t)t * p.heads + kv * G + g0;
-  if constexpr (JOIN) {
-    for (int i = tid; i < parts * 16; i += 256)
-      pml[i / 16][i % 16] = i % 16 < rows ? p.ml[i / 16 * step + row + i % 16] : float2{-INFINITY, 0.0f};
-  }
+  const int k0 = split * p.okeys, k1 = min(count, k0 + p.okeys), rows = min(16, G - g0);
   typename Ops<T>::frag fq[D / KB][1];
   load_queries<T, D, 1>(p, fq, kv, t * G + g0, t * G + g0 + rows, lane);
   Soft<T, D, 1> st;
   st.clear();
   const T* k = static_cast<const T*>(p.k) + (int64_t)kv * p.ldk * p.d;
   const T* vt = static_cast<const T*>(p.vt) + (int64_t)kv * p.d * p.ldv;
-  for (int j = k0 + wave * KB; j < count; j += 4 * KB)
-    take_block<T, D, 1, true>(st, fq, k, vt, p.ldv, first + j, count - j, p.d, p.c, lane);
-  join_waves<T, D, 1>(st, sum, stat, tops, wave, lane);
-  if constexpr (!JOIN) {
-    const int64_t to = (p.psplits + split) * step + row;
-    for (int i = tid; i < rows * (D / 4); i += 256) {
-      const int x = i / (D / 4), e = i % (D / 4) * 4;
-      *reinterpret_cast<float4_t*>(p.part + (to + x) * D + e) = *reinterpret_cast<const float4_t*>(sum + x * P + e);
-      if (e == 0) p.ml[to + x] = stat[x];
-    }
+  for (int j = k0 + wave * KB; j < k1; j += 4 * KB)
+    take_block<T, D, 1, true>(st, fq, k, vt, p.ldv, first + j, k1 - j, p.d, p.c, lane);
+  part.put(st, 0, wave, lane, rows);
+  lds_barrier();
+  const int64_t to = ((int64_t)(p.psplits + split) * p.T + t) * p.heads + kv * G + g0;
+  for (int i = tid; i < rows * (D / 4); i += 256) {
+    const int x = i / (D / 4), e = i % (D / 4) * 4;
+    float m, l;
+    *reinterpret_cast<float4_t*>(p.part + (to + x) * D + e) = part.take(x, e, m, l);
+    if (e == 0) p.ml[to + x] = float2{m, l};
+  }
+}
+
+// The outputs of one token's rows of one key head (8 of them at a time): waves
+// 0 to 3 take the own keys (unless they are among the parts), waves 4 to 7 meanwhile
+// weigh and add the parts, one row to each group of 32 lanes.
+template <class T, int D>
+__global__ __launch_bounds__(512) void shared_join(SharedParams p) {
+  constexpr int KB = Ops<T>::KB, R = kJoinRows, F = D / 32;  // features of a lane
+  __shared__ Joined<D, 5, kJoinRows> part;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = p.heads / p.kvh, tiles = (G + R - 1) / R;
+  const int at = blockIdx.x;
+  const int g0 = at % tiles * R, kv = at / tiles % p.kvh, t = at / tiles / p.kvh;
+  const int s = __builtin_amdgcn_readfirstlane(seq_of(p, t, lane));
+  if (s < 0) return;
+  const int rows = min(R, G - g0), h0 = kv * G + g0;
+  const int64_t row = (int64_t)t * p.heads + h0;
+  if (wave < 4) {
+    int first = 0, count = 0;
+    if (!p.osplits) own_span(p, s, t, first, count);
+    typename Ops<T>::frag fq[D / KB][1];
+    load_queries<T, D, 1>(p, fq, kv, t * G + g0, t * G + g0 + rows, lane);
+    Soft<T, D, 1> st;
+    st.clear();
+    const T* k = static_cast<const T*>(p.k) + (int64_t)kv * p.ldk * p.d;
+    const T* vt = static_cast<const T*>(p.vt) + (int64_t)kv * p.d * p.ldv;
+    for (int j = wave * KB; j < count; j += 4 * KB)
+      take_block<T, D, 1, true>(st, fq, k, vt, p.ldv, first + j, count - j, p.d, p.c, lane);
+    part.put(st, 0, wave, lane, rows);
   } else {
-    // the parts' weights, a row to 16 lanes
-    {
-      const int x = tid / 16, n0 = tid % 16;
-      float m = stat[x].x;
-      for (int n = n0; n < parts; n += 16) m = fmaxf(m, pml[n][x].x);
+    const int x = (tid - 256) / 32, a = tid % 32;
+    const int parts = p.psplits + p.osplits;
+    const int64_t step = (int64_t)p.T * p.heads;
+    if (x < rows) {
+      const float2* ml = p.ml + row + x;
+      float m = -INFINITY;
+      for (int n = a; n < parts; n += 32) m = fmaxf(m, ml[n * step].x);
+      m = fmaxf(m, __shfl_xor(m, 16, 64));
       m = lane_max<16>(m);
       const float ref = m == -INFINITY ? 0.0f : m;
       float l = 0.0f;
-      for (int n = n0; n < parts; n += 16) {
-        const float f = __builtin_amdgcn_exp2f(pml[n][x].x - ref);
-        l = fmaf(pml[n][x].y, f, l);
-        pml[n][x].x = f;
-      }
-      l = sum16(l);
-      if (n0 == 0) {
-        const float f = __builtin_amdgcn_exp2f(stat[x].x - ref);
-        l = fmaf(stat[x].y, f, l);
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
-        stat[x] = float2{f, inv};
-      }
-    }
-    lds_barrier();
-    for (int i = tid; i < rows * (D / 4); i += 256) {
-      const int x = i / (D / 4), e = i % (D / 4) * 4, h = kv * G + g0 + x;
-      if (e >= p.d) continue;
-      const T* gp = static_cast<const T*>(p.gate) + t * p.ldg + h * p.hsg + e;
-      T gate[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) gate[j] = gp[j];
-      float4_t o = *reinterpret_cast<const float4_t*>(sum + x * P + e) * stat[x].x;
-      const float* src = p.part + (row + x) * D + e;
+      float4_t o[F / 4 ? F / 4 : 1] = {};
+      float2_t o2 = {0.f, 0.f};
+      const float* src = p.part + (row + x) * D + a * F;
 #pragma unroll 8
-      for (int n = 0; n < parts; ++n) o += *reinterpret_cast<const float4_t*>(src + n * step * D) * pml[n][x].x;
-      T* y = static_cast<T*>(p.y) + t * p.ldy + (int64_t)h * p.d + e;
+      for (int n = 0; n < parts; ++n) {
+        const float2 w = ml[n * step];
+        const float f = __builtin_amdgcn_exp2f(w.x - ref);
+        l = fmaf(w.y, f, l);
+        if constexpr (F == 2) {
+          o2 += *reinterpret_cast<const float2_t*>(src + n * step * D) * f;
+        } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = cvt_out<T>(o[j] * stat[x].y * sigmoid(to_f32(gate[j])));
+          for (int i = 0; i < F / 4; ++i) o[i] += *reinterpret_cast<const float4_t*>(src + n * step * D + i * 4) * f;
+        }
+      }
+      if constexpr (F == 2) {
+        *reinterpret_cast<float2_t*>(&part.o[4][x][a * F]) = o2;
+      } else {
+#pragma unroll
+        for (int i = 0; i < F / 4; ++i) *reinterpret_cast<float4_t*>(&part.o[4][x][a * F + i * 4]) = o[i];
+      }
+      if (a == 0) part.ml[4][x] = float2{m, l};
     }
+  }
+  lds_barrier();
+  for (int i = tid; i < rows * (D / 4); i += 512) {
+    const int x = i / (D / 4), e = i % (D / 4) * 4;
+    if (e >= p.d) continue;
+    const T* gp = static_cast<const T*>(p.gate) + t * p.ldg + (h0 + x) * p.hsg + e;
+    T gate[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) gate[j] = gp[j];
+    float m, l;
+    const float4_t o = part.take(x, e, m, l);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+    T* y = static_cast<T*>(p.y) + t * p.ldy + (int64_t)(h0 + x) * p.d + e;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = cvt_out<T>(o[j] * inv * sigmoid(to_f32(gate[j])));
   }
 }
 
@@ -634,8 +667,8 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
     parts = (keys + each - 1) / each;
   };
   const int tile = x.many ? 128 : x.tile;
-  if (np) split(np, (rows + tile - 1) / tile * kvh, x.many ? cus : 2 * cus, 128, kMaxParts / 2, x.psplits, x.pkeys);
-  if (max_keys > 1024) split(max_keys, (int64_t)T * kvh, 2 * cus, 512, kMaxParts / 2, x.osplits, x.okeys);
+  if (np) split(np, (rows + tile - 1) / tile * kvh, x.many ? cus : 2 * cus, 128, kMaxParts, x.psplits, x.pkeys);
+  if (max_keys > 1024) split(max_keys, (int64_t)T * kvh, 2 * cus, 512, kMaxParts, x.osplits, x.okeys);
   return x;
 }
 
@@ -658,8 +691,9 @@ int launch(const SharedParams& p, const Plan& x, hipStream_t st) {
       hipLaunchKernelGGL((shared_few_rows<T, D, 1>), dim3((rows + 15) / 16 * each), dim3(256), 0, st, p);
   }
   const unsigned own = (unsigned)p.T * p.kvh * tiles;
-  if (x.osplits) hipLaunchKernelGGL((shared_own<T, D, false>), dim3(own * x.osplits), dim3(256), 0, st, p);
-  hipLaunchKernelGGL((shared_own<T, D, true>), dim3(own), dim3(256), 0, st, p);
+  if (x.osplits) hipLaunchKernelGGL((shared_own<T, D>), dim3(own * x.osplits), dim3(256), 0, st, p);
+  const unsigned join = (unsigned)p.T * p.kvh * ((G + kJoinRows - 1) / kJoinRows);
+  hipLaunchKernelGGL((shared_join<T, D>), dim3(join), dim3(512), 0, st, p);
   return check_launch("shared-prefix attention");
 }
 

@@ -165,12 +165,21 @@ __device__ __forceinline__ float log2_decay(float g) {
 template <class T, int W, int THREADS>
 struct Staged {
   static constexpr int EL = 16 / sizeof(T), VPR = W / EL, N = C * VPR / THREADS;
-  static_assert(C * VPR % THREADS == 0, "whole vectors per thread");
+  static_assert(C * VPR % THREADS == 0 && THREADS % VPR == 0, "whole vectors and rows per thread");
   typedef typename Ops<T>::frag vec;
   static_assert(sizeof(vec) == 16, "16-byte vectors");
   vec x[N];
 
+  // src, stride, rows and width are the wave's
   __device__ __forceinline__ void load(const T* src, int64_t stride, int rows, int width, bool wide, int tid) {
+    constexpr int STEP = THREADS / VPR;  // rows between a thread's vectors
+    if (wide && rows == C && width == W && stride < (int64_t(1) << 22)) {
+      // a whole tile: one 32-bit offset from addresses that the wave shares
+      const uint32_t off = (uint32_t)(tid / VPR) * (uint32_t)stride + tid % VPR * EL;
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const vec*>(src + i * STEP * stride + off);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int at = tid + i * THREADS, r = at / VPR, c = at % VPR * EL;
@@ -209,17 +218,21 @@ struct Shared {
   static constexpr int K = 0, V = K + C * Tile::PK, Q = V + C * Tile::PV;
   static constexpr int P = Q + (OUT ? C * Tile::PQ : 0);
   static constexpr int ALL = P + (OUT ? C * C : 0);
+  // powers of the decay: f32 words behind the tiles.  W[i] = l^{C-1-i}, S[i] =
+  // scale l^{C-1-i}, both 0 from i = C on (tokens behind the query or the chunk)
+  static constexpr int POW = (ALL * (int)sizeof(T) + 15) / 16 * 16;
+  static constexpr int BYTES = POW + 4 * 2 * C * (OUT ? 2 : 1);
 };
 
 // One unit of one v-head.  OUT: walk it from its entering state and write the
 // outputs (and the final state behind a sequence's last unit); else: what it
 // adds to a zero state.
 //
-// f16: at most 128 registers, so that two work-groups share a CU and one's
-// products cover the other's barriers and loads (8 waves with two v-heads each,
+// f16: at most 128 registers a lane, so that two work-groups of 8 waves share a CU
+// and one's products cover the other's barriers and loads (8 waves with two v-heads each,
 // which share the scores, took 133 us for the walk of 16,384 tokens x 32 heads).
 template <class T, class O, int DK, int DV, bool OUT>
-__global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? 4 : 2) void linear_chunks(LinearParams p) {
+__global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1)) void linear_chunks(LinearParams p) {
   constexpr int NW = DV / 16, THREADS = 64 * NW;  // a wave for 16 value columns
   constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL, TPB = Ops<T>::TPB;
   constexpr int NKB = DK / KB;   // k-blocks of a key row
@@ -229,11 +242,13 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? 4 : 2) void linear_chunks(
   constexpr int PQ = Tile::PQ, PV = Tile::PV;
   typedef typename Ops<T>::frag frag;
   typedef Shared<T, DK, DV, OUT> Lds;
-  __shared__ __attribute__((aligned(16))) char smem[Lds::ALL * sizeof(T)];
+  __shared__ __attribute__((aligned(16))) char smem[Lds::BYTES];
   T* const sK = reinterpret_cast<T*>(smem) + Lds::K;
   T* const sV = reinterpret_cast<T*>(smem) + Lds::V;
   T* const sQ = reinterpret_cast<T*>(smem) + Lds::Q;
   T* const sP = reinterpret_cast<T*>(smem) + Lds::P;
+  float* const sW = reinterpret_cast<float*>(smem + Lds::POW);
+  float* const sS = sW + 2 * C;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // heads of one k-head on one XCD (work-groups go round them), to share q and k in its L2
@@ -249,20 +264,26 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? 4 : 2) void linear_chunks(
   const bool last = end == t1;
   if (!OUT && last) return;  // what follows a sequence's last unit is the walk's to write
 
-  float lg = log2_decay(p.g[h]);
+  const float lg = log2_decay(p.g[h]);
+  if (tid < 2 * C) {
+    const float w = tid < C ? __builtin_amdgcn_exp2f(lg * (float)(C - 1 - tid)) : 0.0f;
+    sW[tid] = w;
+    if (OUT) sS[tid] = w * p.scale;
+  }
+  const float first = __builtin_amdgcn_exp2f(lg);
 
   const T* q = static_cast<const T*>(p.q) + (int64_t)hk * p.dk;
   const T* k = static_cast<const T*>(p.k) + (int64_t)hk * p.dk;
   const T* v = static_cast<const T*>(p.v) + (int64_t)h * p.dv;
   Staged<T, DK, THREADS> rq, rk;
   Staged<T, DV, THREADS> rv;
-  auto fetch = [&](int t) {
+  auto fetch = [&](int t, int tid) {
     const int rows = min(C, end - t);
     if (OUT) rq.load(q + t * p.sqk, p.sqk, rows, p.dk, p.vec_qk, tid);
     rk.load(k + t * p.sqk, p.sqk, rows, p.dk, p.vec_qk, tid);
     rv.load(v + t * p.sv, p.sv, rows, p.dv, p.vec_v, tid);
   };
-  if (begin < end) fetch(begin);
+  if (begin < end) fetch(begin, tid);
 
   // ---- the entering state: tile a of S has rows KB (a / TPB) + row(a % TPB, .)
   // and the wave's columns cb + row(ct, .)
@@ -289,15 +310,16 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? 4 : 2) void linear_chunks(
 
   for (int t = begin; t < end; t += C) {
     const int rows = min(C, end - t);
-    // formed anew for each chunk: what the compiler would derive from them once
-    // (powers of the decay, addresses) costs more registers than it saves
-    int r = lane & 15, grp = lane >> 4;
-    asm("" : "+v"(r), "+v"(grp), "+v"(lg));
-    if (OUT) rq.store(sQ, tid, [](int row, int col) { return row * PQ + col; });
-    rk.store(sK, tid, [](int row, int col) { return Tile::key(row, col); });
-    rv.store(sV, tid, [](int row, int col) { return row * PV + col; });
+    // the lane's place anew for each chunk: the addresses that the compiler would
+    // keep from chunk to chunk cost more registers than it saves
+    int ln = lane, at = tid;
+    asm("" : "+v"(ln), "+v"(at));
+    const int r = ln & 15, grp = ln >> 4;
+    if (OUT) rq.store(sQ, at, [](int row, int col) { return row * PQ + col; });
+    rk.store(sK, at, [](int row, int col) { return Tile::key(row, col); });
+    rv.store(sV, at, [](int row, int col) { return row * PV + col; });
     lds_barrier();
-    if (t + C < end) fetch(t + C);
+    if (t + C < end) fetch(t + C, at);
 
     if constexpr (OUT) {
       // ---- scores, transposed: keys of block b x queries of tile qt
@@ -314,25 +336,23 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? 4 : 2) void linear_chunks(
             Mma<T>::mma(acc[x], frag_at(sK + Tile::key(b * KB + Ops<T>::row(x, r), kb * KB + grp * EL)), fq);
         }
         const int i = qt * 16 + r;  // query
-        {
-          frag f;
+        const float* pw = sS + C - 1 - i + b * KB;
+        frag f;
 #pragma unroll
-          for (int x = 0; x < TPB; ++x)
+        for (int x = 0; x < TPB; ++x)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int j = b * KB + Ops<T>::row(x, 4 * grp + e);  // key
-              const float w = acc[x][e] * p.scale * __builtin_amdgcn_exp2f(lg * (float)max(i - j, 0));
-              f[x * 4 + e] = static_cast<T>(j <= i ? w : 0.0f);
-            }
-          *reinterpret_cast<frag*>(sP + (job * 64 + lane) * EL) = f;
-        }
+          for (int e = 0; e < 4; ++e) {
+            const int j = Ops<T>::row(x, 4 * grp + e);  // key of the block
+            f[x * 4 + e] = static_cast<T>(b * KB + j <= i ? acc[x][e] * pw[j] : 0.0f);
+          }
+        *reinterpret_cast<frag*>(sP + (job * 64 + ln) * EL) = f;
       }
       lds_barrier();
 
       // ---- outputs, transposed: value columns x queries
       {
         // f16: the state's copy scaled to at most 2^14 by a power of two
-        float up = 1.0f, down = 1.0f;
+        float up = 1.0f, down = first;
         if constexpr (sizeof(T) == 2) {
           float big = 0.0f;
 #pragma unroll
@@ -344,22 +364,23 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? 4 : 2) void linear_chunks(
           big = fmaxf(big, __shfl_xor(big, 32, 64));
           const uint32_t ex = max(__float_as_uint(big) >> 23, 14u);  // sign clear
           up = __uint_as_float((267u - ex) << 23);                   // 2^(13 - exponent)
-          down = __uint_as_float((ex - 13u) << 23);
+          down *= __uint_as_float((ex - 13u) << 23);
         }
         // An infinite or NaN value times a masked score of 0 is NaN: such values
         // are left out of the product, and added key by key where a query sees them.
         frag fv[NCB];
-        float test = 0.0f;
+        bool odd;
 #pragma unroll
-        for (int b = 0; b < NCB; ++b) fv[b] = transposed(sV + Tile::value_t(b * KB, cb, ct, lane), Tile::VSTEP);
+        for (int b = 0; b < NCB; ++b) fv[b] = transposed(sV + Tile::value_t(b * KB, cb, ct, ln), Tile::VSTEP);
         {
-          frag zero = {};
+          // 0 or -0 from finite values, NaN from others
+          frag zero = fv[0] * T(0);
 #pragma unroll
-          for (int b = 0; b < NCB; ++b) zero += fv[b] * T(0);
-#pragma unroll
-          for (int e = 0; e < EL; ++e) test += to_f32(zero[e]);
+          for (int b = 1; b < NCB; ++b) zero += fv[b] * T(0);
+          const uint4 z = __builtin_bit_cast(uint4, zero);
+          constexpr uint32_t bits = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
+          odd = __any(((z.x | z.y | z.z | z.w) & bits) != 0);
         }
-        const bool odd = __any(test != 0.0f);
         if (odd) {
 #pragma unroll
           for (int b = 0; b < NCB; ++b)
@@ -380,14 +401,13 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? 4 : 2) void linear_chunks(
             Mma<T>::mma(o[qt], fs, frag_at(sQ + (qt * 16 + r) * PQ + kb * KB + grp * EL));
         }
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-          o[qt] *= p.scale * down * __builtin_amdgcn_exp2f(lg * (float)(qt * 16 + r + 1));
+        for (int qt = 0; qt < QT; ++qt) o[qt] *= down * sS[C - 1 - (qt * 16 + r)];
 #pragma unroll
         for (int b = 0; b < NCB; ++b)
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) {
             if (b * KB > qt * 16 + 15) continue;
-            Mma<T>::mma(o[qt], fv[b], frag_at(sP + ((qt * NCB + b) * 64 + lane) * EL));
+            Mma<T>::mma(o[qt], fv[b], frag_at(sP + ((qt * NCB + b) * 64 + ln) * EL));
           }
         if (odd) {
 #pragma unroll 1
@@ -405,13 +425,13 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? 4 : 2) void linear_chunks(
             }
           }
         }
-        O* out = static_cast<O*>(p.out) + t * p.so + (int64_t)h * p.dv;
         const int col = cb + Ops<T>::row(ct, 4 * grp);  // 4 consecutive columns
+        O* out = static_cast<O*>(p.out) + t * p.so + (int64_t)h * p.dv + r * p.so + col;
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
           const int i = qt * 16 + r;
           if (i >= rows) continue;
-          O* dst = out + i * p.so + col;
+          O* dst = out + qt * 16 * p.so;
           typedef O vec __attribute__((ext_vector_type(4)));
           vec w;
 #pragma unroll
@@ -441,18 +461,18 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? 4 : 2) void linear_chunks(
     for (int b = 0; b < NCB; ++b) {
       frag hi, lo;
       {
-        const frag f = transposed(sV + Tile::value_t(b * KB, cb, ct, lane), Tile::VSTEP);
+        const frag f = transposed(sV + Tile::value_t(b * KB, cb, ct, ln), Tile::VSTEP);
+        const float* pw = sW + C - rows + b * KB + grp * EL;
 #pragma unroll
         for (int e = 0; e < EL; ++e) {
-          const float w = __builtin_amdgcn_exp2f(lg * (float)max(rows - 1 - (b * KB + grp * EL + e), 0));
-          const float y = to_f32(f[e]) * w;
+          const float y = to_f32(f[e]) * pw[e];
           hi[e] = cvt_out<T>(y);  // of the rounded product, as the next line takes it
           if constexpr (sizeof(T) == 2) lo[e] = static_cast<T>(y - to_f32(hi[e]));
         }
       }
 #pragma unroll
       for (int a = 0; a < NKB * TPB; ++a) {
-        const frag fk = transposed(sK + Tile::key_t(b * KB, a / TPB * KB, a % TPB, lane), Tile::KSTEP);
+        const frag fk = transposed(sK + Tile::key_t(b * KB, a / TPB * KB, a % TPB, ln), Tile::KSTEP);
         Mma<T>::mma(S[a], fk, hi);
         if constexpr (sizeof(T) == 2) Mma<T>::mma(S[a], fk, lo);
       }
@@ -507,7 +527,7 @@ __global__ __launch_bounds__(256) void linear_join(LinearParams p) {
   const int64_t step = (int64_t)p.Hv * (DK * DV);
   float* at = p.enter + (first_unit(p, s) * (int64_t)p.Hv + h) * (DK * DV) + e;
   float4_t next = *reinterpret_cast<const float4_t*>(at);
-  for (int u = 1; u < n; ++u) {
+  for (int u = 1; u < n; ++u) {  // what a unit adds is read before its entry is written
     const float4_t add = next;
     at += step;
     if (u + 1 < n) next = *reinterpret_cast<const float4_t*>(at);
