@@ -162,63 +162,57 @@ struct Soft {
 };
 
 // ---------------------------------------------------------------------------
-// Keys from memory: a wave takes blocks of KB keys of [first, first + count)
-// straight into operands.  For few rows, where no other wave would use the
-// same keys.
+// Keys from memory: a wave takes blocks of KB keys straight into operands.  For
+// few rows, where no other wave would use the same keys.  (These kernels run
+// for microseconds, most of a short one on instruction fetches: 11.5 us for one
+// tile of keys at d = 256 where d = 64 takes 5.6.  So their code is kept small.)
 
-// One block: keys row0 .. + KB - 1 of k [.][d] and vt [d][ldv], those from
-// `left` on masked (left >= 1): their scores are -inf and their values 0, whatever
-// the buffers hold there.  A lane's 16 bytes of a value row that would end behind
-// the row are taken from its end, and shifted where they reach keys (ANY: row0 at
-// any alignment; otherwise they hold masked keys alone).
-template <class T, int D, int RT, bool ANY>
+// One block: keys c0 .. + KB - 1 of k [.][d] and vt [d][ldv] (c0 a multiple of 8),
+// those outside [lo, hi) masked: scores of -inf and values of 0, whatever the
+// buffers hold there.  FULL: d = D.
+template <class T, int D, int RT, bool FULL>
 __device__ __forceinline__ void take_block(Soft<T, D, RT>& st, const typename Ops<T>::frag (&fq)[D / Ops<T>::KB][RT],
-                                           const T* k, const T* vt, int64_t ldv, int64_t row0, int left, int d, float c,
-                                           int lane) {
+                                           const T* k, const T* vt, int64_t ldv, int c0, int lo, int hi, int d,
+                                           float c, int lane) {
   constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL, TPB = Ops<T>::TPB;
   typedef typename Ops<T>::frag frag;
   const int r = lane & 15, grp = lane >> 4;
+  const int col = c0 + grp * EL;
+  // 16 bytes of a value row: behind the row's end lie masked keys alone
+  const T* vr = vt + r * ldv + min((int64_t)col, ldv - EL);
   frag fv[D / 16];
-  const int64_t col = row0 + grp * EL, col_in = min(col, ldv - EL);
-  const T* vr = vt + r * ldv + col_in;
 #pragma unroll
-  for (int e = 0; e < D / 16; ++e) {
-    fv[e] = frag{};
-    if (e * 16 + r < d) {
-      if (ANY) __builtin_memcpy(&fv[e], vr + e * 16 * ldv, 16);
-      else fv[e] = frag_at(vr + e * 16 * ldv);
-    }
-  }
+  for (int e = 0; e < D / 16; ++e) fv[e] = FULL || e * 16 + r < d ? frag_at(vr + e * 16 * ldv) : frag{};
   float4_t S[TPB][RT] = {};
 #pragma unroll
   for (int x = 0; x < TPB; ++x) {
-    const T* kr = k + (row0 + min(Ops<T>::row(x, r), left - 1)) * d + grp * EL;
+    const T* kr = k + (int64_t)min(max(c0 + Ops<T>::row(x, r), lo), hi - 1) * d + grp * EL;
 #pragma unroll
     for (int kb = 0; kb < D / KB; ++kb) {
-      const frag fk = kb * KB + grp * EL < d ? frag_at(kr + kb * KB) : frag{};
+      const frag fk = FULL || kb * KB + grp * EL < d ? frag_at(kr + kb * KB) : frag{};
 #pragma unroll
       for (int y = 0; y < RT; ++y) Mma<T>::mma(S[x][y], fk, fq[kb][y]);
     }
   }
-  if (left < KB) {
+  if (c0 < lo || c0 + KB > hi) {
+    auto in = [&](int key) { return key >= lo && key < hi; };
 #pragma unroll
     for (int x = 0; x < TPB; ++x)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (Ops<T>::row(x, 4 * grp + i) >= left) {
+      for (int i = 0; i < 4; ++i) {
+        const bool keep = in(c0 + Ops<T>::row(x, 4 * grp + i));
 #pragma unroll
-          for (int y = 0; y < RT; ++y) S[x][y][i] = -INFINITY;
-        }
-    typedef unsigned __int128 bits;
-    constexpr int W = 8 * sizeof(T);
-    const int keep = min(max(left - grp * EL, 0), EL), off = (int)min(col - col_in, (int64_t)EL);
-    const bits mask = keep == 0 ? 0 : ~bits(0) >> (EL - keep) * W;
+        for (int y = 0; y < RT; ++y) S[x][y][i] = keep ? S[x][y][i] : -INFINITY;
+      }
+    typedef uint32_t bits __attribute__((ext_vector_type(4)));
+    bits mask;
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e) {
-      bits x = __builtin_bit_cast(bits, fv[e]);
-      if (ANY && off) x = off < EL ? x >> off * W : 0;
-      fv[e] = __builtin_bit_cast(frag, x & mask);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) mask[i] = (in(col + 2 * i) ? 0xffffu : 0u) | (in(col + 2 * i + 1) ? ~0xffffu : 0u);
+      else mask[i] = in(col + i) ? ~0u : 0u;
     }
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) fv[e] = __builtin_bit_cast(frag, __builtin_bit_cast(bits, fv[e]) & mask);
   }
   frag w[1][RT];
   st.template weights<1>(S, w, c);
@@ -228,9 +222,21 @@ __device__ __forceinline__ void take_block(Soft<T, D, RT>& st, const typename Op
     for (int y = 0; y < RT; ++y) Mma<T>::mma(st.o[e][y], fv[e], w[0][y]);
 }
 
+// The blocks of keys [lo, hi) that are wave `wave`'s of `waves`.
+template <class T, int D, int RT, bool FULL>
+__device__ __forceinline__ void take_keys(Soft<T, D, RT>& st, const typename Ops<T>::frag (&fq)[D / Ops<T>::KB][RT],
+                                          const void* k, int64_t ldk, const void* vt, int64_t ldv, int kv, int lo,
+                                          int hi, int d, float c, int wave, int waves, int lane) {
+  const T* kh = static_cast<const T*>(k) + (int64_t)kv * ldk * d;
+  const T* vh = static_cast<const T*>(vt) + (int64_t)kv * d * ldv;
+#pragma unroll 1
+  for (int c0 = (lo & ~7) + wave * Ops<T>::KB; c0 < hi; c0 += waves * Ops<T>::KB)
+    take_block<T, D, RT, FULL>(st, fq, kh, vh, ldv, c0, lo, hi, d, c, lane);
+}
+
 // The rows of a work-group: query tile y has rows row0 + 16 y + r of the
 // stacked (token, head of the group); fewer than `rows` of them exist.
-template <class T, int D, int RT>
+template <class T, int D, int RT, bool FULL>
 __device__ __forceinline__ void load_queries(const SharedParams& p, typename Ops<T>::frag (&fq)[D / Ops<T>::KB][RT],
                                              int kv, int row0, int rows, int lane) {
   constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL;
@@ -241,7 +247,7 @@ __device__ __forceinline__ void load_queries(const SharedParams& p, typename Ops
     const int row = min(row0 + 16 * y + r, rows - 1);
     const T* src = static_cast<const T*>(p.q) + ((int64_t)(kv * G + row % G) * p.ldq + row / G) * p.d + grp * EL;
 #pragma unroll
-    for (int kb = 0; kb < D / KB; ++kb) fq[kb][y] = kb * KB + grp * EL < p.d ? frag_at(src + kb * KB) : frag{};
+    for (int kb = 0; kb < D / KB; ++kb) fq[kb][y] = FULL || kb * KB + grp * EL < p.d ? frag_at(src + kb * KB) : frag{};
   }
 }
 
@@ -281,7 +287,7 @@ struct Joined {
 };
 
 // Part of the prefix for RT * 16 stacked rows: keys split over the four waves.
-template <class T, int D, int RT>
+template <class T, int D, int RT, bool FULL>
 __global__ __launch_bounds__(256) void shared_few_rows(SharedParams p) {
   constexpr int KB = Ops<T>::KB;
   __shared__ Joined<D, 4, 16> part;
@@ -291,13 +297,10 @@ __global__ __launch_bounds__(256) void shared_few_rows(SharedParams p) {
   const int row0 = blockIdx.x / p.psplits / p.kvh * (RT * 16);
   const int k0 = split * p.pkeys, k1 = min(k0 + p.pkeys, p.np);
   typename Ops<T>::frag fq[D / KB][RT];
-  load_queries<T, D, RT>(p, fq, kv, row0, rows, lane);
+  load_queries<T, D, RT, FULL>(p, fq, kv, row0, rows, lane);
   Soft<T, D, RT> st;
   st.clear();
-  const T* k = static_cast<const T*>(p.pk) + (int64_t)kv * p.ldpk * p.d;
-  const T* vt = static_cast<const T*>(p.pvt) + (int64_t)kv * p.d * p.ldpv;
-  for (int j = k0 + wave * KB; j < k1; j += 4 * KB)
-    take_block<T, D, RT, false>(st, fq, k, vt, p.ldpv, j, k1 - j, p.d, p.c, lane);
+  take_keys<T, D, RT, FULL>(st, fq, p.pk, p.ldpk, p.pvt, p.ldpv, kv, k0, k1, p.d, p.c, wave, 4, lane);
   const int64_t base = (int64_t)split * p.T * p.heads;
 #pragma unroll
   for (int y = 0; y < RT; ++y) {
@@ -533,7 +536,7 @@ __global__ __launch_bounds__(256, 1) void shared_many_rows(SharedParams p) {
 
 // Part `split` of the own keys of one token's rows of one key head (16 of them
 // at a time), the keys split over the four waves.
-template <class T, int D>
+template <class T, int D, bool FULL>
 __global__ __launch_bounds__(256) void shared_own(SharedParams p) {
   constexpr int KB = Ops<T>::KB;
   __shared__ Joined<D, 4, 16> part;
@@ -547,13 +550,10 @@ __global__ __launch_bounds__(256) void shared_own(SharedParams p) {
   own_span(p, s, t, first, count);
   const int k0 = split * p.okeys, k1 = min(count, k0 + p.okeys), rows = min(16, G - g0);
   typename Ops<T>::frag fq[D / KB][1];
-  load_queries<T, D, 1>(p, fq, kv, t * G + g0, t * G + g0 + rows, lane);
+  load_queries<T, D, 1, FULL>(p, fq, kv, t * G + g0, t * G + g0 + rows, lane);
   Soft<T, D, 1> st;
   st.clear();
-  const T* k = static_cast<const T*>(p.k) + (int64_t)kv * p.ldk * p.d;
-  const T* vt = static_cast<const T*>(p.vt) + (int64_t)kv * p.d * p.ldv;
-  for (int j = k0 + wave * KB; j < k1; j += 4 * KB)
-    take_block<T, D, 1, true>(st, fq, k, vt, p.ldv, first + j, k1 - j, p.d, p.c, lane);
+  take_keys<T, D, 1, FULL>(st, fq, p.k, p.ldk, p.vt, p.ldv, kv, first + k0, first + k1, p.d, p.c, wave, 4, lane);
   part.put(st, 0, wave, lane, rows);
   lds_barrier();
   const int64_t to = ((int64_t)(p.psplits + split) * p.T + t) * p.heads + kv * G + g0;
@@ -568,7 +568,7 @@ __global__ __launch_bounds__(256) void shared_own(SharedParams p) {
 // The outputs of one token's rows of one key head (8 of them at a time): waves
 // 0 to 3 take the own keys (unless they are among the parts), waves 4 to 7 meanwhile
 // weigh and add the parts, one row to each group of 32 lanes.
-template <class T, int D>
+template <class T, int D, bool FULL>
 __global__ __launch_bounds__(512) void shared_join(SharedParams p) {
   constexpr int KB = Ops<T>::KB, R = kJoinRows, F = D / 32;  // features of a lane
   __shared__ Joined<D, 5, kJoinRows> part;
@@ -584,13 +584,10 @@ __global__ __launch_bounds__(512) void shared_join(SharedParams p) {
     int first = 0, count = 0;
     if (!p.osplits) own_span(p, s, t, first, count);
     typename Ops<T>::frag fq[D / KB][1];
-    load_queries<T, D, 1>(p, fq, kv, t * G + g0, t * G + g0 + rows, lane);
+    load_queries<T, D, 1, FULL>(p, fq, kv, t * G + g0, t * G + g0 + rows, lane);
     Soft<T, D, 1> st;
     st.clear();
-    const T* k = static_cast<const T*>(p.k) + (int64_t)kv * p.ldk * p.d;
-    const T* vt = static_cast<const T*>(p.vt) + (int64_t)kv * p.d * p.ldv;
-    for (int j = wave * KB; j < count; j += 4 * KB)
-      take_block<T, D, 1, true>(st, fq, k, vt, p.ldv, first + j, count - j, p.d, p.c, lane);
+    take_keys<T, D, 1, FULL>(st, fq, p.k, p.ldk, p.vt, p.ldv, kv, first, first + count, p.d, p.c, wave, 4, lane);
     part.put(st, 0, wave, lane, rows);
   } else {
     const int x = (tid - 256) / 32, a = tid % 32;
@@ -660,25 +657,25 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
   x.many = dtype == CLEF_F16 && rows > 32 && d == padded(d);
   x.tile = rows > 16 ? 32 : 16;
   // splits until the chip is full (many rows: one work-group to a CU), but no
-  // shorter than two tiles of keys
+  // shorter than two tiles of keys, or a block to a wave
   auto split = [&](int keys, int64_t groups, int fill, int least, int most, int& parts, int& each) {
     const int64_t want = std::min<int64_t>(std::max<int64_t>(1, fill / groups), most);
     each = static_cast<int>(((keys + want - 1) / want + least - 1) / least * least);
     parts = (keys + each - 1) / each;
   };
   const int tile = x.many ? 128 : x.tile;
-  if (np) split(np, (rows + tile - 1) / tile * kvh, x.many ? cus : 2 * cus, 128, kMaxParts, x.psplits, x.pkeys);
+  if (np) split(np, (rows + tile - 1) / tile * kvh, x.many ? cus : 2 * cus, dtype == CLEF_F16 ? 128 : 64, kMaxParts, x.psplits, x.pkeys);
   if (max_keys > 1024) split(max_keys, (int64_t)T * kvh, 2 * cus, 512, kMaxParts, x.osplits, x.okeys);
   return x;
 }
 
-template <class T, int D>
+template <class T, int D, bool FULL>
 int launch(const SharedParams& p, const Plan& x, hipStream_t st) {
   const int G = p.heads / p.kvh, tiles = (G + 15) / 16, rows = p.T * G;
   if (x.psplits) {
     const unsigned each = (unsigned)p.kvh * x.psplits;
     bool done = false;
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2 && FULL) {
       // its loads address a key head's values with 32 bits
       if (x.many && p.ldpv * D * 2 < (int64_t(1) << 32)) {
         hipLaunchKernelGGL((shared_many_rows<D>), dim3((rows + 127) / 128 * each), dim3(256), 0, st, p);
@@ -686,22 +683,26 @@ int launch(const SharedParams& p, const Plan& x, hipStream_t st) {
       }
     }
     if (!done && x.tile == 32)
-      hipLaunchKernelGGL((shared_few_rows<T, D, 2>), dim3((rows + 31) / 32 * each), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((shared_few_rows<T, D, 2, FULL>), dim3((rows + 31) / 32 * each), dim3(256), 0, st, p);
     if (!done && x.tile == 16)
-      hipLaunchKernelGGL((shared_few_rows<T, D, 1>), dim3((rows + 15) / 16 * each), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((shared_few_rows<T, D, 1, FULL>), dim3((rows + 15) / 16 * each), dim3(256), 0, st, p);
   }
   const unsigned own = (unsigned)p.T * p.kvh * tiles;
-  if (x.osplits) hipLaunchKernelGGL((shared_own<T, D>), dim3(own * x.osplits), dim3(256), 0, st, p);
+  if (x.osplits) hipLaunchKernelGGL((shared_own<T, D, FULL>), dim3(own * x.osplits), dim3(256), 0, st, p);
   const unsigned join = (unsigned)p.T * p.kvh * ((G + kJoinRows - 1) / kJoinRows);
-  hipLaunchKernelGGL((shared_join<T, D>), dim3(join), dim3(512), 0, st, p);
+  hipLaunchKernelGGL((shared_join<T, D, FULL>), dim3(join), dim3(512), 0, st, p);
   return check_launch("shared-prefix attention");
 }
 
 template <class T>
 int launch_width(const SharedParams& p, const Plan& x, hipStream_t st) {
-  if (padded(p.d) == 64) return launch<T, 64>(p, x, st);
-  if (padded(p.d) == 128) return launch<T, 128>(p, x, st);
-  return launch<T, 256>(p, x, st);
+  switch (p.d) {
+    case 64: return launch<T, 64, true>(p, x, st);
+    case 128: return launch<T, 128, true>(p, x, st);
+    case 256: return launch<T, 256, true>(p, x, st);
+  }
+  if (p.d < 64) return launch<T, 64, false>(p, x, st);
+  return p.d < 128 ? launch<T, 128, false>(p, x, st) : launch<T, 256, false>(p, x, st);
 }
 
 int shared_dims(int T, int nseq, int np, int max_keys, int dtype, int heads, int kv_heads, int d) {
