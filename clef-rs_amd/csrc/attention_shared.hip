@@ -319,16 +319,14 @@ __global__ __launch_bounds__(256) void shared_few_rows(SharedParams p) {
   }
 }
 
-// Part of the prefix for 128 stacked rows (f16, d = D): wave w has rows 32 w +
-// (0..31), one per lane of a half wave, on 32 x 32 x 16 products.  Tiles of 64
-// keys pass through LDS by DMA, double-buffered; the scores of tile j + 1 are
-// formed while tile j's exponentials run on the vector ALU, and the products
-// with V under the next scores' maximum.  Its LDS reads (64 KiB a wave and tile)
-// and its products take the same time at their peak rates, which bounds it.
-//
-// LDS layout: key row x of a tile holds key x with bits 2 and 3 exchanged, so that
-// the 16 weights a lane forms of a 32-key half are its operands in key order;
-// 16-byte slots are permuted by their row (XOR), against bank conflicts.
+// Part of the prefix for 128 stacked rows (f16, d = D): eight waves of 16 rows,
+// two to a SIMD, so that one's exponentials run under the other's products.
+// Tiles of 64 keys pass through LDS by DMA, double-buffered; 16-byte slots are
+// permuted by their row (XOR), so that the 16 rows of an operand, which are
+// 8 (r / 4) + 4 t + r % 4 of the keys, meet different banks.  (Four waves of 32
+// rows with the scores of a tile under the weights of the one before read half as
+// much from LDS, but leave one wave to a SIMD: 91 us for 1,024 rows a key head and
+// 32,768 keys, d = 256.)
 __device__ __forceinline__ void dma16s(const void* base, uint32_t off, void* lds_block) {
   // global_load_lds_dwordx4: lane l writes 16 bytes at M0 + 16 l, awaited by
   // vm_wait_all; the wait states cover M0 and the readfirstlane before it
@@ -340,198 +338,109 @@ __device__ __forceinline__ void dma16s(const void* base, uint32_t off, void* lds
   asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(sb), "{m0}"(m0) : "memory");
 }
 __device__ __forceinline__ void vm_wait_all() { __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8)); }
-__device__ __forceinline__ float halves_max(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
 
 template <int D>
-__global__ __launch_bounds__(256, 1) void shared_many_rows(SharedParams p) {
-  constexpr int BK = 64, NKB = D / 16, NDT = D / 32, KS = D / 8;
-  constexpr int NDMA = D / 32;     // DMA instructions per wave, operand and tile
+__global__ __launch_bounds__(512, 2) void shared_many_rows(SharedParams p) {
+  typedef half_t T;
+  constexpr int BK = 64, KB = 32, EL = 8, KS = D / 8;
+  constexpr int NDMA = D / 64;     // DMA instructions per wave, operand and tile
   constexpr int KROWS = 512 / D;   // key rows of one
-  constexpr int PD = 8;            // operand reads in flight
-  constexpr int NS1 = 2 * NKB, NS2 = 4 * NDT, EPS1 = 32 / NS1, EPS2 = 32 / NS2;
-  __shared__ __attribute__((aligned(1024))) half_t sK[2][BK * D];
-  __shared__ __attribute__((aligned(1024))) half_t sV[2][D * BK];
+  __shared__ __attribute__((aligned(1024))) T sK[2][BK * D];
+  __shared__ __attribute__((aligned(1024))) T sV[2][D * BK];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = lane & 31, g = lane >> 5;
+  const int r = lane & 15, grp = lane >> 4;
   const int G = p.heads / p.kvh, rows = p.T * G;
   const int split = blockIdx.x % p.psplits, kv = blockIdx.x / p.psplits % p.kvh;
-  const int at = blockIdx.x / p.psplits / p.kvh * 128 + 32 * wave + n;  // the lane's row
+  const int row0 = blockIdx.x / p.psplits / p.kvh * 128 + 16 * wave;
   const int k0 = split * p.pkeys, k1 = min(k0 + p.pkeys, p.np);
-  const half_t* K = static_cast<const half_t*>(p.pk) + (int64_t)kv * p.ldpk * D;
-  const half_t* V = static_cast<const half_t*>(p.pvt) + (int64_t)kv * D * p.ldpv;
+  const T* K = static_cast<const T*>(p.pk) + (int64_t)kv * p.ldpk * D;
+  const T* V = static_cast<const T*>(p.pvt) + (int64_t)kv * D * p.ldpv;
 
-  half8 qf[NKB];  // features 16 kb + 8 g .. + 7 of the lane's row
-  {
-    const int row = min(at, rows - 1);
-    const half_t* q = static_cast<const half_t*>(p.q) + ((int64_t)(kv * G + row % G) * p.ldq + row / G) * D;
-#pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) qf[kb] = frag_at(q + 16 * kb + 8 * g);
-  }
-
+  // slot of a 16-byte chunk: of key row x, and of feature row x (two to 256 bytes)
+  auto kslot = [](int x) {
+    return D >= 128 ? (x & 3) << 2 | (x >> 3 & 3) : (x >> 1 & 1) << 2 | (x >> 3 & 3);
+  };
+  auto vslot = [](int x) { return x >> 1 & 7; };
   // DMA instruction wave * NDMA + x writes 1 KiB: KROWS key rows, or 8 feature rows
-  auto key_of = [](int r) { return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1); };
-  auto swizzle = [](int r) { return D >= 128 ? (r & 15) : ((r >> 1) & 7); };
-  uint32_t ko[NDMA], vo[NDMA];
-  int kr[NDMA];
-#pragma unroll
-  for (int x = 0; x < NDMA; ++x) {
-    const int row = (wave * NDMA + x) * KROWS + lane / KS;
-    kr[x] = key_of(row);
-    ko[x] = 16u * ((lane % KS) ^ swizzle(row));
-    const int e = (wave * NDMA + x) * 8 + (lane >> 3);
-    vo[x] = 2u * ((uint32_t)e * (uint32_t)p.ldpv + 8 * ((lane & 7) ^ ((e >> 1) & 7)));
-  }
   auto issue_k = [&](int buf, int j0) {  // keys behind the last: the last again (masked)
-    const half_t* base = K + (int64_t)j0 * D;
+    const T* base = K + (int64_t)j0 * D;
     const int left = p.np - 1 - j0;
 #pragma unroll
-    for (int x = 0; x < NDMA; ++x)
-      dma16s(base, ko[x] + 2u * D * min(kr[x], left), &sK[buf][(wave * NDMA + x) * 512]);
+    for (int x = 0; x < NDMA; ++x) {
+      const int row = (wave * NDMA + x) * KROWS + lane / KS;
+      dma16s(base, 2u * D * min(row, left) + 16u * ((lane % KS) ^ kslot(row)), &sK[buf][(wave * NDMA + x) * 512]);
+    }
   };
   const int vlast = (int)(p.ldpv - 8);
   auto issue_v = [&](int buf, int j0) {  // columns behind the row: its last 8 (zeroed below)
-    const int over = max(0, j0 + 56 - vlast);
-    const half_t* base = V + j0;
 #pragma unroll
     for (int x = 0; x < NDMA; ++x) {
       const int e = (wave * NDMA + x) * 8 + (lane >> 3);
-      const int c = 8 * ((lane & 7) ^ ((e >> 1) & 7));
-      dma16s(base, over ? vo[x] - 2u * max(0, j0 + c - vlast) : vo[x], &sV[buf][(wave * NDMA + x) * 512]);
+      const int c = min(j0 + 8 * ((lane & 7) ^ vslot(e)), vlast);
+      dma16s(V, 2u * ((uint32_t)e * (uint32_t)p.ldpv + c), &sV[buf][(wave * NDMA + x) * 512]);
     }
   };
 
-  constexpr int KPER = D >= 128 ? 8 : 4;
-  int koff[KPER], voff[4];
-#pragma unroll
-  for (int x = 0; x < KPER; ++x) koff[x] = n * 2 * D + 16 * ((2 * x + g) ^ swizzle(n));
-#pragma unroll
-  for (int x = 0; x < 4; ++x) voff[x] = n * 128 + 16 * ((2 * x + g) ^ ((n >> 1) & 7));
-  auto operand = [&](const char* kbase, const char* vbase, int i) {
-    if (i < NS1)  // k-block i / 2, key half i % 2
-      return *reinterpret_cast<const half8*>(kbase + koff[(i >> 1) % KPER] + (i & 1) * 64 * D +
-                                             ((i >> 1) / KPER) * 32 * KPER);
-    i -= NS1;  // 16-key block i / NDT, feature tile i % NDT
-    return *reinterpret_cast<const half8*>(vbase + voff[i / NDT] + (i % NDT) * 32 * 128);
-  };
-  // accumulator x = 16 half + e of a lane is this key of the tile (and 8 g more)
-  auto key_in_tile = [](int x) { return 32 * (x >> 4) + 16 * ((x >> 3) & 1) + (x & 7); };
-
-  float16_t O[NDT] = {}, Sc[2] = {}, Sn[2];
-  float l = 0.0f, m = -INFINITY;
-  half8 fb[PD];
-  const int ntiles = (k1 - k0 + BK - 1) / BK;
   issue_k(0, k0);
   issue_v(0, k0);
-  if (ntiles > 1) issue_k(1, k0 + BK);
+  half8 fq[D / KB][1];
+  load_queries<T, D, 1, true>(p, fq, kv, row0, rows, lane);
+  Soft<T, D, 1> st;
+  st.clear();
   vm_wait_all();
   lds_barrier();
-  {
-    const char* kbase = reinterpret_cast<const char*>(sK[0]);
-#pragma unroll
-    for (int i = 0; i < PD; ++i) fb[i] = operand(kbase, kbase, i);
-#pragma unroll
-    for (int i = 0; i < NS1; ++i) {
-      Sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[i % PD], qf[i >> 1], Sc[i & 1], 0, 0, 0);
-      if (i + PD < NS1) fb[i % PD] = operand(kbase, kbase, i + PD);
-      __builtin_amdgcn_sched_barrier(0);
+  int b = 0;
+#pragma unroll 1
+  for (int j0 = k0; j0 < k1; j0 += BK, b ^= 1) {
+    if (j0 + BK < k1) {
+      issue_k(b ^ 1, j0 + BK);
+      issue_v(b ^ 1, j0 + BK);
     }
-    const int thr = k1 - k0 - 8 * g;
+    float4_t S[4][1] = {};
 #pragma unroll
-    for (int x = 0; x < 32; ++x) {
-      const float y = key_in_tile(x) >= thr ? -INFINITY : Sc[x >> 4][x & 15];
-      Sc[x >> 4][x & 15] = y;
-      m = fmaxf(m, y);
-    }
-    m = halves_max(m);
-  }
-  lds_barrier();  // all waves are done with K(0) before K(2) replaces it
-
-  // iteration j: K(j + 1), V(j) resident, masked scores of tile j in Sc
-  for (int j = 0; j < ntiles; ++j) {
-    const int j0 = k0 + j * BK;
-    if (j + 2 < ntiles) issue_k(j & 1, j0 + 2 * BK);
-    if (j + 1 < ntiles) issue_v((j + 1) & 1, j0 + BK);
-    if (j0 + BK > k1) {  // zero the values behind the last key
-      half_t* v = sV[j & 1];
-      for (int x = tid; x < D * 8; x += 256) {
-        const int e = x >> 3, slot = x & 7, c = j0 + 8 * (slot ^ ((e >> 1) & 7));
+    for (int kb = 0; kb < D / KB; ++kb)
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const int row = a / 2 * KB + Ops<T>::row(a % 2, r);
+        Mma<T>::mma(S[a][0], frag_at(sK[b] + row * D + ((kb * 4 + grp) ^ kslot(row)) * EL), fq[kb][0]);
+      }
+    if (j0 + BK > k1) {
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (j0 + a / 2 * KB + Ops<T>::row(a % 2, 4 * grp + i) >= k1) S[a][0][i] = -INFINITY;
+      for (int x = tid; x < D * 8; x += 512) {  // the values behind the last key
+        const int e = x >> 3, c = j0 + 8 * ((x & 7) ^ vslot(e));
         if (c + 8 > k1) {
-          half8 y = frag_at(v + e * 64 + slot * 8);
+          half8 y = frag_at(sV[b] + x * EL);
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             if (c + i >= k1) y[i] = half_t(0);
-          *reinterpret_cast<half8*>(v + e * 64 + slot * 8) = y;
+          *reinterpret_cast<half8*>(sV[b] + x * EL) = y;
         }
       }
       lds_barrier();
     }
-    const char* kbase = reinterpret_cast<const char*>(sK[(j + 1) & 1]);
-    const char* vbase = reinterpret_cast<const char*>(sV[j & 1]);
-    const float ref = m == -INFINITY ? 0.0f : m * p.c;
-    const int thr = k1 - (j0 + BK) - 8 * g;
+    half8 w[2][1];
+    st.template weights<2>(S, w, p.c);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) Sn[h][e] = 0.0f;
-    half8 w[4];
-    float sum = 0.0f, top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < PD; ++i) fb[i] = operand(kbase, vbase, i);
-    // scores of the next tile (in the last iteration of stale keys, not used) beside this one's weights
-#pragma unroll
-    for (int i = 0; i < NS1; ++i) {
-      Sn[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[i % PD], qf[i >> 1], Sn[i & 1], 0, 0, 0);
-      fb[i % PD] = operand(kbase, vbase, i + PD);
-#pragma unroll
-      for (int u = 0; u < EPS1; ++u) {
-        const int x = i * EPS1 + u;
-        const float y = __builtin_amdgcn_exp2f(fmaf(Sc[x >> 4][x & 15], p.c, -ref));
-        sum += y;
-        w[x >> 3][x & 7] = static_cast<half_t>(y);
+      for (int e = 0; e < D / 16; ++e) {
+        const int row = e * 16 + r;
+        Mma<T>::mma(st.o[e][0], frag_at(sV[b] + row * BK + ((x * 4 + grp) ^ vslot(row)) * EL), w[x][0]);
       }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    auto mask_max = [&](int x) {
-      const float y = key_in_tile(x) >= thr ? -INFINITY : Sn[x >> 4][x & 15];
-      Sc[x >> 4][x & 15] = y;
-      top = fmaxf(top, y);
-    };
-#pragma unroll
-    for (int i = 0; i < NS2; ++i) {
-      O[i % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[(NS1 + i) % PD], w[i / NDT], O[i % NDT], 0, 0, 0);
-      if (i + PD < NS2) fb[(NS1 + i) % PD] = operand(kbase, vbase, NS1 + i + PD);
-      if (i >= 2) {
-#pragma unroll
-        for (int u = 0; u < EPS2; ++u) mask_max((i - 2) * EPS2 + u);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#pragma unroll
-    for (int x = 32 - 2 * EPS2; x < 32; ++x) mask_max(x);
-    l += sum;
-    if (j + 1 < ntiles) {
-      const float to = fmaxf(m, halves_max(top));
-      if (__any((to - m) * p.c > 8.0f)) {
-        const float f = m == to ? 1.0f : __builtin_amdgcn_exp2f((m - to) * p.c);
-#pragma unroll
-        for (int t = 0; t < NDT; ++t) O[t] *= f;
-        l *= f;
-        m = to;
-      }
-    }
     vm_wait_all();
-    lds_barrier();
+    lds_barrier();  // this tile is read, the next one there
   }
-  l += __shfl_xor(l, 32, 64);
+  const int at = row0 + r;
+  const float l = sum4(st.l[0]);
   if (at >= rows) return;
   const int64_t to = (int64_t)split * p.T * p.heads + (int64_t)(at / G) * p.heads + kv * G + at % G;
-  if (g == 0) p.ml[to] = float2{m * p.c, l};
+  if (grp == 0) p.ml[to] = float2{st.m[0], l};
 #pragma unroll
-  for (int t = 0; t < NDT; ++t)
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-      *reinterpret_cast<float4_t*>(p.part + to * D + 32 * t + 8 * x + 4 * g) =
-          float4_t{O[t][4 * x], O[t][4 * x + 1], O[t][4 * x + 2], O[t][4 * x + 3]};
+  for (int e = 0; e < D / 16; ++e) *reinterpret_cast<float4_t*>(p.part + to * D + e * 16 + grp * 4) = st.o[e][0];
 }
 
 // Part `split` of the own keys of one token's rows of one key head (16 of them
@@ -678,7 +587,7 @@ int launch(const SharedParams& p, const Plan& x, hipStream_t st) {
     if constexpr (sizeof(T) == 2 && FULL) {
       // its loads address a key head's values with 32 bits
       if (x.many && p.ldpv * D * 2 < (int64_t(1) << 32)) {
-        hipLaunchKernelGGL((shared_many_rows<D>), dim3((rows + 127) / 128 * each), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((shared_many_rows<D>), dim3((rows + 127) / 128 * each), dim3(512), 0, st, p);
         done = true;
       }
     }
