@@ -356,9 +356,13 @@ __global__ __launch_bounds__(512, 2) void shared_many_rows(SharedParams p) {
   const T* K = static_cast<const T*>(p.pk) + (int64_t)kv * p.ldpk * D;
   const T* V = static_cast<const T*>(p.pvt) + (int64_t)kv * D * p.ldpv;
 
-  // slot of a 16-byte chunk: of key row x, and of feature row x (two to 256 bytes)
+  // slot of a 16-byte chunk: of key row x, and of feature row x (two to 256 bytes).
+  // A 16-byte read takes lanes 0-3, 12-15 and 20-27 of 32 together, then the others:
+  // with the third and fourth quarter's rows exchanged (0, 2, 3, 1) each of these
+  // sixteen meets another bank.
   auto kslot = [](int x) {
-    return D >= 128 ? (x & 3) << 2 | (x >> 3 & 3) : (x >> 1 & 1) << 2 | (x >> 3 & 3);
+    const int q = x >> 3 & 3, f = ((q << 1 ^ q) & 2) | q >> 1;
+    return D >= 128 ? (x & 3) << 2 | f : (x >> 1 & 1) << 2 | f;
   };
   auto vslot = [](int x) { return x >> 1 & 7; };
   // DMA instruction wave * NDMA + x writes 1 KiB: KROWS key rows, or 8 feature rows
@@ -381,36 +385,73 @@ __global__ __launch_bounds__(512, 2) void shared_many_rows(SharedParams p) {
     }
   };
 
+  constexpr int NS = D / KB;           // steps of four products, of the scores and of V
+  constexpr int EACH = 16 / NS;        // scores of a lane to a step
+  auto key_operand = [&](int buf, int kb, half8 (&f)[4]) {
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int row = a / 2 * KB + Ops<T>::row(a % 2, r);
+      f[a] = frag_at(sK[buf] + row * D + ((kb * 4 + grp) ^ kslot(row)) * EL);
+    }
+  };
+  auto value_operand = [&](int buf, int i, half8 (&f)[4]) {  // step i: key half i / (NS / 2), four feature tiles
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int row = (i % (NS / 2) * 4 + a) * 16 + r;
+      f[a] = frag_at(sV[buf] + row * BK + ((i / (NS / 2) * 4 + grp) ^ vslot(row)) * EL);
+    }
+  };
+
+  const int ntiles = (k1 - k0 + BK - 1) / BK;
   issue_k(0, k0);
   issue_v(0, k0);
+  if (ntiles > 1) issue_k(1, k0 + BK);
   half8 fq[D / KB][1];
   load_queries<T, D, 1, true>(p, fq, kv, row0, rows, lane);
-  Soft<T, D, 1> st;
-  st.clear();
+  float4_t o[D / 16] = {};
+  float m = -INFINITY, l = 0.0f;
+  half8 f[2][4];
+  float4_t Sc[4], Sn[4] = {};
   vm_wait_all();
   lds_barrier();
-  int b = 0;
-#pragma unroll 1
-  for (int j0 = k0; j0 < k1; j0 += BK, b ^= 1) {
-    if (j0 + BK < k1) {
-      issue_k(b ^ 1, j0 + BK);
-      issue_v(b ^ 1, j0 + BK);
+#pragma unroll
+  for (int kb = 0; kb < NS; ++kb) {
+    key_operand(0, kb, f[kb & 1]);
+#pragma unroll
+    for (int a = 0; a < 4; ++a) Mma<T>::mma(Sn[a], f[kb & 1][a], fq[kb][0]);
+  }
+  // scores of the tile at j0, masked, and the reference maximum that they need
+  auto mask = [&](int j0, int x) {
+    const int a = x / 4, i = x % 4;
+    const float y = j0 + a / 2 * KB + Ops<T>::row(a % 2, 4 * grp + i) >= k1 ? -INFINITY : Sn[a][i];
+    Sc[a][i] = y;
+    return y;
+  };
+  auto raise = [&](float top) {
+    const float to = fmaxf(m, max4(top) * p.c);
+    if (__any(to > m + 8.0f)) {
+      const float g = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+      m = to;
+      l *= g;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) o[e] *= g;
     }
-    float4_t S[4][1] = {};
+  };
+  {
+    float top = -INFINITY;
 #pragma unroll
-    for (int kb = 0; kb < D / KB; ++kb)
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const int row = a / 2 * KB + Ops<T>::row(a % 2, r);
-        Mma<T>::mma(S[a][0], frag_at(sK[b] + row * D + ((kb * 4 + grp) ^ kslot(row)) * EL), fq[kb][0]);
-      }
+    for (int x = 0; x < 16; ++x) top = fmaxf(top, mask(k0, x));
+    raise(top);
+  }
+  lds_barrier();  // K(0) is read before K(2) replaces it
+  // tile j: its masked scores in Sc, V(j) and K(j + 1) resident
+#pragma unroll 1
+  for (int j = 0; j < ntiles; ++j) {
+    const int j0 = k0 + j * BK, b = j & 1;
+    if (j + 2 < ntiles) issue_k(b, j0 + 2 * BK);
+    if (j + 1 < ntiles) issue_v(b ^ 1, j0 + BK);
     if (j0 + BK > k1) {
-#pragma unroll
-      for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (j0 + a / 2 * KB + Ops<T>::row(a % 2, 4 * grp + i) >= k1) S[a][0][i] = -INFINITY;
-      for (int x = tid; x < D * 8; x += 512) {  // the values behind the last key
+      for (int x = tid; x < D * 8; x += 512) {  // zero the values behind the last key
         const int e = x >> 3, c = j0 + 8 * ((x & 7) ^ vslot(e));
         if (c + 8 > k1) {
           half8 y = frag_at(sV[b] + x * EL);
@@ -422,25 +463,53 @@ __global__ __launch_bounds__(512, 2) void shared_many_rows(SharedParams p) {
       }
       lds_barrier();
     }
-    half8 w[2][1];
-    st.template weights<2>(S, w, p.c);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    half8 w[2];
+    float top = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int a = 0; a < 4; ++a) Sn[a] = float4_t{0.f, 0.f, 0.f, 0.f};
+    key_operand(b ^ 1, 0, f[0]);
+    // the next tile's scores (in the last round of stale keys, not used) beside this one's weights
 #pragma unroll
-      for (int e = 0; e < D / 16; ++e) {
-        const int row = e * 16 + r;
-        Mma<T>::mma(st.o[e][0], frag_at(sV[b] + row * BK + ((x * 4 + grp) ^ vslot(row)) * EL), w[x][0]);
+    for (int kb = 0; kb < NS; ++kb) {
+      if (kb + 1 < NS) key_operand(b ^ 1, kb + 1, f[(kb + 1) & 1]);
+      else value_operand(b, 0, f[(kb + 1) & 1]);
+#pragma unroll
+      for (int a = 0; a < 4; ++a) Mma<T>::mma(Sn[a], f[kb & 1][a], fq[kb][0]);
+#pragma unroll
+      for (int u = 0; u < EACH; ++u) {
+        const int x = kb * EACH + u;
+        const float y = __builtin_amdgcn_exp2f(fmaf(Sc[x / 4][x % 4], p.c, -ref));
+        l += y;
+        w[x / 8][x % 8] = static_cast<T>(y);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // the products with V beside the next scores' maximum
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      if (i + 1 < NS) value_operand(b, i + 1, f[(i + 1 + NS) & 1]);
+#pragma unroll
+      for (int a = 0; a < 4; ++a) Mma<T>::mma(o[i % (NS / 2) * 4 + a], f[(i + NS) & 1][a], w[i / (NS / 2)]);
+      if (i > 0) {
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) top = fmaxf(top, mask(j0 + BK, (i - 1) * EACH + u));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int x = 16 - EACH; x < 16; ++x) top = fmaxf(top, mask(j0 + BK, x));
+    if (j + 1 < ntiles) raise(top);
     vm_wait_all();
-    lds_barrier();  // this tile is read, the next one there
+    lds_barrier();
   }
   const int at = row0 + r;
-  const float l = sum4(st.l[0]);
+  l = sum4(l);
   if (at >= rows) return;
   const int64_t to = (int64_t)split * p.T * p.heads + (int64_t)(at / G) * p.heads + kv * G + at % G;
-  if (grp == 0) p.ml[to] = float2{st.m[0], l};
+  if (grp == 0) p.ml[to] = float2{m, l};
 #pragma unroll
-  for (int e = 0; e < D / 16; ++e) *reinterpret_cast<float4_t*>(p.part + to * D + e * 16 + grp * 4) = st.o[e][0];
+  for (int e = 0; e < D / 16; ++e) *reinterpret_cast<float4_t*>(p.part + to * D + e * 16 + grp * 4) = o[e];
 }
 
 // Part `split` of the own keys of one token's rows of one key head (16 of them

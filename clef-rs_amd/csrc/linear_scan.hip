@@ -106,7 +106,10 @@ struct Tiles {
   static constexpr bool XOR = sizeof(T) == 2 && DK == 128;
   static constexpr int PQ = DK + EL, PK = XOR ? DK : DK + EL, PV = sizeof(T) == 2 ? DV + 32 : DV + EL;
   static __device__ __forceinline__ int key(int row, int col) {  // col a multiple of EL
-    return XOR ? row * DK + (((col >> 3) ^ ((row & 3) << 2 | (row >> 3 & 3))) << 3) : row * PK + col;
+    // quarters of 8 rows as 0, 2, 3, 1: a 16-byte read takes lanes 0-3, 12-15 and
+    // 20-27 of 32 together, then the others
+    const int q = row >> 3 & 3, f = ((q << 1 ^ q) & 2) | q >> 1;
+    return XOR ? row * DK + (((col >> 3) ^ ((row & 3) << 2 | f)) << 3) : row * PK + col;
   }
   // what lane names for key columns c0 + row(t, .) of tokens t0 + EL (lane / 16) ..
   static __device__ __forceinline__ int key_t(int t0, int c0, int t, int lane) {
