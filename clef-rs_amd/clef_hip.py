@@ -390,7 +390,7 @@ class LinearScan:
         n = lib().clef_linear_scan_workspace(T, nseq, Hk, Hv, self.key_dim, self.value_dim, _dt(q))
         if n == 0:
             raise ClefError(-1, last_error())
-        return _scratch(n, q.device)
+        return _scratch(n, q.device) if n > 256 else None  # 256: the call keeps nothing there
 
     def prefill(self, q, k, v, g, initial=None, out_dtype=torch.float32, want_final=True, out=None):
         """q, k [T, Hk, dk], v [T, Hv, dv], g [Hv]; initial None or [Hv, dk, dv] f32.
@@ -403,11 +403,11 @@ class LinearScan:
             raise ClefError(-1, "initial state must be contiguous f32 [Hv, dk, dv]")
         if initial is not None:
             _here(initial)
-        final = torch.empty((Hv, dk, dv), dtype=torch.float32, device=q.device) if want_final else None
+        final = g.new_empty((Hv, dk, dv)) if want_final else None
         ws = self._workspace(T, 1, Hk, Hv, q)
         _check(lib().clef_linear_scan(
             _ptr(q), _ptr(k), _ptr(v), sqk, sv, _dt(q), _ptr(g), T, Hk, Hv, dk, dv, self.scale, _ptr(initial),
-            _ptr(out), so, _dt(out), _ptr(final), _ptr(ws), ws.numel(), _stream()))
+            _ptr(out), so, _dt(out), _ptr(final), _ptr(ws), 0 if ws is None else ws.numel(), _stream()))
         return out, final
 
     def prefill_varlen(self, q, k, v, g, cu_seqlens, initial=None, out_dtype=torch.float32, want_final=True,
@@ -430,10 +430,10 @@ class LinearScan:
                 raise ClefError(-1, "initial state must be [Hv, dk, dv] or [nseq, Hv, dk, dv]")
         _here(cu_seqlens, initial)
         ws = self._workspace(T, nseq, Hk, Hv, q)
-        final = torch.empty((nseq, Hv, dk, dv), dtype=torch.float32, device=q.device) if want_final else None
+        final = g.new_empty((nseq, Hv, dk, dv)) if want_final else None
         _check(lib().clef_linear_scan_varlen(
             _ptr(q), _ptr(k), _ptr(v), sqk, sv, _dt(q), _ptr(g), _ptr(cu_seqlens), nseq, T, Hk, Hv, dk, dv,
-            self.scale, _ptr(initial), stride, _ptr(out), so, _dt(out), _ptr(final), _ptr(ws), ws.numel(), _stream()))
+            self.scale, _ptr(initial), stride, _ptr(out), so, _dt(out), _ptr(final), _ptr(ws), 0 if ws is None else ws.numel(), _stream()))
         return out, final
 
     def step(self, q, k, v, g, states, slots=None, new_states=None, out_dtype=torch.float32, out=None):

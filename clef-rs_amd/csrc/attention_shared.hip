@@ -100,8 +100,6 @@ __device__ __forceinline__ void own_span(const SharedParams& p, int s, int t, in
   count = max(len - left, 0);
 }
 
-typedef float float2_t __attribute__((ext_vector_type(2)));
-
 __device__ __forceinline__ float max4(float x) {  // over the 4 lanes of a query
   x = fmaxf(x, __shfl_xor(x, 16, 64));
   return fmaxf(x, __shfl_xor(x, 32, 64));
@@ -558,6 +556,15 @@ __global__ __launch_bounds__(512) void shared_join(SharedParams p) {
   if (s < 0) return;
   const int rows = min(R, G - g0), h0 = kv * G + g0;
   const int64_t row = (int64_t)t * p.heads + h0;
+  // the thread's four features of the output, and their gate
+  const int x = tid / (D / 4), e = tid % (D / 4) * 4;
+  const bool mine = x < rows && e < p.d;
+  T gate[4] = {};
+  if (mine) {
+    const T* gp = static_cast<const T*>(p.gate) + t * p.ldg + (h0 + x) * p.hsg + e;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) gate[j] = gp[j];
+  }
   if (wave < 4) {
     int first = 0, count = 0;
     if (!p.osplits) own_span(p, s, t, first, count);
@@ -567,57 +574,38 @@ __global__ __launch_bounds__(512) void shared_join(SharedParams p) {
     st.clear();
     take_keys<T, D, 1, FULL>(st, fq, p.k, p.ldk, p.vt, p.ldv, kv, first, first + count, p.d, p.c, wave, 4, lane);
     part.put(st, 0, wave, lane, rows);
-  } else {
-    const int x = (tid - 256) / 32, a = tid % 32;
+  } else if (const int y = (tid - 256) / 32; y < rows) {
+    const int a = tid % 32;
     const int parts = p.psplits + p.osplits;
     const int64_t step = (int64_t)p.T * p.heads;
-    if (x < rows) {
-      const float2* ml = p.ml + row + x;
-      float m = -INFINITY;
-      for (int n = a; n < parts; n += 32) m = fmaxf(m, ml[n * step].x);
-      m = fmaxf(m, __shfl_xor(m, 16, 64));
-      m = lane_max<16>(m);
-      const float ref = m == -INFINITY ? 0.0f : m;
-      float l = 0.0f;
-      float4_t o[F / 4 ? F / 4 : 1] = {};
-      float2_t o2 = {0.f, 0.f};
-      const float* src = p.part + (row + x) * D + a * F;
+    const float2* ml = p.ml + row + y;
+    const float* src = p.part + (row + y) * D + a * F;
+    typedef float vec __attribute__((ext_vector_type(F)));
+    float m = -INFINITY;
+    for (int n = a; n < parts; n += 32) m = fmaxf(m, ml[n * step].x);
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = lane_max<16>(m);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    vec o = {};
 #pragma unroll 8
-      for (int n = 0; n < parts; ++n) {
-        const float2 w = ml[n * step];
-        const float f = __builtin_amdgcn_exp2f(w.x - ref);
-        l = fmaf(w.y, f, l);
-        if constexpr (F == 2) {
-          o2 += *reinterpret_cast<const float2_t*>(src + n * step * D) * f;
-        } else {
-#pragma unroll
-          for (int i = 0; i < F / 4; ++i) o[i] += *reinterpret_cast<const float4_t*>(src + n * step * D + i * 4) * f;
-        }
-      }
-      if constexpr (F == 2) {
-        *reinterpret_cast<float2_t*>(&part.o[4][x][a * F]) = o2;
-      } else {
-#pragma unroll
-        for (int i = 0; i < F / 4; ++i) *reinterpret_cast<float4_t*>(&part.o[4][x][a * F + i * 4]) = o[i];
-      }
-      if (a == 0) part.ml[4][x] = float2{m, l};
+    for (int n = 0; n < parts; ++n) {
+      const float2 w = ml[n * step];
+      const float f = __builtin_amdgcn_exp2f(w.x - ref);
+      l = fmaf(w.y, f, l);
+      o += *reinterpret_cast<const vec*>(src + n * step * D) * f;
     }
+    *reinterpret_cast<vec*>(&part.o[4][y][a * F]) = o;
+    if (a == 0) part.ml[4][y] = float2{m, l};
   }
   lds_barrier();
-  for (int i = tid; i < rows * (D / 4); i += 512) {
-    const int x = i / (D / 4), e = i % (D / 4) * 4;
-    if (e >= p.d) continue;
-    const T* gp = static_cast<const T*>(p.gate) + t * p.ldg + (h0 + x) * p.hsg + e;
-    T gate[4];
+  if (!mine) return;
+  float m, l;
+  const float4_t o = part.take(x, e, m, l);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+  T* y = static_cast<T*>(p.y) + t * p.ldy + (int64_t)(h0 + x) * p.d + e;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) gate[j] = gp[j];
-    float m, l;
-    const float4_t o = part.take(x, e, m, l);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
-    T* y = static_cast<T*>(p.y) + t * p.ldy + (int64_t)(h0 + x) * p.d + e;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = cvt_out<T>(o[j] * inv * sigmoid(to_f32(gate[j])));
-  }
+  for (int j = 0; j < 4; ++j) y[j] = cvt_out<T>(o[j] * inv * sigmoid(to_f32(gate[j])));
 }
 
 int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
@@ -634,15 +622,18 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
   const int cus = device_cus();
   x.many = dtype == CLEF_F16 && rows > 32 && d == padded(d);
   x.tile = rows > 16 ? 32 : 16;
-  // splits until the chip is full (many rows: one work-group to a CU), but no
-  // shorter than two tiles of keys, or a block to a wave
+  // splits until the chip is full (many rows: one work-group to a CU), but not so
+  // short that the parts cost more than they save: 32 requests behind 4,096 keys at
+  // 64, 128 and 256 keys a part take 38, 34 and 33 us with their joining; few rows
+  // take one block to each of two waves (2 requests behind 512 keys: 12.8 us at 64,
+  // 16.1 at 128, where every wave has one)
   auto split = [&](int keys, int64_t groups, int fill, int least, int most, int& parts, int& each) {
     const int64_t want = std::min<int64_t>(std::max<int64_t>(1, fill / groups), most);
     each = static_cast<int>(((keys + want - 1) / want + least - 1) / least * least);
     parts = (keys + each - 1) / each;
   };
   const int tile = x.many ? 128 : x.tile;
-  if (np) split(np, (rows + tile - 1) / tile * kvh, x.many ? cus : 2 * cus, dtype == CLEF_F16 ? 128 : 64, kMaxParts, x.psplits, x.pkeys);
+  if (np) split(np, (rows + tile - 1) / tile * kvh, x.many ? cus : 2 * cus, x.many ? 256 : 64, kMaxParts, x.psplits, x.pkeys);
   if (max_keys > 1024) split(max_keys, (int64_t)T * kvh, 2 * cus, 512, kMaxParts, x.osplits, x.okeys);
   return x;
 }

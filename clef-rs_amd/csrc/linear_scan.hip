@@ -45,6 +45,7 @@ namespace {
 constexpr int kMaxSeq = 4096;
 constexpr int kMaxWidth = 128;
 constexpr int C = 64;  // tokens of a chunk
+constexpr size_t kNoWorkspace = 256;  // said of calls that keep nothing there
 
 struct LinearParams {
   const void *q, *k, *v;
@@ -52,7 +53,7 @@ struct LinearParams {
   const int* cu;         // [nseq + 1] or null (one sequence of T tokens)
   const float* initial;  // sequence s at initial + s * init_stride; null: zeros
   float* final_state;    // [nseq][Hv][dk][dv] or null
-  float* enter;          // [units][Hv][DK * DV]: unit states in register order
+  float* enter;          // [T / unit][Hv][DK * DV]: unit states in register order
   void* out;
   int64_t sqk, sv, so, init_stride;
   int T, nseq, Hk, Hv, dk, dv;
@@ -135,9 +136,15 @@ __device__ __forceinline__ void span_of(const LinearParams& p, int s, int& t0, i
 
 // Units are numbered without a table: sequence s's first is cu[s] / unit + s,
 // so that the ceil(len / unit) of one never reach the next one's first.
-// Numbers that no sequence uses are idle.
+// Numbers that no sequence uses are idle.  Those that start inside a sequence
+// have an entry for their state, unit i >= 1 of sequence s entry cu[s] / unit + i - 1:
+// there are at most T / unit, and again none reaches the next sequence's.
 __device__ __forceinline__ int first_unit(const LinearParams& p, int s) {
   return p.cu ? min(max(p.cu[s], 0), p.T) / p.unit + s : 0;
+}
+__device__ __forceinline__ float* entry(const LinearParams& p, int s, int i, int h, int state) {
+  const int at = (p.cu ? min(max(p.cu[s], 0), p.T) / p.unit : 0) + i - 1;
+  return p.enter + ((int64_t)at * p.Hv + h) * state;
 }
 // The sequence of unit u: the last one whose first unit is at most u, by 64-way
 // steps (every lane of a wave probes one sequence).
@@ -295,7 +302,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
   {
     const int r = lane & 15, grp = lane >> 4;
     if (OUT && index > 0) {
-      const float* src = p.enter + ((int64_t)u * p.Hv + h) * (DK * DV) + wave * (DK * 16);
+      const float* src = entry(p, s, index, h, DK * DV) + wave * (DK * 16);
 #pragma unroll
       for (int a = 0; a < NKB * TPB; ++a) S[a] = *reinterpret_cast<const float4_t*>(src + (a * 64 + lane) * 4);
     } else {
@@ -486,7 +493,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
   {
     const int r = lane & 15, grp = lane >> 4;
     if constexpr (!OUT) {
-      float* dst = p.enter + ((int64_t)u * p.Hv + h) * (DK * DV) + wave * (DK * 16);
+      float* dst = entry(p, s, index + 1, h, DK * DV) + wave * (DK * 16);
 #pragma unroll
       for (int a = 0; a < NKB * TPB; ++a) *reinterpret_cast<float4_t*>(dst + (a * 64 + lane) * 4) = S[a];
     } else if (p.final_state && last) {
@@ -503,9 +510,9 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
   }
 }
 
-// The state that each unit starts from: enter[u] holds what unit u adds, and
-// becomes what it starts with (units behind a sequence's first).  A thread owns
-// 4 elements of one (sequence, head).
+// The state that each unit starts from: its entry holds what the unit before it
+// adds, and becomes what it starts from.  A thread owns 4 elements of one
+// (sequence, head).
 template <class T, int DK, int DV>
 __global__ __launch_bounds__(256) void linear_join(LinearParams p) {
   constexpr int KB = Ops<T>::KB, TPB = Ops<T>::TPB;
@@ -528,12 +535,11 @@ __global__ __launch_bounds__(256) void linear_join(LinearParams p) {
   }
   const float w = __builtin_amdgcn_exp2f(log2_decay(p.g[h]) * (float)p.unit);
   const int64_t step = (int64_t)p.Hv * (DK * DV);
-  float* at = p.enter + (first_unit(p, s) * (int64_t)p.Hv + h) * (DK * DV) + e;
+  float* at = entry(p, s, 1, h, DK * DV) + e;
   float4_t next = *reinterpret_cast<const float4_t*>(at);
-  for (int u = 1; u < n; ++u) {  // what a unit adds is read before its entry is written
+  for (int i = 1; i < n; ++i, at += step) {
     const float4_t add = next;
-    at += step;
-    if (u + 1 < n) next = *reinterpret_cast<const float4_t*>(at);
+    if (i + 1 < n) next = *reinterpret_cast<const float4_t*>(at + step);
     run = run * w + add;
     *reinterpret_cast<float4_t*>(at) = run;
   }
@@ -564,8 +570,8 @@ int padded(int d) { return d <= 64 ? 64 : 128; }
 
 size_t workspace_bytes(int T, int nseq, int Hk, int Hv, int dk, int dv, int dtype) {
   const int unit = unit_tokens(T, Hv, dtype);
-  if (T <= unit) return 256;  // every sequence is one unit
-  return ((size_t)T / unit + nseq) * Hv * padded(dk) * padded(dv) * 4;
+  if (T <= unit) return kNoWorkspace;  // every sequence is one unit
+  return (size_t)(T / unit) * Hv * padded(dk) * padded(dv) * 4;
 }
 
 template <class T, class O, int DK, int DV>
@@ -606,7 +612,8 @@ int linear_scan(const void* q, const void* k, const void* v, int64_t sqk, int64_
     const uintptr_t ea = a + 4 * (size_t)((nseq - 1) * initial_stride + state), eb = b + 4 * (size_t)(nseq * state);
     CLEF_REQUIRE(ea <= b || eb <= a, "linear attention scan: initial and final states overlap");
   }
-  CLEF_REQUIRE(workspace && workspace_size >= workspace_bytes(T, nseq, Hk, Hv, dk, dv, dtype_qkv),
+  const size_t need = workspace_bytes(T, nseq, Hk, Hv, dk, dv, dtype_qkv);
+  CLEF_REQUIRE(need == kNoWorkspace || (workspace && workspace_size >= need),
                "linear attention scan: workspace too small");
   CLEF_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
                "linear attention scan: workspace must be 256-byte aligned");

@@ -154,7 +154,8 @@ int clef_delta_scan_varlen(const void* q, const void* k, const void* v, int64_t 
  * and scores beyond 65504 overflow.
  * Limits: 1 <= T <= 1048576; 1 <= Hk <= Hv <= 256; Hv % Hk == 0;
  * 1 <= dk <= 128; 1 <= dv <= 128.  workspace: clef_linear_scan_workspace
- * (nseq 1 for a single sequence) bytes, 256-byte aligned.
+ * (nseq 1 for a single sequence) bytes, 256-byte aligned; where that is 256
+ * (short prompts), nothing is kept there and workspace may be NULL.
  */
 size_t clef_linear_scan_workspace(int T, int nseq, int Hk, int Hv, int dk, int dv, int dtype_qkv);
 int clef_linear_scan(const void* q, const void* k, const void* v, int64_t sqk, int64_t sv, int dtype_qkv,

@@ -18,8 +18,8 @@ def scan(**kw):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(q=None), dict(k=None), dict(v=None), dict(g=None), dict(out=None), dict(cu=None), dict(ws=None), dict(wsb=0),
-    dict(ws=257), dict(T=0), dict(T=(1 << 20) + 1), dict(nseq=0), dict(nseq=4097), dict(Hk=0), dict(Hk=3), dict(Hv=257),
+    dict(q=None), dict(k=None), dict(v=None), dict(g=None), dict(out=None), dict(cu=None), dict(T=3000, ws=None),
+    dict(T=3000, wsb=0), dict(ws=257), dict(T=0), dict(T=(1 << 20) + 1), dict(nseq=0), dict(nseq=4097), dict(Hk=0), dict(Hk=3), dict(Hv=257),
     dict(dk=0), dict(dk=129), dict(dv=0), dict(dv=129), dict(dt=2), dict(dto=2), dict(sqk=127), dict(sv=255),
     dict(so=255), dict(stride=-1), dict(stride=4 * 64 * 64 - 1), dict(scale=float("nan")), dict(scale=float("inf")),
     dict(initial=1 << 20, stride=4 * 64 * 64, final=(1 << 20) + 64)], ids=str)
@@ -34,7 +34,9 @@ def test_linear_scan_workspace(L):
     assert L.clef_linear_scan_workspace(10, 0, 1, 1, 64, 64, 1) == 0
     assert L.clef_linear_scan_workspace(10, 1, 2, 3, 64, 64, 1) == 0
     assert L.clef_linear_scan_workspace(10, 1, 1, 1, 64, 64, 3) == 0
-    assert L.clef_linear_scan_varlen(*scan(wsb=L.clef_linear_scan_workspace(100, 3, 2, 4, 64, 64, 1) - 1)) < 0
+    n = L.clef_linear_scan_workspace(3000, 3, 2, 4, 64, 64, 1)
+    assert n > 256 and L.clef_linear_scan_varlen(*scan(T=3000, wsb=n - 1)) < 0
+    assert L.clef_linear_scan_workspace(1 << 20, 4096, 1, 2, 128, 128, 0) % 256 == 0
 
 
 def step(kind, **kw):
