@@ -100,7 +100,8 @@ __device__ __forceinline__ float4_t transposed(const float* p, int pitch) {
 // columns exchanged by a function of the row (XOR) that spreads both the 16 rows
 // of a score operand (8 (r / 4) + 4 t + r % 4) and the 4 tokens x 4 columns of a
 // transposed read over the banks.  Elsewhere rows are padded: by 16 bytes, which
-// spreads consecutive rows, and value rows of f16 by 64, for the transposed reads.
+// spreads consecutive rows, and value rows of f16 by 64, with every other 8 of
+// them 32 bytes on, so that the 8 rows x 32 bytes of two transposed reads differ.
 template <class T, int DK, int DV>
 struct Tiles {
   static constexpr int EL = Ops<T>::EL;
@@ -117,9 +118,13 @@ struct Tiles {
     if constexpr (sizeof(T) == 2) return key(t0 + 8 * (lane >> 4) + (lane >> 2 & 3), c0 + 8 * (lane & 3)) + 4 * t;
     else return (t0 + 4 * (lane >> 4)) * PK + c0 + (lane & 15);
   }
-  static __device__ __forceinline__ int value_t(int t0, int c0, int t, int lane) {
-    if constexpr (sizeof(T) == 2) return (t0 + 8 * (lane >> 4) + (lane >> 2 & 3)) * PV + c0 + 8 * (lane & 3) + 4 * t;
-    else return (t0 + 4 * (lane >> 4)) * PV + c0 + (lane & 15);
+  // value columns c0 + 0 .. 15
+  static __device__ __forceinline__ int value(int row, int col) {
+    return sizeof(T) == 2 ? row * PV + (row >> 3 & 1) * 16 + col : row * PV + col;
+  }
+  static __device__ __forceinline__ int value_t(int t0, int c0, int lane) {
+    if constexpr (sizeof(T) == 2) return value(t0 + 8 * (lane >> 4) + (lane >> 2 & 3), c0 + 4 * (lane & 3));
+    else return value(t0 + 4 * (lane >> 4), c0 + (lane & 15));
   }
   static constexpr int KSTEP = sizeof(T) == 2 ? 4 * PK : PK, VSTEP = sizeof(T) == 2 ? 4 * PV : PV;
 };
@@ -249,7 +254,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
   constexpr int NCB = C / KB;    // k-blocks of a chunk
   constexpr int QT = C / 16;     // query tiles of a chunk
   typedef Tiles<T, DK, DV> Tile;
-  constexpr int PQ = Tile::PQ, PV = Tile::PV;
+  constexpr int PQ = Tile::PQ;
   typedef typename Ops<T>::frag frag;
   typedef Shared<T, DK, DV, OUT> Lds;
   __shared__ __attribute__((aligned(16))) char smem[Lds::BYTES];
@@ -296,8 +301,8 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
   if (begin < end) fetch(begin, tid);
 
   // ---- the entering state: tile a of S has rows KB (a / TPB) + row(a % TPB, .)
-  // and the wave's columns cb + row(ct, .)
-  const int cb = wave / TPB * KB, ct = wave % TPB;
+  // and the wave's 16 columns
+  const int cb = wave * 16;
   float4_t S[NKB * TPB];
   {
     const int r = lane & 15, grp = lane >> 4;
@@ -307,7 +312,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
       for (int a = 0; a < NKB * TPB; ++a) S[a] = *reinterpret_cast<const float4_t*>(src + (a * 64 + lane) * 4);
     } else {
       const float* src = OUT && p.initial ? p.initial + s * p.init_stride + (int64_t)h * p.dk * p.dv : nullptr;
-      const int col = cb + Ops<T>::row(ct, r);
+      const int col = cb + r;
 #pragma unroll
       for (int a = 0; a < NKB * TPB; ++a)
 #pragma unroll
@@ -327,7 +332,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
     const int r = ln & 15, grp = ln >> 4;
     if (OUT) rq.store(sQ, at, [](int row, int col) { return row * PQ + col; });
     rk.store(sK, at, [](int row, int col) { return Tile::key(row, col); });
-    rv.store(sV, at, [](int row, int col) { return row * PV + col; });
+    rv.store(sV, at, [](int row, int col) { return Tile::value(row, col); });
     lds_barrier();
     if (t + C < end) fetch(t + C, at);
 
@@ -381,7 +386,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
         frag fv[NCB];
         bool odd;
 #pragma unroll
-        for (int b = 0; b < NCB; ++b) fv[b] = transposed(sV + Tile::value_t(b * KB, cb, ct, ln), Tile::VSTEP);
+        for (int b = 0; b < NCB; ++b) fv[b] = transposed(sV + Tile::value_t(b * KB, cb, ln), Tile::VSTEP);
         {
           // 0 or -0 from finite values, NaN from others
           frag zero = fv[0] * T(0);
@@ -422,7 +427,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
         if (odd) {
 #pragma unroll 1
           for (int j = 0; j < rows; ++j) {
-            const T* vj = sV + j * PV + cb + Ops<T>::row(ct, 4 * grp);
+            const T* vj = sV + Tile::value(j, cb + 4 * grp);
             // the scores of key j lie EL apart in their fragments
             const T* pj = sP + (j / KB * 64 + j % KB / EL * 16 + r) * EL + j % EL;
 #pragma unroll
@@ -435,7 +440,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
             }
           }
         }
-        const int col = cb + Ops<T>::row(ct, 4 * grp);  // 4 consecutive columns
+        const int col = cb + 4 * grp;  // 4 consecutive columns
         O* out = static_cast<O*>(p.out) + t * p.so + (int64_t)h * p.dv + r * p.so + col;
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
@@ -471,7 +476,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
     for (int b = 0; b < NCB; ++b) {
       frag hi, lo;
       {
-        const frag f = transposed(sV + Tile::value_t(b * KB, cb, ct, ln), Tile::VSTEP);
+        const frag f = transposed(sV + Tile::value_t(b * KB, cb, ln), Tile::VSTEP);
         const float* pw = sW + C - rows + b * KB + grp * EL;
 #pragma unroll
         for (int e = 0; e < EL; ++e) {
@@ -498,7 +503,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
       for (int a = 0; a < NKB * TPB; ++a) *reinterpret_cast<float4_t*>(dst + (a * 64 + lane) * 4) = S[a];
     } else if (p.final_state && last) {
       float* dst = p.final_state + ((int64_t)s * p.Hv + h) * p.dk * p.dv;
-      const int col = cb + Ops<T>::row(ct, r);
+      const int col = cb + r;
 #pragma unroll
       for (int a = 0; a < NKB * TPB; ++a)
 #pragma unroll
@@ -527,7 +532,7 @@ __global__ __launch_bounds__(256) void linear_join(LinearParams p) {
   if (p.initial) {
     const int lane = e / 4 % 64, a = e / 256 % (DK / 16), wave = e / (DK * 16);
     const float* src = p.initial + s * p.init_stride + (int64_t)h * p.dk * p.dv;
-    const int col = wave / TPB * KB + Ops<T>::row(wave % TPB, lane & 15);
+    const int col = wave * 16 + (lane & 15);
     for (int i = 0; i < 4; ++i) {
       const int row = a / TPB * KB + Ops<T>::row(a % TPB, 4 * (lane >> 4) + i);
       if (row < p.dk && col < p.dv) run[i] = src[row * p.dv + col];
