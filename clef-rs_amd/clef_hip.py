@@ -188,7 +188,7 @@ def _scratch(n, device):
 
 
 def _index(t, n, name):
-    if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
         raise ClefError(-1, f"{name} must be a contiguous int32 device tensor [{n}]")
 
 
@@ -684,6 +684,15 @@ def attention_gated_varlen(q, k, vt, gate, cu_seqlens, prefix_k=None, prefix_vt=
     return y
 
 
+def _keys(k, vt, d, dtype, name):
+    """(kv_heads, keys, value row) of contiguous keys [kv_heads, keys, d] and values [kv_heads, d, >= keys]."""
+    if k.dim() != 3 or vt.dim() != 3 or k.shape[2] != d or vt.shape[:2] != (k.shape[0], d):
+        raise ClefError(-1, f"{name} keys must be [kv_heads, keys, d] and values [kv_heads, d, keys]")
+    if k.dtype != dtype or vt.dtype != dtype or not k.is_contiguous() or not vt.is_contiguous():
+        raise ClefError(-1, f"{name} keys and values must be contiguous and of q's dtype")
+    return k.shape[0], k.shape[1], vt.shape[2]
+
+
 def attention_gated_shared(q, k, vt, gate, cu_seqlens, key_starts, key_lens, prefix_k=None, prefix_vt=None,
                            max_keys=None, out=None):
     """Requests of one to a few tokens behind one shared prefix, which is read once for
@@ -697,43 +706,38 @@ def attention_gated_shared(q, k, vt, gate, cu_seqlens, key_starts, key_lens, pre
     heads, T, d = q.shape
     nseq = cu_seqlens.numel() - 1
     _index(cu_seqlens, nseq + 1, "cu_seqlens")
-    if (prefix_k is None) != (prefix_vt is None) or (k is None) != (vt is None):
-        raise ClefError(-1, "keys and values come together")
-    if k is None and prefix_k is None:
-        raise ClefError(-1, "no keys: neither a prefix nor own keys")
-    kvh = (prefix_k if k is None else k).shape[0]
-    for name, a, b in (("prefix", prefix_k, prefix_vt), ("own", k, vt)):
-        if a is None:
-            continue
-        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != kvh or a.shape[2] != d or b.shape[:2] != (kvh, d):
-            raise ClefError(-1, f"{name} keys must be [kv_heads, keys, d] and values [kv_heads, d, keys]")
-        if a.dtype != q.dtype or b.dtype != q.dtype or not a.is_contiguous() or not b.is_contiguous():
-            raise ClefError(-1, f"{name} keys and values must be contiguous and of q's dtype")
-    np_ = 0 if prefix_k is None else prefix_k.shape[1]
-    rows, ldv = (0, 0) if k is None else (k.shape[1], vt.shape[2])
-    if k is not None:
+    kvh = np_ = rows = ldpv = ldv = 0
+    if prefix_k is not None and prefix_vt is not None:
+        kvh, np_, ldpv = _keys(prefix_k, prefix_vt, d, q.dtype, "prefix")
+    if k is not None and vt is not None:
+        own_kvh, rows, ldv = _keys(k, vt, d, q.dtype, "own")
+        if kvh and own_kvh != kvh:
+            raise ClefError(-1, "prefix and own keys must have the same heads")
+        kvh = own_kvh
         _index(key_starts, nseq, "key_starts")
         _index(key_lens, nseq, "key_lens")
+        _here(key_starts, k, vt, key_lens)
+    if (prefix_k is None) != (prefix_vt is None) or (k is None) != (vt is None) or not kvh:
+        raise ClefError(-1, "keys and values come together, of a prefix, of the requests or of both")
     max_keys = rows if max_keys is None else min(int(max_keys), rows)
-    if gate.dim() != 3 or gate.shape[:2] != (T, heads) or gate.shape[2] < d or gate.stride(2) != 1 or \
-            gate.dtype != q.dtype:
+    gs = gate.stride()
+    if len(gs) != 3 or gs[2] != 1 or gate.shape[:2] != (T, heads) or gate.shape[2] < d or gate.dtype != q.dtype:
         raise ClefError(-1, "gate must be a [T, heads, d] view of q's dtype")
     if out is None:
-        out = torch.empty((T, heads * d), dtype=q.dtype, device=q.device)
-    if out.shape != (T, heads * d) or out.stride(1) != 1 or out.dtype != q.dtype:
+        out = q.new_empty((T, heads * d))
+    elif out.shape != (T, heads * d) or out.stride(1) != 1 or out.dtype != q.dtype:
         raise ClefError(-1, "out must be [T, heads * d] rows of q's dtype")
-    _here(q, k, vt, gate, cu_seqlens, prefix_k, prefix_vt, out)
-    if k is not None:
-        _here(key_starts, key_lens)
-    n = lib().clef_attention_shared_workspace(T, nseq, np_, max_keys, _dt(q), heads, kvh, d)
+    _here(q, gate, cu_seqlens, out, prefix_k, prefix_vt)
+    dt = _dt(q)
+    L = lib()
+    n = L.clef_attention_shared_workspace(T, nseq, np_, max_keys, dt, heads, kvh, d)
     if n == 0:
         raise ClefError(-1, last_error())
-    ws = _scratch(n, q.device)
-    _check(lib().clef_attention_gated_shared(
-        _ptr(q), T, _ptr(prefix_k), np_, _ptr(prefix_vt), 0 if prefix_vt is None else prefix_vt.shape[2], np_,
-        _ptr(k), rows, _ptr(vt), ldv, _ptr(cu_seqlens), None if k is None else _ptr(key_starts),
-        None if k is None else _ptr(key_lens), nseq, T, max_keys, _dt(q), heads, kvh, d, _ptr(gate), gate.stride(0),
-        gate.stride(1), _ptr(out), out.stride(0), _ptr(ws), ws.numel(), _stream()))
+    ws = _scratch(n, q.device) if n > 256 else None  # 256: the call keeps nothing there
+    _check(L.clef_attention_gated_shared(
+        q.data_ptr(), T, _ptr(prefix_k), np_, _ptr(prefix_vt), ldpv, np_, _ptr(k), rows, _ptr(vt), ldv,
+        cu_seqlens.data_ptr(), _ptr(key_starts), _ptr(key_lens), nseq, T, max_keys, dt, heads, kvh, d,
+        gate.data_ptr(), gs[0], gs[1], out.data_ptr(), out.stride(0), _ptr(ws), n if ws is not None else 0, _stream()))
     return out
 
 

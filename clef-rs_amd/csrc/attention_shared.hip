@@ -37,6 +37,8 @@ constexpr int kMaxSeq = 4096;
 constexpr int kMaxKeys = 1 << 24;
 constexpr int kMaxParts = 64;  // of a row over the prefix, and over its own keys
 constexpr int kJoinRows = 8;     // rows of a joining work-group
+constexpr int kOwnKeys = 1024;   // own keys that the joining launch takes itself
+constexpr size_t kNoWorkspace = 256;  // said of calls that keep nothing there
 
 struct SharedParams {
   const void* q;           // [heads][ldq][d]
@@ -541,13 +543,14 @@ __global__ __launch_bounds__(256) void shared_own(SharedParams p) {
   }
 }
 
-// The outputs of one token's rows of one key head (8 of them at a time): waves
+// The outputs of one token's rows of one key head (8 of them at a time).  Waves
 // 0 to 3 take the own keys (unless they are among the parts), waves 4 to 7 meanwhile
-// weigh and add the parts, one row to each group of 32 lanes.
-template <class T, int D, bool FULL>
+// weigh and add the parts, one row to each group of 32 lanes.  WALK: no parts; all
+// eight waves take the keys of a short prefix and the own ones, in this one launch.
+template <class T, int D, bool FULL, bool WALK>
 __global__ __launch_bounds__(512) void shared_join(SharedParams p) {
   constexpr int KB = Ops<T>::KB, R = kJoinRows, F = D / 32;  // features of a lane
-  __shared__ Joined<D, 5, kJoinRows> part;
+  __shared__ Joined<D, WALK ? 8 : 5, kJoinRows> part;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.heads / p.kvh, tiles = (G + R - 1) / R;
   const int at = blockIdx.x;
@@ -565,14 +568,23 @@ __global__ __launch_bounds__(512) void shared_join(SharedParams p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) gate[j] = gp[j];
   }
-  if (wave < 4) {
+  if (WALK || wave < 4) {
     int first = 0, count = 0;
     if (!p.osplits) own_span(p, s, t, first, count);
     typename Ops<T>::frag fq[D / KB][1];
     load_queries<T, D, 1, FULL>(p, fq, kv, t * G + g0, t * G + g0 + rows, lane);
     Soft<T, D, 1> st;
     st.clear();
-    take_keys<T, D, 1, FULL>(st, fq, p.k, p.ldk, p.vt, p.ldv, kv, first, first + count, p.d, p.c, wave, 4, lane);
+    if constexpr (WALK) {
+      // the own keys' blocks go on where the prefix's end
+#pragma unroll 1
+      for (int own = 0; own < 2; ++own)
+        take_keys<T, D, 1, FULL>(st, fq, own ? p.k : p.pk, own ? p.ldk : p.ldpk, own ? p.vt : p.pvt,
+                                 own ? p.ldv : p.ldpv, kv, own ? first : 0, own ? first + count : p.np, p.d, p.c,
+                                 own ? (wave - (p.np + KB - 1) / KB) & 7 : wave, 8, lane);
+    } else {
+      take_keys<T, D, 1, FULL>(st, fq, p.k, p.ldk, p.vt, p.ldv, kv, first, first + count, p.d, p.c, wave, 4, lane);
+    }
     part.put(st, 0, wave, lane, rows);
   } else if (const int y = (tid - 256) / 32; y < rows) {
     const int a = tid % 32;
@@ -595,8 +607,9 @@ __global__ __launch_bounds__(512) void shared_join(SharedParams p) {
       l = fmaf(w.y, f, l);
       o += *reinterpret_cast<const vec*>(src + n * step * D) * f;
     }
-    *reinterpret_cast<vec*>(&part.o[4][y][a * F]) = o;
-    if (a == 0) part.ml[4][y] = float2{m, l};
+    constexpr int at = WALK ? 0 : 4;  // (WALK: never here)
+    *reinterpret_cast<vec*>(&part.o[at][y][a * F]) = o;
+    if (a == 0) part.ml[at][y] = float2{m, l};
   }
   lds_barrier();
   if (!mine) return;
@@ -612,6 +625,7 @@ int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 // How the work is split, from the shapes alone (the workspace follows from it).
 struct Plan {
+  bool walk;  // one launch
   bool many;  // 128 rows to a work-group
   int tile;   // rows of a work-group otherwise
   int psplits, pkeys, osplits, okeys;
@@ -620,6 +634,12 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
   Plan x{};
   const int64_t rows = (int64_t)T * (heads / kvh);
   const int cus = device_cus();
+  // At most one block of the prefix to a wave: one launch of 8 waves per token and
+  // key head, which read the prefix for themselves.  (A block takes a CU about 5 us,
+  // most of it the 256 KiB that its waves read: 2 requests behind 512 keys, two
+  // blocks to a wave, took 20.7 us so and 12.4 us in parts.)
+  x.walk = np <= 8 * (dtype == CLEF_F16 ? Ops<half_t>::KB : Ops<float>::KB) && max_keys <= kOwnKeys;
+  if (x.walk) return x;
   x.many = dtype == CLEF_F16 && rows > 32 && d == padded(d);
   x.tile = rows > 16 ? 32 : 16;
   // splits until the chip is full (many rows: one work-group to a CU), but not so
@@ -634,7 +654,7 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
   };
   const int tile = x.many ? 128 : x.tile;
   if (np) split(np, (rows + tile - 1) / tile * kvh, x.many ? cus : 2 * cus, x.many ? 256 : 64, kMaxParts, x.psplits, x.pkeys);
-  if (max_keys > 1024) split(max_keys, (int64_t)T * kvh, 2 * cus, 512, kMaxParts, x.osplits, x.okeys);
+  if (max_keys > kOwnKeys) split(max_keys, (int64_t)T * kvh, 2 * cus, 512, kMaxParts, x.osplits, x.okeys);
   return x;
 }
 
@@ -659,7 +679,8 @@ int launch(const SharedParams& p, const Plan& x, hipStream_t st) {
   const unsigned own = (unsigned)p.T * p.kvh * tiles;
   if (x.osplits) hipLaunchKernelGGL((shared_own<T, D, FULL>), dim3(own * x.osplits), dim3(256), 0, st, p);
   const unsigned join = (unsigned)p.T * p.kvh * ((G + kJoinRows - 1) / kJoinRows);
-  hipLaunchKernelGGL((shared_join<T, D, FULL>), dim3(join), dim3(512), 0, st, p);
+  if (x.walk) hipLaunchKernelGGL((shared_join<T, D, FULL, true>), dim3(join), dim3(512), 0, st, p);
+  else hipLaunchKernelGGL((shared_join<T, D, FULL, false>), dim3(join), dim3(512), 0, st, p);
   return check_launch("shared-prefix attention");
 }
 
@@ -689,6 +710,7 @@ int shared_dims(int T, int nseq, int np, int max_keys, int dtype, int heads, int
 
 size_t workspace_bytes(int T, int nseq, int np, int max_keys, int dtype, int heads, int kv_heads, int d) {
   const Plan x = plan_of(T, np, max_keys, dtype, heads, kv_heads, d);
+  if (x.walk) return kNoWorkspace;
   const size_t rows = (size_t)(x.psplits + x.osplits) * T * heads;
   return rows * padded(d) * 4 + rows * sizeof(float2) + 256;
 }
@@ -725,7 +747,8 @@ extern "C" int clef_attention_gated_shared(
   CLEF_REQUIRE(!misaligned(q) && !(np && (misaligned(prefix_k) || misaligned(prefix_vt))) &&
                    !(max_keys && (misaligned(k) || misaligned(vt))),
                "shared-prefix attention: q, keys and values must be 16-byte aligned");
-  CLEF_REQUIRE(workspace && workspace_bytes >= clef::workspace_bytes(T, nseq, np, max_keys, dtype, heads, kv_heads, d) &&
+  const size_t need = clef::workspace_bytes(T, nseq, np, max_keys, dtype, heads, kv_heads, d);
+  CLEF_REQUIRE((need == clef::kNoWorkspace || (workspace && workspace_bytes >= need)) &&
                    !(reinterpret_cast<uintptr_t>(workspace) & 255),
                "shared-prefix attention: workspace too small or not 256-byte aligned");
   clef::SharedParams p{};

@@ -419,7 +419,8 @@ int clef_attention_gated_varlen(const void* q, int64_t ldq_tok, const void* k, i
  * np and max_keys up to 2^24, not both 0 (0: the buffers may be NULL); q, keys
  * and values 16-byte aligned, ldpv_tok and ldv_tok multiples of 8.  A table
  * that does not fit gives unspecified values, never an access out of bounds.
- * workspace: clef_attention_shared_workspace bytes, 256-byte aligned.  No
+ * workspace: clef_attention_shared_workspace bytes, 256-byte aligned; where that
+ * is 256 (short prefixes), nothing is kept there and workspace may be NULL.  No
  * counterpart in the reference (one request per flash-attention call there).
  */
 size_t clef_attention_shared_workspace(int T, int nseq, int np, int max_keys, int dtype, int heads, int kv_heads,

@@ -119,6 +119,12 @@ CASES = [
     (12, 1, 256, 130, [3] * 11, [3] * 11),
     (32, 1, 64, 700, [1, 2], [300, 2]),
     (2, 2, 248, 129, [70], [90]),
+    (8, 1, 256, 1500, [1], [5]),
+    (16, 2, 256, 513, [1, 1], [20, 3]),
+    (2, 1, 128, 3001, [2, 1], [9, 40]),
+    (4, 2, 64, 600, [1, 2, 1], [1500, 1100, 1]),
+    (24, 1, 128, 530, [1, 1], [1200, 33]),
+    (20, 1, 64, 40, [1, 3], [1, 100]),
 ]
 
 

@@ -70,7 +70,7 @@ def test_steps_refuse(L, kind, bad):
 
 
 def shared(**kw):
-    a = dict(q=256, ldq=9, pk=256, ldpk=100, pvt=256, ldpv=104, np=100, k=256, ldk=300, vt=256, ldv=304, cu=256,
+    a = dict(q=256, ldq=9, pk=256, ldpk=1000, pvt=256, ldpv=1000, np=999, k=256, ldk=300, vt=256, ldv=304, cu=256,
              starts=256, lens=256, nseq=4, T=9, max_keys=50, dt=1, heads=8, kvh=2, d=64, gate=256, ldg=512, hsg=64,
              y=256, ldy=512, ws=256, wsb=1 << 40)
     assert set(kw) <= set(a)
@@ -81,7 +81,7 @@ def shared(**kw):
 @pytest.mark.parametrize("bad", [
     dict(q=None), dict(gate=None), dict(y=None), dict(cu=None), dict(pk=None), dict(pvt=None), dict(k=None),
     dict(vt=None), dict(starts=None), dict(lens=None), dict(ws=None), dict(wsb=0), dict(ws=264), dict(ldq=8),
-    dict(ldpk=99), dict(ldpv=96), dict(ldpv=105), dict(ldv=303), dict(ldk=0), dict(ldv=0), dict(ldk=1 << 31),
+    dict(ldpk=998), dict(ldpv=992), dict(ldpv=1001), dict(ldv=303), dict(ldk=0), dict(ldv=0), dict(ldk=1 << 31),
     dict(ldv=1 << 31), dict(nseq=0), dict(nseq=4097), dict(T=0), dict(T=65537), dict(np=-1), dict(np=(1 << 24) + 1),
     dict(max_keys=-1), dict(max_keys=(1 << 24) + 1), dict(np=0, max_keys=0), dict(dt=2), dict(heads=0), dict(heads=257),
     dict(kvh=0), dict(kvh=3), dict(d=0), dict(d=60), dict(d=264), dict(hsg=63), dict(ldg=511), dict(ldy=511),
@@ -96,8 +96,8 @@ def test_shared_attention_workspace(L):
     assert L.clef_attention_shared_workspace(0, 1, 8, 8, 1, 8, 2, 64) == 0
     assert L.clef_attention_shared_workspace(4, 1, 0, 0, 1, 8, 2, 64) == 0
     assert L.clef_attention_shared_workspace(4, 1, 8, 8, 1, 8, 2, 65) == 0
-    n = L.clef_attention_shared_workspace(9, 4, 100, 50, 1, 8, 2, 64)
-    assert n > 0 and L.clef_attention_gated_shared(*shared(wsb=n - 1)) < 0
+    n = L.clef_attention_shared_workspace(9, 4, 999, 50, 1, 8, 2, 64)
+    assert n > 256 and L.clef_attention_gated_shared(*shared(wsb=n - 1)) < 0
 
 
 def test_binding_refuses_host_tensors_and_shapes():
