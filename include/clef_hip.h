@@ -144,7 +144,8 @@ int clef_delta_scan_varlen(const void* q, const void* k, const void* v, int64_t 
  * whose linear layers are gated DeltaNet.
  * q, k: [T, Hk, dk] (token strides sqk, dtype_qkv); v: [T, Hv, dv] (token
  * stride sv, dtype_qkv); g: [Hv] f32 log-decays (<= 0; -infinity forgets all);
- * out: [T, Hv, dv] (token stride so, dtype_out).  initial: [Hv, dk, dv] f32 or
+ * out: [T, Hv, dv] (token stride so, dtype_out; apart from the inputs, here and
+ * below).  initial: [Hv, dk, dv] f32 or
  * NULL (zero state); final_state [Hv, dk, dv] f32 or NULL receives the state
  * after token T; the two may not overlap.
  * CLEF_F32 inputs are multiplied in f32 (f32 MFMA).  CLEF_F16 inputs are

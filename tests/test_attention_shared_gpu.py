@@ -273,3 +273,28 @@ def test_two_streams_at_once(clef):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+@gpu
+@pytest.mark.parametrize("many", [True, False])
+def test_offsets_past_32_bits(clef, many):
+    """Prefix values of a key head over 2^32 bytes, and own keys behind 2^31 elements of the cache."""
+    heads, d, prefix, own = (40 if many else 8), 64, 600, 70
+    b = _batch(F16, heads, 1, d, prefix, [1], [own], gap=0)
+    args = b.cuda()
+    rows = (1 << 25) + 512
+    free = torch.cuda.mem_get_info()[0]
+    if free < 16 << 30:
+        pytest.skip("needs 16 GiB of device memory")
+    big_pvt = torch.empty((1, d, 1 << 25), dtype=F16, device="cuda")
+    big_pvt[:, :, :prefix] = args["prefix_vt"][:, :, :prefix]
+    k = torch.empty((1, rows, d), dtype=F16, device="cuda")
+    vt = torch.empty((1, d, rows), dtype=F16, device="cuda")
+    at = rows - own - 1
+    k[:, at:at + own] = args["k"][:, b.starts[0]:b.starts[0] + own]
+    vt[:, :, at:at + own] = args["vt"][:, :, b.starts[0]:b.starts[0] + own]
+    vt[:, :, at + own:] = float("nan")
+    y = clef.attention_gated_shared(args["q"], k, vt, args["gate"], args["cu_seqlens"],
+                                    torch.tensor([at], dtype=torch.int32, device="cuda"), args["key_lens"],
+                                    prefix_k=args["prefix_k"], prefix_vt=big_pvt, max_keys=128)
+    b.check(y)

@@ -262,6 +262,23 @@ def test_long_prompt_tail(clef):
     assert ((final.double().cpu() - ef).abs() <= 2.0 ** -14 * mf).all()
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_offsets_past_32_bits(clef, dtype):
+    """Token strides of 2^23 elements: 600 tokens reach past 2^32."""
+    T, H, d, stride = 600, 1, 64, 1 << 23
+    if torch.cuda.mem_get_info()[0] < 32 << 30:
+        pytest.skip("needs 32 GiB of device memory")
+    q, k, v = _inputs(8, T, H, H, d, d, dtype)
+    flat = torch.empty((T - 1) * stride + 4 * d, dtype=dtype, device="cuda")
+    views = [torch.as_strided(flat, (T, H, d), (stride, d, 1), i * d) for i in range(4)]
+    for x, y in zip(views, (q, k, v)):
+        x.copy_(y)
+    g = _slopes(H)
+    _, final = clef.LinearScan(d, d).prefill(*views[:3], g.cuda(), out=views[3])
+    check(views[3], final, q, k, v, g, d ** -0.5)
+
+
 # ---------------------------------------------------------------------------- single tokens
 def step_reference(kind, q, k, v, g, beta, slots, states, new, scale):
     """Row after row; returns (out of the live rows, new states, and both over absolute values)."""
@@ -377,6 +394,31 @@ def test_step_rows_of_one_request(clef, in_place, kind):
 def test_step_many_rows(clef, kind):
     run_step(clef, kind, F16, 1500, 1, 1, 16, 8)
     run_step(clef, kind, F16, 600, 1, 2, 128, 128, slots=[(7 * i) % 601 for i in range(600)], nslots=601)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["delta", "linear"])
+def test_step_pool_past_32_bits(clef, kind):
+    """States behind 2^31 elements of the pool, in place."""
+    Hv, d, n = 32, 128, 4098
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GiB of device memory")
+    pool = torch.empty((n, Hv, d, d), device="cuda")
+    slots = [n - 1, 5, n - 2]
+    old = _randn(1, 3, Hv, d, d)
+    for i, s in enumerate(slots):
+        pool[s] = old[i].cuda()
+    q, k, v = _inputs(3, 3, 16, Hv, d, d, F32)
+    g = _slopes(Hv) if kind == "linear" else -_randn(8, 3, Hv).abs()
+    beta = torch.sigmoid(_randn(7, 3, Hv))
+    scan = clef.DeltaScan(d, d) if kind == "delta" else clef.LinearScan(d, d)
+    args = _cuda(q, k, v, g) + ([beta.cuda()] if kind == "delta" else [])
+    out = scan.step(*args, pool, slots=torch.tensor(slots, dtype=torch.int32, device="cuda"))
+    eo, en, mo, mn = step_reference(kind, q, k, v, g, beta, None, old, old, d ** -0.5)
+    sums = (2 * d + 24) * 2.0 ** -24
+    assert ((out.double().cpu() - eo).abs() <= sums * mo).all()
+    for i, s in enumerate(slots):
+        assert ((pool[s].double().cpu() - en[i]).abs() <= sums * mn[i]).all()
 
 
 @gpu
