@@ -59,7 +59,7 @@ struct LinearParams {
   int T, nseq, Hk, Hv, dk, dv;
   int unit;              // tokens of a unit, a multiple of C
   int nunits;            // at most T / unit + nseq
-  int vec_qk, vec_v, vec_out;  // 16-byte accesses allowed
+  int wide, whole, vec_out;  // 16-byte accesses to the inputs; to whole tiles of them; to out
   float scale;
 };
 
@@ -175,48 +175,55 @@ __device__ __forceinline__ float log2_decay(float g) {
   return x < -1e30f ? -1e30f : x;
 }
 
-// 64 rows of a [rows][W] tile in registers, 16 bytes at a time, zeros behind
-// `rows` and `width`.
+// 64 rows of a [rows][W] tile in registers, 16 bytes at a time; src, stride,
+// rows and width are the wave's.  The loads of a chunk's tiles stand in one branch
+// each of three (whole, wide, any): with a choice per tile the compiler waits for
+// one tile's loads before it issues the next one's (3,300 of a chunk's 13,900 cycles).
 template <class T, int W, int THREADS>
 struct Staged {
   static constexpr int EL = 16 / sizeof(T), VPR = W / EL, N = C * VPR / THREADS;
+  static constexpr int STEP = THREADS / VPR;  // rows between a thread's vectors
   static_assert(C * VPR % THREADS == 0 && THREADS % VPR == 0, "whole vectors and rows per thread");
   typedef typename Ops<T>::frag vec;
   static_assert(sizeof(vec) == 16, "16-byte vectors");
   vec x[N];
 
-  // src, stride, rows and width are the wave's
-  __device__ __forceinline__ void load(const T* src, int64_t stride, int rows, int width, bool wide, int tid) {
-    constexpr int STEP = THREADS / VPR;  // rows between a thread's vectors
-    if (wide && rows == C && width == W && stride < (int64_t(1) << 22)) {
-      // a whole tile: one 32-bit offset from addresses that the wave shares
-      const uint32_t off = (uint32_t)(tid / VPR) * (uint32_t)stride + tid % VPR * EL;
+  // a whole tile of aligned rows, stride below 2^22: one 32-bit offset from
+  // addresses that the wave shares
+  __device__ __forceinline__ void load_whole(const T* src, int64_t stride, int tid) {
+    const uint32_t off = (uint32_t)(tid / VPR) * (uint32_t)stride + tid % VPR * EL;
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const vec*>(src + i * STEP * stride + off);
-      return;
-    }
+    for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const vec*>(src + i * STEP * stride + off);
+  }
+  // aligned rows of whole vectors: what lies behind `rows` and `width` is read from
+  // the tile's last row and vector, and left out when it is stored
+  __device__ __forceinline__ void load_wide(const T* src, int64_t stride, int rows, int width, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      x[i] = *reinterpret_cast<const vec*>(src + min(tid / VPR + i * STEP, rows - 1) * stride +
+                                           min(tid % VPR * EL, width - EL));
+  }
+  // rows at any alignment: value by value
+  __device__ __forceinline__ void load_any(const T* src, int64_t stride, int rows, int width, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = tid + i * THREADS, r = at / VPR, c = at % VPR * EL;
+      const int r = tid / VPR + i * STEP, c = tid % VPR * EL;
       vec y = {};
-      if (r < rows) {
-        if (wide) {
-          if (c < width) y = *reinterpret_cast<const vec*>(src + r * stride + c);
-        } else {
 #pragma unroll
-          for (int e = 0; e < EL; ++e)
-            if (c + e < width) y[e] = src[r * stride + c + e];
-        }
-      }
+      for (int e = 0; e < EL; ++e)
+        if (r < rows && c + e < width) y[e] = src[r * stride + c + e];
       x[i] = y;
     }
   }
-  template <class At>  // at(row, column): the vector's place in the tile
-  __device__ __forceinline__ void store(T* tile, int tid, At place) const {
+  // place(row, column): the vector's place in the tile; cut: zeros behind `rows` and `width`
+  template <class At>
+  __device__ __forceinline__ void store(T* tile, int tid, bool cut, int rows, int width, At place) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = tid + i * THREADS;
-      *reinterpret_cast<vec*>(tile + place(at / VPR, at % VPR * EL)) = x[i];
+      const int r = tid / VPR + i * STEP, c = tid % VPR * EL;
+      vec y = x[i];
+      if (cut && (r >= rows || c >= width)) y = vec{};
+      *reinterpret_cast<vec*>(tile + place(r, c)) = y;
     }
   }
 };
@@ -294,9 +301,20 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
   Staged<T, DV, THREADS> rv;
   auto fetch = [&](int t, int tid) {
     const int rows = min(C, end - t);
-    if (OUT) rq.load(q + t * p.sqk, p.sqk, rows, p.dk, p.vec_qk, tid);
-    rk.load(k + t * p.sqk, p.sqk, rows, p.dk, p.vec_qk, tid);
-    rv.load(v + t * p.sv, p.sv, rows, p.dv, p.vec_v, tid);
+    const T *qt = q + t * p.sqk, *kt = k + t * p.sqk, *vt = v + t * p.sv;
+    if (p.whole && rows == C) {
+      if (OUT) rq.load_whole(qt, p.sqk, tid);
+      rk.load_whole(kt, p.sqk, tid);
+      rv.load_whole(vt, p.sv, tid);
+    } else if (p.wide) {
+      if (OUT) rq.load_wide(qt, p.sqk, rows, p.dk, tid);
+      rk.load_wide(kt, p.sqk, rows, p.dk, tid);
+      rv.load_wide(vt, p.sv, rows, p.dv, tid);
+    } else {
+      if (OUT) rq.load_any(qt, p.sqk, rows, p.dk, tid);
+      rk.load_any(kt, p.sqk, rows, p.dk, tid);
+      rv.load_any(vt, p.sv, rows, p.dv, tid);
+    }
   };
   if (begin < end) fetch(begin, tid);
 
@@ -330,9 +348,10 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
     int ln = lane, at = tid;
     asm("" : "+v"(ln), "+v"(at));
     const int r = ln & 15, grp = ln >> 4;
-    if (OUT) rq.store(sQ, at, [](int row, int col) { return row * PQ + col; });
-    rk.store(sK, at, [](int row, int col) { return Tile::key(row, col); });
-    rv.store(sV, at, [](int row, int col) { return Tile::value(row, col); });
+    const bool cut = !(p.whole && rows == C);
+    if (OUT) rq.store(sQ, at, cut, rows, p.dk, [](int row, int col) { return row * PQ + col; });
+    rk.store(sK, at, cut, rows, p.dk, [](int row, int col) { return Tile::key(row, col); });
+    rv.store(sV, at, cut, rows, p.dv, [](int row, int col) { return Tile::value(row, col); });
     lds_barrier();
     if (t + C < end) fetch(t + C, at);
 
@@ -631,12 +650,10 @@ int linear_scan(const void* q, const void* k, const void* v, int64_t sqk, int64_
   p.unit = unit_tokens(T, Hv, dtype_qkv);
   p.nunits = (cu_seqlens ? T / p.unit : (T + p.unit - 1) / p.unit - 1) + nseq;
   p.enter = static_cast<float*>(workspace);
-  auto wide = [](const void* x, int64_t stride, int width, int dtype) {
-    const int el = dtype == CLEF_F16 ? 8 : 4;
-    return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && stride % el == 0 && width % el == 0;
-  };
-  p.vec_qk = wide(q, sqk, dk, dtype_qkv) && wide(k, sqk, dk, dtype_qkv);
-  p.vec_v = wide(v, sv, dv, dtype_qkv);
+  const int el = dtype_qkv == CLEF_F16 ? 8 : 4;
+  p.wide = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0 &&
+           sqk % el == 0 && sv % el == 0 && dk % el == 0 && dv % el == 0;
+  p.whole = p.wide && dk == padded(dk) && dv == padded(dv) && sqk < (int64_t(1) << 22) && sv < (int64_t(1) << 22);
   p.vec_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && so % 4 == 0 && dv % 4 == 0;
   if (dtype_qkv == CLEF_F16)
     return dtype_out == CLEF_F16 ? launch_widths<half_t, half_t>(p, st) : launch_widths<half_t, float>(p, st);
