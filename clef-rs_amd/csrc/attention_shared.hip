@@ -640,7 +640,10 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
   // blocks to a wave, took 20.7 us so and 12.4 us in parts.)
   x.walk = np <= 8 * (dtype == CLEF_F16 ? Ops<half_t>::KB : Ops<float>::KB) && max_keys <= kOwnKeys;
   if (x.walk) return x;
-  x.many = dtype == CLEF_F16 && rows > 32 && d == padded(d);
+  // 24 rows of a key head behind 8,192 and 32,768 keys take 28 and 42 us with the
+  // 128-row groups and took 33 and 50 with 32-row ones; 16 rows behind 32,768 keys
+  // take 38 us with 16-row ones.
+  x.many = dtype == CLEF_F16 && rows > 16 && d == padded(d);
   x.tile = rows > 16 ? 32 : 16;
   // splits until the chip is full (many rows: one work-group to a CU), but not so
   // short that the parts cost more than they save: 32 requests behind 4,096 keys at
