@@ -9,9 +9,10 @@
 // sum_p e^{m_p - M} O_p / sum_p e^{m_p - M} l_p.  So the queries of all requests
 // are stacked as rows of one product against the prefix (rows (token, head) of
 // one key head), which is read once per 128 rows instead of once per request,
-// its keys split over work-groups until the chip is full; and a second launch
-// takes each request's own keys and joins the parts, per token.  4 d flops per
-// (row, key): few rows are bound by the keys' bytes, many by MFMA.
+// its keys split over work-groups until the chip is full.  Each request's own
+// keys are further parts, of further work-groups of that launch, or are taken by
+// the second launch, which joins the parts of a row.  4 d flops per (row, key):
+// few rows are bound by the keys' bytes, many by MFMA.
 //
 // Scores are formed transposed (K Q^T), so a lane holds one query and several
 // keys of a tile, its row maximum and sum are per-lane values, and the
@@ -36,8 +37,8 @@ namespace {
 constexpr int kMaxSeq = 4096;
 constexpr int kMaxKeys = 1 << 24;
 constexpr int kMaxParts = 64;  // of a row over the prefix, and over its own keys
-constexpr int kJoinRows = 8;     // rows of a joining work-group
-constexpr int kOwnKeys = 1024;   // own keys that the joining launch takes itself
+constexpr int kFinishRows = 8;     // rows of a work-group that takes own keys and finishes
+constexpr int kFinishKeys = 1024;  // own keys of a request there
 constexpr size_t kNoWorkspace = 256;  // said of calls that keep nothing there
 
 struct SharedParams {
@@ -54,7 +55,8 @@ struct SharedParams {
   float* part;             // [psplits + osplits][T * heads][D]
   float2* ml;              // [psplits + osplits][T * heads] {m, l}
   int psplits, pkeys;      // prefix parts and the keys of each
-  int osplits, okeys;      // parts of the own keys (0: taken by the joining launch)
+  int osplits, okeys;      // parts of the own keys
+  int pgroups;             // work-groups of the prefix
 };
 
 // as in the linear scan: fragments of KB k-indices (EL per lane), TPB tiles of
@@ -286,15 +288,63 @@ struct Joined {
   }
 };
 
-// Part of the prefix for RT * 16 stacked rows: keys split over the four waves.
+// four features of one output: their gate, and the output itself
+template <class T>
+__device__ __forceinline__ void load_gate(const SharedParams& p, T (&gate)[4], int t, int h, int e) {
+  const T* gp = static_cast<const T*>(p.gate) + t * p.ldg + h * p.hsg + e;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) gate[j] = gp[j];
+}
+template <class T>
+__device__ __forceinline__ void finish(const SharedParams& p, const T (&gate)[4], float4_t o, float l, int t, int h, int e) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+  T* y = static_cast<T*>(p.y) + t * p.ldy + (int64_t)h * p.d + e;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y[j] = cvt_out<T>(o[j] * inv * sigmoid(to_f32(gate[j])));
+}
+
+// Part `split` of the own keys of one token's rows of one key head (16 of them at a
+// time), the keys split over a work-group's NW waves.
+template <class T, int D, bool FULL, int NW>
+__device__ __forceinline__ void own_part(const SharedParams& p, int group, Joined<D, NW, 16>& part, int tid, int lane,
+                                         int wave) {
+  constexpr int KB = Ops<T>::KB;
+  const int G = p.heads / p.kvh, tiles = (G + 15) / 16;
+  const int split = group % p.osplits, at = group / p.osplits;
+  const int g0 = at % tiles * 16, kv = at / tiles % p.kvh, t = at / tiles / p.kvh;
+  const int s = __builtin_amdgcn_readfirstlane(seq_of(p, t, lane));
+  if (s < 0) return;
+  int first, count;
+  own_span(p, s, t, first, count);
+  const int k0 = split * p.okeys, k1 = min(count, k0 + p.okeys), rows = min(16, G - g0);
+  typename Ops<T>::frag fq[D / KB][1];
+  load_queries<T, D, 1, FULL>(p, fq, kv, t * G + g0, t * G + g0 + rows, lane);
+  Soft<T, D, 1> st;
+  st.clear();
+  take_keys<T, D, 1, FULL>(st, fq, p.k, p.ldk, p.vt, p.ldv, kv, first + k0, first + k1, p.d, p.c, wave, NW, lane);
+  part.put(st, 0, wave, lane, rows);
+  lds_barrier();
+  const int64_t to = ((int64_t)(p.psplits + split) * p.T + t) * p.heads + kv * G + g0;
+  for (int i = tid; i < rows * (D / 4); i += 64 * NW) {
+    const int x = i / (D / 4), e = i % (D / 4) * 4;
+    float m, l;
+    *reinterpret_cast<float4_t*>(p.part + (to + x) * D + e) = part.take(x, e, m, l);
+    if (e == 0) p.ml[to + x] = float2{m, l};
+  }
+}
+
+// Part of the prefix for RT * 16 stacked rows, keys split over the four waves; the
+// work-groups behind those of the prefix take the own keys.
 template <class T, int D, int RT, bool FULL>
 __global__ __launch_bounds__(256) void shared_few_rows(SharedParams p) {
   constexpr int KB = Ops<T>::KB;
   __shared__ Joined<D, 4, 16> part;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = blockIdx.x;
+  if (group >= p.pgroups) return own_part<T, D, FULL, 4>(p, group - p.pgroups, part, tid, lane, wave);
   const int G = p.heads / p.kvh, rows = p.T * G;
-  const int split = blockIdx.x % p.psplits, kv = blockIdx.x / p.psplits % p.kvh;
-  const int row0 = blockIdx.x / p.psplits / p.kvh * (RT * 16);
+  const int split = group % p.psplits, kv = group / p.psplits % p.kvh;
+  const int row0 = group / p.psplits / p.kvh * (RT * 16);
   const int k0 = split * p.pkeys, k1 = min(k0 + p.pkeys, p.np);
   typename Ops<T>::frag fq[D / KB][RT];
   load_queries<T, D, RT, FULL>(p, fq, kv, row0, rows, lane);
@@ -319,7 +369,7 @@ __global__ __launch_bounds__(256) void shared_few_rows(SharedParams p) {
   }
 }
 
-// Part of the prefix for 128 stacked rows (f16, d = D): eight waves of 16 rows,
+// The same for 128 stacked rows (f16, d = D): eight waves of 16 rows,
 // two to a SIMD, so that one's exponentials run under the other's products.
 // Tiles of 64 keys pass through LDS by DMA, double-buffered; 16-byte slots are
 // permuted by their row (XOR), so that the 16 rows of an operand, which are
@@ -345,13 +395,18 @@ __global__ __launch_bounds__(512, 2) void shared_many_rows(SharedParams p) {
   constexpr int BK = 64, KB = 32, EL = 8, KS = D / 8;
   constexpr int NDMA = D / 64;     // DMA instructions per wave, operand and tile
   constexpr int KROWS = 512 / D;   // key rows of one
-  __shared__ __attribute__((aligned(1024))) T sK[2][BK * D];
-  __shared__ __attribute__((aligned(1024))) T sV[2][D * BK];
+  constexpr int TILES = 4 * BK * D * (int)sizeof(T), OWN = (int)sizeof(Joined<D, 8, 16>);
+  __shared__ __attribute__((aligned(1024))) char lds[TILES > OWN ? TILES : OWN];
+  T(*sK)[BK * D] = reinterpret_cast<T(*)[BK * D]>(lds);
+  T(*sV)[D * BK] = reinterpret_cast<T(*)[D * BK]>(lds + TILES / 2);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, grp = lane >> 4;
+  const int group = blockIdx.x;
+  if (group >= p.pgroups)
+    return own_part<T, D, true, 8>(p, group - p.pgroups, *reinterpret_cast<Joined<D, 8, 16>*>(lds), tid, lane, wave);
   const int G = p.heads / p.kvh, rows = p.T * G;
-  const int split = blockIdx.x % p.psplits, kv = blockIdx.x / p.psplits % p.kvh;
-  const int row0 = blockIdx.x / p.psplits / p.kvh * 128 + 16 * wave;
+  const int split = group % p.psplits, kv = group / p.psplits % p.kvh;
+  const int row0 = group / p.psplits / p.kvh * 128 + 16 * wave;
   const int k0 = split * p.pkeys, k1 = min(k0 + p.pkeys, p.np);
   const T* K = static_cast<const T*>(p.pk) + (int64_t)kv * p.ldpk * D;
   const T* V = static_cast<const T*>(p.pvt) + (int64_t)kv * D * p.ldpv;
@@ -512,45 +567,14 @@ __global__ __launch_bounds__(512, 2) void shared_many_rows(SharedParams p) {
   for (int e = 0; e < D / 16; ++e) *reinterpret_cast<float4_t*>(p.part + to * D + e * 16 + grp * 4) = o[e];
 }
 
-// Part `split` of the own keys of one token's rows of one key head (16 of them
-// at a time), the keys split over the four waves.
-template <class T, int D, bool FULL>
-__global__ __launch_bounds__(256) void shared_own(SharedParams p) {
-  constexpr int KB = Ops<T>::KB;
-  __shared__ Joined<D, 4, 16> part;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int G = p.heads / p.kvh, tiles = (G + 15) / 16;
-  const int split = blockIdx.x % p.osplits, at = blockIdx.x / p.osplits;
-  const int g0 = at % tiles * 16, kv = at / tiles % p.kvh, t = at / tiles / p.kvh;
-  const int s = __builtin_amdgcn_readfirstlane(seq_of(p, t, lane));
-  if (s < 0) return;
-  int first, count;
-  own_span(p, s, t, first, count);
-  const int k0 = split * p.okeys, k1 = min(count, k0 + p.okeys), rows = min(16, G - g0);
-  typename Ops<T>::frag fq[D / KB][1];
-  load_queries<T, D, 1, FULL>(p, fq, kv, t * G + g0, t * G + g0 + rows, lane);
-  Soft<T, D, 1> st;
-  st.clear();
-  take_keys<T, D, 1, FULL>(st, fq, p.k, p.ldk, p.vt, p.ldv, kv, first + k0, first + k1, p.d, p.c, wave, 4, lane);
-  part.put(st, 0, wave, lane, rows);
-  lds_barrier();
-  const int64_t to = ((int64_t)(p.psplits + split) * p.T + t) * p.heads + kv * G + g0;
-  for (int i = tid; i < rows * (D / 4); i += 256) {
-    const int x = i / (D / 4), e = i % (D / 4) * 4;
-    float m, l;
-    *reinterpret_cast<float4_t*>(p.part + (to + x) * D + e) = part.take(x, e, m, l);
-    if (e == 0) p.ml[to + x] = float2{m, l};
-  }
-}
-
-// The outputs of one token's rows of one key head (8 of them at a time).  Waves
-// 0 to 3 take the own keys (unless they are among the parts), waves 4 to 7 meanwhile
-// weigh and add the parts, one row to each group of 32 lanes.  WALK: no parts; all
-// eight waves take the keys of a short prefix and the own ones, in this one launch.
+// The outputs of one token's rows of one key head (8 of them at a time).  Waves 0 to
+// 3 take the own keys, waves 4 to 7 meanwhile weigh and add the prefix's parts, one
+// row to each group of 32 lanes.  WALK: no parts; all eight waves take the keys of a
+// short prefix and the own ones, in this one launch.
 template <class T, int D, bool FULL, bool WALK>
-__global__ __launch_bounds__(512) void shared_join(SharedParams p) {
-  constexpr int KB = Ops<T>::KB, R = kJoinRows, F = D / 32;  // features of a lane
-  __shared__ Joined<D, WALK ? 8 : 5, kJoinRows> part;
+__global__ __launch_bounds__(512) void shared_finish(SharedParams p) {
+  constexpr int KB = Ops<T>::KB, R = kFinishRows, F = D / 32;  // features of a lane
+  __shared__ Joined<D, WALK ? 8 : 5, R> part;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.heads / p.kvh, tiles = (G + R - 1) / R;
   const int at = blockIdx.x;
@@ -558,19 +582,14 @@ __global__ __launch_bounds__(512) void shared_join(SharedParams p) {
   const int s = __builtin_amdgcn_readfirstlane(seq_of(p, t, lane));
   if (s < 0) return;
   const int rows = min(R, G - g0), h0 = kv * G + g0;
-  const int64_t row = (int64_t)t * p.heads + h0;
   // the thread's four features of the output, and their gate
   const int x = tid / (D / 4), e = tid % (D / 4) * 4;
   const bool mine = x < rows && e < p.d;
   T gate[4] = {};
-  if (mine) {
-    const T* gp = static_cast<const T*>(p.gate) + t * p.ldg + (h0 + x) * p.hsg + e;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) gate[j] = gp[j];
-  }
+  if (mine) load_gate(p, gate, t, h0 + x, e);
   if (WALK || wave < 4) {
-    int first = 0, count = 0;
-    if (!p.osplits) own_span(p, s, t, first, count);
+    int first, count;
+    own_span(p, s, t, first, count);
     typename Ops<T>::frag fq[D / KB][1];
     load_queries<T, D, 1, FULL>(p, fq, kv, t * G + g0, t * G + g0 + rows, lane);
     Soft<T, D, 1> st;
@@ -588,20 +607,19 @@ __global__ __launch_bounds__(512) void shared_join(SharedParams p) {
     part.put(st, 0, wave, lane, rows);
   } else if (const int y = (tid - 256) / 32; y < rows) {
     const int a = tid % 32;
-    const int parts = p.psplits + p.osplits;
-    const int64_t step = (int64_t)p.T * p.heads;
-    const float2* ml = p.ml + row + y;
-    const float* src = p.part + (row + y) * D + a * F;
+    const int64_t row = (int64_t)t * p.heads + h0 + y, step = (int64_t)p.T * p.heads;
+    const float2* ml = p.ml + row;
+    const float* src = p.part + row * D + a * F;
     typedef float vec __attribute__((ext_vector_type(F)));
     float m = -INFINITY;
-    for (int n = a; n < parts; n += 32) m = fmaxf(m, ml[n * step].x);
+    for (int n = a; n < p.psplits; n += 32) m = fmaxf(m, ml[n * step].x);
     m = fmaxf(m, __shfl_xor(m, 16, 64));
     m = lane_max<16>(m);
     const float ref = m == -INFINITY ? 0.0f : m;
     float l = 0.0f;
     vec o = {};
 #pragma unroll 8
-    for (int n = 0; n < parts; ++n) {
+    for (int n = 0; n < p.psplits; ++n) {
       const float2 w = ml[n * step];
       const float f = __builtin_amdgcn_exp2f(w.x - ref);
       l = fmaf(w.y, f, l);
@@ -615,10 +633,49 @@ __global__ __launch_bounds__(512) void shared_join(SharedParams p) {
   if (!mine) return;
   float m, l;
   const float4_t o = part.take(x, e, m, l);
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
-  T* y = static_cast<T*>(p.y) + t * p.ldy + (int64_t)(h0 + x) * p.d + e;
+  finish<T>(p, gate, o, l, t, h0 + x, e);
+}
+
+// The output of one (token, head): its parts, weighed and added by as many groups
+// of D / 4 threads as a work-group has, a part to each in turn.
+template <class T, int D>
+__global__ __launch_bounds__(256) void shared_join(SharedParams p) {
+  constexpr int L = D / 4, N = 256 / L;
+  __shared__ __attribute__((aligned(16))) float4_t so[N][L];
+  __shared__ float sl[N];
+  const int tid = threadIdx.x, lane = tid & 63, n0 = tid / L, e = tid % L * 4;
+  const int t = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
+  const int parts = p.psplits + p.osplits;
+  const int64_t step = (int64_t)p.T * p.heads;
+  const float2* ml = p.ml + blockIdx.x;
+  const float* src = p.part + (int64_t)blockIdx.x * D + e;
+  if (seq_of(p, t, lane) < 0) return;
+  const bool mine = n0 == 0 && e < p.d;
+  T gate[4] = {};
+  if (mine) load_gate(p, gate, t, h, e);
+  float m = -INFINITY;
+  for (int n = lane; n < parts; n += 64) m = fmaxf(m, ml[n * step].x);
+  m = max4(lane_max<16>(m));
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+  float4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int n = n0; n < parts; n += N) {
+    const float2 w = ml[n * step];
+    const float f = __builtin_amdgcn_exp2f(w.x - ref);
+    l = fmaf(w.y, f, l);
+    o += *reinterpret_cast<const float4_t*>(src + n * step * D) * f;
+  }
+  so[n0][tid % L] = o;
+  if (e == 0) sl[n0] = l;
+  lds_barrier();
+  if (!mine) return;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) y[j] = cvt_out<T>(o[j] * inv * sigmoid(to_f32(gate[j])));
+  for (int n = 1; n < N; ++n) {
+    o += so[n][tid % L];
+    l += sl[n];
+  }
+  finish<T>(p, gate, o, l, t, h, e);
 }
 
 int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
@@ -626,6 +683,7 @@ int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 // How the work is split, from the shapes alone (the workspace follows from it).
 struct Plan {
   bool walk;  // one launch
+  bool fused; // the own keys beside the joining
   bool many;  // 128 rows to a work-group
   int tile;   // rows of a work-group otherwise
   int psplits, pkeys, osplits, okeys;
@@ -638,7 +696,7 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
   // key head, which read the prefix for themselves.  (A block takes a CU about 5 us,
   // most of it the 256 KiB that its waves read: 2 requests behind 512 keys, two
   // blocks to a wave, took 20.7 us so and 12.4 us in parts.)
-  x.walk = np <= 8 * (dtype == CLEF_F16 ? Ops<half_t>::KB : Ops<float>::KB) && max_keys <= kOwnKeys;
+  x.walk = np <= 8 * (dtype == CLEF_F16 ? Ops<half_t>::KB : Ops<float>::KB) && max_keys <= kFinishKeys;
   if (x.walk) return x;
   // 24 rows of a key head behind 8,192 and 32,768 keys take 28 and 42 us with the
   // 128-row groups and took 33 and 50 with 32-row ones; 16 rows behind 32,768 keys
@@ -657,33 +715,35 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
   };
   const int tile = x.many ? 128 : x.tile;
   if (np) split(np, (rows + tile - 1) / tile * kvh, x.many ? cus : 2 * cus, x.many ? 256 : 64, kMaxParts, x.psplits, x.pkeys);
-  if (max_keys > kOwnKeys) split(max_keys, (int64_t)T * kvh, 2 * cus, 512, kMaxParts, x.osplits, x.okeys);
+  // Own keys as parts beside the prefix's while that leaves work-groups short of the
+  // chip, beside the joining when they would be another round of it: at 64, 128, 200
+  // and 256 (token, key head) behind 4,096 keys with up to 1,024 own, d = 256, f16,
+  // 30, 42, 69 and 76 us as parts, 52, 53, 63 and 67 beside the joining.
+  x.fused = np && max_keys <= kFinishKeys && (int64_t)T * kvh * 4 >= cus * 3;
+  if (max_keys && !x.fused) split(max_keys, (int64_t)T * kvh, 2 * cus, x.many && np ? 256 : 128, kMaxParts, x.osplits, x.okeys);
   return x;
 }
 
 template <class T, int D, bool FULL>
-int launch(const SharedParams& p, const Plan& x, hipStream_t st) {
-  const int G = p.heads / p.kvh, tiles = (G + 15) / 16, rows = p.T * G;
-  if (x.psplits) {
-    const unsigned each = (unsigned)p.kvh * x.psplits;
-    bool done = false;
-    if constexpr (sizeof(T) == 2 && FULL) {
-      // its loads address a key head's values with 32 bits
-      if (x.many && p.ldpv * D * 2 < (int64_t(1) << 32)) {
-        hipLaunchKernelGGL((shared_many_rows<D>), dim3((rows + 127) / 128 * each), dim3(512), 0, st, p);
-        done = true;
-      }
-    }
-    if (!done && x.tile == 32)
-      hipLaunchKernelGGL((shared_few_rows<T, D, 2, FULL>), dim3((rows + 31) / 32 * each), dim3(256), 0, st, p);
-    if (!done && x.tile == 16)
-      hipLaunchKernelGGL((shared_few_rows<T, D, 1, FULL>), dim3((rows + 15) / 16 * each), dim3(256), 0, st, p);
+int launch(SharedParams p, const Plan& x, hipStream_t st) {
+  const int G = p.heads / p.kvh, rows = p.T * G;
+  const unsigned last = (unsigned)p.T * p.kvh * ((G + kFinishRows - 1) / kFinishRows);
+  if (x.walk) {
+    hipLaunchKernelGGL((shared_finish<T, D, FULL, true>), dim3(last), dim3(512), 0, st, p);
+    return check_launch("shared-prefix attention");
   }
-  const unsigned own = (unsigned)p.T * p.kvh * tiles;
-  if (x.osplits) hipLaunchKernelGGL((shared_own<T, D, FULL>), dim3(own * x.osplits), dim3(256), 0, st, p);
-  const unsigned join = (unsigned)p.T * p.kvh * ((G + kJoinRows - 1) / kJoinRows);
-  if (x.walk) hipLaunchKernelGGL((shared_join<T, D, FULL, true>), dim3(join), dim3(512), 0, st, p);
-  else hipLaunchKernelGGL((shared_join<T, D, FULL, false>), dim3(join), dim3(512), 0, st, p);
+  // the wide groups' loads address a key head's values with 32 bits
+  const bool many = sizeof(T) == 2 && FULL && x.many && p.np && p.ldpv * D * 2 < (int64_t(1) << 32);
+  const int tile = many ? 128 : p.np ? x.tile : 16;
+  p.pgroups = (rows + tile - 1) / tile * p.kvh * x.psplits;
+  const unsigned groups = p.pgroups + (unsigned)p.T * p.kvh * ((G + 15) / 16) * x.osplits;
+  if constexpr (sizeof(T) == 2 && FULL) {
+    if (many) hipLaunchKernelGGL((shared_many_rows<D>), dim3(groups), dim3(512), 0, st, p);
+  }
+  if (tile == 32) hipLaunchKernelGGL((shared_few_rows<T, D, 2, FULL>), dim3(groups), dim3(256), 0, st, p);
+  if (tile == 16) hipLaunchKernelGGL((shared_few_rows<T, D, 1, FULL>), dim3(groups), dim3(256), 0, st, p);
+  if (x.fused) hipLaunchKernelGGL((shared_finish<T, D, FULL, false>), dim3(last), dim3(512), 0, st, p);
+  else hipLaunchKernelGGL((shared_join<T, D>), dim3((unsigned)p.T * p.heads), dim3(256), 0, st, p);
   return check_launch("shared-prefix attention");
 }
 

@@ -141,6 +141,33 @@ def test_batch(clef, case, dtype):
     assert torch.equal(y, clef.attention_gated_shared(**args, max_keys=max(b.lens)))
 
 
+SPLITS = [
+    # heads, kvh, d, prefix, requests, tokens of each, own keys at most, rows behind the last sequence
+    (4, 4, 64, 530, 60, 1, 200, 0),       # own keys beside the joining, 60 rows of a key head
+    (8, 8, 72, 300, 9, 3, 90, 5),         # the same, a padded width, 32 rows
+    (16, 2, 256, 600, 97, 1, 130, 70),
+    (24, 24, 64, 257, 9, 1, 40, 0),       # 16 rows
+    (12, 3, 128, 400, 5, 2, 70, 3),       # own keys as parts, 40 rows
+    (5, 5, 128, 400, 13, 1, 1000, 2),     # 13 rows
+    (34, 2, 64, 0, 40, 1, 300, 1),        # no prefix, 17 heads of a key head
+    (34, 1, 40, 300, 3, 1, 300, 1),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("split", SPLITS, ids=lambda c: "-".join(str(x) for x in c))
+def test_split_of_the_own_keys(clef, split, dtype):
+    heads, kvh, d, prefix, requests, tokens, most, behind = split
+    lens = [max(tokens, 1 + (37 * s) % most) for s in range(requests)]
+    b = _batch(dtype, heads, kvh, d, prefix, [tokens] * requests, lens, behind=behind)
+    out = torch.full((b.T, heads * d), 7.0, dtype=dtype, device="cuda")
+    y = clef.attention_gated_shared(**b.cuda(), max_keys=max(lens), out=out)
+    b.check(y)
+    assert (y[b.T - behind:] == 7.0).all()
+    assert torch.equal(y, clef.attention_gated_shared(**b.cuda(), max_keys=max(lens), out=out.clone()))
+
+
 @gpu
 @pytest.mark.parametrize("dtype", [F16, F32])
 def test_without_prefix_or_own_keys(clef, dtype):
