@@ -13,18 +13,19 @@
 // is cut into units of whole chunks: one launch forms what each unit adds to
 // a zero state, a second joins these into the state that each unit starts
 // from, a third walks the units side by side.  Prompts of one unit take the
-// third alone.
+// third alone.  16,384 tokens of 32 heads, 128 x 128, f16: 54 + 11 + 130 us, where
+// q, k, v and o once are 82 us at the rate of a copy; keys and values pass twice,
+// and the walk is bound by a chunk's chain of products, barriers and LDS reads.
 //
 // A work-group owns one unit of one v-head and holds its state in the f32
-// accumulators of its waves, 16 value columns to a wave.  Products are laid out so that every
-// accumulator is the next product's operand as it stands: the scores are
-// formed transposed (K Q^T: a lane has one query and 4 keys of a tile), the
-// state as S[dk][dv] and the output transposed (o^T = S^T q^T + V^T P^T: a
-// lane has one query and 4 value columns).  For f16,
-// whose operands hold 8 consecutive k-indices a lane, the tiles' rows are
-// taken in the order 8 (r / 4) + 4 t + r % 4 (two tiles t to a block of 32), and
-// then a lane's accumulators of both tiles are exactly its operand.  V^T and
-// K^T come out of LDS transposed (ds_read_b64_tr_b16).
+// accumulators of its waves, 16 value columns to a wave.  Products are laid out so
+// that every accumulator is the next product's operand as it stands: the scores are
+// formed transposed (K Q^T: a lane has one query and 4 keys of a tile), the state as
+// S[dk][dv] and the output transposed (o^T = S^T q^T + V^T P^T: a lane has one query
+// and 4 value columns).  For f16, whose operands hold 8 consecutive k-indices a
+// lane, the tiles' rows are taken in the order 8 (r / 4) + 4 t + r % 4 (two tiles t
+// to a block of 32), and then a lane's accumulators of both tiles are exactly its
+// operand.  V^T and K^T come out of LDS transposed (ds_read_b64_tr_b16).
 //
 // Precision.  The states, their sums and the scores are f32.  Rounded once, to
 // f16, because the f16 matrix product takes no other factor: the decayed
@@ -588,13 +589,20 @@ int linear_dims(int T, int nseq, int Hk, int Hv, int dk, int dv, int dtype_qkv) 
   return 0;
 }
 
-// Tokens of a unit: enough units that the work-groups fill the chip once, and
-// none shorter than 2 chunks, since a cut costs two launches and passes over a
-// state.
+// Tokens of a unit: enough units that the work-groups fill the chip, one to a CU,
+// or two for f16 once the units are long enough that one covering the other's
+// waits saves more than the joining of twice the units costs.  us at one and two
+// to a CU, 128 x 128: 1,200 tokens of 32 heads 33 and 38, 2,400 46 and 50, 8,192
+// of 8 heads 49 and 59; 6,000 of 32 heads 88 and 84, 16,384 230 and 214; for f32
+// (which has LDS for one) 4,096 of 32 heads 172 and 186.  And no f16 unit shorter
+// than 2 chunks (600 tokens of 32 heads 31 us, in chunks 33; of f32, whose chunks
+// take longer, 300 tokens 48 us in units of two, 37 in chunks).
 int unit_tokens(int T, int Hv, int dtype) {
-  const int64_t fill = (int64_t)device_cus() * (dtype == CLEF_F16 ? 2 : 1);
-  const int64_t want = ((int64_t)T * Hv + fill - 1) / fill;
-  return static_cast<int>((std::max<int64_t>(want, 2 * C) + C - 1) / C * C);
+  const int cus = device_cus();
+  const int64_t work = (int64_t)T * Hv, once = (work + cus - 1) / cus, twice = (once + 1) / 2;
+  const bool half = dtype == CLEF_F16;
+  const int64_t unit = std::max<int64_t>(half && once > 6 * C ? twice : once, half ? 2 * C : C);
+  return static_cast<int>((unit + C - 1) / C * C);
 }
 int padded(int d) { return d <= 64 ? 64 : 128; }
 
