@@ -348,8 +348,9 @@ class DeltaScan:
         sqk, sv, so = _token_stride(q, "q"), _token_stride(v, "v"), _token_stride(out, "out")
         _token_stride(k, "k")
         _check(lib().clef_delta_step(
-            _ptr(q), _ptr(k), _ptr(v), sqk, sv, _dt(q), _ptr(g), _ptr(beta), g.stride(0) if B > 1 else 0, _dt(g), _ptr(slots), B, Hk,
-            Hv, dk, dv, _ptr(states), stride, _ptr(new_states), nslots, _ptr(out), so, _dt(out), _stream()))
+            _ptr(q), _ptr(k), _ptr(v), sqk, sv, _dt(q), _ptr(g), _ptr(beta), g.stride(0) if B > 1 else 0, _dt(g),
+            _ptr(slots), B, Hk, Hv, dk, dv, _ptr(states), stride, _ptr(new_states), nslots, _ptr(out), so, _dt(out),
+            _stream()))
         return out
 
 
@@ -433,7 +434,8 @@ class LinearScan:
         final = g.new_empty((nseq, Hv, dk, dv)) if want_final else None
         _check(lib().clef_linear_scan_varlen(
             _ptr(q), _ptr(k), _ptr(v), sqk, sv, _dt(q), _ptr(g), _ptr(cu_seqlens), nseq, T, Hk, Hv, dk, dv,
-            self.scale, _ptr(initial), stride, _ptr(out), so, _dt(out), _ptr(final), _ptr(ws), 0 if ws is None else ws.numel(), _stream()))
+            self.scale, _ptr(initial), stride, _ptr(out), so, _dt(out), _ptr(final), _ptr(ws),
+            0 if ws is None else ws.numel(), _stream()))
         return out, final
 
     def step(self, q, k, v, g, states, slots=None, new_states=None, out_dtype=torch.float32, out=None):
