@@ -36,7 +36,7 @@ namespace {
 
 constexpr int kMaxSeq = 4096;
 constexpr int kMaxKeys = 1 << 24;
-constexpr int kMaxParts = 64;  // of a row over the prefix, and over its own keys
+constexpr int kMaxParts = 64;      // of a row over the prefix, and over its own keys
 constexpr int kFinishRows = 8;     // rows of a work-group that takes own keys and finishes
 constexpr int kFinishKeys = 1024;  // own keys of a request there
 constexpr size_t kNoWorkspace = 256;  // said of calls that keep nothing there
@@ -703,24 +703,47 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
   // take 38 us with 16-row ones.
   x.many = dtype == CLEF_F16 && rows > 16 && d == padded(d);
   x.tile = rows > 16 ? 32 : 16;
-  // splits until the chip is full (many rows: one work-group to a CU), but not so
-  // short that the parts cost more than they save: 32 requests behind 4,096 keys at
-  // 64, 128 and 256 keys a part take 38, 34 and 33 us with their joining; few rows
-  // take one block to each of two waves (2 requests behind 512 keys: 12.8 us at 64,
-  // 16.1 at 128, where every wave has one)
-  auto split = [&](int keys, int64_t groups, int fill, int least, int most, int& parts, int& each) {
-    const int64_t want = std::min<int64_t>(std::max<int64_t>(1, fill / groups), most);
-    each = static_cast<int>(((keys + want - 1) / want + least - 1) / least * least);
+  // work-groups that run at once: by the LDS of 128 rows, the registers of 32 and 16
+  const int tile = x.many ? 128 : x.tile, at_once = np && tile > 16 ? cus : 2 * cus;
+  // Parts until the chip is full, but not so short that they cost more than they
+  // save: 32 requests behind 4,096 keys at 64, 128 and 256 keys a part took 38, 34 and
+  // 33 us with their joining; few rows take one block to each of two waves (2 requests
+  // behind 512 keys: 12.8 us at 64, 16.1 at 128, where every wave has one).
+  auto split = [&](int keys, int64_t groups, int64_t fill, int least, int step, int& parts, int& each) {
+    const int64_t want = std::min<int64_t>(std::max<int64_t>(1, fill / groups), kMaxParts);
+    each = std::max(least, static_cast<int>(((keys + want - 1) / want + step - 1) / step * step));
     parts = (keys + each - 1) / each;
   };
-  const int tile = x.many ? 128 : x.tile;
-  if (np) split(np, (rows + tile - 1) / tile * kvh, x.many ? cus : 2 * cus, x.many ? 256 : 64, kMaxParts, x.psplits, x.pkeys);
   // Own keys as parts beside the prefix's while that leaves work-groups short of the
   // chip, beside the joining when they would be another round of it: at 64, 128, 200
   // and 256 (token, key head) behind 4,096 keys with up to 1,024 own, d = 256, f16,
   // 30, 42, 69 and 76 us as parts, 52, 53, 63 and 67 beside the joining.
   x.fused = np && max_keys <= kFinishKeys && (int64_t)T * kvh * 4 >= cus * 3;
-  if (max_keys && !x.fused) split(max_keys, (int64_t)T * kvh, 2 * cus, x.many && np ? 256 : 128, kMaxParts, x.osplits, x.okeys);
+  int64_t own = 0;
+  if (max_keys && !x.fused) {
+    // half of the chip for short ones (32 requests, up to 1,024 own: 26 us, 30 with all
+    // of it), all of it for long ones (up to 4,096: 59 us, 76 with half)
+    own = (int64_t)T * kvh * ((heads / kvh + 15) / 16);
+    const int least = x.many && np ? 256 : 128;
+    split(max_keys, own, max_keys > kFinishKeys ? at_once : at_once / 2, least, least, x.osplits, x.okeys);
+    own *= x.osplits;
+  }
+  if (!np) return x;
+  // The prefix's parts fill the chip with the own keys' groups behind them, or leave
+  // these their place: by which way the longest chain is shorter, where an own group
+  // counts as so many keys of a part.  (32 requests, f16, behind 16,384 keys 40 and
+  // 33 us; f32, behind 4,096 keys 52 and 61.)
+  const int64_t groups = (rows + tile - 1) / tile * kvh;
+  const int least = x.many ? 256 : 64, after = x.many ? 384 : 192;
+  split(np, groups, at_once, least, 64, x.psplits, x.pkeys);
+  if (own && groups * x.psplits + own > at_once) {
+    int parts, each;
+    split(np, groups, std::max<int64_t>(at_once - own, groups), least, 64, parts, each);
+    if (groups * parts + own <= at_once && each < x.pkeys + after) {
+      x.psplits = parts;
+      x.pkeys = each;
+    }
+  }
   return x;
 }
 
