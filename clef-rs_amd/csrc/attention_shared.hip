@@ -695,7 +695,7 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
   // At most one block of the prefix to a wave: one launch of 8 waves per token and
   // key head, which read the prefix for themselves.  (A block takes a CU about 5 us,
   // most of it the 256 KiB that its waves read: 2 requests behind 512 keys, two
-  // blocks to a wave, took 20.7 us so and 12.4 us in parts.)
+  // blocks to a wave, took 20.7 us so and take 10.4 us in parts.)
   x.walk = np <= 8 * (dtype == CLEF_F16 ? Ops<half_t>::KB : Ops<float>::KB) && max_keys <= kFinishKeys;
   if (x.walk) return x;
   // 24 rows of a key head behind 8,192 and 32,768 keys take 28 and 42 us with the
@@ -706,9 +706,10 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
   // work-groups that run at once: by the LDS of 128 rows, the registers of 32 and 16
   const int tile = x.many ? 128 : x.tile, at_once = np && tile > 16 ? cus : 2 * cus;
   // Parts until the chip is full, but not so short that they cost more than they
-  // save: 32 requests behind 4,096 keys at 64, 128 and 256 keys a part took 38, 34 and
-  // 33 us with their joining; few rows take one block to each of two waves (2 requests
-  // behind 512 keys: 12.8 us at 64, 16.1 at 128, where every wave has one).
+  // save: 32 requests behind 4,096 keys at 64, 128 and 256 keys a part take 35, 26 and
+  // 26 us, behind 8,192 36, 36 and 26; few rows take one block to each of two waves (2
+  // requests behind 512 keys, on the GPU: 12.8 us at 64, 16.1 at 128, where every wave
+  // has one).
   auto split = [&](int keys, int64_t groups, int64_t fill, int least, int step, int& parts, int& each) {
     const int64_t want = std::min<int64_t>(std::max<int64_t>(1, fill / groups), kMaxParts);
     each = std::max(least, static_cast<int>(((keys + want - 1) / want + step - 1) / step * step));
