@@ -36,6 +36,7 @@ namespace {
 
 constexpr int kMaxSeq = 4096;
 constexpr int kMaxKeys = 1 << 24;
+constexpr int64_t kMaxRows = 1 << 30;  // of the own keys' cache: blocks of keys are numbered with 32 bits
 constexpr int kMaxParts = 64;      // of a row over the prefix, and over its own keys
 constexpr int kFinishRows = 8;     // rows of a work-group that takes own keys and finishes
 constexpr int kFinishKeys = 1024;  // own keys of a request there
@@ -172,31 +173,41 @@ struct Soft {
 // One block: keys c0 .. + KB - 1 of k [.][d] and vt [d][ldv] (c0 a multiple of 8),
 // those outside [lo, hi) masked: scores of -inf and values of 0, whatever the
 // buffers hold there.  FULL: d = D.
-template <class T, int D, int RT, bool FULL>
-__device__ __forceinline__ void take_block(Soft<T, D, RT>& st, const typename Ops<T>::frag (&fq)[D / Ops<T>::KB][RT],
-                                           const T* k, const T* vt, int64_t ldv, int c0, int lo, int hi, int d,
-                                           float c, int lane) {
-  constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL, TPB = Ops<T>::TPB;
+template <class T, int D, bool FULL>
+struct Block {
+  static constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL, TPB = Ops<T>::TPB;
   typedef typename Ops<T>::frag frag;
-  const int r = lane & 15, grp = lane >> 4;
-  const int col = c0 + grp * EL;
-  // 16 bytes of a value row: behind the row's end lie masked keys alone
-  const T* vr = vt + r * ldv + min((int64_t)col, ldv - EL);
-  frag fv[D / 16];
+  frag k[TPB][D / KB], v[D / 16];
+
+  __device__ __forceinline__ void load_keys(const T* keys, int c0, int lo, int hi, int d, int lane) {
+    const int r = lane & 15, grp = lane >> 4;
 #pragma unroll
-  for (int e = 0; e < D / 16; ++e) fv[e] = FULL || e * 16 + r < d ? frag_at(vr + e * 16 * ldv) : frag{};
-  float4_t S[TPB][RT] = {};
+    for (int x = 0; x < TPB; ++x) {
+      const T* kr = keys + (int64_t)min(max(c0 + Ops<T>::row(x, r), lo), hi - 1) * d + grp * EL;
 #pragma unroll
-  for (int x = 0; x < TPB; ++x) {
-    const T* kr = k + (int64_t)min(max(c0 + Ops<T>::row(x, r), lo), hi - 1) * d + grp * EL;
-#pragma unroll
-    for (int kb = 0; kb < D / KB; ++kb) {
-      const frag fk = FULL || kb * KB + grp * EL < d ? frag_at(kr + kb * KB) : frag{};
-#pragma unroll
-      for (int y = 0; y < RT; ++y) Mma<T>::mma(S[x][y], fk, fq[kb][y]);
+      for (int kb = 0; kb < D / KB; ++kb) k[x][kb] = FULL || kb * KB + grp * EL < d ? frag_at(kr + kb * KB) : frag{};
     }
   }
-  if (c0 < lo || c0 + KB > hi) {
+  __device__ __forceinline__ void load_values(const T* vt, int64_t ldv, int c0, int d, int lane) {
+    const int r = lane & 15, grp = lane >> 4;
+    // 16 bytes of a value row: behind the row's end lie masked keys alone
+    const T* vr = vt + r * ldv + min((int64_t)(c0 + grp * EL), ldv - EL);
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) v[e] = FULL || e * 16 + r < d ? frag_at(vr + e * 16 * ldv) : frag{};
+  }
+  template <int RT>
+  __device__ __forceinline__ void scores(float4_t (&S)[TPB][RT], const frag (&fq)[D / KB][RT]) const {
+#pragma unroll
+    for (int x = 0; x < TPB; ++x)
+#pragma unroll
+      for (int kb = 0; kb < D / KB; ++kb)
+#pragma unroll
+        for (int y = 0; y < RT; ++y) Mma<T>::mma(S[x][y], k[x][kb], fq[kb][y]);
+  }
+  template <int RT>
+  __device__ __forceinline__ void mask(float4_t (&S)[TPB][RT], int c0, int lo, int hi, int lane) {
+    if (c0 >= lo && c0 + KB <= hi) return;
+    const int grp = lane >> 4, col = c0 + grp * EL;
     auto in = [&](int key) { return key >= lo && key < hi; };
 #pragma unroll
     for (int x = 0; x < TPB; ++x)
@@ -207,33 +218,58 @@ __device__ __forceinline__ void take_block(Soft<T, D, RT>& st, const typename Op
         for (int y = 0; y < RT; ++y) S[x][y][i] = keep ? S[x][y][i] : -INFINITY;
       }
     typedef uint32_t bits __attribute__((ext_vector_type(4)));
-    bits mask;
+    bits keep;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 2) mask[i] = (in(col + 2 * i) ? 0xffffu : 0u) | (in(col + 2 * i + 1) ? ~0xffffu : 0u);
-      else mask[i] = in(col + i) ? ~0u : 0u;
+      if constexpr (sizeof(T) == 2) keep[i] = (in(col + 2 * i) ? 0xffffu : 0u) | (in(col + 2 * i + 1) ? ~0xffffu : 0u);
+      else keep[i] = in(col + i) ? ~0u : 0u;
     }
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e) fv[e] = __builtin_bit_cast(frag, __builtin_bit_cast(bits, fv[e]) & mask);
+    for (int e = 0; e < D / 16; ++e) v[e] = __builtin_bit_cast(frag, __builtin_bit_cast(bits, v[e]) & keep);
   }
-  frag w[1][RT];
-  st.template weights<1>(S, w, c);
+  template <int RT>
+  __device__ __forceinline__ void values(Soft<T, D, RT>& st, const frag (&w)[1][RT]) const {
 #pragma unroll
-  for (int e = 0; e < D / 16; ++e)
+    for (int e = 0; e < D / 16; ++e)
 #pragma unroll
-    for (int y = 0; y < RT; ++y) Mma<T>::mma(st.o[e][y], fv[e], w[0][y]);
-}
+      for (int y = 0; y < RT; ++y) Mma<T>::mma(st.o[e][y], v[e], w[0][y]);
+  }
+};
 
-// The blocks of keys [lo, hi) that are wave `wave`'s of `waves`.
+// The blocks of keys [lo, hi) that are wave `wave`'s of `waves`.  Two query tiles
+// leave one or two waves to a SIMD: there the next block's keys are loaded under this
+// one's weights and values, and its values under its scores (128 rows a key head behind
+// 32,768 keys, f32, d = 256: 151 -> 105 us).
 template <class T, int D, int RT, bool FULL>
 __device__ __forceinline__ void take_keys(Soft<T, D, RT>& st, const typename Ops<T>::frag (&fq)[D / Ops<T>::KB][RT],
                                           const void* k, int64_t ldk, const void* vt, int64_t ldv, int kv, int lo,
                                           int hi, int d, float c, int wave, int waves, int lane) {
+  constexpr int KB = Ops<T>::KB;
+  constexpr bool AHEAD = RT > 1;
   const T* kh = static_cast<const T*>(k) + (int64_t)kv * ldk * d;
   const T* vh = static_cast<const T*>(vt) + (int64_t)kv * d * ldv;
+  int c0 = (lo & ~7) + wave * KB;
+  Block<T, D, FULL> b;
+  if (AHEAD && c0 < hi) {
+    b.load_keys(kh, c0, lo, hi, d, lane);
+    b.load_values(vh, ldv, c0, d, lane);
+  }
 #pragma unroll 1
-  for (int c0 = (lo & ~7) + wave * Ops<T>::KB; c0 < hi; c0 += waves * Ops<T>::KB)
-    take_block<T, D, RT, FULL>(st, fq, kh, vh, ldv, c0, lo, hi, d, c, lane);
+  for (; c0 < hi; c0 += waves * KB) {
+    const int next = c0 + waves * KB;
+    if constexpr (!AHEAD) {
+      b.load_values(vh, ldv, c0, d, lane);
+      b.load_keys(kh, c0, lo, hi, d, lane);
+    }
+    float4_t S[Ops<T>::TPB][RT] = {};
+    b.scores(S, fq);
+    if constexpr (AHEAD) b.load_keys(kh, next, lo, hi, d, lane);
+    b.mask(S, c0, lo, hi, lane);
+    typename Ops<T>::frag w[1][RT];
+    st.template weights<1>(S, w, c);
+    b.values(st, w);
+    if constexpr (AHEAD) b.load_values(vh, ldv, next, d, lane);
+  }
 }
 
 // The rows of a work-group: query tile y has rows row0 + 16 y + r of the
@@ -703,8 +739,11 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
   // take 38 us with 16-row ones.
   x.many = dtype == CLEF_F16 && rows > 16 && d == padded(d);
   x.tile = rows > 16 ? 32 : 16;
-  // work-groups that run at once: by the LDS of 128 rows, the registers of 32 and 16
-  const int tile = x.many ? 128 : x.tile, at_once = np && tile > 16 ? cus : 2 * cus;
+  // Work-groups that run at once: one to a CU by the LDS or the registers (wide heads,
+  // more than 16 rows), else two.  (1,024 rows a key head behind 32,768 keys, f16, d =
+  // 72: 89 us at one, 68 at two; 800 behind 8,192, f32, d = 128: 89 and 99, MFMA bound.)
+  const int tile = x.many ? 128 : x.tile, width = d * (dtype == CLEF_F16 ? 2 : 4);
+  const int at_once = np && tile > 16 && width > (x.many ? 128 : 256) ? cus : 2 * cus;
   // Parts until the chip is full, but not so short that they cost more than they
   // save: 32 requests behind 4,096 keys at 64, 128 and 256 keys a part take 35, 26 and
   // 26 us, behind 8,192 36, 36 and 26; few rows take one block to each of two waves (2
@@ -825,9 +864,9 @@ extern "C" int clef_attention_gated_shared(
   CLEF_REQUIRE(ldq_tok >= T, "shared-prefix attention: query stride");
   CLEF_REQUIRE(np == 0 || (ldpk_tok >= np && ldpv_tok >= np && ldpv_tok % 8 == 0),
                "shared-prefix attention: prefix strides (ldpv_tok must be a multiple of 8)");
-  CLEF_REQUIRE(max_keys == 0 || (ldk_tok >= 1 && ldv_tok >= 8 && ldv_tok % 8 == 0 && ldk_tok < (int64_t(1) << 31) &&
-                                 ldv_tok < (int64_t(1) << 31)),
-               "shared-prefix attention: own-key strides (below 2^31, ldv_tok a multiple of 8)");
+  CLEF_REQUIRE(max_keys == 0 || (ldk_tok >= 1 && ldv_tok >= 8 && ldv_tok % 8 == 0 &&
+                                 ldk_tok <= clef::kMaxRows && ldv_tok <= clef::kMaxRows),
+               "shared-prefix attention: own-key strides (up to 2^30, ldv_tok a multiple of 8)");
   CLEF_REQUIRE(hsg >= d && ldg >= (int64_t)(heads - 1) * hsg + d && ldy >= (int64_t)heads * d,
                "shared-prefix attention: gate or output strides");
   auto misaligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) != 0; };

@@ -418,8 +418,9 @@ int clef_attention_gated_varlen(const void* q, int64_t ldq_tok, const void* k, i
  * values, gate and y, with f32 sums and softmax.  1 <= T <= 65536, 1 <= nseq
  * <= 4096, heads <= 256, heads % kv_heads == 0, d a multiple of 8 up to 256;
  * np and max_keys up to 2^24, not both 0 (0: the buffers may be NULL); q, keys
- * and values 16-byte aligned, ldpv_tok and ldv_tok multiples of 8.  A table
- * that does not fit gives unspecified values, never an access out of bounds.
+ * and values 16-byte aligned, ldpv_tok and ldv_tok multiples of 8, ldk_tok and
+ * ldv_tok up to 2^30.  A table that does not fit gives unspecified values, never
+ * an access out of bounds.
  * workspace: clef_attention_shared_workspace bytes, 256-byte aligned; where that
  * is 256 (short prefixes), nothing is kept there and workspace may be NULL.  No
  * counterpart in the reference (one request per flash-attention call there).

@@ -92,6 +92,12 @@ def test_shared_attention_refuses(L, bad):
     assert "shared-prefix attention" in clef_hip.last_error()
 
 
+@pytest.mark.parametrize("bad", [dict(ldk=(1 << 30) + 1), dict(ldv=(1 << 30) + 8)], ids=str)
+def test_shared_attention_refuses_rows_past_its_block_numbers(L, bad):
+    """Blocks of keys are numbered with 32 bits, a step of the waves behind the last one included."""
+    assert L.clef_attention_gated_shared(*shared(**bad)) < 0
+
+
 def test_shared_attention_workspace(L):
     assert L.clef_attention_shared_workspace(0, 1, 8, 8, 1, 8, 2, 64) == 0
     assert L.clef_attention_shared_workspace(4, 1, 0, 0, 1, 8, 2, 64) == 0
