@@ -205,7 +205,7 @@ struct Staged {
     for (int i = 0; i < N; ++i)
       __builtin_memcpy(&x[i], src + min(tid / VPR + i * STEP, rows - 1) * stride + min(tid % VPR * EL, width - EL), 16);
   }
-  // narrower rows: value by value
+  // any rows: value by value, zeros behind `rows` and `width`
   __device__ __forceinline__ void load_any(const T* src, int64_t stride, int rows, int width, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -217,9 +217,10 @@ struct Staged {
       x[i] = y;
     }
   }
-  // place(row, column): the vector's place in the tile; cut: zeros behind `rows` and `width`
+  // place(row, column): the vector's place in the tile; cut: zeros behind `rows` and `width`;
+  // wide: from load_wide, whose vectors at a row's end are shifted to their place
   template <class At>
-  __device__ __forceinline__ void store(T* tile, int tid, bool cut, int rows, int width, At place) const {
+  __device__ __forceinline__ void store(T* tile, int tid, bool cut, bool wide, int rows, int width, At place) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int r = tid / VPR + i * STEP, c = tid % VPR * EL;
@@ -228,7 +229,7 @@ struct Staged {
         typedef unsigned __int128 bits;
         const int over = c + EL - width;  // elements behind the row's end
         if (r >= rows || over >= EL) y = vec{};
-        else if (over > 0 && width >= EL) y = __builtin_bit_cast(vec, __builtin_bit_cast(bits, y) >> over * 8 * (int)sizeof(T));
+        else if (over > 0 && wide) y = __builtin_bit_cast(vec, __builtin_bit_cast(bits, y) >> over * 8 * (int)sizeof(T));
       }
       *reinterpret_cast<vec*>(tile + place(r, c)) = y;
     }
@@ -355,10 +356,10 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
     int ln = lane, at = tid;
     asm("" : "+v"(ln), "+v"(at));
     const int r = ln & 15, grp = ln >> 4;
-    const bool cut = !(p.whole && rows == C);
-    if (OUT) rq.store(sQ, at, cut, rows, p.dk, [](int row, int col) { return row * PQ + col; });
-    rk.store(sK, at, cut, rows, p.dk, [](int row, int col) { return Tile::key(row, col); });
-    rv.store(sV, at, cut, rows, p.dv, [](int row, int col) { return Tile::value(row, col); });
+    const bool cut = !(p.whole && rows == C), wide = p.dk >= EL && p.dv >= EL;  // as fetch() takes them
+    if (OUT) rq.store(sQ, at, cut, wide, rows, p.dk, [](int row, int col) { return row * PQ + col; });
+    rk.store(sK, at, cut, wide, rows, p.dk, [](int row, int col) { return Tile::key(row, col); });
+    rv.store(sV, at, cut, wide, rows, p.dv, [](int row, int col) { return Tile::value(row, col); });
     lds_barrier();
     if (t + C < end) fetch(t + C, at);
 
