@@ -29,8 +29,8 @@
 //
 // Precision.  The states, their sums and the scores are f32.  Rounded once, to
 // f16, because the f16 matrix product takes no other factor: the decayed
-// scores, and a copy of the state scaled by a power of two (so that no state
-// overflows) for S^T q.  The decayed values of the state update are split into
+// scores, and a copy of the state for S^T q, each value column scaled by a power
+// of two (so that no state overflows, and columns of any size keep their bits).  The decayed values of the state update are split into
 // two f16 factors (22 bits), since the f32 states are results themselves.
 #include <hip/hip_runtime.h>
 
@@ -393,20 +393,23 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
 
       // ---- outputs, transposed: value columns x queries
       {
-        // f16: the state's copy scaled to at most 2^14 by a power of two
-        float up = 1.0f, down = first;
+        // f16: each column of the state's copy scaled to 2^13 .. 2^14 at its largest, by a
+        // power of two of its own, so that no column's size (or infinity) costs another its
+        // bits; its outputs are scaled back
+        float up = 1.0f, down[4] = {first, first, first, first};
         if constexpr (sizeof(T) == 2) {
           float big = 0.0f;
 #pragma unroll
           for (int a = 0; a < NKB * TPB; ++a)
 #pragma unroll
             for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(S[a][i]));
-          big = lane_max<16>(big);
           big = fmaxf(big, __shfl_xor(big, 16, 64));
           big = fmaxf(big, __shfl_xor(big, 32, 64));
           const uint32_t ex = max(__float_as_uint(big) >> 23, 14u);  // sign clear
           up = __uint_as_float((267u - ex) << 23);                   // 2^(13 - exponent)
-          down *= __uint_as_float((ex - 13u) << 23);
+          const float back = first * __uint_as_float((ex - 13u) << 23);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) down[e] = __shfl(back, 4 * grp + e, 64);  // of the lane's output columns
         }
         // An infinite or NaN value times a masked score of 0 is NaN: such values
         // are left out of the product, and added key by key where a query sees them.
@@ -443,7 +446,11 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
             Mma<T>::mma(o[qt], fs, frag_at(sQ + (qt * 16 + r) * PQ + kb * KB + grp * EL));
         }
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) o[qt] *= down * sS[C - 1 - (qt * 16 + r)];
+        for (int qt = 0; qt < QT; ++qt) {
+          const float w = sS[C - 1 - (qt * 16 + r)];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[qt][e] *= down[e] * w;
+        }
 #pragma unroll
         for (int b = 0; b < NCB; ++b)
 #pragma unroll

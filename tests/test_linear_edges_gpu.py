@@ -47,3 +47,54 @@ def test_one_narrow_width(clef, dk, dv, dtype):
             check(out[a:a + n], final[s], q[a:a + n], k[a:a + n], v[a:a + n], g, scan.scale, init)
         else:
             assert torch.equal(final[s].cpu(), init)
+
+
+# ---------------------------------------------------------------------------- states
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("T", [1, 70, 900])
+def test_infinite_state_entry_stays_in_its_column(clef, T, value, dtype):
+    """One infinite or NaN entry of the initial state: the other value columns come out as without it."""
+    H, dk, dv, row, col = 3, 64, 48, 7, 5
+    q, k, v = _inputs(T, T, H, H, dk, dv, dtype)
+    g = torch.tensor([-0.05, 0.0, -0.3])
+    init = _randn(6, H, dk, dv)
+    scan = clef.LinearScan(dk, dv)
+    cq, ck, cv, cg = _cuda(q, k, v, g)
+    clean, cfinal = scan.prefill(cq, ck, cv, cg, initial=init.cuda())
+    check(clean, cfinal, q, k, v, g, scan.scale, init)
+    init[1, row, col] = value
+    out, final = scan.prefill(cq, ck, cv, cg, initial=init.cuda())
+    hit = torch.zeros((H, dv), dtype=torch.bool, device="cuda")
+    hit[1, col] = True
+    assert torch.equal(out[:, ~hit], clean[:, ~hit])
+    assert not torch.isfinite(out[:, hit]).any()
+    entry = torch.zeros_like(final, dtype=torch.bool)
+    entry[1, row, col] = True
+    assert torch.equal(final[~entry], cfinal[~entry])
+    assert torch.equal(final[entry].cpu(), torch.tensor([value])) or value != value and final[entry].isnan().all()
+
+
+@gpu
+@pytest.mark.parametrize("T", [3, 70, 500])
+def test_state_columns_of_different_size(clef, T):
+    """Each column of an f16 scan's state to its own scale, 2^-30 to 2^30 side by side.  The copy of the state
+    is rounded relative to a column's largest entry, which is scaled to 2^13 or more, so the part below the
+    normal range of f16 is off by at most 2^-25 2^-13 of that entry; here against the column's sums of
+    absolute values, and with decays of 0, so that the entries stay where they are."""
+    H, dk, dv = 2, 64, 32
+    q, k, v = _inputs(T, T, H, H, dk, dv, F16)
+    k[:] = 0  # the state alone
+    g = torch.zeros(H)
+    sizes = torch.exp2(torch.tensor([(-30, 30, 0, -15)[c % 4] for c in range(dv)], dtype=F32))
+    init = _randn(6, H, dk, dv) * sizes
+    scan = clef.LinearScan(dk, dv)
+    out, final = scan.prefill(*_cuda(q, k, v, g), initial=init.cuda())
+    assert torch.equal(final.cpu(), init)
+    want, _ = reference(q, k, v, g, scan.scale, init)
+    size, _ = reference(q.abs(), k, v, g, scan.scale, init.abs())
+    top = init.abs().double().amax(1) * q.double().abs().sum(2).max() * scan.scale  # [H, dv]
+    bound = (2.0 ** -11 + (dk + T + 8) * 2.0 ** -24) * size + 2.0 ** -38 * top
+    err = (out.double().cpu() - want).abs()
+    assert (err <= bound).all(), f"{float((err / bound).max()):.3g} of the bound"
