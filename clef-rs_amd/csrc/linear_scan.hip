@@ -32,10 +32,18 @@
 // scores, and a copy of the state for S^T q, each value column scaled by a power
 // of two (so that no state overflows, and columns of any size keep their bits).  The decayed values of the state update are split into
 // two f16 factors (22 bits), since the f32 states are results themselves.
+//
+// Infinities and NaN.  Masked scores, padded keys and the halves of a split factor
+// are zeros that the products would turn into NaN beside an infinity.  Whatever was
+// not finite in a unit's keys, values or entering state is still so in the state at
+// its end, so only that is looked at; units where it is not finite are walked again,
+// with such factors taken out of the products and added key by key.  (A test of each
+// chunk's tiles instead cost 16 % of the states' launch and 5 % of the walk.)
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "../../include/clef_hip.h"
 #include "common.hpp"
@@ -169,6 +177,17 @@ __device__ __forceinline__ int unit_seq(const LinearParams& p, int u, int lane) 
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
+// S <- l^n S, w = l^n: an infinite or NaN entry stays what it is where l^n, but not l
+// (`first`), leaves the range of f32.
+__device__ __forceinline__ float4_t decayed(float4_t s, float w, float first) {
+  if (w == 0.0f && first > 0.0f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = finite(s[i]) ? 0.0f : s[i];
+    return s;
+  }
+  return s * w;
+}
+
 // e^g as a power of two per token: l^n = 2^{lg n}; an infinite decay stays
 // finite, so that l^0 = 1.
 __device__ __forceinline__ float log2_decay(float g) {
@@ -218,9 +237,11 @@ struct Staged {
     }
   }
   // place(row, column): the vector's place in the tile; cut: zeros behind `rows` and `width`;
-  // wide: from load_wide, whose vectors at a row's end are shifted to their place
+  // wide: from load_wide, whose vectors at a row's end are shifted to their place.
+  // Returns the sum of what it stored, times 0 (for any_nan).
   template <class At>
-  __device__ __forceinline__ void store(T* tile, int tid, bool cut, bool wide, int rows, int width, At place) const {
+  __device__ __forceinline__ vec store(T* tile, int tid, bool cut, bool wide, int rows, int width, At place) const {
+    vec zero = {};
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int r = tid / VPR + i * STEP, c = tid % VPR * EL;
@@ -232,13 +253,31 @@ struct Staged {
         else if (over > 0 && wide) y = __builtin_bit_cast(vec, __builtin_bit_cast(bits, y) >> over * 8 * (int)sizeof(T));
       }
       *reinterpret_cast<vec*>(tile + place(r, c)) = y;
+      zero += y * T(0);
     }
+    return zero;
   }
 };
 
 template <class T>
 __device__ __forceinline__ typename Ops<T>::frag frag_at(const T* p) {
   return *reinterpret_cast<const typename Ops<T>::frag*>(p);
+}
+
+// 0 or -0 in every element from finite vectors, NaN in some from others: of a sum of x * 0.
+template <class T>
+__device__ __forceinline__ bool any_nan(const typename Ops<T>::frag& zero) {
+  const uint4 z = __builtin_bit_cast(uint4, zero);
+  constexpr uint32_t bits = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
+  return ((z.x | z.y | z.z | z.w) & bits) != 0;
+}
+
+template <class T>
+__device__ __forceinline__ typename Ops<T>::frag finite_only(typename Ops<T>::frag x) {
+#pragma unroll
+  for (int e = 0; e < Ops<T>::EL; ++e)
+    if (!finite(to_f32(x[e]))) x[e] = T(0);
+  return x;
 }
 
 // LDS of a work-group (elements of T): k, v, q, scores.
@@ -251,7 +290,8 @@ struct Shared {
   // powers of the decay: f32 words behind the tiles.  W[i] = l^{C-1-i}, S[i] =
   // scale l^{C-1-i}, both 0 from i = C on (tokens behind the query or the chunk)
   static constexpr int POW = (ALL * (int)sizeof(T) + 15) / 16 * 16;
-  static constexpr int BYTES = POW + 4 * 2 * C * (OUT ? 2 : 1);
+  static constexpr int ODD = POW + 4 * 2 * C * (OUT ? 2 : 1);  // a word for each wave
+  static constexpr int BYTES = ODD + 4 * (DV / 16);
 };
 
 // One unit of one v-head.  OUT: walk it from its entering state and write the
@@ -279,6 +319,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
   T* const sP = reinterpret_cast<T*>(smem) + Lds::P;
   float* const sW = reinterpret_cast<float*>(smem + Lds::POW);
   float* const sS = sW + 2 * C;
+  int* const sOdd = reinterpret_cast<int*>(smem + Lds::ODD);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // heads of one k-head on one XCD (work-groups go round them), to share q and k in its L2
@@ -324,13 +365,12 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
       rv.load_any(vt, p.sv, rows, p.dv, tid);
     }
   };
-  if (begin < end) fetch(begin, tid);
 
   // ---- the entering state: tile a of S has rows KB (a / TPB) + row(a % TPB, .)
   // and the wave's 16 columns
   const int cb = wave * 16;
   float4_t S[NKB * TPB];
-  {
+  auto enter = [&]() {
     const int r = lane & 15, grp = lane >> 4;
     if (OUT && index > 0) {
       const float* src = entry(p, s, index, h, DK * DV) + wave * (DK * 16);
@@ -347,186 +387,235 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
           S[a][i] = src && row < p.dk && col < p.dv ? src[row * p.dv + col] : 0.0f;
         }
     }
-  }
+  };
 
-  for (int t = begin; t < end; t += C) {
-    const int rows = min(C, end - t);
-    // the lane's place anew for each chunk: the addresses that the compiler would
-    // keep from chunk to chunk cost more registers than it saves
-    int ln = lane, at = tid;
-    asm("" : "+v"(ln), "+v"(at));
-    const int r = ln & 15, grp = ln >> 4;
-    const bool cut = !(p.whole && rows == C), wide = p.dk >= EL && p.dv >= EL;  // as fetch() takes them
-    if (OUT) rq.store(sQ, at, cut, wide, rows, p.dk, [](int row, int col) { return row * PQ + col; });
-    rk.store(sK, at, cut, wide, rows, p.dk, [](int row, int col) { return Tile::key(row, col); });
-    rv.store(sV, at, cut, wide, rows, p.dv, [](int row, int col) { return Tile::value(row, col); });
-    lds_barrier();
-    if (t + C < end) fetch(t + C, at);
+  if (begin < end) fetch(begin, tid);
+  enter();
 
-    if constexpr (OUT) {
-      // ---- scores, transposed: keys of block b x queries of tile qt
-#pragma unroll
-      for (int job = wave; job < QT * NCB; job += NW) {
-        const int qt = job / NCB, b = job % NCB;
-        if (b * KB > qt * 16 + 15) continue;  // keys behind every query of the tile
-        float4_t acc[TPB] = {};
-#pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) {
-          const frag fq = frag_at(sQ + (qt * 16 + r) * PQ + kb * KB + grp * EL);
-#pragma unroll
-          for (int x = 0; x < TPB; ++x)
-            Mma<T>::mma(acc[x], frag_at(sK + Tile::key(b * KB + Ops<T>::row(x, r), kb * KB + grp * EL)), fq);
-        }
-        const int i = qt * 16 + r;  // query
-        const float* pw = sS + C - 1 - i + b * KB;
-        frag f;
-#pragma unroll
-        for (int x = 0; x < TPB; ++x)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = Ops<T>::row(x, 4 * grp + e);  // key of the block
-            f[x * 4 + e] = static_cast<T>(b * KB + j <= i ? acc[x][e] * pw[j] : 0.0f);
-          }
-        *reinterpret_cast<frag*>(sP + (job * 64 + ln) * EL) = f;
+  // The unit's chunks.  CAREFUL: with infinite and NaN keys, values and states as the
+  // recurrence has them, at a price; all others come out the same, to the bit.
+  auto walk = [&](auto careful) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(careful)::value;
+    for (int t = begin; t < end; t += C) {
+      const int rows = min(C, end - t);
+      // the lane's place anew for each chunk: the addresses that the compiler would
+      // keep from chunk to chunk cost more registers than it saves
+      int ln = lane, at = tid;
+      asm("" : "+v"(ln), "+v"(at));
+      const int r = ln & 15, grp = ln >> 4;
+      const bool cut = !(p.whole && rows == C), wide = p.dk >= EL && p.dv >= EL;  // as fetch() takes them
+      if (OUT) rq.store(sQ, at, cut, wide, rows, p.dk, [](int row, int col) { return row * PQ + col; });
+      frag zero = rk.store(sK, at, cut, wide, rows, p.dk, [](int row, int col) { return Tile::key(row, col); });
+      zero += rv.store(sV, at, cut, wide, rows, p.dv, [](int row, int col) { return Tile::value(row, col); });
+      if constexpr (CAREFUL) {
+        const bool mine = __any(any_nan<T>(zero));
+        if (ln == 0) sOdd[wave] = mine;
       }
       lds_barrier();
+      if (t + C < end) fetch(t + C, at);
 
-      // ---- outputs, transposed: value columns x queries
-      {
-        // f16: each column of the state's copy scaled to 2^13 .. 2^14 at its largest, by a
-        // power of two of its own, so that no column's size (or infinity) costs another its
-        // bits; its outputs are scaled back
-        float up = 1.0f, down[4] = {first, first, first, first};
-        if constexpr (sizeof(T) == 2) {
-          float big = 0.0f;
+      // infinite or NaN keys or values in the chunk
+      const bool odd = CAREFUL && __any(sOdd[ln % NW]);
+      if constexpr (OUT) {
+        // ---- scores, transposed: keys of block b x queries of tile qt
 #pragma unroll
-          for (int a = 0; a < NKB * TPB; ++a)
+        for (int job = wave; job < QT * NCB; job += NW) {
+          const int qt = job / NCB, b = job % NCB;
+          if (b * KB > qt * 16 + 15) continue;  // keys behind every query of the tile
+          float4_t acc[TPB] = {};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(S[a][i]));
-          big = fmaxf(big, __shfl_xor(big, 16, 64));
-          big = fmaxf(big, __shfl_xor(big, 32, 64));
-          const uint32_t ex = max(__float_as_uint(big) >> 23, 14u);  // sign clear
-          up = __uint_as_float((267u - ex) << 23);                   // 2^(13 - exponent)
-          const float back = first * __uint_as_float((ex - 13u) << 23);
+          for (int kb = 0; kb < NKB; ++kb) {
+            const frag fq = frag_at(sQ + (qt * 16 + r) * PQ + kb * KB + grp * EL);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) down[e] = __shfl(back, 4 * grp + e, 64);  // of the lane's output columns
+            for (int x = 0; x < TPB; ++x)
+              Mma<T>::mma(acc[x], frag_at(sK + Tile::key(b * KB + Ops<T>::row(x, r), kb * KB + grp * EL)), fq);
+          }
+          const int i = qt * 16 + r;  // query
+          const float* pw = sS + C - 1 - i + b * KB;
+          frag f;
+#pragma unroll
+          for (int x = 0; x < TPB; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int j = Ops<T>::row(x, 4 * grp + e);  // key of the block
+              f[x * 4 + e] = static_cast<T>(b * KB + j <= i ? acc[x][e] * pw[j] : 0.0f);
+            }
+          *reinterpret_cast<frag*>(sP + (job * 64 + ln) * EL) = f;
         }
-        // An infinite or NaN value times a masked score of 0 is NaN: such values
-        // are left out of the product, and added key by key where a query sees them.
-        frag fv[NCB];
-        bool odd;
-#pragma unroll
-        for (int b = 0; b < NCB; ++b) fv[b] = transposed(sV + Tile::value_t(b * KB, cb, ln), Tile::VSTEP);
+        lds_barrier();
+
+        // ---- outputs, transposed: value columns x queries
         {
-          // 0 or -0 from finite values, NaN from others
-          frag zero = fv[0] * T(0);
+          // f16: each column of the state's copy scaled to 2^13 .. 2^14 at its largest, by a
+          // power of two of its own, so that no column's size (or infinity) costs another its
+          // bits; its outputs are scaled back
+          float up = 1.0f, down[4] = {first, first, first, first};
+          if constexpr (sizeof(T) == 2) {
+            float big = 0.0f;
 #pragma unroll
-          for (int b = 1; b < NCB; ++b) zero += fv[b] * T(0);
-          const uint4 z = __builtin_bit_cast(uint4, zero);
-          constexpr uint32_t bits = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
-          odd = __any(((z.x | z.y | z.z | z.w) & bits) != 0);
-        }
-        if (odd) {
+            for (int a = 0; a < NKB * TPB; ++a)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(S[a][i]));
+            big = fmaxf(big, __shfl_xor(big, 16, 64));
+            big = fmaxf(big, __shfl_xor(big, 32, 64));
+            const uint32_t ex = max(__float_as_uint(big) >> 23, 14u);  // sign clear
+            up = __uint_as_float((267u - ex) << 23);                   // 2^(13 - exponent)
+            const float back = first * __uint_as_float((ex - 13u) << 23);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) down[e] = __shfl(back, 4 * grp + e, 64);  // of the lane's output columns
+          }
+          // An infinite or NaN value times a masked score of 0 is NaN: such values
+          // are left out of the product, and added key by key where a query sees them.
+          frag fv[NCB];
+#pragma unroll
+          for (int b = 0; b < NCB; ++b) fv[b] = transposed(sV + Tile::value_t(b * KB, cb, ln), Tile::VSTEP);
+          if (odd) {
+#pragma unroll
+            for (int b = 0; b < NCB; ++b) fv[b] = finite_only<T>(fv[b]);
+          }
+          float4_t o[QT] = {};
+#pragma unroll
+          for (int kb = 0; kb < NKB; ++kb) {
+            frag fs;
+#pragma unroll
+            for (int y = 0; y < TPB; ++y)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) fs[y * 4 + e] = static_cast<T>(S[kb * TPB + y][e] * up);
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+              Mma<T>::mma(o[qt], fs, frag_at(sQ + (qt * 16 + r) * PQ + kb * KB + grp * EL));
+          }
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) {
+            const float w = sS[C - 1 - (qt * 16 + r)];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[qt][e] *= down[e] * w;
+          }
 #pragma unroll
           for (int b = 0; b < NCB; ++b)
 #pragma unroll
-            for (int e = 0; e < EL; ++e)
-              if (!finite(to_f32(fv[b][e]))) fv[b][e] = T(0);
-        }
-        float4_t o[QT] = {};
+            for (int qt = 0; qt < QT; ++qt) {
+              if (b * KB > qt * 16 + 15) continue;
+              Mma<T>::mma(o[qt], fv[b], frag_at(sP + ((qt * NCB + b) * 64 + ln) * EL));
+            }
+          if (odd) {
+#pragma unroll 1
+            for (int j = 0; j < rows; ++j) {
+              const T* vj = sV + Tile::value(j, cb + 4 * grp);
+              // the scores of key j lie EL apart in their fragments
+              const T* pj = sP + (j / KB * 64 + j % KB / EL * 16 + r) * EL + j % EL;
 #pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) {
-          frag fs;
+              for (int e = 0; e < 4; ++e) {
+                const float v = to_f32(vj[e]);
+                if (finite(v)) continue;
 #pragma unroll
-          for (int y = 0; y < TPB; ++y)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) fs[y * 4 + e] = static_cast<T>(S[kb * TPB + y][e] * up);
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
-            Mma<T>::mma(o[qt], fs, frag_at(sQ + (qt * 16 + r) * PQ + kb * KB + grp * EL));
-        }
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-          const float w = sS[C - 1 - (qt * 16 + r)];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[qt][e] *= down[e] * w;
-        }
-#pragma unroll
-        for (int b = 0; b < NCB; ++b)
+                for (int qt = 0; qt < QT; ++qt)
+                  if (j <= qt * 16 + r) o[qt][e] = fmaf(to_f32(pj[qt * NCB * 64 * EL]), v, o[qt][e]);
+              }
+            }
+          }
+          const int col = cb + 4 * grp;  // 4 consecutive columns
+          O* out = static_cast<O*>(p.out) + t * p.so + (int64_t)h * p.dv + r * p.so + col;
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) {
-            if (b * KB > qt * 16 + 15) continue;
-            Mma<T>::mma(o[qt], fv[b], frag_at(sP + ((qt * NCB + b) * 64 + ln) * EL));
-          }
-        if (odd) {
-#pragma unroll 1
-          for (int j = 0; j < rows; ++j) {
-            const T* vj = sV + Tile::value(j, cb + 4 * grp);
-            // the scores of key j lie EL apart in their fragments
-            const T* pj = sP + (j / KB * 64 + j % KB / EL * 16 + r) * EL + j % EL;
+            const int i = qt * 16 + r;
+            if (i >= rows) continue;
+            O* dst = out + qt * 16 * p.so;
+            typedef O vec __attribute__((ext_vector_type(4)));
+            vec w;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float v = to_f32(vj[e]);
-              if (finite(v)) continue;
+              float y = o[qt][e];
+              asm("" : "+v"(y));  // one value from either side of the branch above (or the stores are formed twice)
+              w[e] = cvt_out<O>(y);
+            }
+            if (p.vec_out) {
+              if (col < p.dv) *reinterpret_cast<vec*>(dst) = w;
+            } else {
 #pragma unroll
-              for (int qt = 0; qt < QT; ++qt)
-                if (j <= qt * 16 + r) o[qt][e] = fmaf(to_f32(pj[qt * NCB * 64 * EL]), v, o[qt][e]);
+              for (int e = 0; e < 4; ++e)
+                if (col + e < p.dv) dst[e] = w[e];
             }
           }
         }
-        const int col = cb + 4 * grp;  // 4 consecutive columns
-        O* out = static_cast<O*>(p.out) + t * p.so + (int64_t)h * p.dv + r * p.so + col;
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-          const int i = qt * 16 + r;
-          if (i >= rows) continue;
-          O* dst = out + qt * 16 * p.so;
-          typedef O vec __attribute__((ext_vector_type(4)));
-          vec w;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float y = o[qt][e];
-            asm("" : "+v"(y));  // one value from either side of the branch above (or the stores are formed twice)
-            w[e] = cvt_out<O>(y);
-          }
-          if (p.vec_out) {
-            if (col < p.dv) *reinterpret_cast<vec*>(dst) = w;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (col + e < p.dv) dst[e] = w[e];
-          }
-        }
       }
-    }
 
-    // ---- S <- l^rows S + K^T (l^{rows-1-j} V)
-    {
-      const float w = __builtin_amdgcn_exp2f(lg * (float)rows);
-#pragma unroll
-      for (int a = 0; a < NKB * TPB; ++a) S[a] *= w;
-    }
-#pragma unroll
-    for (int b = 0; b < NCB; ++b) {
-      frag hi, lo;
+      // ---- S <- l^rows S + K^T (l^{rows-1-j} V)
       {
-        const frag f = transposed(sV + Tile::value_t(b * KB, cb, ln), Tile::VSTEP);
-        const float* pw = sW + C - rows + b * KB + grp * EL;
+        const float w = __builtin_amdgcn_exp2f(lg * (float)rows);
 #pragma unroll
-        for (int e = 0; e < EL; ++e) {
-          const float y = to_f32(f[e]) * pw[e];
-          hi[e] = cvt_out<T>(y);  // of the rounded product, as the next line takes it
-          if constexpr (sizeof(T) == 2) lo[e] = static_cast<T>(y - to_f32(hi[e]));
+        for (int a = 0; a < NKB * TPB; ++a) S[a] = CAREFUL ? decayed(S[a], w, first) : S[a] * w;
+      }
+      // Infinite and NaN keys and values are left out of the products and added key by key:
+      // the difference of an infinite value and its f16 half, and the product of one with
+      // the zeros that pad a key, are NaN where the recurrence has an infinity.
+      if (odd) {
+#pragma unroll 1
+        for (int j = 0; j < rows; ++j) {
+          int width = p.dk, g4 = grp;
+          asm("" : "+s"(width), "+v"(g4));  // nothing of this rare loop is kept over the chunk
+          const float v = to_f32(sV[Tile::value(j, cb + r)]), w = sW[C - rows + j];
+          const float y = first == 0.0f ? v * w : v;  // the decay changes an infinity as in decayed()
+          const bool take = !finite(v);
+#pragma unroll
+          for (int a = 0; a < NKB * TPB; ++a) {
+            const int row = a / TPB * KB + EL * g4;
+            typedef T four __attribute__((ext_vector_type(4)));
+            const four k = *reinterpret_cast<const four*>(sK + Tile::key(j, row) + a % TPB * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float x = to_f32(k[i]);
+              if (row + a % TPB * 4 + i < width && (take || !finite(x))) S[a][i] = fmaf(x, y, S[a][i]);
+            }
+          }
+        }
+        lds_barrier();  // (all waves are here)
+        for (int x = at * EL; x < C * Tile::PK; x += THREADS * EL)
+          *reinterpret_cast<frag*>(sK + x) = finite_only<T>(frag_at(sK + x));
+        lds_barrier();
+      }
+#pragma unroll
+      for (int b = 0; b < NCB; ++b) {
+        frag hi, lo;
+        {
+          frag f = transposed(sV + Tile::value_t(b * KB, cb, ln), Tile::VSTEP);
+          if (odd) f = finite_only<T>(f);
+          const float* pw = sW + C - rows + b * KB + grp * EL;
+#pragma unroll
+          for (int e = 0; e < EL; ++e) {
+            const float y = to_f32(f[e]) * pw[e];
+            hi[e] = cvt_out<T>(y);  // of the rounded product, as the next line takes it
+            if constexpr (sizeof(T) == 2) lo[e] = static_cast<T>(y - to_f32(hi[e]));
+          }
+        }
+#pragma unroll
+        for (int a = 0; a < NKB * TPB; ++a) {
+          const frag fk = transposed(sK + Tile::key_t(b * KB, a / TPB * KB, a % TPB, ln), Tile::KSTEP);
+          Mma<T>::mma(S[a], fk, hi);
+          if constexpr (sizeof(T) == 2) Mma<T>::mma(S[a], fk, lo);
         }
       }
-#pragma unroll
-      for (int a = 0; a < NKB * TPB; ++a) {
-        const frag fk = transposed(sK + Tile::key_t(b * KB, a / TPB * KB, a % TPB, ln), Tile::KSTEP);
-        Mma<T>::mma(S[a], fk, hi);
-        if constexpr (sizeof(T) == 2) Mma<T>::mma(S[a], fk, lo);
-      }
+      lds_barrier();  // everyone is done with the tiles
     }
-    lds_barrier();  // everyone is done with the tiles
+  };
+  walk(std::false_type{});
+  if (begin < end) {
+    // what was not finite is in the state still: then once more from the start
+    float zero = 0.0f;  // NaN from an infinity or a NaN
+#pragma unroll
+    for (int a = 0; a < NKB * TPB; ++a)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) zero = fmaf(S[a][i], 0.0f, zero);
+    const bool mine = __any(zero != zero);
+    if (lane == 0) sOdd[wave] = mine;
+    lds_barrier();
+    const bool odd = __any(sOdd[lane % NW]);
+    lds_barrier();  // read before a wave writes it again
+    if (odd) {
+      fetch(begin, tid);
+      enter();
+      walk(std::true_type{});
+    }
   }
 
   {
@@ -572,14 +661,15 @@ __global__ __launch_bounds__(256) void linear_join(LinearParams p) {
       if (row < p.dk && col < p.dv) run[i] = src[row * p.dv + col];
     }
   }
-  const float w = __builtin_amdgcn_exp2f(log2_decay(p.g[h]) * (float)p.unit);
+  const float lg = log2_decay(p.g[h]), first = __builtin_amdgcn_exp2f(lg);
+  const float w = __builtin_amdgcn_exp2f(lg * (float)p.unit);
   const int64_t step = (int64_t)p.Hv * (DK * DV);
   float* at = entry(p, s, 1, h, DK * DV) + e;
   float4_t next = *reinterpret_cast<const float4_t*>(at);
   for (int i = 1; i < n; ++i, at += step) {
     const float4_t add = next;
     if (i + 1 < n) next = *reinterpret_cast<const float4_t*>(at + step);
-    run = run * w + add;
+    run = decayed(run, w, first) + add;
     *reinterpret_cast<float4_t*>(at) = run;
   }
 }

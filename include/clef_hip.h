@@ -153,6 +153,9 @@ int clef_delta_scan_varlen(const void* q, const void* k, const void* v, int64_t 
  * exp(g n)) and a scaled copy of the state are rounded to f16 as factors of
  * an output, the f32 states themselves are not (their factors keep 22 bits),
  * and scores beyond 65504 overflow.
+ * Infinite and NaN keys, values and state entries leave infinities and NaN in
+ * the state where the recurrence does, and there alone; work-groups that meet
+ * one walk their tokens a second time.
  * Limits: 1 <= T <= 1048576; 1 <= Hk <= Hv <= 256; Hv % Hk == 0;
  * 1 <= dk <= 128; 1 <= dv <= 128.  workspace: clef_linear_scan_workspace
  * (nseq 1 for a single sequence) bytes, 256-byte aligned; where that is 256

@@ -98,3 +98,68 @@ def test_state_columns_of_different_size(clef, T):
     bound = (2.0 ** -11 + (dk + T + 8) * 2.0 ** -24) * size + 2.0 ** -38 * top
     err = (out.double().cpu() - want).abs()
     assert (err <= bound).all(), f"{float((err / bound).max()):.3g} of the bound"
+
+
+def recurrence(q, k, v, g, scale, initial=None):
+    """Token by token in 64 bits: infinities as the operator's definition has them."""
+    T, Hv = v.shape[0], v.shape[1]
+    rep = Hv // q.shape[1]
+    q, k = (x.double().repeat_interleave(rep, 1) for x in (q, k))
+    v, lam = v.double(), torch.exp(g.double())[:, None, None]
+    s = torch.zeros((Hv, q.shape[2], v.shape[2]), dtype=torch.float64) if initial is None else initial.double()
+    out = torch.empty(v.shape, dtype=torch.float64)
+    for t in range(T):
+        s = s * lam + k[t][:, :, None] * v[t][:, None, :]
+        out[t] = scale * (q[t][:, :, None] * s).sum(1)
+    return out, s
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("which", ["value", "key"])
+@pytest.mark.parametrize("T,dk,dv", [(1, 1, 1), (70, 64, 64), (150, 40, 24), (300, 128, 128), (900, 100, 13)])
+def test_infinities_in_the_state(clef, T, dk, dv, which, dtype):
+    """An infinite value (key) makes its column (row) of the state infinite, not NaN, and so it stays; all
+    factors are positive, so that outputs are infinite too wherever the recurrence has them so."""
+    Hk, Hv = 1, 2
+    q, k, v = (x.abs() + 0.125 for x in _inputs(T, T, Hk, Hv, dk, dv, dtype))
+    at = [t for t in (T // 3, T // 2) if t < T]
+    if which == "value":
+        for n, t in enumerate(at):
+            v[t, n % Hv, (3 * n + 1) % dv] = float("inf") * (1 - 2 * n)
+    else:
+        for n, t in enumerate(at):
+            k[t, 0, (3 * n + 1) % dk] = float("inf")
+    g = torch.tensor([-0.01, -0.2])
+    scan = clef.LinearScan(dk, dv)
+    cq, ck, cv, cg = _cuda(q, k, v, g)
+    eo, ef = recurrence(q, k, v, g, scan.scale)
+    mo, mf = eo.abs(), ef.abs()
+    cu = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    for out, final in (scan.prefill(cq, ck, cv, cg), [x if i == 0 else x[0] for i, x in enumerate(
+            scan.prefill_varlen(cq, ck, cv, cg, cu))]):
+        out, final = out.double().cpu(), final.double().cpu()
+        for got, want, size, rel in ((out, eo, mo, 2.0 ** -11 if dtype == F16 else 0.0), (final, ef, mf, 2.0 ** -21)):
+            odd = ~torch.isfinite(want)
+            assert torch.equal(got[odd & ~want.isnan()], want[odd & ~want.isnan()])
+            assert torch.isnan(got[want.isnan()]).all()
+            bound = ((dk + T + 8) * 2.0 ** -24 + rel) * size
+            assert ((got - want).abs()[~odd] <= bound[~odd]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_infinite_states_under_strong_decay(clef, dtype):
+    """Where e^{g n} of a chunk or a unit leaves the range of f32, an infinite entry is still infinite."""
+    T, H, d = 700, 1, 64
+    q, k, v = (x.abs() + 0.125 for x in _inputs(1, T, H, H, d, d, dtype))
+    v[10, 0, 3] = float("inf")
+    g = torch.tensor([-5.0])
+    init = _randn(2, H, d, d)
+    init[0, 9, 8] = float("-inf")
+    _, final = clef.LinearScan(d, d).prefill(*_cuda(q, k, v, g), initial=init.cuda())
+    _, want = recurrence(q, k, v, g, d ** -0.5, init)
+    final = final.double().cpu()
+    odd = ~torch.isfinite(want)
+    assert odd.sum() == d + 1 and torch.equal(final[odd], want[odd])
+    assert ((final - want).abs()[~odd] <= ((d + T + 8) * 2.0 ** -24 + 2.0 ** -21) * want.abs()[~odd]).all()
