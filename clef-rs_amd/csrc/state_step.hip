@@ -170,9 +170,11 @@ __global__ __launch_bounds__(kStepThreads) void state_step(StepParams p) {
     }
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-      const float e = kn * sk[rg + i * GROUPS];
+      const int r = rg + i * GROUPS;
+      const float e = kn * sk[r];
+      // (rows behind the key's end stay 0 beside an infinite d: the request's next row sums over them)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) S[i][j] = fmaf(e, d[j], S[i][j]);
+      for (int j = 0; j < 4; ++j) S[i][j] = r < p.dk ? fmaf(e, d[j], S[i][j]) : 0.0f;
     }
     if (next >= p.B) break;
     // ---- the request's next row

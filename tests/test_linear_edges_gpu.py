@@ -163,3 +163,26 @@ def test_infinite_states_under_strong_decay(clef, dtype):
     odd = ~torch.isfinite(want)
     assert odd.sum() == d + 1 and torch.equal(final[odd], want[odd])
     assert ((final - want).abs()[~odd] <= ((d + T + 8) * 2.0 ** -24 + 2.0 ** -21) * want.abs()[~odd]).all()
+
+
+# ---------------------------------------------------------------------------- single tokens
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("dk", [1, 40, 128])
+def test_step_after_an_infinite_value(clef, dk, dtype):
+    """Two tokens of one request in one call, an infinite value in the first: as one call for each."""
+    H, dv, col = 2, 24, 3
+    q, k, v = (x.abs() + 0.125 for x in _inputs(dk, 2, H, H, dk, dv, dtype))
+    v[0, 1, col] = float("inf")
+    g = _slopes(H).cuda()
+    cq, ck, cv = _cuda(q, k, v)
+    scan = clef.LinearScan(dk, dv)
+    old = _randn(4, 1, H, dk, dv).abs().cuda()
+    both, each = old.clone(), old.clone()
+    out = scan.step(cq, ck, cv, g, both, slots=torch.zeros(2, dtype=torch.int32, device="cuda"))
+    want = torch.cat([scan.step(cq[i:i + 1], ck[i:i + 1], cv[i:i + 1], g, each) for i in range(2)])
+    assert torch.equal(both, each) and torch.equal(out, want)
+    assert (out[:, 1, col] == float("inf")).all() and (both[0, 1, :, col] == float("inf")).all()
+    rest = torch.ones((H, dv), dtype=torch.bool, device="cuda")
+    rest[1, col] = False
+    assert torch.isfinite(out[:, rest]).all()
