@@ -29,8 +29,9 @@
 //
 // Precision.  The states, their sums and the scores are f32.  Rounded once, to
 // f16, because the f16 matrix product takes no other factor: the decayed
-// scores, and a copy of the state for S^T q, each value column scaled by a power
-// of two (so that no state overflows, and columns of any size keep their bits).  The decayed values of the state update are split into
+// scores, and a copy of the state for S^T q; each query's scores of a key block, and
+// each value column of the state, scaled by a power of two of its own (so that
+// nothing overflows, and any size keeps its bits).  The decayed values of the state update are split into
 // two f16 factors (22 bits), since the f32 states are results themselves.
 //
 // Infinities and NaN.  Masked scores, padded keys and the halves of a split factor
@@ -280,6 +281,22 @@ __device__ __forceinline__ typename Ops<T>::frag finite_only(typename Ops<T>::fr
   return x;
 }
 
+__device__ __forceinline__ float max4(float x) {  // over the 4 lanes of one column
+  x = fmaxf(x, __shfl_xor(x, 16, 64));
+  return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+// The power of two that brings `big` >= 0 to 2^13 .. 2^14, as a factor for f16, and its
+// inverse; up to 2^(140 - least).
+struct Scale {
+  float up, down;
+};
+__device__ __forceinline__ Scale scale_of(float big, uint32_t least) {
+  const uint32_t ex = max(__float_as_uint(big) >> 23, least);  // sign clear
+  return {__uint_as_float((267u - ex) << 23), __uint_as_float((ex - 13u) << 23)};
+}
+// the inverse of a power of two (a normal one)
+__device__ __forceinline__ float inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+
 // LDS of a work-group (elements of T): k, v, q, scores.
 template <class T, int DK, int DV, bool OUT>
 struct Shared {
@@ -290,7 +307,10 @@ struct Shared {
   // powers of the decay: f32 words behind the tiles.  W[i] = l^{C-1-i}, S[i] =
   // scale l^{C-1-i}, both 0 from i = C on (tokens behind the query or the chunk)
   static constexpr int POW = (ALL * (int)sizeof(T) + 15) / 16 * 16;
-  static constexpr int ODD = POW + 4 * 2 * C * (OUT ? 2 : 1);  // a word for each wave
+  // f16: what the scores of a query and key block are scaled back by
+  static constexpr int DOWN = POW + 4 * 2 * C * (OUT ? 2 : 1);
+  static constexpr int SCALED = DOWN + (OUT && sizeof(T) == 2 ? 4 * C * (C / Ops<T>::KB) : 0);  // a word for each wave
+  static constexpr int ODD = SCALED + (OUT && sizeof(T) == 2 ? 4 * (DV / 16) : 0);  // the same
   static constexpr int BYTES = ODD + 4 * (DV / 16);
 };
 
@@ -319,6 +339,8 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
   T* const sP = reinterpret_cast<T*>(smem) + Lds::P;
   float* const sW = reinterpret_cast<float*>(smem + Lds::POW);
   float* const sS = sW + 2 * C;
+  float* const sD = reinterpret_cast<float*>(smem + Lds::DOWN);
+  int* const sScaled = reinterpret_cast<int*>(smem + Lds::SCALED);
   int* const sOdd = reinterpret_cast<int*>(smem + Lds::ODD);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -418,6 +440,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
       const bool odd = CAREFUL && __any(sOdd[ln % NW]);
       if constexpr (OUT) {
         // ---- scores, transposed: keys of block b x queries of tile qt
+        int scaled = 0;  // any of the wave's scores
 #pragma unroll
         for (int job = wave; job < QT * NCB; job += NW) {
           const int qt = job / NCB, b = job % NCB;
@@ -432,16 +455,41 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
           }
           const int i = qt * 16 + r;  // query
           const float* pw = sS + C - 1 - i + b * KB;
-          frag f;
+          float y[EL];
 #pragma unroll
           for (int x = 0; x < TPB; ++x)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int j = Ops<T>::row(x, 4 * grp + e);  // key of the block
-              f[x * 4 + e] = static_cast<T>(b * KB + j <= i ? acc[x][e] * pw[j] : 0.0f);
+              y[x * 4 + e] = b * KB + j <= i ? acc[x][e] * pw[j] : 0.0f;
             }
+          frag f;
+          float up = 1.0f;
+          if constexpr (sizeof(T) == 2) {
+            // f16: where a query's largest score of the block is not in 2^-10 .. 2^15, scaled to
+            // 2^13 .. 2^14, by up to 2^40 (the output of the state meets the scores at that
+            // scale, and fits it up to 2^86)
+            float big = 0.0f, down = 1.0f;
+#pragma unroll
+            for (int e = 0; e < EL; ++e) big = fmaxf(big, fabsf(y[e]));
+            auto of_queries = [](uint64_t m) { return (uint32_t)(m | m >> 32) | (uint32_t)((m | m >> 32) >> 16); };
+            const uint32_t some = of_queries(__ballot(big > 0.0f)), enough = of_queries(__ballot(big >= 0x1p-10f));
+            if (((some & ~enough) & 0xffffu) || __any(big >= 0x1p15f)) {
+              big = max4(big);
+              if (big < 0x1p-10f || big >= 0x1p15f) {  // the others as if these were not there
+                const Scale x = scale_of(big, 100);
+                up = x.up;
+                down = x.down;
+              }
+              scaled = 1;
+            }
+            if (grp == 0) sD[job * 16 + r] = down;
+          }
+#pragma unroll
+          for (int e = 0; e < EL; ++e) f[e] = static_cast<T>(y[e] * up);
           *reinterpret_cast<frag*>(sP + (job * 64 + ln) * EL) = f;
         }
+        if (sizeof(T) == 2 && ln == 0) sScaled[wave] = scaled;
         lds_barrier();
 
         // ---- outputs, transposed: value columns x queries
@@ -456,11 +504,9 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
             for (int a = 0; a < NKB * TPB; ++a)
 #pragma unroll
               for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(S[a][i]));
-            big = fmaxf(big, __shfl_xor(big, 16, 64));
-            big = fmaxf(big, __shfl_xor(big, 32, 64));
-            const uint32_t ex = max(__float_as_uint(big) >> 23, 14u);  // sign clear
-            up = __uint_as_float((267u - ex) << 23);                   // 2^(13 - exponent)
-            const float back = first * __uint_as_float((ex - 13u) << 23);
+            const Scale scale = scale_of(max4(big), 14);  // (both normal f32 numbers)
+            up = scale.up;
+            const float back = first * scale.down;
 #pragma unroll
             for (int e = 0; e < 4; ++e) down[e] = __shfl(back, 4 * grp + e, 64);  // of the lane's output columns
           }
@@ -491,13 +537,21 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[qt][e] *= down[e] * w;
           }
+          auto add_values = [&](auto scaled) __attribute__((always_inline)) {
 #pragma unroll
-          for (int b = 0; b < NCB; ++b)
+            for (int b = 0; b < NCB; ++b)
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-              if (b * KB > qt * 16 + 15) continue;
-              Mma<T>::mma(o[qt], fv[b], frag_at(sP + ((qt * NCB + b) * 64 + ln) * EL));
-            }
+              for (int qt = 0; qt < QT; ++qt) {
+                if (b * KB > qt * 16 + 15) continue;
+                const int job = qt * NCB + b;
+                const float down = decltype(scaled)::value ? sD[job * 16 + r] : 1.0f;
+                if (scaled) o[qt] *= inverse(down);
+                Mma<T>::mma(o[qt], fv[b], frag_at(sP + (job * 64 + ln) * EL));
+                if (scaled) o[qt] *= down;
+              }
+          };
+          if (sizeof(T) == 2 && __any(sScaled[ln % NW])) add_values(std::true_type{});
+          else add_values(std::false_type{});
           if (odd) {
 #pragma unroll 1
             for (int j = 0; j < rows; ++j) {
@@ -510,7 +564,11 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
                 if (finite(v)) continue;
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt)
-                  if (j <= qt * 16 + r) o[qt][e] = fmaf(to_f32(pj[qt * NCB * 64 * EL]), v, o[qt][e]);
+                  if (j <= qt * 16 + r) {
+                    float score = to_f32(pj[qt * NCB * 64 * EL]);
+                    if constexpr (sizeof(T) == 2) score *= sD[(qt * NCB + j / KB) * 16 + r];
+                    o[qt][e] = fmaf(score, v, o[qt][e]);
+                  }
               }
             }
           }

@@ -150,9 +150,9 @@ int clef_delta_scan_varlen(const void* q, const void* k, const void* v, int64_t 
  * after token T; the two may not overlap.
  * CLEF_F32 inputs are multiplied in f32 (f32 MFMA).  CLEF_F16 inputs are
  * multiplied on f16 MFMA with f32 accumulation; there the scores (scale q.k
- * exp(g n)) and a scaled copy of the state are rounded to f16 as factors of
- * an output, the f32 states themselves are not (their factors keep 22 bits),
- * and scores beyond 65504 overflow.
+ * exp(g n)) and a copy of the state are rounded to f16 as factors of an output
+ * (scaled by powers of two, so at any size), the f32 states themselves are not
+ * (their factors keep 22 bits).
  * Infinite and NaN keys, values and state entries leave infinities and NaN in
  * the state where the recurrence does, and there alone; work-groups that meet
  * one walk their tokens a second time.

@@ -186,3 +186,50 @@ def test_step_after_an_infinite_value(clef, dk, dtype):
     rest = torch.ones((H, dv), dtype=torch.bool, device="cuda")
     rest[1, col] = False
     assert torch.isfinite(out[:, rest]).all()
+
+
+# ---------------------------------------------------------------------------- ranges of f16
+@gpu
+@pytest.mark.parametrize("size", [2.0 ** -11, 2.0 ** -6, 1.0, 2.0 ** 8])
+@pytest.mark.parametrize("T,d", [(33, 64), (64, 128), (300, 64)])
+def test_scores_of_any_size(clef, T, d, size):
+    """Queries and keys of about `size`: scores of f16 inputs from 2^-22 to beyond 65,504.  A score is rounded
+    by 2^-11 of itself, or, below the normal range of f16, by 2^-25 where the largest score of its query in a
+    block of keys is at least 2^-10, and elsewhere by 2^-25 2^-13 of that largest one: by 2^-15 of it at most."""
+    Hk, Hv = 1, 2
+    q, k, v = _inputs(T, T, Hk, Hv, d, d, F16)
+    q, k = (q.float() * size).to(F16), (k.float() * size).to(F16)
+    g = _slopes(Hv)
+    scan = clef.LinearScan(d, d)
+    out, final = scan.prefill(*_cuda(q, k, v, g))
+    want, state = reference(q, k, v, g, scan.scale)
+    mo, ms = reference(q.abs(), k.abs(), v.abs(), g, scan.scale)
+    top = (q[:, 0].double().abs() @ k[:, 0].double().abs().t()).amax(1) * scan.scale  # [T]
+    small = top[:, None, None] * v.double().abs().sum(0)[None]
+    _, kept = reference(q.abs(), k.abs(), v.abs(), torch.zeros(Hv), scan.scale)  # no state of a chunk is larger
+    enter = kept.amax() * q.double().abs().sum(2).max() * scan.scale
+    bound = (2.0 ** -11 + (d + T + 8) * 2.0 ** -24) * mo + 2.0 ** -15 * small + 2.0 ** -38 * enter
+    err = (out.double().cpu() - want).abs()
+    assert (err <= bound).all(), f"{float((err / bound).max()):.3g} of the bound"
+    sbound = ((d + T + 8) * 2.0 ** -24 + 2.0 ** -21) * ms + 2.0 ** -25 * k.double().abs().sum(0).max()
+    assert ((final.double().cpu() - state).abs() <= sbound).all()
+
+
+@gpu
+def test_queries_of_different_size(clef):
+    """A query of another size than its neighbours (2^-20 and 2^12 of them) changes its own row alone."""
+    T, H, d = 130, 2, 64
+    q, k, v = _inputs(3, T, H, H, d, d, F16)
+    g = torch.tensor([-0.01, -0.5])
+    scan = clef.LinearScan(d, d)
+    clean, _ = scan.prefill(*_cuda(q, k, v, g))
+    for at, factor in ((3, 2.0 ** -20), (70, 2.0 ** 12), (129, 2.0 ** -14)):
+        other = q.clone()
+        other[at] = (q[at].float() * factor).to(F16)
+        out, _ = scan.prefill(*_cuda(other, k, v, g))
+        rest = torch.arange(T, device="cuda") != at
+        assert torch.equal(out[rest], clean[rest])
+        eo, _ = reference(other, k, v, g, scan.scale)
+        mo, _ = reference(other.abs(), k.abs(), v.abs(), g, scan.scale)
+        err = (out.double().cpu() - eo).abs()[at]
+        assert (err <= (2.0 ** -10 + (d + T + 8) * 2.0 ** -24) * mo[at]).all()
