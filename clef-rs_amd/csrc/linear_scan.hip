@@ -32,7 +32,8 @@
 // scores, and a copy of the state for S^T q; each query's scores of a key block, and
 // each value column of the state, scaled by a power of two of its own (so that
 // nothing overflows, and any size keeps its bits).  The decayed values of the state update are split into
-// two f16 factors (22 bits), since the f32 states are results themselves.
+// two f16 factors, since the f32 states are results themselves: to 22 bits, or to
+// 2^-25, the step of f16's smallest numbers, where that is more.
 //
 // Infinities and NaN.  Masked scores, padded keys and the halves of a split factor
 // are zeros that the products would turn into NaN beside an infinity.  Whatever was

@@ -152,7 +152,7 @@ int clef_delta_scan_varlen(const void* q, const void* k, const void* v, int64_t 
  * multiplied on f16 MFMA with f32 accumulation; there the scores (scale q.k
  * exp(g n)) and a copy of the state are rounded to f16 as factors of an output
  * (scaled by powers of two, so at any size), the f32 states themselves are not
- * (their factors keep 22 bits).
+ * (their factors keep 22 bits, or 2^-25 where that is more, as of f16 values).
  * Infinite and NaN keys, values and state entries leave infinities and NaN in
  * the state where the recurrence does, and there alone; work-groups that meet
  * one walk their tokens a second time.
