@@ -57,6 +57,7 @@ constexpr int kMaxSeq = 4096;
 constexpr int kMaxWidth = 128;
 constexpr int C = 64;  // tokens of a chunk
 constexpr size_t kNoWorkspace = 256;  // said of calls that keep nothing there
+constexpr int kJoinSeqs = 256;        // sequences that a launch joins side by side
 
 struct LinearParams {
   const void *q, *k, *v;
@@ -698,38 +699,40 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
 }
 
 // The state that each unit starts from: its entry holds what the unit before it
-// adds, and becomes what it starts from.  A thread owns 4 elements of one
-// (sequence, head).
+// adds, and becomes what it starts from.  A thread owns 4 elements of one head, of one
+// sequence or (so that the launch keeps within 2^32 threads) of every kJoinSeqs-th.
 template <class T, int DK, int DV>
 __global__ __launch_bounds__(256) void linear_join(LinearParams p) {
   constexpr int KB = Ops<T>::KB, TPB = Ops<T>::TPB;
   const int per = DK * DV / 4 / 256;  // work-groups of a state
-  const int part = blockIdx.x % per, h = blockIdx.x / per % p.Hv, s = blockIdx.x / per / p.Hv;
-  int t0, t1;
-  span_of(p, s, t0, t1);
-  const int n = (t1 - t0 + p.unit - 1) / p.unit;
-  if (n < 2) return;
+  const int part = blockIdx.x % per, h = blockIdx.x / per % p.Hv;
   const int e = (part * 256 + threadIdx.x) * 4;  // wave * DK * 16 + (a * 64 + lane) * 4
-  float4_t run = {0.f, 0.f, 0.f, 0.f};
-  if (p.initial) {
-    const int lane = e / 4 % 64, a = e / 256 % (DK / 16), wave = e / (DK * 16);
-    const float* src = p.initial + s * p.init_stride + (int64_t)h * p.dk * p.dv;
-    const int col = wave * 16 + (lane & 15);
-    for (int i = 0; i < 4; ++i) {
-      const int row = a / TPB * KB + Ops<T>::row(a % TPB, 4 * (lane >> 4) + i);
-      if (row < p.dk && col < p.dv) run[i] = src[row * p.dv + col];
+  for (int s = blockIdx.x / per / p.Hv; s < p.nseq; s += kJoinSeqs) {
+    int t0, t1;
+    span_of(p, s, t0, t1);
+    const int n = (t1 - t0 + p.unit - 1) / p.unit;
+    if (n < 2) continue;
+    float4_t run = {0.f, 0.f, 0.f, 0.f};
+    if (p.initial) {
+      const int lane = e / 4 % 64, a = e / 256 % (DK / 16), wave = e / (DK * 16);
+      const float* src = p.initial + s * p.init_stride + (int64_t)h * p.dk * p.dv;
+      const int col = wave * 16 + (lane & 15);
+      for (int i = 0; i < 4; ++i) {
+        const int row = a / TPB * KB + Ops<T>::row(a % TPB, 4 * (lane >> 4) + i);
+        if (row < p.dk && col < p.dv) run[i] = src[row * p.dv + col];
+      }
     }
-  }
-  const float lg = log2_decay(p.g[h]), first = __builtin_amdgcn_exp2f(lg);
-  const float w = __builtin_amdgcn_exp2f(lg * (float)p.unit);
-  const int64_t step = (int64_t)p.Hv * (DK * DV);
-  float* at = entry(p, s, 1, h, DK * DV) + e;
-  float4_t next = *reinterpret_cast<const float4_t*>(at);
-  for (int i = 1; i < n; ++i, at += step) {
-    const float4_t add = next;
-    if (i + 1 < n) next = *reinterpret_cast<const float4_t*>(at + step);
-    run = decayed(run, w, first) + add;
-    *reinterpret_cast<float4_t*>(at) = run;
+    const float lg = log2_decay(p.g[h]), first = __builtin_amdgcn_exp2f(lg);
+    const float w = __builtin_amdgcn_exp2f(lg * (float)p.unit);
+    const int64_t step = (int64_t)p.Hv * (DK * DV);
+    float* at = entry(p, s, 1, h, DK * DV) + e;
+    float4_t next = *reinterpret_cast<const float4_t*>(at);
+    for (int i = 1; i < n; ++i, at += step) {
+      const float4_t add = next;
+      if (i + 1 < n) next = *reinterpret_cast<const float4_t*>(at + step);
+      run = decayed(run, w, first) + add;
+      *reinterpret_cast<float4_t*>(at) = run;
+    }
   }
 }
 
@@ -774,7 +777,8 @@ int launch(const LinearParams& p, hipStream_t st) {
   const dim3 grid((unsigned)p.nunits * p.Hv), block(DV * 4);
   if (p.unit < p.T) {
     hipLaunchKernelGGL((linear_chunks<T, T, DK, DV, false>), grid, block, 0, st, p);
-    hipLaunchKernelGGL((linear_join<T, DK, DV>), dim3((unsigned)p.nseq * p.Hv * (DK * DV / 1024)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((linear_join<T, DK, DV>), dim3((unsigned)std::min(p.nseq, kJoinSeqs) * p.Hv * (DK * DV / 1024)),
+                       dim3(256), 0, st, p);
   }
   hipLaunchKernelGGL((linear_chunks<T, O, DK, DV, true>), grid, block, 0, st, p);
   return check_launch("linear attention scan");

@@ -233,3 +233,42 @@ def test_queries_of_different_size(clef):
         mo, _ = reference(other.abs(), k.abs(), v.abs(), g, scan.scale)
         err = (out.double().cpu() - eo).abs()[at]
         assert (err <= (2.0 ** -10 + (d + T + 8) * 2.0 ** -24) * mo[at]).all()
+
+
+# ---------------------------------------------------------------------------- limits
+@gpu
+def test_most_sequences_of_most_heads(clef):
+    """4,096 sequences of 256 heads at 128 x 128, the limits of a ragged batch, in units that are joined."""
+    nseq, Hk, Hv, d, long = 4096, 1, 256, 128, 1300
+    T = long + 64
+    q, k, v = _inputs(3, T, Hk, Hv, d, d, F16)
+    lens = [0] * nseq
+    lens[7] = long
+    for s in range(100, 164):
+        lens[s] = 1
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    g = _slopes(Hv)
+    scan = clef.LinearScan(d, d)
+    cq, ck, cv, cg = _cuda(q, k, v, g)
+    out, none = scan.prefill_varlen(cq, ck, cv, cg, torch.tensor(cu, dtype=torch.int32, device="cuda"),
+                                    want_final=False, out_dtype=F16)
+    assert none is None
+    check(out[:long, :2].contiguous(), None, q[:long], k[:long], v[:long, :2], g[:2], scan.scale)
+    for t in (long, T - 1):
+        check(out[t:t + 1], None, q[t:t + 1], k[t:t + 1], v[t:t + 1], g, scan.scale)
+
+
+@gpu
+def test_many_sequences_of_two_units(clef):
+    """400 sequences of one head, each cut into two units, more than are joined side by side."""
+    nseq, n, H, d = 400, 400, 1, 64
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = (torch.randn((nseq * n, H, d), generator=gen, device="cuda", dtype=F16) for _ in range(3))
+    init = torch.randn((nseq, H, d, d), generator=gen, device="cuda")
+    g = torch.tensor([-0.003])
+    scan = clef.LinearScan(d, d)
+    cu = torch.arange(0, nseq * n + 1, n, dtype=torch.int32, device="cuda")
+    out, final = scan.prefill_varlen(q, k, v, g.cuda(), cu, initial=init)
+    for s in (0, 143, 255, 256, 257, 399):
+        part = slice(s * n, (s + 1) * n)
+        check(out[part], final[s], q[part].cpu(), k[part].cpu(), v[part].cpu(), g, scan.scale, init[s].cpu())
