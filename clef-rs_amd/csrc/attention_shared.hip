@@ -58,6 +58,7 @@ struct SharedParams {
   int psplits, pkeys;      // prefix parts and the keys of each
   int osplits, okeys;      // parts of the own keys
   int pgroups;             // work-groups of the prefix
+  int first;               // work-group that this launch begins with
 };
 
 // as in the linear scan: fragments of KB k-indices (EL per lane), TPB tiles of
@@ -376,7 +377,7 @@ __global__ __launch_bounds__(256) void shared_few_rows(SharedParams p) {
   constexpr int KB = Ops<T>::KB;
   __shared__ Joined<D, 4, 16> part;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int group = blockIdx.x;
+  const int group = p.first + blockIdx.x;
   if (group >= p.pgroups) return own_part<T, D, FULL, 4>(p, group - p.pgroups, part, tid, lane, wave);
   const int G = p.heads / p.kvh, rows = p.T * G;
   const int split = group % p.psplits, kv = group / p.psplits % p.kvh;
@@ -437,7 +438,7 @@ __global__ __launch_bounds__(512, 2) void shared_many_rows(SharedParams p) {
   T(*sV)[D * BK] = reinterpret_cast<T(*)[D * BK]>(lds + TILES / 2);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, grp = lane >> 4;
-  const int group = blockIdx.x;
+  const int group = p.first + blockIdx.x;
   if (group >= p.pgroups)
     return own_part<T, D, true, 8>(p, group - p.pgroups, *reinterpret_cast<Joined<D, 8, 16>*>(lds), tid, lane, wave);
   const int G = p.heads / p.kvh, rows = p.T * G;
@@ -613,7 +614,7 @@ __global__ __launch_bounds__(512) void shared_finish(SharedParams p) {
   __shared__ Joined<D, WALK ? 8 : 5, R> part;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.heads / p.kvh, tiles = (G + R - 1) / R;
-  const int at = blockIdx.x;
+  const int at = p.first + blockIdx.x;
   const int g0 = at % tiles * R, kv = at / tiles % p.kvh, t = at / tiles / p.kvh;
   const int s = __builtin_amdgcn_readfirstlane(seq_of(p, t, lane));
   if (s < 0) return;
@@ -680,11 +681,11 @@ __global__ __launch_bounds__(256) void shared_join(SharedParams p) {
   __shared__ __attribute__((aligned(16))) float4_t so[N][L];
   __shared__ float sl[N];
   const int tid = threadIdx.x, lane = tid & 63, n0 = tid / L, e = tid % L * 4;
-  const int t = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
+  const int row = p.first + blockIdx.x, t = row / p.heads, h = row % p.heads;
   const int parts = p.psplits + p.osplits;
   const int64_t step = (int64_t)p.T * p.heads;
-  const float2* ml = p.ml + blockIdx.x;
-  const float* src = p.part + (int64_t)blockIdx.x * D + e;
+  const float2* ml = p.ml + row;
+  const float* src = p.part + (int64_t)row * D + e;
   if (seq_of(p, t, lane) < 0) return;
   const bool mine = n0 == 0 && e < p.d;
   T gate[4] = {};
@@ -787,26 +788,36 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
   return x;
 }
 
+// A launch of `groups` work-groups, or several: each of at most 2^31 threads (one takes
+// less than 2^32; 65,536 tokens of 128 key heads finish in 2^32 of them).
+void launch_groups(void (*kernel)(SharedParams), int64_t groups, int threads, SharedParams p, hipStream_t st) {
+  const int64_t most = (int64_t(1) << 31) / threads;
+  for (int64_t first = 0; first < groups; first += most) {
+    p.first = static_cast<int>(first);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(groups - first, most)), dim3(threads), 0, st, p);
+  }
+}
+
 template <class T, int D, bool FULL>
 int launch(SharedParams p, const Plan& x, hipStream_t st) {
   const int G = p.heads / p.kvh, rows = p.T * G;
-  const unsigned last = (unsigned)p.T * p.kvh * ((G + kFinishRows - 1) / kFinishRows);
+  const int64_t last = (int64_t)p.T * p.kvh * ((G + kFinishRows - 1) / kFinishRows);
   if (x.walk) {
-    hipLaunchKernelGGL((shared_finish<T, D, FULL, true>), dim3(last), dim3(512), 0, st, p);
+    launch_groups(shared_finish<T, D, FULL, true>, last, 512, p, st);
     return check_launch("shared-prefix attention");
   }
   // the wide groups' loads address a key head's values with 32 bits
   const bool many = sizeof(T) == 2 && FULL && x.many && p.np && p.ldpv * D * 2 < (int64_t(1) << 32);
   const int tile = many ? 128 : p.np ? x.tile : 16;
   p.pgroups = (rows + tile - 1) / tile * p.kvh * x.psplits;
-  const unsigned groups = p.pgroups + (unsigned)p.T * p.kvh * ((G + 15) / 16) * x.osplits;
+  const int64_t groups = p.pgroups + (int64_t)p.T * p.kvh * ((G + 15) / 16) * x.osplits;
   if constexpr (sizeof(T) == 2 && FULL) {
-    if (many) hipLaunchKernelGGL((shared_many_rows<D>), dim3(groups), dim3(512), 0, st, p);
+    if (many) launch_groups(shared_many_rows<D>, groups, 512, p, st);
   }
-  if (tile == 32) hipLaunchKernelGGL((shared_few_rows<T, D, 2, FULL>), dim3(groups), dim3(256), 0, st, p);
-  if (tile == 16) hipLaunchKernelGGL((shared_few_rows<T, D, 1, FULL>), dim3(groups), dim3(256), 0, st, p);
-  if (x.fused) hipLaunchKernelGGL((shared_finish<T, D, FULL, false>), dim3(last), dim3(512), 0, st, p);
-  else hipLaunchKernelGGL((shared_join<T, D>), dim3((unsigned)p.T * p.heads), dim3(256), 0, st, p);
+  if (tile == 32) launch_groups(shared_few_rows<T, D, 2, FULL>, groups, 256, p, st);
+  if (tile == 16) launch_groups(shared_few_rows<T, D, 1, FULL>, groups, 256, p, st);
+  if (x.fused) launch_groups(shared_finish<T, D, FULL, false>, last, 512, p, st);
+  else launch_groups(shared_join<T, D>, (int64_t)p.T * p.heads, 256, p, st);
   return check_launch("shared-prefix attention");
 }
 

@@ -1,0 +1,53 @@
+"""Attention behind a shared prefix at the limits of its launches and with tables
+that do not fit the cache, against the same references as test_attention_shared_gpu.
+"""
+import pytest
+import torch
+
+from test_attention_shared_gpu import Batch
+
+gpu = pytest.mark.gpu
+F16, F32 = torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def clef():
+    import clef_hip
+    clef_hip.lib()
+    return clef_hip
+
+
+@gpu
+@pytest.mark.parametrize("prefix,max_keys", [(16, 8), (300, 8), (300, 2000)], ids=["one launch", "fused", "parts"])
+def test_most_tokens_of_most_heads(clef, prefix, max_keys):
+    """65,536 tokens of 256 key heads, the limits of a call, in each of its forms.  An f16 output is off by 2^-11
+    of itself, its f16 weights by 2^-11 of the sum of |v| under them or by 2^-25 of the largest, its f32 sums
+    (and those of the f32 reference) by far less than another 2^-12."""
+    T, heads, d, nseq, own = 65536, 256, 8, 16, 8
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GiB of device memory")
+    gen = torch.Generator(device="cuda").manual_seed(prefix)
+    randn = lambda *shape: torch.randn(shape, generator=gen, device="cuda", dtype=F16)  # noqa: E731
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    q, gate = randn(heads, T, d), randn(T, heads, d)
+    pk, pvt = randn(heads, prefix, d), randn(heads, d, (prefix + 7) // 8 * 8)
+    k, vt = randn(heads, nseq * own, d), randn(heads, d, nseq * own)
+    each = T // nseq
+    y = clef.attention_gated_shared(q, k, vt, gate, ints([each * s for s in range(nseq + 1)]),
+                                    ints([own * s for s in range(nseq)]), ints([own] * nseq), prefix_k=pk,
+                                    prefix_vt=pvt, max_keys=max_keys)
+    for s in range(nseq):  # the last `own` queries of a request see own keys, 1 to all of them
+        a, b = each * s, each * (s + 1)
+        keys = torch.cat([pk, k[:, own * s:own * (s + 1)]], 1).float()
+        values = torch.cat([pvt[:, :, :prefix], vt[:, :, own * s:own * (s + 1)]], 2).float()
+        values = values.transpose(1, 2).contiguous()
+        scores = q[:, a:b].float() @ keys.transpose(1, 2).contiguous() / d ** 0.5
+        sees = (torch.arange(a, b, device="cuda") - (b - own) + 1).clamp(min=0)
+        scores.masked_fill_(torch.arange(prefix + own, device="cuda")[None] >= prefix + sees[:, None], float("-inf"))
+        w = torch.softmax(scores, -1)
+        g = torch.sigmoid(gate[a:b].float()).transpose(0, 1)
+        want, size = (w @ values) * g, (w @ values.abs()) * g
+        small = w.amax(-1, keepdim=True) * values.abs().sum(1)[:, None] * g
+        bound = (2.0 ** -11 + 2.0 ** -12) * size + 2.0 ** -25 * small + 2.0 ** -11 * want.abs() + 2.0 ** -25
+        err = (y[a:b].view(each, heads, d).transpose(0, 1).float() - want).abs()
+        assert (err <= bound).all(), f"request {s}: {float((err / bound).max()):.3g} of the bound"
