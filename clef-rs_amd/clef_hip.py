@@ -201,7 +201,7 @@ def _step_args(q, k, v, states, slots, new_states, out_dtype, out):
     Hv, dv = v.shape[1], v.shape[2]
     if k.shape != q.shape or v.shape[0] != B:
         raise ClefError(-1, "step tensor shapes")
-    if q.dtype != k.dtype or q.dtype != v.dtype or q.stride(0) != k.stride(0):
+    if q.dtype != k.dtype or q.dtype != v.dtype or (B > 1 and q.stride(0) != k.stride(0)):
         raise ClefError(-1, "q, k, v must share a dtype; q and k a token stride")
     if new_states is None:
         new_states = states
@@ -371,7 +371,7 @@ class LinearScan:
         Hv, dv = v.shape[1], v.shape[2]
         if k.shape != q.shape or v.shape[0] != T or dk != self.key_dim or dv != self.value_dim:
             raise ClefError(-1, "linear attention tensor shapes")
-        if q.dtype != k.dtype or q.dtype != v.dtype or q.stride(0) != k.stride(0):
+        if q.dtype != k.dtype or q.dtype != v.dtype or (T > 1 and q.stride(0) != k.stride(0)):
             raise ClefError(-1, "q, k, v must share a dtype; q and k a token stride")
         self._decays(g, Hv)
         if out is None:

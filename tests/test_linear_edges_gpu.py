@@ -272,3 +272,34 @@ def test_many_sequences_of_two_units(clef):
     for s in (0, 143, 255, 256, 257, 399):
         part = slice(s * n, (s + 1) * n)
         check(out[part], final[s], q[part].cpu(), k[part].cpu(), v[part].cpu(), g, scan.scale, init[s].cpu())
+
+
+# ---------------------------------------------------------------------------- views
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_one_token_from_different_buffers(clef, dtype):
+    """A single row has no token stride: q, k, v (and g, beta) as rows of buffers of any pitch."""
+    Hk, Hv, dk, dv = 2, 4, 64, 32
+    q, k, v = _inputs(1, 1, Hk, Hv, dk, dv, dtype)
+    g, gates, beta = _slopes(Hv), -_randn(2, 1, Hv).abs(), torch.sigmoid(_randn(3, 1, Hv))
+
+    def view(x, pitch):  # the row as the second of a wider buffer
+        n = x[0].numel()
+        buf = torch.zeros((3, n + pitch), dtype=x.dtype, device="cuda")
+        buf[1, :n] = x.reshape(-1).cuda()
+        return torch.as_strided(buf, x.shape, (n + pitch,) + x.stride()[1:], n + pitch)
+
+    cq, ck, cv = view(q, 8), view(k, 24), view(v, 40)
+    state = _randn(4, 1, Hv, dk, dv).cuda()
+    linear, delta = clef.LinearScan(dk, dv), clef.DeltaScan(dk, dv)
+    packed = _cuda(q, k, v)
+    a, b = state.clone(), state.clone()
+    assert torch.equal(linear.step(cq, ck, cv, g.cuda(), a), linear.step(*packed, g.cuda(), b)) and torch.equal(a, b)
+    a, b = state.clone(), state.clone()
+    assert torch.equal(delta.step(cq, ck, cv, view(gates, 3), view(beta, 5), a),
+                       delta.step(*packed, gates.cuda(), beta.cuda(), b)) and torch.equal(a, b)
+    one, two = (linear.prefill(*x, g.cuda(), initial=state[0]) for x in ((cq, ck, cv), packed))
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    one, two = (linear.prefill_varlen(*x, g.cuda(), cu) for x in ((cq, ck, cv), packed))
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
