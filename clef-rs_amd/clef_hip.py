@@ -725,6 +725,9 @@ def attention_gated_shared(q, k, vt, gate, cu_seqlens, key_starts, key_lens, pre
     gs = gate.stride()
     if len(gs) != 3 or gs[2] != 1 or gate.shape[:2] != (T, heads) or gate.shape[2] < d or gate.dtype != q.dtype:
         raise ClefError(-1, "gate must be a [T, heads, d] view of q's dtype")
+    # one row, or one head, has no stride
+    hsg = gs[1] if heads > 1 else d
+    ldg = gs[0] if T > 1 else (heads - 1) * hsg + d
     if out is None:
         out = q.new_empty((T, heads * d))
     elif out.shape != (T, heads * d) or out.stride(1) != 1 or out.dtype != q.dtype:
@@ -739,7 +742,8 @@ def attention_gated_shared(q, k, vt, gate, cu_seqlens, key_starts, key_lens, pre
     _check(L.clef_attention_gated_shared(
         q.data_ptr(), T, _ptr(prefix_k), np_, _ptr(prefix_vt), ldpv, np_, _ptr(k), rows, _ptr(vt), ldv,
         cu_seqlens.data_ptr(), _ptr(key_starts), _ptr(key_lens), nseq, T, max_keys, dt, heads, kvh, d,
-        gate.data_ptr(), gs[0], gs[1], out.data_ptr(), out.stride(0), _ptr(ws), n if ws is not None else 0, _stream()))
+        gate.data_ptr(), ldg, hsg, out.data_ptr(), out.stride(0) if T > 1 else heads * d, _ptr(ws),
+        n if ws is not None else 0, _stream()))
     return out
 
 

@@ -18,6 +18,21 @@ def clef():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_one_token_of_strided_views(clef, dtype):
+    """One query row: the gate may be a head-major view, whose token stride is shorter than a row, and out any row."""
+    heads, kvh, d, prefix = 6, 2, 64, 40
+    b = Batch(dtype, heads, kvh, d, prefix, [1], [9], [3], 16)
+    args = b.cuda()
+    want = clef.attention_gated_shared(**args)
+    b.check(want)
+    gate = args["gate"].transpose(0, 1).contiguous().transpose(0, 1)
+    assert gate.stride() == (d, d, 1)
+    out = torch.as_strided(torch.zeros(heads * d, dtype=dtype, device="cuda"), (1, heads * d), (1, 1))
+    assert torch.equal(clef.attention_gated_shared(**{**args, "gate": gate}, out=out), want)
+
+
+@gpu
 @pytest.mark.parametrize("prefix,max_keys", [(16, 8), (300, 8), (300, 2000)], ids=["one launch", "fused", "parts"])
 def test_most_tokens_of_most_heads(clef, prefix, max_keys):
     """65,536 tokens of 256 key heads, the limits of a call, in each of its forms.  An f16 output is off by 2^-11
