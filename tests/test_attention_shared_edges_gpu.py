@@ -66,3 +66,30 @@ def test_most_tokens_of_most_heads(clef, prefix, max_keys):
         bound = (2.0 ** -11 + 2.0 ** -12) * size + 2.0 ** -25 * small + 2.0 ** -11 * want.abs() + 2.0 ** -25
         err = (y[a:b].view(each, heads, d).transpose(0, 1).float() - want).abs()
         assert (err <= bound).all(), f"request {s}: {float((err / bound).max()):.3g} of the bound"
+
+
+TABLES = [
+    # heads, kvh, d, prefix, requests, rows of the cache, max_keys
+    (4, 2, 64, 50, 5, 176, 176),       # one launch
+    (16, 2, 256, 600, 5, 176, 100),    # own keys as parts, 40 rows of a key head
+    (16, 2, 256, 600, 97, 176, 130),   # beside the joining, 128-row groups
+    (4, 4, 72, 300, 9, 176, 90),       # as parts, 16-row groups of a padded width
+    (8, 8, 72, 300, 30, 2048, 1500),   # long own keys in many parts
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("table", TABLES, ids=lambda c: "-".join(str(x) for x in c))
+def test_starts_and_lengths_that_do_not_fit(clef, table, dtype):
+    """key_starts and key_lens outside the cache: cut to it, in every form of the call."""
+    heads, kvh, d, prefix, requests, rows, max_keys = table
+    b = Batch(dtype, heads, kvh, d, prefix, [1] * requests, [rows] + [0] * (requests - 1), [0] * requests, rows)
+    odd = [(-5, 10), (10 ** 9, 10), (2 ** 31 - 1, 10), (-2 ** 31, 2 ** 31 - 1), (0, -1), (rows - 6, 2 ** 31 - 1),
+           (3, 10 ** 6), (rows, 1), (rows - 1, 1), (17, -2 ** 31), (rows // 2, rows)]
+    pairs = [odd[s % len(odd)] for s in range(requests)]
+    args = b.cuda()
+    args["key_starts"], args["key_lens"] = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in zip(*pairs))
+    b.starts = [min(max(a, 0), rows) for a, _ in pairs]
+    b.lens = [min(max(n, 0), max_keys, rows - a) for a, (_, n) in zip(b.starts, pairs)]
+    b.check(clef.attention_gated_shared(**args, max_keys=max_keys))
