@@ -22,7 +22,8 @@
 // values stored by feature, whose rows are operands as they lie in memory.
 // The maximum only moves (and O is only rescaled) when it grows by more than 8
 // in log2 units; sums and O are f32, the weights are rounded once, to the
-// operands' type.
+// operands' type.  f16 weights, sums and O are 2^7 times as large (up to 2^15), so
+// that weights down to 2^-32 of the reference's are not lost in sums of many.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -62,16 +63,18 @@ struct SharedParams {
 };
 
 // as in the linear scan: fragments of KB k-indices (EL per lane), TPB tiles of
-// 16 accumulator rows to a block of KB
+// 16 accumulator rows to a block of KB; UP: log2 of what weights are multiplied by
 template <class T> struct Ops;
 template <> struct Ops<half_t> {
   typedef half8 frag;
   static constexpr int KB = 32, EL = 8, TPB = 2;
+  static constexpr float UP = 7.0f;
   static __device__ __forceinline__ int row(int t, int r) { return 8 * (r >> 2) + 4 * t + (r & 3); }
 };
 template <> struct Ops<float> {
   typedef float4_t frag;
   static constexpr int KB = 16, EL = 4, TPB = 1;
+  static constexpr float UP = 0.0f;
   static __device__ __forceinline__ int row(int, int r) { return r; }
 };
 
@@ -152,7 +155,7 @@ struct Soft {
 #pragma unroll
         for (int e = 0; e < NE; ++e) o[e][x] *= f;
       }
-      const float ref = m[x] == -INFINITY ? 0.0f : m[x];
+      const float ref = (m[x] == -INFINITY ? 0.0f : m[x]) - Ops<T>::UP;
 #pragma unroll
       for (int a = 0; a < NB * TPB; ++a)
 #pragma unroll
@@ -555,7 +558,7 @@ __global__ __launch_bounds__(512, 2) void shared_many_rows(SharedParams p) {
       }
       lds_barrier();
     }
-    const float ref = m == -INFINITY ? 0.0f : m;
+    const float ref = (m == -INFINITY ? 0.0f : m) - Ops<T>::UP;
     half8 w[2];
     float top = -INFINITY;
 #pragma unroll

@@ -93,3 +93,31 @@ def test_starts_and_lengths_that_do_not_fit(clef, table, dtype):
     b.starts = [min(max(a, 0), rows) for a, _ in pairs]
     b.lens = [min(max(n, 0), max_keys, rows - a) for a, (_, n) in zip(b.starts, pairs)]
     b.check(clef.attention_gated_shared(**args, max_keys=max_keys))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d", [64, 72])
+def test_many_far_keys_beside_a_near_one(clef, d, dtype):
+    """2^18 keys 17.5 below the score of one: each has a weight of 2^-25.2 of the largest, all of them 0.66 % of the
+    sum.  Rows enough that no work-group has fewer than all keys.  A weight is rounded to f16 by 2^-11 of itself
+    or by 2^-25 of 2^-7 of the row's reference (the largest key's, or up to 2^8 times less), 2^-32 n = 2^-14 in
+    all; scores and sums of n equal terms in f32 by 2^-24 of the score and, running, of n: 2^-18 and 2^-7 at the
+    very worst, of these 0.66 %."""
+    T, heads, n = 2100, 16, 1 << 18
+    if dtype == F32:
+        n = 1 << 15
+    gap = 17.5
+    q = torch.zeros((heads, T, d), dtype=dtype, device="cuda")
+    q[:, :, 0] = 16.0
+    pk = torch.zeros((1, n, d), dtype=dtype, device="cuda")
+    pk[0, 3, 0] = gap * d ** 0.5 / 16
+    pvt = torch.ones((1, d, n), dtype=dtype, device="cuda")
+    pvt[0, :, 3] = 0.0
+    gate = torch.full((T, heads, d), 100.0, dtype=dtype, device="cuda")  # open
+    cu = torch.arange(T + 1, dtype=torch.int32, device="cuda")
+    y = clef.attention_gated_shared(q, None, None, gate, cu, None, None, prefix_k=pk, prefix_vt=pvt)
+    far = (n - 1) * torch.exp(-q[0, 0, 0].double() * pk[0, 3, 0].double() / d ** 0.5)
+    want = far / (1 + far)
+    bound = want * (2.0 ** -10 + 2.0 ** -18 + 2.0 ** -7) + 2.0 ** -14
+    assert ((y.double() - want).abs() <= bound).all(), f"{float(y.double().mean())} for {float(want)}"
