@@ -469,8 +469,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
           float up = 1.0f;
           if constexpr (sizeof(T) == 2) {
             // f16: where a query's largest score of the block is not in 2^-10 .. 2^15, scaled to
-            // 2^13 .. 2^14, by up to 2^40 (the output of the state meets the scores at that
-            // scale, and fits it up to 2^86)
+            // 2^13 .. 2^14, by up to 2^40 (the output of the state meets them at that scale)
             float big = 0.0f, down = 1.0f;
 #pragma unroll
             for (int e = 0; e < EL; ++e) big = fmaxf(big, fabsf(y[e]));
@@ -547,9 +546,16 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
                 if (b * KB > qt * 16 + 15) continue;
                 const int job = qt * NCB + b;
                 const float down = decltype(scaled)::value ? sD[job * 16 + r] : 1.0f;
+                const float4_t before = o[qt];
                 if (scaled) o[qt] *= inverse(down);
                 Mma<T>::mma(o[qt], fv[b], frag_at(sP + (job * 64 + ln) * EL));
-                if (scaled) o[qt] *= down;
+                if (scaled) {
+                  o[qt] *= down;
+                  // beside what is too large for that scale, scores that were scaled up vanish
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    if (down < 1.0f && fabsf(before[e]) >= 0x1p80f) o[qt][e] = before[e];
+                }
               }
           };
           if (sizeof(T) == 2 && __any(sScaled[ln % NW])) add_values(std::true_type{});

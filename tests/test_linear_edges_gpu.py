@@ -303,3 +303,22 @@ def test_one_token_from_different_buffers(clef, dtype):
     cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
     one, two = (linear.prefill_varlen(*x, g.cuda(), cu) for x in ((cq, ck, cv), packed))
     assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+
+
+@gpu
+@pytest.mark.parametrize("size", [1e28, 1e34])
+def test_huge_states_beside_small_scores(clef, size):
+    """The output of a state far beyond f16 next to scores that have to be scaled up."""
+    T, H, d = 70, 1, 64
+    q, k, v = _inputs(5, T, H, H, d, d, F16)
+    q = (q.float() * 2.0 ** -6).to(F16)
+    k = (k.float() * 2.0 ** -12).to(F16)
+    init = _randn(6, H, d, d) * size
+    init[:, :, ::2] = 0.0  # every other column has its scores alone
+    g = torch.tensor([-0.05])
+    scan = clef.LinearScan(d, d)
+    out, _ = scan.prefill(*_cuda(q, k, v, g), initial=init.cuda())
+    want, _ = reference(q, k, v, g, scan.scale, init)
+    mo, _ = reference(q.abs(), k.abs(), v.abs(), g, scan.scale, init.abs())
+    bound = (2.0 ** -10 + (d + T + 8) * 2.0 ** -24) * mo
+    assert ((out.double().cpu() - want).abs() <= bound).all()
