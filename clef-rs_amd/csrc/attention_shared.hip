@@ -732,11 +732,17 @@ Plan plan_of(int T, int np, int max_keys, int dtype, int heads, int kvh, int d) 
   Plan x{};
   const int64_t rows = (int64_t)T * (heads / kvh);
   const int cus = device_cus();
-  // At most one block of the prefix to a wave: one launch of 8 waves per token and
-  // key head, which read the prefix for themselves.  (A block takes a CU about 5 us,
-  // most of it the 256 KiB that its waves read: 2 requests behind 512 keys, two
-  // blocks to a wave, took 20.7 us so and take 10.4 us in parts.)
-  x.walk = np <= 8 * (dtype == CLEF_F16 ? Ops<half_t>::KB : Ops<float>::KB) && max_keys <= kFinishKeys;
+  // At most one block of the prefix to a wave, and a few work-groups to a CU: one launch
+  // of 8 waves per token and 8 heads of a key head, which read the prefix for themselves.
+  // (A block takes a CU about 5 us, most of it the 256 KiB that its waves read: 2 requests
+  // behind 512 keys, two blocks to a wave, took 20.7 us so and take 10.4 us in parts.  16
+  // heads of 2 key heads, d = 256, f16, behind 256 keys with up to 64 own, at 64, 256, 1,024
+  // and 4,096 requests: 15, 29, 106 and 466 us so, 21, 31, 69 and 263 in parts; 8 heads of
+  // one, d = 64: 13, 13, 16 and 59 so, 17, 17, 18 and 42; 16 of 2, d = 256, f32, behind 128
+  // keys: 20, 44, 173 and 718 so, 21, 42, 143 and 592.)
+  const int64_t walks = (int64_t)T * kvh * ((heads / kvh + kFinishRows - 1) / kFinishRows);
+  x.walk = np <= 8 * (dtype == CLEF_F16 ? Ops<half_t>::KB : Ops<float>::KB) && max_keys <= kFinishKeys &&
+           (np == 0 || walks <= 4 * cus);
   if (x.walk) return x;
   // 24 rows of a key head behind 8,192 and 32,768 keys take 28 and 42 us with the
   // 128-row groups and took 33 and 50 with 32-row ones; 16 rows behind 32,768 keys

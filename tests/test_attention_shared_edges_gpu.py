@@ -33,7 +33,8 @@ def test_one_token_of_strided_views(clef, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("prefix,max_keys", [(16, 8), (300, 8), (300, 2000)], ids=["one launch", "fused", "parts"])
+@pytest.mark.parametrize("prefix,max_keys", [(16, 8), (0, 8), (300, 8), (300, 2000)],
+                         ids=["short", "one launch", "beside", "parts"])
 def test_most_tokens_of_most_heads(clef, prefix, max_keys):
     """65,536 tokens of 256 key heads, the limits of a call, in each of its forms.  An f16 output is off by 2^-11
     of itself, its f16 weights by 2^-11 of the sum of |v| under them or by 2^-25 of the largest, its f32 sums
@@ -46,11 +47,12 @@ def test_most_tokens_of_most_heads(clef, prefix, max_keys):
     ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
     q, gate = randn(heads, T, d), randn(T, heads, d)
     pk, pvt = randn(heads, prefix, d), randn(heads, d, (prefix + 7) // 8 * 8)
+    before = dict(prefix_k=pk, prefix_vt=pvt) if prefix else {}
     k, vt = randn(heads, nseq * own, d), randn(heads, d, nseq * own)
     each = T // nseq
     y = clef.attention_gated_shared(q, k, vt, gate, ints([each * s for s in range(nseq + 1)]),
-                                    ints([own * s for s in range(nseq)]), ints([own] * nseq), prefix_k=pk,
-                                    prefix_vt=pvt, max_keys=max_keys)
+                                    ints([own * s for s in range(nseq)]), ints([own] * nseq), max_keys=max_keys,
+                                    **before)
     for s in range(nseq):  # the last `own` queries of a request see own keys, 1 to all of them
         a, b = each * s, each * (s + 1)
         keys = torch.cat([pk, k[:, own * s:own * (s + 1)]], 1).float()
@@ -59,7 +61,7 @@ def test_most_tokens_of_most_heads(clef, prefix, max_keys):
         scores = q[:, a:b].float() @ keys.transpose(1, 2).contiguous() / d ** 0.5
         sees = (torch.arange(a, b, device="cuda") - (b - own) + 1).clamp(min=0)
         scores.masked_fill_(torch.arange(prefix + own, device="cuda")[None] >= prefix + sees[:, None], float("-inf"))
-        w = torch.softmax(scores, -1)
+        w = torch.softmax(scores, -1).nan_to_num(0.0)  # no key: zeros
         g = torch.sigmoid(gate[a:b].float()).transpose(0, 1)
         want, size = (w @ values) * g, (w @ values.abs()) * g
         small = w.amax(-1, keepdim=True) * values.abs().sum(1)[:, None] * g
