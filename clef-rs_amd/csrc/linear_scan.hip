@@ -299,6 +299,12 @@ __device__ __forceinline__ Scale scale_of(float big, uint32_t least) {
 // the inverse of a power of two (a normal one)
 __device__ __forceinline__ float inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
 
+// A bit for each r = 0 .. 15 that is set in `m` at r, r + 16, r + 32 or r + 48.
+__device__ __forceinline__ uint32_t of_queries(uint64_t m) {
+  m |= m >> 32;
+  return (uint32_t)(m | m >> 16) & 0xffffu;
+}
+
 // LDS of a work-group (elements of T): k, v, q, scores.
 template <class T, int DK, int DV, bool OUT>
 struct Shared {
@@ -309,10 +315,11 @@ struct Shared {
   // powers of the decay: f32 words behind the tiles.  W[i] = l^{C-1-i}, S[i] =
   // scale l^{C-1-i}, both 0 from i = C on (tokens behind the query or the chunk)
   static constexpr int POW = (ALL * (int)sizeof(T) + 15) / 16 * 16;
-  // f16: what the scores of a query and key block are scaled back by
-  static constexpr int DOWN = POW + 4 * 2 * C * (OUT ? 2 : 1);
-  static constexpr int SCALED = DOWN + (OUT && sizeof(T) == 2 ? 4 * C * (C / Ops<T>::KB) : 0);  // a word for each wave
-  static constexpr int ODD = SCALED + (OUT && sizeof(T) == 2 ? 4 * (DV / 16) : 0);  // the same
+  // f16: what the scores of a query and key block are scaled back by, and whether any of a
+  // job's (16 queries, a key block) are
+  static constexpr int JOBS = OUT && sizeof(T) == 2 ? C / 16 * (C / Ops<T>::KB) : 0;
+  static constexpr int DOWN = POW + 4 * 2 * C * (OUT ? 2 : 1), SCALED = DOWN + 4 * 16 * JOBS;
+  static constexpr int ODD = SCALED + 4 * JOBS;  // a word for each wave
   static constexpr int BYTES = ODD + 4 * (DV / 16);
 };
 
@@ -442,7 +449,6 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
       const bool odd = CAREFUL && __any(sOdd[ln % NW]);
       if constexpr (OUT) {
         // ---- scores, transposed: keys of block b x queries of tile qt
-        int scaled = 0;  // any of the wave's scores
 #pragma unroll
         for (int job = wave; job < QT * NCB; job += NW) {
           const int qt = job / NCB, b = job % NCB;
@@ -471,26 +477,26 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
             // f16: where a query's largest score of the block is not in 2^-10 .. 2^15, scaled to
             // 2^13 .. 2^14, by up to 2^40 (the output of the state meets them at that scale)
             float big = 0.0f, down = 1.0f;
+            int scaled = 0;
 #pragma unroll
             for (int e = 0; e < EL; ++e) big = fmaxf(big, fabsf(y[e]));
-            auto of_queries = [](uint64_t m) { return (uint32_t)(m | m >> 32) | (uint32_t)((m | m >> 32) >> 16); };
             const uint32_t some = of_queries(__ballot(big > 0.0f)), enough = of_queries(__ballot(big >= 0x1p-10f));
-            if (((some & ~enough) & 0xffffu) || __any(big >= 0x1p15f)) {
+            if ((some & ~enough) || __any(big >= 0x1p15f)) {
               big = max4(big);
               if (big < 0x1p-10f || big >= 0x1p15f) {  // the others as if these were not there
                 const Scale x = scale_of(big, 100);
                 up = x.up;
                 down = x.down;
               }
+              if (grp == 0) sD[job * 16 + r] = down;
               scaled = 1;
             }
-            if (grp == 0) sD[job * 16 + r] = down;
+            if (ln == 0) sScaled[job] = scaled;
           }
 #pragma unroll
           for (int e = 0; e < EL; ++e) f[e] = static_cast<T>(y[e] * up);
           *reinterpret_cast<frag*>(sP + (job * 64 + ln) * EL) = f;
         }
-        if (sizeof(T) == 2 && ln == 0) sScaled[wave] = scaled;
         lds_barrier();
 
         // ---- outputs, transposed: value columns x queries
@@ -538,27 +544,36 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[qt][e] *= down[e] * w;
           }
-          auto add_values = [&](auto scaled) __attribute__((always_inline)) {
+          // a bit for each job whose scores are scaled (those of keys behind every query: none)
+          uint32_t scaled = 0;
+          if constexpr (sizeof(T) == 2) {
+            constexpr uint32_t jobs = 0xf5;
+            static_assert(QT == 4 && NCB == 2 && NW <= QT * NCB, "jobs 1 and 3 hold no keys that a query sees");
+            scaled = (uint32_t)__ballot(sScaled[ln % (QT * NCB)] != 0) & jobs;
+          }
+          auto add_values = [&](auto any) __attribute__((always_inline)) {
 #pragma unroll
             for (int b = 0; b < NCB; ++b)
 #pragma unroll
               for (int qt = 0; qt < QT; ++qt) {
                 if (b * KB > qt * 16 + 15) continue;
                 const int job = qt * NCB + b;
-                const float down = decltype(scaled)::value ? sD[job * 16 + r] : 1.0f;
-                const float4_t before = o[qt];
-                if (scaled) o[qt] *= inverse(down);
-                Mma<T>::mma(o[qt], fv[b], frag_at(sP + (job * 64 + ln) * EL));
-                if (scaled) {
+                if (any && (scaled >> job & 1)) {
+                  const float down = sD[job * 16 + r];
+                  const float4_t before = o[qt];
+                  o[qt] *= inverse(down);
+                  Mma<T>::mma(o[qt], fv[b], frag_at(sP + (job * 64 + ln) * EL));
                   o[qt] *= down;
                   // beside what is too large for that scale, scores that were scaled up vanish
 #pragma unroll
                   for (int e = 0; e < 4; ++e)
                     if (down < 1.0f && fabsf(before[e]) >= 0x1p80f) o[qt][e] = before[e];
+                } else {
+                  Mma<T>::mma(o[qt], fv[b], frag_at(sP + (job * 64 + ln) * EL));
                 }
               }
           };
-          if (sizeof(T) == 2 && __any(sScaled[ln % NW])) add_values(std::true_type{});
+          if (scaled) add_values(std::true_type{});
           else add_values(std::false_type{});
           if (odd) {
 #pragma unroll 1
@@ -574,7 +589,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
                 for (int qt = 0; qt < QT; ++qt)
                   if (j <= qt * 16 + r) {
                     float score = to_f32(pj[qt * NCB * 64 * EL]);
-                    if constexpr (sizeof(T) == 2) score *= sD[(qt * NCB + j / KB) * 16 + r];
+                    if (scaled >> (qt * NCB + j / KB) & 1) score *= sD[(qt * NCB + j / KB) * 16 + r];
                     o[qt][e] = fmaf(score, v, o[qt][e]);
                   }
               }
