@@ -188,7 +188,7 @@ def _scratch(n, device):
 
 
 def _index(t, n, name):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+    if t is None or t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
         raise ClefError(-1, f"{name} must be a contiguous int32 device tensor [{n}]")
 
 

@@ -184,3 +184,14 @@ def test_bad_unit_tables_stay_inside(nseq, T, unit):
         for _ in units.walk():
             pass
         units.join()
+
+
+def test_missing_starts_and_lengths_are_refused():
+    torch = pytest.importorskip("torch")
+    clef = pytest.importorskip("clef_hip")
+    q, gate = torch.zeros(4, 2, 64), torch.zeros(2, 4, 64)
+    k, vt = torch.zeros(2, 16, 64), torch.zeros(2, 64, 16)
+    cu, table = torch.tensor([0, 1, 2], dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for starts, lens in ((None, table), (table, None), (None, None)):
+        with pytest.raises(clef.ClefError, match="int32 device tensor"):
+            clef.attention_gated_shared(q, k, vt, gate, cu, starts, lens)
