@@ -13,7 +13,7 @@
 // is cut into units of whole chunks: one launch forms what each unit adds to
 // a zero state, a second joins these into the state that each unit starts
 // from, a third walks the units side by side.  Prompts of one unit take the
-// third alone.  16,384 tokens of 32 heads, 128 x 128, f16: 54 + 11 + 130 us, where
+// third alone.  16,384 tokens of 32 heads, 128 x 128, f16: 56 + 12 + 140 us, where
 // q, k, v and o once are 82 us at the rate of a copy; keys and values pass twice,
 // and the walk is bound by a chunk's chain of products, barriers and LDS reads.
 //
@@ -220,8 +220,8 @@ struct Staged {
   }
   // Rows of at least a vector, at any alignment: what lies behind `rows` is read from
   // the last row, a vector that would end behind `width` from the row's end; store()
-  // mends both.  (Value by value, 4096 tokens of 32 heads took 115 us at 128 x 13 and
-  // 119 us at 100 x 72; so, 54 and 67.)
+  // mends both.  (Value by value, 4096 tokens of 32 heads take 119 us at 128 x 13 and
+  // 122 us at 100 x 72; so, 59 and 68.)
   __device__ __forceinline__ void load_wide(const T* src, int64_t stride, int rows, int width, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -329,7 +329,8 @@ struct Shared {
 //
 // f16: at most 128 registers a lane, so that two work-groups of 8 waves share a CU
 // and one's products cover the other's barriers and loads (8 waves with two v-heads each,
-// which share the scores, took 133 us for the walk of 16,384 tokens x 32 heads).
+// which share the scores, took 133 us for the walk of 16,384 tokens x 32 heads where
+// this then took 131).
 template <class T, class O, int DK, int DV, bool OUT>
 __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1)) void linear_chunks(LinearParams p) {
   constexpr int NW = DV / 16, THREADS = 64 * NW;  // a wave for 16 value columns
@@ -773,11 +774,11 @@ int linear_dims(int T, int nseq, int Hk, int Hv, int dk, int dv, int dtype_qkv) 
 // Tokens of a unit: enough units that the work-groups fill the chip, one to a CU,
 // or two for f16 once the units are long enough that one covering the other's
 // waits saves more than the joining of twice the units costs.  us at one and two
-// to a CU, 128 x 128: 1,200 tokens of 32 heads 33 and 38, 2,400 46 and 50, 8,192
-// of 8 heads 49 and 59; 6,000 of 32 heads 88 and 84, 16,384 230 and 214; for f32
-// (which has LDS for one) 4,096 of 32 heads 172 and 186.  And no f16 unit shorter
-// than 2 chunks (600 tokens of 32 heads 31 us, in chunks 33; of f32, whose chunks
-// take longer, 300 tokens 48 us in units of two, 37 in chunks).
+// to a CU, 128 x 128: 1,200 tokens of 32 heads 37 and 41, 2,400 51 and 54, 8,192
+// of 8 heads 52 and 61; 6,000 of 32 heads 95 and 88, 16,384 229 and 200; for f32
+// (which has LDS for one) 4,096 of 32 heads 179 and 191.  And no f16 unit shorter
+// than 2 chunks (400 tokens of 32 heads 27.5 us, in chunks 28.5; of f32, whose chunks
+// take longer, 300 tokens 50 us in units of two, 38 in chunks).
 int unit_tokens(int T, int Hv, int dtype) {
   const int cus = device_cus();
   const int64_t work = (int64_t)T * Hv, once = (work + cus - 1) / cus, twice = (once + 1) / 2;

@@ -410,7 +410,8 @@ int clef_attention_gated_varlen(const void* q, int64_t ldq_tok, const void* k, i
  * query i sees the np prefix keys and the sequence's own keys 0 .. len - n + i,
  *   y[t, h*d + e] = attn(...)[h, t, e] * sigmoid(gate[t, h, e]).
  * Own keys live in a cache with room: key j of sequence s is row key_starts[s]
- * + j of k [kv_heads, ldk_tok, d] and vt [kv_heads, d, ldv_tok] (any start).
+ * + j of k [kv_heads, ldk_tok, d] and vt [kv_heads, d, ldv_tok] (any start; the
+ * cache ends with the shorter of the two).
  * max_keys bounds len (longer ones are cut to it), so that cu_seqlens,
  * key_starts and key_lens, all device int32, may change under a captured
  * launch.  A query that sees no key gives zeros; keys that no query of its
@@ -425,7 +426,7 @@ int clef_attention_gated_varlen(const void* q, int64_t ldq_tok, const void* k, i
  * ldv_tok up to 2^30.  A table that does not fit gives unspecified values, never
  * an access out of bounds.
  * workspace: clef_attention_shared_workspace bytes, 256-byte aligned; where that
- * is 256 (short prefixes), nothing is kept there and workspace may be NULL.  No
+ * is 256 (a few rows behind a short prefix), nothing is kept there and workspace may be NULL.  No
  * counterpart in the reference (one request per flash-attention call there).
  */
 size_t clef_attention_shared_workspace(int T, int nseq, int np, int max_keys, int dtype, int heads, int kv_heads,
