@@ -288,12 +288,12 @@ __device__ __forceinline__ float max4(float x) {  // over the 4 lanes of one col
   return fmaxf(x, __shfl_xor(x, 32, 64));
 }
 // The power of two that brings `big` >= 0 to 2^13 .. 2^14, as a factor for f16, and its
-// inverse; up to 2^(140 - least).
+// inverse; from 2^-113 on, so that both are normal f32 numbers.
 struct Scale {
   float up, down;
 };
-__device__ __forceinline__ Scale scale_of(float big, uint32_t least) {
-  const uint32_t ex = max(__float_as_uint(big) >> 23, least);  // sign clear
+__device__ __forceinline__ Scale scale_of(float big) {
+  const uint32_t ex = max(__float_as_uint(big) >> 23, 14u);  // sign clear
   return {__uint_as_float((267u - ex) << 23), __uint_as_float((ex - 13u) << 23)};
 }
 // the inverse of a power of two (a normal one)
@@ -476,7 +476,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
           float up = 1.0f;
           if constexpr (sizeof(T) == 2) {
             // f16: where a query's largest score of the block is not in 2^-10 .. 2^15, scaled to
-            // 2^13 .. 2^14, by up to 2^40 (the output of the state meets them at that scale)
+            // 2^13 .. 2^14 (the output of the state meets them at that scale)
             float big = 0.0f, down = 1.0f;
             int scaled = 0;
 #pragma unroll
@@ -485,7 +485,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
             if ((some & ~enough) || __any(big >= 0x1p15f)) {
               big = max4(big);
               if (big < 0x1p-10f || big >= 0x1p15f) {  // the others as if these were not there
-                const Scale x = scale_of(big, 100);
+                const Scale x = scale_of(big);
                 up = x.up;
                 down = x.down;
               }
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
             for (int a = 0; a < NKB * TPB; ++a)
 #pragma unroll
               for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(S[a][i]));
-            const Scale scale = scale_of(max4(big), 14);  // (both normal f32 numbers)
+            const Scale scale = scale_of(max4(big));
             up = scale.up;
             const float back = first * scale.down;
 #pragma unroll
@@ -568,7 +568,7 @@ __global__ __launch_bounds__(DV * 4, (sizeof(T) == 2 ? 4 : 2) / (DK > DV ? 2 : 1
                   // beside what is too large for that scale, scores that were scaled up vanish
 #pragma unroll
                   for (int e = 0; e < 4; ++e)
-                    if (down < 1.0f && fabsf(before[e]) >= 0x1p80f) o[qt][e] = before[e];
+                    if (down < 1.0f && fabsf(before[e]) >= down * 0x1p120f) o[qt][e] = before[e];
                 } else {
                   Mma<T>::mma(o[qt], fv[b], frag_at(sP + (job * 64 + ln) * EL));
                 }

@@ -306,6 +306,29 @@ def test_one_token_from_different_buffers(clef, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("scale", [1e-30, 1e-20, -3.0, 1e20])
+def test_any_scale(clef, scale, dtype):
+    """The scale of the outputs is any finite number: scores of 2^-100 and 2^66 keep f16's relative precision."""
+    T, H, d = 150, 2, 64
+    q, k, v = _inputs(4, T, H, H, d, d, dtype)
+    init = _randn(6, H, d, d)
+    g = torch.tensor([-0.01, -0.1])
+    out, _ = clef.LinearScan(d, d, scale=scale).prefill(*_cuda(q, k, v, g), initial=init.cuda())
+    want, _ = reference(q, k, v, g, scale, init)
+    mo, _ = reference(q.abs(), k.abs(), v.abs(), g, abs(scale), init.abs())
+    top = (q.double().abs().transpose(0, 1) @ k.double().abs().permute(1, 2, 0)).amax(2).t()[..., None] * abs(scale)
+    rel = 2.0 ** -11 if dtype == F16 else 0.0
+    bound = (rel + (d + T + 8) * 2.0 ** -24) * mo
+    if dtype == F16:  # factors below f16's normal range, of the largest score and of the largest state entry
+        kept = reference(q.abs(), k.abs(), v.abs(), torch.zeros(H), 1.0, init.abs())[1].amax()
+        bound = bound + 2.0 ** -15 * top * v.double().abs().sum(0) + \
+            2.0 ** -38 * kept * abs(scale) * q.double().abs().sum(2)[..., None]
+    err = (out.double().cpu() - want).abs()
+    assert (err <= bound).all(), f"{float((err / bound).max()):.3g} of the bound"
+
+
+@gpu
 @pytest.mark.parametrize("size", [1e28, 1e34])
 def test_huge_states_beside_small_scores(clef, size):
     """The output of a state far beyond f16 next to scores that have to be scaled up."""
