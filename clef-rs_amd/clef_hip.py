@@ -87,6 +87,13 @@ SIGNATURES = {
     "clef_attention_shared_workspace": (_z, [_i] * 8),
     "clef_attention_gated_shared": (_i, [_p, _l, _p, _l, _p, _l, _i, _p, _l, _p, _l, _p, _p, _p, _i, _i, _i, _i, _i,
                                          _i, _i, _p, _l, _l, _p, _l, _p, _z, _p]),
+    "clef_paged_append": (_i, [_p, _p, _i, _p, _p, _i, _i, _p, _l, _l, _p, _l, _p, _l, _i, _p, _p, _f, _p, _l, _i, _p, _i,
+                               _d, _p, _l, _p]),
+    "clef_attention_paged_workspace": (_z, [_i] * 8),
+    "clef_attention_gated_paged": (_i, [_p, _p, _i, _p, _p, _i, _i, _p, _l, _i, _p, _l, _l, _i, _i, _p, _l, _p, _p, _z,
+                                        _p]),
+    "clef_paged_weights": (_i, [_p, _p, _i, _p, _p, _i, _i, _p, _l, _i, _p, _i, _i, _p, _p, _p]),
+    "clef_paged_evict": (_i, [_p, _p, _i, _p, _i, _p, _i, _i, _i, _p, _p, _i, _p, _p, _p, _p]),
     "clef_embed": (_i, [_p, _i, _p, _i, _i, _i, _p, _p]),
     "clef_head_logits": (_i, [_p, _i, _p, _i, _p, _p]),
 }
@@ -695,6 +702,22 @@ def _keys(k, vt, d, dtype, name):
     return k.shape[0], k.shape[1], vt.shape[2]
 
 
+def _gate_and_out(q, gate, out):
+    """(gate token stride, gate head stride, out) of a gated attention of q [heads, T, d]."""
+    heads, T, d = q.shape
+    gs = gate.stride()
+    if len(gs) != 3 or gs[2] != 1 or gate.shape[:2] != (T, heads) or gate.shape[2] < d or gate.dtype != q.dtype:
+        raise ClefError(-1, "gate must be a [T, heads, d] view of q's dtype")
+    # one row, or one head, has no stride
+    hsg = gs[1] if heads > 1 else d
+    ldg = gs[0] if T > 1 else (heads - 1) * hsg + d
+    if out is None:
+        out = q.new_empty((T, heads * d))
+    elif out.shape != (T, heads * d) or out.stride(1) != 1 or out.dtype != q.dtype:
+        raise ClefError(-1, "out must be [T, heads * d] rows of q's dtype")
+    return ldg, hsg, out
+
+
 def attention_gated_shared(q, k, vt, gate, cu_seqlens, key_starts, key_lens, prefix_k=None, prefix_vt=None,
                            max_keys=None, out=None):
     """Requests of one to a few tokens behind one shared prefix, which is read once for
@@ -722,16 +745,7 @@ def attention_gated_shared(q, k, vt, gate, cu_seqlens, key_starts, key_lens, pre
     if (prefix_k is None) != (prefix_vt is None) or (k is None) != (vt is None) or not kvh:
         raise ClefError(-1, "keys and values come together, of a prefix, of the requests or of both")
     max_keys = rows if max_keys is None else min(int(max_keys), rows)
-    gs = gate.stride()
-    if len(gs) != 3 or gs[2] != 1 or gate.shape[:2] != (T, heads) or gate.shape[2] < d or gate.dtype != q.dtype:
-        raise ClefError(-1, "gate must be a [T, heads, d] view of q's dtype")
-    # one row, or one head, has no stride
-    hsg = gs[1] if heads > 1 else d
-    ldg = gs[0] if T > 1 else (heads - 1) * hsg + d
-    if out is None:
-        out = q.new_empty((T, heads * d))
-    elif out.shape != (T, heads * d) or out.stride(1) != 1 or out.dtype != q.dtype:
-        raise ClefError(-1, "out must be [T, heads * d] rows of q's dtype")
+    ldg, hsg, out = _gate_and_out(q, gate, out)
     _here(q, gate, cu_seqlens, out, prefix_k, prefix_vt)
     dt = _dt(q)
     L = lib()
@@ -745,6 +759,173 @@ def attention_gated_shared(q, k, vt, gate, cu_seqlens, key_starts, key_lens, pre
         gate.data_ptr(), ldg, hsg, out.data_ptr(), out.stride(0) if T > 1 else heads * d, _ptr(ws),
         n if ws is not None else 0, _stream()))
     return out
+
+
+# ---------------------------------------------------------------------------
+# A paged cache of keys and values
+# ---------------------------------------------------------------------------
+class PagedCacheDesc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("vt", C.c_void_p), ("k_stride", C.c_int64), ("vt_stride", C.c_int64)] + [
+        (n, C.c_int) for n in ("num_pages", "page", "kv_heads", "d", "dtype")]
+
+
+class PagedCache:
+    """Keys and values of many requests in the pages of one pool: k [pages, kvh, page, d]
+    and vt [pages, kvh, d, page] (views of a larger buffer may skip between pages; page
+    is 16, 32, 64, 128 or 256).  Request s's key j stands in slot j % page of page
+    pages[s, j // page] (`pages`: int32 [nseq, most pages of a request]).
+
+    The calls take a batch: T new tokens packed by cu_seqlens (int32 [nseq + 1]), and
+    key_lens (int32 [nseq]), each request's keys with the new tokens' own, which are the
+    last of them."""
+
+    def __init__(self, k, vt):
+        if k.dim() != 4 or vt.dim() != 4 or vt.shape != (k.shape[0], k.shape[1], k.shape[3], k.shape[2]):
+            raise ClefError(-1, "a cache has keys [pages, kvh, page, d] and values [pages, kvh, d, page]")
+        if k.dtype != vt.dtype:
+            raise ClefError(-1, "keys and values must share a dtype")
+        n = k.shape[0]
+        for t in (k, vt):
+            if n and not t[0].is_contiguous():
+                raise ClefError(-1, "a page must be contiguous")
+            if n > 1 and t.stride(0) < t[0].numel():
+                raise ClefError(-1, "pages must not overlap")
+        self.k, self.vt = k, vt
+        self.num_pages, self.kv_heads, self.page, self.d = k.shape
+        self.dtype = _dt(k)
+        self._desc = PagedCacheDesc(k.data_ptr(), vt.data_ptr(), k.stride(0) if n > 1 else 0,
+                                    vt.stride(0) if n > 1 else 0, n, self.page, self.kv_heads, self.d, self.dtype)
+        self._at = C.addressof(self._desc)
+
+    def _batch(self, cu_seqlens, key_lens, pages):
+        nseq = cu_seqlens.numel() - 1
+        _index(cu_seqlens, nseq + 1, "cu_seqlens")
+        return self._requests(key_lens, pages, nseq)
+
+    @staticmethod
+    def _requests(key_lens, pages, nseq):
+        _index(key_lens, nseq, "key_lens")
+        if pages.dtype != torch.int32 or pages.dim() != 2 or pages.shape[0] != nseq or not pages.is_contiguous():
+            raise ClefError(-1, "pages must be a contiguous int32 device tensor [nseq, pages of a request]")
+        return nseq, pages.shape[1]
+
+    def _queries(self, q):
+        if q.dim() != 3 or not q.is_contiguous() or q.shape[2] != self.d or q.dtype != self.k.dtype:
+            raise ClefError(-1, "q must be contiguous [heads, T, d] of the cache's dtype")
+        return q.shape[0], q.shape[1]
+
+    def _scores(self, t, name):
+        if t.shape != (self.num_pages, self.kv_heads, self.page) or t.dtype != torch.float32 or not t.is_contiguous():
+            raise ClefError(-1, f"{name} must be contiguous f32 [pages, kvh, page]")
+
+    def append(self, q, k, v, q_norm, k_norm, cu_seqlens, key_lens, pages, rot_dim, theta, positions=None,
+               axis_of=None, eps=1e-6, out=None):
+        """New tokens enter the cache: q [T, heads, d] (a view; heads may be further apart),
+        k, v [T, kvh, d]; q and k normalised per head (q_norm, k_norm [d] f32) and rotated on
+        their first rot_dim features, k and v written to their pages.  positions: int32
+        [axes, T] (or [T]), and axis_of the axis of each of the rot_dim / 2 rotary pairs
+        (default: all on axis 0); None: each token's index among its request's keys.
+        Returns the queries [heads, T, d]."""
+        nseq, width = self._batch(cu_seqlens, key_lens, pages)
+        if q.dim() != 3 or q.shape[2] != self.d or q.stride(2) != 1:
+            raise ClefError(-1, "q must be [T, heads, d] with contiguous features")
+        T, heads, d = q.shape
+        if k.shape != (T, self.kv_heads, d) or v.shape != k.shape:
+            raise ClefError(-1, "k and v must be [T, kvh, d]")
+        dt = self.k.dtype
+        if q.dtype != dt or k.dtype != dt or v.dtype != dt:
+            raise ClefError(-1, "q, k and v must have the cache's dtype")
+        for w in (q_norm, k_norm):
+            if w.shape != (d,) or w.dtype != torch.float32 or not w.is_contiguous():
+                raise ClefError(-1, "q_norm and k_norm must be contiguous f32 [d]")
+        axes, ldpos = 1, T
+        if positions is not None:
+            if positions.dtype != torch.int32 or positions.dim() not in (1, 2) or positions.shape[-1] != T or \
+                    not positions.is_contiguous():
+                raise ClefError(-1, "positions must be a contiguous int32 device tensor [axes, T]")
+            axes = positions.shape[0] if positions.dim() == 2 else 1
+        if axis_of is not None:
+            if len(axis_of) != rot_dim // 2 or not all(0 <= a < axes for a in axis_of):
+                raise ClefError(-1, "axis_of must name the axis of each of the rot_dim / 2 rotary pairs")
+            axis_of = bytes(axis_of)
+        hsq = q.stride(1) if heads > 1 else d
+        ldq = q.stride(0) if T > 1 else (heads - 1) * hsq + d
+        if hsq < d or ldq < (heads - 1) * hsq + d:
+            raise ClefError(-1, "q rows must not overlap")
+        ldk, ldv = _token_stride(k, "k"), _token_stride(v, "v")
+        if out is None:
+            out = q.new_empty((heads, T, d))
+        elif out.shape != (heads, T, d) or out.dtype != dt or not out.is_contiguous():
+            raise ClefError(-1, "out must be contiguous [heads, T, d] of the cache's dtype")
+        _here(q, k, v, q_norm, k_norm, cu_seqlens, key_lens, pages, self.k, self.vt, out, positions)
+        _check(lib().clef_paged_append(
+            self._at, pages.data_ptr(), width, cu_seqlens.data_ptr(), key_lens.data_ptr(), nseq, T, q.data_ptr(), ldq,
+            hsq, k.data_ptr(), ldk, v.data_ptr(), ldv, heads, q_norm.data_ptr(), k_norm.data_ptr(), float(eps),
+            _ptr(positions), ldpos, axes, axis_of, rot_dim, float(theta), out.data_ptr(), T, _stream()))
+        return out
+
+    def attention_gated(self, q, gate, cu_seqlens, key_lens, pages, window=0, sinks=0, lse=None, out=None):
+        """Causal attention of each request's new tokens over its cached keys, gated:
+        q [heads, T, d], gate [T, heads, *] view; window > 0: each query sees the last
+        `window` keys up to its own and the first `sinks`.  lse: f32 [T, heads], receives
+        the logarithm of each row's sum.  Returns y [T, heads * d]."""
+        nseq, width = self._batch(cu_seqlens, key_lens, pages)
+        heads, T = self._queries(q)
+        d = self.d
+        ldg, hsg, out = _gate_and_out(q, gate, out)
+        if lse is not None and (lse.shape != (T, heads) or lse.dtype != torch.float32 or not lse.is_contiguous()):
+            raise ClefError(-1, "lse must be contiguous f32 [T, heads]")
+        _here(q, gate, cu_seqlens, key_lens, pages, self.k, self.vt, out, lse)
+        L = lib()
+        n = L.clef_attention_paged_workspace(T, nseq, width, self.page, self.dtype, heads, self.kv_heads, d)
+        if n == 0:
+            raise ClefError(-1, last_error())
+        ws = _scratch(n, q.device)
+        _check(L.clef_attention_gated_paged(
+            self._at, pages.data_ptr(), width, cu_seqlens.data_ptr(), key_lens.data_ptr(), nseq, T, q.data_ptr(), T,
+            heads, gate.data_ptr(), ldg, hsg, int(window), int(sinks), out.data_ptr(),
+            out.stride(0) if T > 1 else heads * d, _ptr(lse), ws.data_ptr(), n, _stream()))
+        return out
+
+    def add_weights(self, q, lse, cu_seqlens, key_lens, pages, scores, new_scores=None, window=0, sinks=0):
+        """Adds to each cached key's score [pages, kvh, page] (f32) the attention weights
+        that the new tokens' rows give it (lse from attention_gated, for the same window and
+        sinks); the new tokens' own keys start from 0.  Writes new_scores (default: in place)
+        and returns it."""
+        nseq, width = self._batch(cu_seqlens, key_lens, pages)
+        heads, T = self._queries(q)
+        if lse.shape != (T, heads) or lse.dtype != torch.float32 or not lse.is_contiguous():
+            raise ClefError(-1, "lse must be contiguous f32 [T, heads]")
+        if new_scores is None:
+            new_scores = scores
+        self._scores(scores, "scores")
+        self._scores(new_scores, "new_scores")
+        _here(q, lse, cu_seqlens, key_lens, pages, self.k, self.vt, scores, new_scores)
+        _check(lib().clef_paged_weights(
+            self._at, pages.data_ptr(), width, cu_seqlens.data_ptr(), key_lens.data_ptr(), nseq, T, q.data_ptr(), T,
+            heads, lse.data_ptr(), int(window), int(sinks), scores.data_ptr(), new_scores.data_ptr(), _stream()))
+        return new_scores
+
+    def evict(self, scores, key_lens, pages, budget, to, to_pages, to_scores, sinks=0, recent=0):
+        """Cuts each request to `budget` keys: the first `sinks`, the last `recent` and those of
+        largest score between them (per key head; ties: the lowest index), in their order,
+        copied with their scores to the pages to_pages [nseq, pages of a request] of the cache
+        `to`.  Those must not be pages that the call reads.  Returns (new key_lens [nseq], kept
+        indices [nseq, kvh, budget], -1 behind the last)."""
+        nseq, width = self._requests(key_lens, pages, key_lens.numel())
+        _, to_width = self._requests(key_lens, to_pages, nseq)
+        self._scores(scores, "scores")
+        to._scores(to_scores, "to_scores")
+        _here(scores, key_lens, pages, self.k, self.vt, to.k, to.vt, to_pages, to_scores)
+        if budget < 1:
+            raise ClefError(-1, "the budget must be at least 1")
+        lens = key_lens.new_empty(nseq)
+        keep = key_lens.new_empty((nseq, self.kv_heads, budget))
+        _check(lib().clef_paged_evict(
+            self._at, pages.data_ptr(), width, key_lens.data_ptr(), nseq, scores.data_ptr(), int(budget), int(sinks),
+            int(recent), to._at, to_pages.data_ptr(), to_width, to_scores.data_ptr(), lens.data_ptr(), keep.data_ptr(),
+            _stream()))
+        return lens, keep
 
 
 # ---------------------------------------------------------------------------

@@ -439,6 +439,104 @@ int clef_attention_gated_shared(const void* q, int64_t ldq_tok, const void* pref
                                 void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------- */
+/* A paged cache of keys and values                                        */
+/* ---------------------------------------------------------------------- */
+/*
+ * Keys and values of many requests in pages of one pool, where requests come,
+ * grow, are cut and go.  Page x holds the keys k [kv_heads][page][d] and the
+ * values vt [kv_heads][d][page] (transposed, as clef_values_transposed lays them
+ * out) of `page` consecutive keys of a request; pages are k_stride and vt_stride
+ * elements apart (0: contiguous).  Request s's key j stands in slot j % page of
+ * page table[s * max_pages + j / page] (device int32).  A request's last page
+ * may be full or not; its other entries, and slots behind its last key, may hold
+ * anything.  page is 16, 32, 64, 128 or 256, d a multiple of 8 up to 256, dtype
+ * CLEF_F16 or CLEF_F32, kv_heads <= 256; both pools 16-byte aligned, strides
+ * multiples of 8 elements; max_pages * page <= 2^24.
+ *
+ * The calls below take a batch of nseq requests (1 .. 4096) with T packed new
+ * tokens (1 .. 65536): cu_seqlens (device int32, nseq + 1 offsets), key_lens
+ * (device int32: each request's keys, its n new tokens, which are the last of them,
+ * included).  The tables may change under a captured launch.  Tables that do not
+ * fit give unspecified values, never an access out of bounds: an entry that is
+ * no page of the pool is read as some page, and never written to.  Heads are
+ * grouped as elsewhere (heads % kv_heads == 0, heads <= 256).  No counterpart in
+ * the reference (one request per call, flat keys).
+ */
+typedef struct {
+    void *k, *vt;
+    int64_t k_stride, vt_stride;
+    int num_pages, page, kv_heads, d, dtype;
+} clef_paged_cache;
+/*
+ * New tokens enter the cache: per-head RMS norm and rotary of q and k as in
+ * clef_qk_norm_rotary, but with each token's own position on each of `axes` axes
+ * (1 .. 4; time, height and width of pictures), and v as it is.  Rotary pair i <
+ * rot_dim / 2 (features i and i + rot_dim / 2) turns by positions[axis_of[i] * ldpos
+ * + t] * theta^(-2i/rot_dim): axis_of is a host array of rot_dim / 2 axis numbers, read
+ * during the call (NULL: all on axis 0), positions device int32 [axes][ldpos]; NULL
+ * positions: the token's index among its request's keys.  Angles are reduced in
+ * f64, so that far positions keep their fraction; norm and rotation in f32, rounded
+ * once.  q: (token, head) at t * ldq + h * hsq; k, v: [T, kv_heads, d] with token
+ * strides ldk, ldv (all in the cache's dtype); q_norm, k_norm [d] f32, already offset;
+ * q_out [heads, ldq_tok, d].  Query rows behind the last request leave q_out as it was.
+ * A token whose index is negative (key_lens < n) or has no page is not written.
+ */
+int clef_paged_append(const clef_paged_cache* cache, const int32_t* table, int max_pages, const int32_t* cu_seqlens,
+                      const int32_t* key_lens, int nseq, int T, const void* q, int64_t ldq, int64_t hsq, const void* k,
+                      int64_t ldk, const void* v, int64_t ldv, int heads, const float* q_norm, const float* k_norm,
+                      float eps, const int32_t* positions, int64_t ldpos, int axes, const uint8_t* axis_of, int rot_dim,
+                      double theta, void* q_out, int64_t ldq_tok, void* stream);
+/*
+ * Gated attention of each request's new tokens over its cached keys (its new
+ * ones among them), causal: query i of n stands at p = len - n + i and sees keys j
+ * <= p, and with window > 0 of those only j > p - window and the first `sinks`:
+ *   y[t, h*d + e] = attn(...)[h, t, e] * sigmoid(gate[t, h, e]).
+ * From single tokens of many requests to chunks of a prompt, and both in one
+ * batch.  lse (NULL, or f32 [T, heads]) receives log sum exp(q.k / sqrt(d)) of each
+ * row over the keys it sees.  A query that sees no key gives zeros and an lse of
+ * -inf; keys that no query of its request sees may hold anything.  Rows behind the
+ * last request leave y and lse as they were.  q [heads, ldq_tok, d] (rows 0..T-1,
+ * 16-byte aligned), gate as in clef_attention_gated_shared; f32 sums and softmax.
+ * workspace: clef_attention_paged_workspace bytes, 256-byte aligned.
+ */
+size_t clef_attention_paged_workspace(int T, int nseq, int max_pages, int page, int dtype, int heads, int kv_heads,
+                                      int d);
+int clef_attention_gated_paged(const clef_paged_cache* cache, const int32_t* table, int max_pages,
+                               const int32_t* cu_seqlens, const int32_t* key_lens, int nseq, int T, const void* q,
+                               int64_t ldq_tok, int heads, const void* gate, int64_t ldg, int64_t hsg, int window,
+                               int sinks, void* y, int64_t ldy, float* lse, void* workspace, size_t workspace_bytes,
+                               void* stream);
+/*
+ * What the new tokens attend to, added up per cached key and key head:
+ *   new_scores[j] = scores[j] + sum over rows (t, h of the group) that see j of
+ *                   exp(q.k_j / sqrt(d) - lse[t, h])
+ * with scores and new_scores f32 [num_pages][kv_heads][page], paged as the keys
+ * (new_scores may be scores itself); the new tokens' own keys start from 0.  Every
+ * key of each request is written, all else is left as it was.  lse: as
+ * clef_attention_gated_paged gives it for the same window and sinks.  The sum's
+ * order is fixed: no atomics.  Requests of one call that share a page each write its
+ * scores: that page receives the sums of one of them.
+ */
+int clef_paged_weights(const clef_paged_cache* cache, const int32_t* table, int max_pages, const int32_t* cu_seqlens,
+                       const int32_t* key_lens, int nseq, int T, const void* q, int64_t ldq_tok, int heads,
+                       const float* lse, int window, int sinks, const float* scores, float* new_scores, void* stream);
+/*
+ * Caches cut to `budget` keys each: of a request's len keys the first `sinks`, the
+ * last `recent` and, of those between, the ones of largest score (per key head; NaN
+ * counts as lowest, ties go to the lowest index) stay, in their order, and are copied
+ * with their scores into the pages that to_table [nseq][to_max_pages] names in `to`
+ * (the same geometry; slots behind them are left as they were).  Requests of no more
+ * than budget keys are copied whole.  new_lens (device int32 [nseq]) receives min(len,
+ * budget), keep (device int32 [nseq][kv_heads][budget]) the kept indices, -1 behind
+ * them.  The pages written must not be pages that this call reads.  sinks + recent <=
+ * budget <= to_max_pages * page.
+ */
+int clef_paged_evict(const clef_paged_cache* cache, const int32_t* table, int max_pages, const int32_t* key_lens,
+                     int nseq, const float* scores, int budget, int sinks, int recent, const clef_paged_cache* to,
+                     const int32_t* to_table, int to_max_pages, float* to_scores, int32_t* new_lens, int32_t* keep,
+                     void* stream);
+
+/* ---------------------------------------------------------------------- */
 /* Embedding gather and pooled head                                         */
 /* ---------------------------------------------------------------------- */
 /* h[t, :] = f32(table[ids[t], :]); ids are int32 and must be < vocab. */
