@@ -30,7 +30,7 @@ struct PagedAttn {
   void* y;           // [T][ldy]
   float* lse;        // [T][heads] or null
   int64_t ldq, ldg, hsg, ldy;
-  int heads;
+  int heads, vec;    // vec: gate and y in pieces of four
   float scale;       // log2(e) / sqrt(d): scores in log2 units
   int64_t least;     // shortest stretch of a work-group, on the line
   int groups;        // work-groups of the first launch
@@ -49,8 +49,22 @@ __device__ __forceinline__ void write_out(const PagedAttn& p, float4_t o, float 
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
   const T* gp = static_cast<const T*>(p.gate) + t * p.ldg + h * p.hsg + e;
   T* y = static_cast<T*>(p.y) + t * p.ldy + (int64_t)h * p.c.d + e;
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  vec4 g;
+  if (p.vec) {
+    g = *reinterpret_cast<const vec4*>(gp);
+  } else {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) y[j] = cvt_out<T>(o[j] * inv * sigmoid(to_f32(gp[j])));
+    for (int j = 0; j < 4; ++j) g[j] = gp[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) g[j] = cvt_out<T>(o[j] * inv * sigmoid(to_f32(g[j])));
+  if (p.vec) {
+    *reinterpret_cast<vec4*>(y) = g;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = g[j];
+  }
 }
 // log of the row's sum: m in log2 units, l 2^UP times as large
 template <class T>
@@ -63,6 +77,16 @@ __device__ __forceinline__ void write_lse(const PagedAttn& p, float m, float l, 
 // One block of KB keys, c0 .. + KB - 1 (c0 a multiple of KB), straight from the
 // pages into operands.  The pages hold at least 16 keys each, so a block lies in
 // one or in two.  FULL: d = D.
+// a wave's own writes to LDS are done, and none of its accesses moves across
+__device__ __forceinline__ void lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// all ones where a 16-bit half, or a float, is infinite or NaN
+template <class T>
+__device__ __forceinline__ uint32_t odd_bits(uint32_t x) {
+  if constexpr (sizeof(T) == 4) return (x & 0x7f800000u) == 0x7f800000u ? ~0u : 0u;
+  return ((x & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((x & 0x7c000000u) == 0x7c000000u ? ~0xffffu : 0u);
+}
+
 template <class T, int D, bool FULL>
 struct PageBlock {
   static constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL, TPB = Ops<T>::TPB;
@@ -70,18 +94,18 @@ struct PageBlock {
   frag k[TPB][D / KB], v[D / 16];
 
   // kp, vp: the key head's rows of the pages of the block's first and last 16 keys
-  __device__ __forceinline__ void load(const Paged& c, const T* const (&kp)[2], const T* const (&vp)[2], int c0,
-                                       int lane) {
-    const int r = lane & 15, grp = lane >> 4, in = (1 << c.shift) - 1, d = c.d;
-    const int col = grp * EL;  // the lane's EL keys of a value row
-    const T* vr = (col >= 16 ? vp[1] : vp[0]) + ((int64_t)r << c.shift) + ((c0 + col) & in);
+  __device__ __forceinline__ void load_values(const Paged& c, const T* const (&vp)[2], int c0, int lane) {
+    const int r = lane & 15, col = (lane >> 4) * EL;  // the lane's EL keys of a value row
+    const T* vr = (col >= 16 ? vp[1] : vp[0]) + (r << c.shift) + ((c0 + col) & ((1 << c.shift) - 1));
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e)
-      v[e] = FULL || e * 16 + r < d ? frag_at(vr + ((int64_t)(e * 16) << c.shift)) : frag{};
+    for (int e = 0; e < D / 16; ++e) v[e] = FULL || e * 16 + r < c.d ? frag_at(vr + (e * 16 << c.shift)) : frag{};
+  }
+  __device__ __forceinline__ void load_keys(const Paged& c, const T* const (&kp)[2], int c0, int lane) {
+    const int r = lane & 15, grp = lane >> 4, in = (1 << c.shift) - 1, d = c.d;
 #pragma unroll
     for (int x = 0; x < TPB; ++x) {
       const int row = Ops<T>::row(x, r);
-      const T* kr = (row >= 16 ? kp[1] : kp[0]) + (int64_t)((c0 + row) & in) * d + grp * EL;
+      const T* kr = (row >= 16 ? kp[1] : kp[0]) + ((c0 + row) & in) * d + grp * EL;
 #pragma unroll
       for (int kb = 0; kb < D / KB; ++kb) k[x][kb] = FULL || kb * KB + grp * EL < d ? frag_at(kr + kb * KB) : frag{};
     }
@@ -92,19 +116,23 @@ struct PageBlock {
 #pragma unroll
       for (int kb = 0; kb < D / KB; ++kb) Mma<T>::mma(S[x][0], k[x][kb], fq[kb]);
   }
-  // scores that the lane's query, at position at, does not see: -inf; values that no
-  // row of the tile sees: 0, whatever stands there
-  __device__ __forceinline__ void mask(float4_t (&S)[TPB][1], const Rows& t, const Seen& seen, int at, int c0,
-                                       int lane) {
+  typedef uint32_t bits __attribute__((ext_vector_type(4)));
+  // scores that the lane's query, at position at, does not see: -inf
+  __device__ __forceinline__ void hide(float4_t (&S)[TPB][1], const Rows& t, int at, int c0, int lane) const {
     const int grp = lane >> 4;
 #pragma unroll
     for (int x = 0; x < TPB; ++x)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (!sees(t, at, c0 + Ops<T>::row(x, 4 * grp + i))) S[x][0][i] = -INFINITY;
+        S[x][0][i] = sees(t, at, c0 + Ops<T>::row(x, 4 * grp + i)) ? S[x][0][i] : -INFINITY;
+  }
+  // values that no row of the tile sees: 0, whatever stands there.  So are infinite and NaN
+  // ones, which times a weight of 0 would reach rows that do not see them; whether there
+  // are any (of the lane's).
+  __device__ __forceinline__ bool clean(const Seen& seen, int c0, int lane) {
     typedef uint32_t bits __attribute__((ext_vector_type(4)));
     bits keep;
-    const int col = c0 + grp * EL;
+    const int col = c0 + (lane >> 4) * EL;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (sizeof(T) == 2)
@@ -112,8 +140,19 @@ struct PageBlock {
       else
         keep[i] = seen.any(col + i) ? ~0u : 0u;
     }
+    uint32_t odd = 0;
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e) v[e] = __builtin_bit_cast(frag, __builtin_bit_cast(bits, v[e]) & keep);
+    for (int e = 0; e < D / 16; ++e) {
+      bits y = __builtin_bit_cast(bits, v[e]) & keep;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t bad = odd_bits<T>(y[i]);
+        y[i] &= ~bad;
+        odd |= bad;
+      }
+      v[e] = __builtin_bit_cast(frag, y);
+    }
+    return odd != 0;
   }
   __device__ __forceinline__ void values(Soft<T, D, 1>& st, const frag (&w)[1][1]) const {
 #pragma unroll
@@ -121,11 +160,18 @@ struct PageBlock {
   }
 };
 
-// Tiles of 16 rows, for single tokens and short chunks: the NW waves of a work-group
-// take blocks of a piece in turn, and their parts are joined in LDS.
+// A piece of a tile of 16 rows or fewer, as the NW waves of a work-group take it.
+template <class T, int D, int NW>
+struct FewRows {
+  Joined<D, NW, 16> parts;
+  float weights[NW][Ops<T>::KB][16];  // of a block, in the rare path
+};
+
+// Single tokens and short chunks: the waves of a work-group take blocks of a piece in
+// turn, and their parts are joined in LDS.
 template <class T, int D, bool FULL, int NW>
 __device__ __forceinline__ void few_rows(const PagedAttn& p, const Request& r, const Seen& seen, const Piece& x,
-                                         int row0, int rows, Joined<D, NW, 16>& sh, int w) {
+                                         int row0, int rows, FewRows<T, D, NW>& sh, int w) {
   constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL, PER = kWalkBlock / KB;
   typedef typename Ops<T>::frag frag;
   const Paged& c = p.c;
@@ -133,43 +179,88 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Request& r, c
   const int lr = lane & 15, grp = lane >> 4, G = p.t.G;
   // the lane's query (rows behind the last: the last again)
   const int row = row0 + min(lr, rows - 1), at = r.len - r.n + row / G;
-  const T* src =
-      static_cast<const T*>(p.q) + ((int64_t)(x.kv * G + row % G) * p.ldq + r.first + row / G) * c.d + grp * EL;
   frag fq[D / KB];
+  auto load_queries = [&]() {
+    const T* src =
+        static_cast<const T*>(p.q) + ((int64_t)(x.kv * G + row % G) * p.ldq + r.first + row / G) * c.d + grp * EL;
 #pragma unroll
-  for (int kb = 0; kb < D / KB; ++kb) fq[kb] = FULL || kb * KB + grp * EL < c.d ? frag_at(src + kb * KB) : frag{};
+    for (int kb = 0; kb < D / KB; ++kb) fq[kb] = FULL || kb * KB + grp * EL < c.d ? frag_at(src + kb * KB) : frag{};
+  };
+  load_queries();
   const T* K = static_cast<const T*>(c.k) + ((int64_t)x.kv << c.shift) * c.d;
   const T* V = static_cast<const T*>(c.vt) + ((int64_t)x.kv << c.shift) * c.d;
+  auto key0 = [&](int b) { return seen.key0(b / PER) + b % PER * KB; };
+  auto none = [&](int c0) { return c0 >= seen.to || (c0 >= seen.sink && c0 + KB <= seen.from); };
+  // whether rows at low .. high all see the block's keys
+  auto all = [&](int c0) {
+    return c0 + KB - 1 <= seen.low && (p.t.window == 0 || c0 > seen.high - p.t.window || c0 + KB <= p.t.sinks);
+  };
   Soft<T, D, 1> st;
   st.clear();
+  bool odd = false;
 #pragma unroll 1
   for (int b = x.b0 * PER + wave; b < x.b1 * PER; b += NW) {
-    const int c0 = seen.key0(b / PER) + b % PER * KB;
-    if (c0 >= seen.to) break;
-    if (c0 >= seen.sink && c0 + KB <= seen.from) continue;
+    const int c0 = key0(b);
+    if (none(c0)) continue;
     const int first = page_of(c, x.s, c0), second = KB > 16 ? page_of(c, x.s, c0 + 16) : first;
     const T* const kp[2] = {K + first * c.ks, K + second * c.ks};
     const T* const vp[2] = {V + first * c.vs, V + second * c.vs};
     PageBlock<T, D, FULL> blk;
-    blk.load(c, kp, vp, c0, lane);
+    blk.load_values(c, vp, c0, lane);
+    blk.load_keys(c, kp, c0, lane);
     float4_t S[Ops<T>::TPB][1] = {};
     blk.scores(S, fq);
-    // rows at low .. high all see the block's keys
-    const bool all = c0 + KB - 1 <= seen.low &&
-                     (p.t.window == 0 || c0 > seen.high - p.t.window || c0 + KB <= p.t.sinks);
-    if (!all) blk.mask(S, p.t, seen, at, c0, lane);
+    if (!all(c0)) {
+      blk.hide(S, p.t, at, c0, lane);
+      odd |= blk.clean(seen, c0, lane);
+    }
     frag wt[1][1];
     st.template weights<1>(S, wt, p.scale);
     blk.values(st, wt);
   }
-  sh.put(st, 0, wave, lane, rows);
+  sh.parts.put(st, 0, wave, lane, rows);
+  if (__any(odd)) {  // (rare) the infinite and NaN values, key by key, to the rows that see them
+    lds_done();
+    const float m = lr < rows ? sh.parts.ml[wave][lr].x : 0.0f, ref = (m == -INFINITY ? 0.0f : m) - Ops<T>::UP;
+    load_queries();
+#pragma unroll 1
+    for (int b = x.b0 * PER + wave; b < x.b1 * PER; b += NW) {
+      const int c0 = key0(b);
+      if (none(c0) || all(c0)) continue;
+      const int first = page_of(c, x.s, c0), second = KB > 16 ? page_of(c, x.s, c0 + 16) : first;
+      const T* const kp[2] = {K + first * c.ks, K + second * c.ks};
+      PageBlock<T, D, FULL> blk;
+      blk.load_keys(c, kp, c0, lane);
+      float4_t S[Ops<T>::TPB][1] = {};
+      blk.scores(S, fq);
+#pragma unroll
+      for (int y = 0; y < Ops<T>::TPB; ++y)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          sh.weights[wave][Ops<T>::row(y, 4 * grp + i)][lr] =
+              __builtin_amdgcn_exp2f(fmaf(S[y][0][i], p.scale, -ref));
+      lds_done();
+#pragma unroll 1
+      for (int j = 0; j < KB; ++j) {
+        if (lr >= rows || !sees(p.t, at, c0 + j)) continue;
+        const float f = sh.weights[wave][j][lr];
+        const T* v = V + (j < 16 ? first : second) * c.vs + ((c0 + j) & ((1 << c.shift) - 1));
+#pragma unroll 1
+        for (int e = grp; e < c.d; e += 4) {
+          const float y = to_f32(v[e << c.shift]);
+          if (!(fabsf(y) < INFINITY)) sh.parts.o[wave][lr][e] += f * y;
+        }
+      }
+      lds_done();
+    }
+  }
   lds_barrier();
   const bool whole = x.head && x.tail;
   const int64_t to = ((int64_t)w * 2 + (x.head ? 1 : 0)) * p.t.R;
   for (int i = tid; i < rows * (D / 4); i += 64 * NW) {
     const int y = i / (D / 4), e = i % (D / 4) * 4;
     float m, l;
-    const float4_t o = sh.take(y, e, m, l);
+    const float4_t o = sh.parts.take(y, e, m, l);
     if (whole) {
       const int t = r.first + (row0 + y) / G, h = x.kv * G + (row0 + y) % G;
       if (e < c.d) write_out<T>(p, o, l, t, h, e);
@@ -181,22 +272,18 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Request& r, c
   }
 }
 
-template <class T, int D, bool FULL>
-__global__ __launch_bounds__(256) void paged_few_rows(PagedAttn p) {
-  __shared__ Joined<D, 4, 16> sh;
-  __shared__ WalkShared walk;
-  const int tid = threadIdx.x;
-  Stretch x;
-  const bool work = walk_begin<256>(p.c, p.t, p.least, blockIdx.x, p.groups, walk, x);
+// The pieces of a work-group's stretch, each given to `take`, which leaves its part or its
+// output; and which tile's first part the work-group holds.
+template <int NT, class F>
+__device__ __forceinline__ void walk_pieces(const PagedAttn& p, WalkShared& walk, F take) {
   PagedAttn::Split split = {};
-  if (work) {
+  Stretch x;
+  if (walk_begin<NT>(p.c, p.t, p.least, blockIdx.x, p.groups, walk, x)) {
     Piece piece;
     Request r;
     Seen seen;
     while (next_piece(p.c, p.t, x, piece, r, seen)) {
-      const int row0 = piece.tile * 16, rows = min(16, r.n * p.t.G - row0);
-      few_rows<T, D, FULL, 4>(p, r, seen, piece, row0, rows, sh, x.w);
-      lds_barrier();  // the parts in LDS are read before the next ones replace them
+      take(r, seen, piece, x.w);
       if (piece.head && !piece.tail) {
         int lo = x.w + 1, hi = x.W - 1;  // the first work-group that ends at or behind the tile's end
         while (lo < hi) {
@@ -208,7 +295,311 @@ __global__ __launch_bounds__(256) void paged_few_rows(PagedAttn p) {
       }
     }
   }
-  if (tid == 0) p.split[blockIdx.x] = split;
+  if (threadIdx.x == 0) p.split[blockIdx.x] = split;
+}
+
+template <class T, int D, bool FULL>
+__global__ __launch_bounds__(256, 2) void paged_few_rows(PagedAttn p) {
+  __shared__ FewRows<T, D, 4> sh;
+  __shared__ WalkShared walk;
+  walk_pieces<256>(p, walk, [&](const Request& r, const Seen& seen, const Piece& piece, int w) {
+    const int row0 = piece.tile * 16, rows = min(16, r.n * p.t.G - row0);
+    few_rows<T, D, FULL, 4>(p, r, seen, piece, row0, rows, sh, w);
+    lds_barrier();  // the parts in LDS are read before the next ones replace them
+  });
+}
+
+// ---------------------------------------------------------------------------
+// Tiles of 256 rows, for chunks (f16, d = D): eight waves of 32 rows, two to a SIMD,
+// so that one's exponentials run under the other's products.  Tiles of 64 keys pass
+// through LDS by DMA, double-buffered, and feed products of 32 x 32 x 16: each operand
+// read from LDS serves 32 rows.  (With 16 rows a wave the LDS reads alone take twice
+// the time of the products.)  16-byte slots are permuted by their row (XOR) against
+// bank conflicts; key row r of LDS holds key r with bits 2 and 3 exchanged, so that the
+// 16 weights that a lane holds of 32 keys are operands of the next product as they stand.
+__device__ __forceinline__ void dma16(const void* src, void* lds_block) {
+  // global_load_lds_dwordx4: lane l writes 16 bytes at M0 + 16 l; awaited by vm_wait_all
+  const uint32_t m0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_block));
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+}
+__device__ __forceinline__ void dma16s(const void* base, uint32_t off, void* lds_block) {
+  // the same from a base that is uniform; the wait states cover M0 and the readfirstlane
+  const uint32_t m0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_block));
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(b >> 32)));
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(b)));
+  const uint64_t sb = (static_cast<uint64_t>(hi) << 32) | lo;
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(sb), "{m0}"(m0) : "memory");
+}
+__device__ __forceinline__ void vm_wait_all() { __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8)); }
+
+__device__ __forceinline__ float halves_max(float x) {  // of lanes l and l ^ 32
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+constexpr int kManyRows = 256;
+
+template <int D>
+struct Tiles {
+  __attribute__((aligned(1024))) half_t k[2][64 * D];  // [key][d]
+  half_t v[2][D * 64];                                 // [d][key]
+};
+
+// The eight pages that a wave's DMA of a tile touches at most: of its 16-key quarters.
+struct TilePages {
+  int page[4];
+};
+
+template <int D>
+__device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, const Seen& seen, const Piece& x,
+                                          int row0, int rows, Tiles<D>& sh, int* odd_flag, int w) {
+  typedef half_t T;
+  constexpr int BK = 64, KS = D / 8, NDMA = D / 64, KROWS = 512 / D, NKB = D / 16, NDT = D / 32;
+  constexpr int PER = D >= 128 ? 8 : 4;  // 16-wide steps of a key row per swizzle period
+  constexpr int PD = 4;                  // operands read ahead
+  const Paged& c = p.c;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 31, g = lane >> 5, G = p.t.G, shift = c.shift, in = (1 << shift) - 1;
+  const bool idle = 32 * wave >= rows;  // a wave without rows moves tiles for the others
+  const int row = row0 + min(32 * wave + n, rows - 1), at = r.len - r.n + row / G;
+  const char* K = static_cast<const char*>(c.k) + (((int64_t)x.kv << shift) * D) * 2;
+  const char* V = static_cast<const char*>(c.vt) + (((int64_t)x.kv << shift) * D) * 2;
+  auto kswz = [](int y) { return D >= 128 ? y & 15 : y >> 1 & 7; };
+  typedef const __attribute__((address_space(4))) int* ctable;
+  const ctable table = (ctable)(uintptr_t)(c.table + (int64_t)x.s * c.max_pages);
+
+  auto pages_at = [&](int k0, TilePages& y) {  // uniform: scalar loads
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      y.page[i] = min(max(table[min((k0 + 16 * i) >> shift, c.max_pages - 1)], 0), c.num - 1);
+  };
+  // DMA instruction wave * NDMA + q writes 1 KiB: KROWS key rows, or 8 feature rows.  A
+  // wave's 8 key rows are of one 16-key quarter of the tile, so of one page.
+  auto issue = [&](int buf, int k0, const TilePages& y) {
+    const char* kb = K + y.page[wave >> 1] * (c.ks * 2);
+#pragma unroll
+    for (int q = 0; q < NDMA; ++q) {
+      const int lrow = wave * 8 + q * KROWS + lane / KS;  // LDS row; its key:
+      const int key = (lrow & ~12) | (lrow & 4) << 1 | (lrow & 8) >> 1;
+      const uint32_t off = 2 * D * ((k0 + key) & in) + 16 * ((lane % KS) ^ kswz(lrow));
+      dma16s(kb, off, &sh.k[buf][(wave * NDMA + q) * 512]);
+    }
+    const int64_t vs = c.vs * 2;
+    if (shift >= 6) {
+      const char* vb = V + y.page[0] * vs;
+#pragma unroll
+      for (int q = 0; q < NDMA; ++q) {
+        const int e = (wave * NDMA + q) * 8 + (lane >> 3), chunk = (lane & 7) ^ (e >> 1 & 7);
+        dma16s(vb, 2 * ((e << shift) + (k0 & in) + 8 * chunk), &sh.v[buf][(wave * NDMA + q) * 512]);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < NDMA; ++q) {
+        const int e = (wave * NDMA + q) * 8 + (lane >> 3), chunk = (lane & 7) ^ (e >> 1 & 7), i = chunk >> 1;
+        const int page = i < 2 ? (i == 0 ? y.page[0] : y.page[1]) : (i == 2 ? y.page[2] : y.page[3]);
+        dma16(V + page * vs + 2 * ((e << shift) + ((k0 + 8 * chunk) & in)), &sh.v[buf][(wave * NDMA + q) * 512]);
+      }
+    }
+  };
+
+  // operands: key rows 32 kh + n, 16-byte chunk 2 kb + g; feature rows 32 t + n, chunk 2 y + g
+  const int koff = n * 2 * D + 16 * (g ^ kswz(n)), voff = n * 128 + 16 * (g ^ (n >> 1 & 7));
+  auto key_at = [&](const char* base, int kh, int kb) {
+    return *reinterpret_cast<const half8*>(base + (koff ^ 32 * (kb % PER)) + kh * 64 * D + kb / PER * 32 * PER);
+  };
+  auto value_at = [&](const char* base, int y, int t) {
+    return *reinterpret_cast<const half8*>(base + (voff ^ 32 * y) + t * 32 * 128);
+  };
+
+  lds_barrier();  // the piece before is done with the tiles
+  if (tid == 0) *odd_flag = 0;
+  TilePages pages;
+  pages_at(seen.key0(x.b0), pages);
+  if (x.b0 < x.b1) issue(0, seen.key0(x.b0), pages);
+  half8 fq[NKB];
+  {
+    const T* src = static_cast<const T*>(p.q) + ((int64_t)(x.kv * G + row % G) * p.ldq + r.first + row / G) * D + 8 * g;
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) fq[kb] = *reinterpret_cast<const half8*>(src + 16 * kb);
+  }
+  float16_t o[NDT];
+#pragma unroll
+  for (int t = 0; t < NDT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[t][e] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  if (x.b0 + 1 < x.b1) pages_at(seen.key0(x.b0 + 1), pages);
+
+#pragma unroll 1
+  for (int b = x.b0; b < x.b1; ++b) {
+    const int k0 = seen.key0(b), buf = (b - x.b0) & 1;
+    vm_wait_all();
+    lds_barrier();  // tile b is there; tile b - 1 is done with
+    if (b + 1 < x.b1) {
+      issue(buf ^ 1, seen.key0(b + 1), pages);
+      if (b + 2 < x.b1) pages_at(seen.key0(b + 2), pages);
+    }
+    const bool all = k0 + BK - 1 <= seen.low &&
+                     (p.t.window == 0 || k0 > seen.high - p.t.window || k0 + BK <= p.t.sinks);
+    if (!all) {
+      // values that no row sees, and infinite and NaN ones (see FewRows): 0
+      bool odd = false;
+      for (int i = tid; i < D * 8; i += 512) {
+        const int e = i >> 3, key = k0 + 8 * ((i & 7) ^ (e >> 1 & 7));
+        typedef uint32_t bits __attribute__((ext_vector_type(4)));
+        bits* const at = reinterpret_cast<bits*>(sh.v[buf] + i * 8);
+        bits y = *at;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          y[j] &= (seen.any(key + 2 * j) ? 0xffffu : 0u) | (seen.any(key + 2 * j + 1) ? ~0xffffu : 0u);
+          const uint32_t bad = odd_bits<T>(y[j]);
+          odd |= bad != 0;
+          y[j] &= ~bad;
+        }
+        *at = y;
+      }
+      if (odd) *odd_flag = 1;
+      lds_barrier();
+    }
+    if (idle) continue;
+    const char* kbase = reinterpret_cast<const char*>(sh.k[buf]);
+    const char* vbase = reinterpret_cast<const char*>(sh.v[buf]);
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh) {
+      float16_t S;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) S[e] = 0.0f;
+      half8 f[PD];
+#pragma unroll
+      for (int i = 0; i < PD; ++i) f[i] = key_at(kbase, kh, i);
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+        S = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[kb % PD], fq[kb], S, 0, 0, 0);
+        if (kb + PD < NKB) f[kb % PD] = key_at(kbase, kh, kb + PD);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // element e of lane group g: key k0 + 32 kh + 16 (e / 8) + 8 g + e % 8
+      if (!all) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          S[e] = sees(p.t, at, k0 + 32 * kh + 16 * (e >> 3) + 8 * g + (e & 7)) ? S[e] : -INFINITY;
+      }
+      float top = S[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, S[e]);
+      const float to = fmaxf(m, halves_max(top) * p.scale);
+      if (__any(to > m + 8.0f)) {
+        const float a = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= a;
+#pragma unroll
+        for (int t = 0; t < NDT; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[t][e] *= a;
+      }
+      const float ref = (m == -INFINITY ? 0.0f : m) - Ops<T>::UP;
+#pragma unroll
+      for (int i = 0; i < PD; ++i) f[i] = value_at(vbase, 2 * kh + i / NDT, i % NDT);
+      half8 wt[2];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float y = __builtin_amdgcn_exp2f(fmaf(S[e], p.scale, -ref));
+        l += y;
+        wt[e >> 3][e & 7] = static_cast<T>(y);
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * NDT; ++i) {
+        o[i % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % PD], wt[i / NDT], o[i % NDT], 0, 0, 0);
+        if (i + PD < 2 * NDT) f[i % PD] = value_at(vbase, 2 * kh + (i + PD) / NDT, (i + PD) % NDT);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  if (idle) return;
+  l = halves_sum(l);
+  const bool whole = x.head && x.tail, mine = 32 * wave + n < rows;
+  const bool odd = *odd_flag != 0;
+  // (a whole tile needs no part; the second is free until the last piece)
+  const int64_t to = ((int64_t)w * 2 + (x.head ? 1 : 0)) * kManyRows + 32 * wave + n;
+  const int tok = r.first + row / G, h = x.kv * G + row % G;
+  auto feature = [&](int t, int i) { return 32 * t + 8 * i + 4 * g; };  // of o[t][4 i]
+  if (mine && g == 0) {
+    if (whole) write_lse<T>(p, m, l, tok, h);
+    else p.ml[to] = float2{m, l};
+  }
+#pragma unroll
+  for (int t = 0; t < NDT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4_t y = {o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+      if (!mine) continue;
+      if (whole && !odd) write_out<T>(p, y, l, tok, h, feature(t, i));
+      else *reinterpret_cast<float4_t*>(p.part + to * D + feature(t, i)) = y;
+    }
+  if (!odd) return;
+  // (rare) the infinite and NaN values, key by key, to the rows that see them; each lane adds
+  // to the features that it has written
+  const T* qrow = static_cast<const T*>(p.q) + ((int64_t)h * p.ldq + tok) * D;
+  const float ref = (m == -INFINITY ? 0.0f : m) - Ops<T>::UP;
+#pragma unroll 1
+  for (int b = x.b0; b < x.b1; ++b) {
+    const int k0 = seen.key0(b);
+#pragma unroll 1
+    for (int j = k0; j < k0 + BK; ++j) {
+      if (!seen.any(j)) continue;
+      const int page = page_of(c, x.s, j);
+      const T* v = reinterpret_cast<const T*>(V) + page * c.vs + (j & in);
+      bool any = false;
+#pragma unroll 1
+      for (int e = lane; e < D; e += 64) any |= !(fabsf(to_f32(v[e << shift])) < INFINITY);
+      if (!__any(any)) continue;
+      const T* key = reinterpret_cast<const T*>(K) + page * c.ks + (j & in) * D;
+      float s = 0.0f;
+#pragma unroll 1
+      for (int e = g; e < D; e += 2) s = fmaf(to_f32(qrow[e]), to_f32(key[e]), s);
+      s = halves_sum(s);
+      // where all rows see a tile its products have them already
+      const int t0 = j / BK * BK;
+      const bool all = t0 + BK - 1 <= seen.low &&
+                       (p.t.window == 0 || t0 > seen.high - p.t.window || t0 + BK <= p.t.sinks);
+      if (all || !mine || !sees(p.t, at, j)) continue;
+      const float f = __builtin_amdgcn_exp2f(fmaf(s, p.scale, -ref));
+#pragma unroll 1
+      for (int i = 0; i < D / 8; ++i) {
+#pragma unroll 1
+        for (int e = 8 * i + 4 * g; e < 8 * i + 4 * g + 4; ++e) {
+          const float y = to_f32(v[e << shift]);
+          if (!(fabsf(y) < INFINITY)) p.part[to * D + e] += f * y;
+        }
+      }
+    }
+  }
+  if (whole && mine) {
+#pragma unroll 1
+    for (int i = 0; i < D / 8; ++i)
+      write_out<T>(p, *reinterpret_cast<const float4_t*>(p.part + to * D + 8 * i + 4 * g), l, tok, h, 8 * i + 4 * g);
+  }
+}
+
+// Requests of at most 16 rows in a batch with chunks go the other way, with eight waves.
+template <int D>
+__global__ __launch_bounds__(512, 2) void paged_many_rows(PagedAttn p) {
+  typedef half_t T;
+  constexpr size_t TILES = sizeof(Tiles<D>), FEW = sizeof(FewRows<T, D, 8>);
+  __shared__ __attribute__((aligned(1024))) char lds[TILES > FEW ? TILES : FEW];
+  __shared__ WalkShared walk;
+  __shared__ int odd;
+  walk_pieces<512>(p, walk, [&](const Request& r, const Seen& seen, const Piece& piece, int w) {
+    const int row0 = piece.tile * kManyRows, rows = min(kManyRows, r.n * p.t.G - row0);
+    if (r.n * p.t.G <= 16) few_rows<T, D, true, 8>(p, r, seen, piece, row0, rows, *reinterpret_cast<FewRows<T, D, 8>*>(lds), w);
+    else many_rows<D>(p, r, seen, piece, row0, rows, *reinterpret_cast<Tiles<D>*>(lds), &odd, w);
+    lds_barrier();
+  });
 }
 
 // The output of one row of a tile that was split: its parts, weighed and added by as
@@ -258,17 +649,20 @@ int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 // How a call is launched, from the shapes alone (the workspace follows from it).
 struct PagedPlan {
+  bool many;   // tiles of 256 rows, else of 16
   int R;       // rows of a tile
   int groups;  // work-groups, a multiple of 8
 };
-PagedPlan plan_of(int T, int nseq, int max_keys, int heads, int kvh) {
+PagedPlan plan_of(int T, int nseq, int max_keys, int dtype, int heads, int kvh, int d) {
   PagedPlan x;
-  x.R = 16;
   const int64_t rows = (int64_t)T * (heads / kvh);
+  x.many = dtype == CLEF_F16 && d == padded(d) && rows > 16 * (int64_t)nseq;
+  x.R = x.many ? kManyRows : 16;
   // no more than blocks of keys that there can be
   const int64_t tiles = (rows / x.R + std::min(T, nseq)) * kvh;
   const int64_t blocks = tiles * ((max_keys + kTileCost) / kWalkBlock + 1);
-  x.groups = static_cast<int>(std::min<int64_t>(2 * device_cus(), blocks) + 7) / 8 * 8;
+  // as many as run at once: one to a CU by the LDS, or two
+  x.groups = static_cast<int>(std::min<int64_t>((x.many ? 1 : 2) * device_cus(), blocks) + 7) / 8 * 8;
   return x;
 }
 size_t parts_bytes(const PagedPlan& x, int d) {
@@ -280,7 +674,10 @@ size_t workspace_bytes(const PagedPlan& x, int d) {
 
 template <class T, int D, bool FULL>
 int launch(const PagedAttn& p, const PagedPlan& x, hipStream_t st) {
-  hipLaunchKernelGGL((paged_few_rows<T, D, FULL>), dim3(x.groups), dim3(256), 0, st, p);
+  if constexpr (sizeof(T) == 2 && FULL) {
+    if (x.many) hipLaunchKernelGGL((paged_many_rows<D>), dim3(x.groups), dim3(512), 0, st, p);
+  }
+  if (!x.many) hipLaunchKernelGGL((paged_few_rows<T, D, FULL>), dim3(x.groups), dim3(256), 0, st, p);
   hipLaunchKernelGGL((paged_join<T, D>), dim3(x.groups * x.R), dim3(256), 0, st, p);
   return check_launch("paged attention");
 }
@@ -302,7 +699,7 @@ extern "C" size_t clef_attention_paged_workspace(int T, int nseq, int max_pages,
                                                  int kv_heads, int d) {
   if (clef::paged_shape("paged attention", page, max_pages, dtype, kv_heads, d)) return 0;
   if (clef::paged_batch("paged attention", nseq, T, heads, kv_heads)) return 0;
-  return clef::workspace_bytes(clef::plan_of(T, nseq, max_pages * page, heads, kv_heads), d);
+  return clef::workspace_bytes(clef::plan_of(T, nseq, max_pages * page, dtype, heads, kv_heads, d), d);
 }
 
 extern "C" int clef_attention_gated_paged(const clef_paged_cache* cache, const int32_t* table, int max_pages,
@@ -321,7 +718,7 @@ extern "C" int clef_attention_gated_paged(const clef_paged_cache* cache, const i
   CLEF_REQUIRE(window >= 0 && window <= clef::kPagedKeys && sinks >= 0 && sinks <= clef::kPagedKeys,
                "paged attention: window and sinks must be in 0..2^24");
   CLEF_REQUIRE(!clef::misaligned(q), "paged attention: q must be 16-byte aligned");
-  const clef::PagedPlan x = clef::plan_of(T, nseq, p.c.max_keys, heads, p.c.kvh);
+  const clef::PagedPlan x = clef::plan_of(T, nseq, p.c.max_keys, cache->dtype, heads, p.c.kvh, d);
   CLEF_REQUIRE(workspace && workspace_bytes >= clef::workspace_bytes(x, d) &&
                    !(reinterpret_cast<uintptr_t>(workspace) & 255),
                "paged attention: workspace too small or not 256-byte aligned");
@@ -330,6 +727,9 @@ extern "C" int clef_attention_gated_paged(const clef_paged_cache* cache, const i
   p.q = q; p.gate = gate; p.y = y; p.lse = lse;
   p.ldq = ldq_tok; p.ldg = ldg; p.hsg = hsg; p.ldy = ldy;
   p.heads = heads;
+  const size_t four = cache->dtype == CLEF_F16 ? 8 : 16;
+  p.vec = !(reinterpret_cast<uintptr_t>(gate) % four || reinterpret_cast<uintptr_t>(y) % four || ldg % 4 || hsg % 4 ||
+            ldy % 4);
   p.scale = static_cast<float>(1.44269504088896340736 / std::sqrt(static_cast<double>(d)));
   p.least = (int64_t)clef::kWalkBlock * p.t.G;
   p.groups = x.groups;

@@ -202,6 +202,47 @@ def test_attention_pages(clef, page):
 
 
 @gpu
+@pytest.mark.parametrize("window,sinks", [(0, 0), (30, 4)])
+@pytest.mark.parametrize("dtype,page,d", [(F16, 16, 64), (F16, 64, 256), (F16, 32, 72), (F32, 16, 128)], ids=str)
+@pytest.mark.parametrize("requests", [[(5, 40)], [(100, 230), (3, 70), (60, 60)]], ids=str)
+def test_infinite_and_nan_values(clef, window, sinks, dtype, page, d, requests):
+    """Infinite and NaN values reach the rows that see their key, in their feature, and no
+    others; everything else keeps the bits that it has with finite values there."""
+    heads = 8
+    b = Batch(requests, page, 2, d, dtype, seed=d)
+    q, gate = b.randn(heads, b.T, d), b.randn(b.T, heads, d)
+    cache = clef.PagedCache(b.k, b.vt)
+    run = lambda: cache.attention_gated(q, gate, b.cu, b.len, b.table, window=window, sinks=sinks).view(b.T, heads, d)  # noqa: E731
+    odd = [(0, 1, 3, math.inf), (0, 0, d - 1, -math.inf), (0, 1, 9, NAN), (0, 0, 0, math.inf), (0, 0, 0, NAN)]
+    places = []
+    for s, (n, m) in enumerate(requests):
+        first = m - n
+        for (_, kv, f, x), j in zip(odd, (first + n // 2, m - 1, first + 1, max(first - 1, 0), max(first - 2, 0))):
+            places.append((s, kv, f, j, x))
+            b.values[s][kv, j, f] = 0.0
+        b.fill(b.vt.transpose(2, 3), s, b.values[s])
+    plain = run()
+    for s, kv, f, j, x in places:
+        b.values[s][kv, j, f] = x
+        b.fill(b.vt.transpose(2, 3), s, b.values[s])
+    got = run()
+    torch.cuda.synchronize()
+    want = plain.float()
+    t = 0
+    for s, (n, m) in enumerate(requests):
+        for s2, kv, f, j, x in places:
+            if s2 != s:
+                continue
+            for i in range(n):
+                p = m - n + i
+                if j <= p and (not window or j > p - window or j < sinks):
+                    # an infinity, or NaN where it meets NaN or the other infinity
+                    want[t + i, kv * 4:kv * 4 + 4, f] += x
+        t += n
+    assert torch.equal(got.float().nan_to_num(5.0, 6.0, 7.0), want.nan_to_num(5.0, 6.0, 7.0))
+
+
+@gpu
 def test_many_requests(clef):
     """More requests than threads deal with at once, most of them short."""
     requests = [(s % 3, s % 3 + s * 7 % 90) for s in range(1500)]
