@@ -342,17 +342,35 @@ __device__ __forceinline__ float halves_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The lane's number, formed where it is used instead of kept in a register.
+__device__ __forceinline__ int fresh_lane() {
+  int y;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(y));
+  return y;
+}
+
 constexpr int kManyRows = 256;
+
+// Query operands of a wave that stand in LDS: at D = 256 registers hold 13 of the 16 beside
+// the outputs (128 registers) and what a tile needs.
+template <int D>
+constexpr int kQueryLds() { return D == 256 ? 3 : 0; }
 
 template <int D>
 struct Tiles {
   __attribute__((aligned(1024))) half_t k[2][64 * D];  // [key][d]
   half_t v[2][D * 64];                                 // [d][key]
+  half8 q[kQueryLds<D>() ? 8 : 1][kQueryLds<D>() ? kQueryLds<D>() : 1][64];
 };
 
-// The eight pages that a wave's DMA of a tile touches at most: of its 16-key quarters.
+// The pages of a tile's 16-key quarters (read through scalar registers: a choice among
+// fields would be made on their addresses, and loads from there wait for the tiles in flight).
 struct TilePages {
-  int page[4];
+  int a, b, c, d;
+  __device__ __forceinline__ int of(int i) const {
+    const int x = uniform(a), y = uniform(b), z = uniform(c), w = uniform(d);
+    return i < 2 ? (i == 0 ? x : y) : (i == 2 ? z : w);
+  }
 };
 
 template <int D>
@@ -361,6 +379,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
   typedef half_t T;
   constexpr int BK = 64, KS = D / 8, NDMA = D / 64, KROWS = 512 / D, NKB = D / 16, NDT = D / 32;
   constexpr int PER = D >= 128 ? 8 : 4;  // 16-wide steps of a key row per swizzle period
+  constexpr float kLow = -1e30f;         // stands for a maximum of -inf where one is subtracted
   constexpr int PD = 4;                  // operands read ahead
   const Paged& c = p.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -374,14 +393,25 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
   const ctable table = (ctable)(uintptr_t)(c.table + (int64_t)x.s * c.max_pages);
 
   auto pages_at = [&](int k0, TilePages& y) {  // uniform: scalar loads
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      y.page[i] = min(max(table[min((k0 + 16 * i) >> shift, c.max_pages - 1)], 0), c.num - 1);
+    auto entry = [&](int key) { return table[min(key >> shift, c.max_pages - 1)]; };
+    auto page = [&](int z) { return uniform(min(max(z, 0), c.num - 1)); };
+    if (shift >= 6) {
+      y.a = y.b = y.c = y.d = page(entry(k0));
+    } else {
+      const int e0 = entry(k0), e1 = entry(k0 + 16), e2 = entry(k0 + 32), e3 = entry(k0 + 48);
+      y.a = page(e0);
+      y.b = page(e1);
+      y.c = page(e2);
+      y.d = page(e3);
+    }
   };
   // DMA instruction wave * NDMA + q writes 1 KiB: KROWS key rows, or 8 feature rows.  A
   // wave's 8 key rows are of one 16-key quarter of the tile, so of one page.
   auto issue = [&](int buf, int k0, const TilePages& y) {
-    const char* kb = K + y.page[wave >> 1] * (c.ks * 2);
+    // formed anew for each tile: offsets kept for the loop would be spilled, and a spilled
+    // register's load waits for the tiles in flight
+    const int lane = fresh_lane();
+    const char* kb = K + y.of(wave >> 1) * (c.ks * 2);
 #pragma unroll
     for (int q = 0; q < NDMA; ++q) {
       const int lrow = wave * 8 + q * KROWS + lane / KS;  // LDS row; its key:
@@ -391,7 +421,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
     }
     const int64_t vs = c.vs * 2;
     if (shift >= 6) {
-      const char* vb = V + y.page[0] * vs;
+      const char* vb = V + y.a * vs;
 #pragma unroll
       for (int q = 0; q < NDMA; ++q) {
         const int e = (wave * NDMA + q) * 8 + (lane >> 3), chunk = (lane & 7) ^ (e >> 1 & 7);
@@ -400,20 +430,26 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
     } else {
 #pragma unroll
       for (int q = 0; q < NDMA; ++q) {
-        const int e = (wave * NDMA + q) * 8 + (lane >> 3), chunk = (lane & 7) ^ (e >> 1 & 7), i = chunk >> 1;
-        const int page = i < 2 ? (i == 0 ? y.page[0] : y.page[1]) : (i == 2 ? y.page[2] : y.page[3]);
-        dma16(V + page * vs + 2 * ((e << shift) + ((k0 + 8 * chunk) & in)), &sh.v[buf][(wave * NDMA + q) * 512]);
+        const int e = (wave * NDMA + q) * 8 + (lane >> 3), chunk = (lane & 7) ^ (e >> 1 & 7);
+        dma16(V + y.of(chunk >> 1) * vs + 2 * ((e << shift) + ((k0 + 8 * chunk) & in)), &sh.v[buf][(wave * NDMA + q) * 512]);
       }
     }
   };
 
   // operands: key rows 32 kh + n, 16-byte chunk 2 kb + g; feature rows 32 t + n, chunk 2 y + g
+  // (each read's variant is formed where it is used, in one instruction that the compiler
+  // neither shares nor moves: kept for the loop they cost the registers of three Q operands)
   const int koff = n * 2 * D + 16 * (g ^ kswz(n)), voff = n * 128 + 16 * (g ^ (n >> 1 & 7));
+  auto variant = [](int off, int bits) {
+    int y;
+    asm volatile("v_xor_b32 %0, %1, %2" : "=v"(y) : "i"(bits), "v"(off));
+    return y;
+  };
   auto key_at = [&](const char* base, int kh, int kb) {
-    return *reinterpret_cast<const half8*>(base + (koff ^ 32 * (kb % PER)) + kh * 64 * D + kb / PER * 32 * PER);
+    return *reinterpret_cast<const half8*>(base + variant(koff, 32 * (kb % PER)) + kh * 64 * D + kb / PER * 32 * PER);
   };
   auto value_at = [&](const char* base, int y, int t) {
-    return *reinterpret_cast<const half8*>(base + (voff ^ 32 * y) + t * 32 * 128);
+    return *reinterpret_cast<const half8*>(base + variant(voff, 32 * y) + t * 32 * 128);
   };
 
   lds_barrier();  // the piece before is done with the tiles
@@ -421,11 +457,14 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
   TilePages pages;
   pages_at(seen.key0(x.b0), pages);
   if (x.b0 < x.b1) issue(0, seen.key0(x.b0), pages);
-  half8 fq[NKB];
+  constexpr int QL = kQueryLds<D>(), QR = NKB - QL;
+  half8 fq[QR];
   {
     const T* src = static_cast<const T*>(p.q) + ((int64_t)(x.kv * G + row % G) * p.ldq + r.first + row / G) * D + 8 * g;
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) fq[kb] = *reinterpret_cast<const half8*>(src + 16 * kb);
+    for (int kb = 0; kb < QR; ++kb) fq[kb] = *reinterpret_cast<const half8*>(src + 16 * kb);
+#pragma unroll
+    for (int kb = 0; kb < QL; ++kb) sh.q[wave][kb][lane] = *reinterpret_cast<const half8*>(src + 16 * (QR + kb));
   }
   float16_t o[NDT];
 #pragma unroll
@@ -449,7 +488,8 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
     if (!all) {
       // values that no row sees, and infinite and NaN ones (see FewRows): 0
       bool odd = false;
-      for (int i = tid; i < D * 8; i += 512) {
+#pragma unroll 1
+      for (int i = 64 * wave + fresh_lane(); i < D * 8; i += 512) {
         const int e = i >> 3, key = k0 + 8 * ((i & 7) ^ (e >> 1 & 7));
         typedef uint32_t bits __attribute__((ext_vector_type(4)));
         bits* const at = reinterpret_cast<bits*>(sh.v[buf] + i * 8);
@@ -474,27 +514,36 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
       float16_t S;
 #pragma unroll
       for (int e = 0; e < 16; ++e) S[e] = 0.0f;
-      half8 f[PD];
+      half8 f[PD], lq = {};
 #pragma unroll
       for (int i = 0; i < PD; ++i) f[i] = key_at(kbase, kh, i);
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
-        S = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[kb % PD], fq[kb], S, 0, 0, 0);
+        S = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[kb % PD], kb < QR ? fq[kb < QR ? kb : 0] : lq, S, 0, 0, 0);
+        if constexpr (QL > 0) {
+          if (kb + 1 >= QR && kb + 1 < NKB) lq = sh.q[wave][kb + 1 - QR][fresh_lane()];
+        }
         if (kb + PD < NKB) f[kb % PD] = key_at(kbase, kh, kb + PD);
         __builtin_amdgcn_sched_barrier(0);
       }
       // element e of lane group g: key k0 + 32 kh + 16 (e / 8) + 8 g + e % 8
       if (!all) {
+        const int first = k0 + 32 * kh + 8 * (fresh_lane() >> 5);
+        float hidden;
+        asm volatile("v_mov_b32 %0, 0xff800000" : "=v"(hidden));  // -inf
+        const int last = at - first, left = p.t.window ? last - p.t.window : -1, sink = p.t.sinks - first;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          S[e] = sees(p.t, at, k0 + 32 * kh + 16 * (e >> 3) + 8 * g + (e & 7)) ? S[e] : -INFINITY;
+        for (int e = 0; e < 16; ++e) {
+          const int key = 16 * (e >> 3) + (e & 7);
+          S[e] = key <= last && (key > left || key < sink) ? S[e] : hidden;
+        }
       }
       float top = S[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, S[e]);
       const float to = fmaxf(m, halves_max(top) * p.scale);
       if (__any(to > m + 8.0f)) {
-        const float a = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+        const float a = __builtin_amdgcn_exp2f(fmaxf(m, kLow) - fmaxf(to, kLow));
         m = to;
         l *= a;
 #pragma unroll
@@ -502,9 +551,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[t][e] *= a;
       }
-      const float ref = (m == -INFINITY ? 0.0f : m) - Ops<T>::UP;
-#pragma unroll
-      for (int i = 0; i < PD; ++i) f[i] = value_at(vbase, 2 * kh + i / NDT, i % NDT);
+      const float ref = fmaxf(m, kLow) - Ops<T>::UP;
       half8 wt[2];
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -512,6 +559,9 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
         l += y;
         wt[e >> 3][e & 7] = static_cast<T>(y);
       }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < PD; ++i) f[i] = value_at(vbase, 2 * kh + i / NDT, i % NDT);
 #pragma unroll
       for (int i = 0; i < 2 * NDT; ++i) {
         o[i % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % PD], wt[i / NDT], o[i % NDT], 0, 0, 0);
@@ -602,44 +652,52 @@ __global__ __launch_bounds__(512, 2) void paged_many_rows(PagedAttn p) {
   });
 }
 
-// The output of one row of a tile that was split: its parts, weighed and added by as
-// many groups of D / 4 threads as a work-group has, a part to each in turn.
-template <class T, int D>
+// The outputs of the rows of tiles that were split: their parts, weighed and added by
+// groups of D / 4 threads.  FEW: one row to a work-group, whose groups take its parts in
+// turn (a row of a single request can have hundreds); else a row to each group.
+template <class T, int D, bool FEW>
 __global__ __launch_bounds__(256) void paged_join(PagedAttn p) {
-  constexpr int L = D / 4, N = 256 / L;
+  constexpr int L = D / 4, N = 256 / L, STEP = FEW ? N : 1, ROWS = FEW ? 1 : N;
   __shared__ __attribute__((aligned(16))) float4_t so[N][L];
   __shared__ float sl[N];
-  const int tid = threadIdx.x, lane = tid & 63, n0 = tid / L, e = tid % L * 4;
-  const int y = blockIdx.x % p.t.R;
-  const PagedAttn::Split x = p.split[blockIdx.x / p.t.R];
+  const int tid = threadIdx.x, n0 = tid / L, e = tid % L * 4, per = p.t.R / ROWS;
+  const PagedAttn::Split x = p.split[blockIdx.x / per];
   if (x.parts == 0) return;
   const Request r = request_of(p.c, x.s);
-  const int row = x.tile * p.t.R + y;
-  if (row >= r.n * p.t.G) return;
-  const int parts = x.parts;  // the second of work-group w, the first of those behind it
+  const int y = blockIdx.x % per * ROWS + (FEW ? 0 : n0), row = x.tile * p.t.R + y, rows = r.n * p.t.G;
+  if (FEW ? row >= rows : row - n0 >= rows) return;
+  const bool live = FEW || row < rows;
+  const int parts = live ? x.parts : 0;  // the second of work-group w, the first of those behind it
   auto place = [&](int n) { return ((int64_t)(x.w + n) * 2 + (n == 0 ? 1 : 0)) * p.t.R + y; };
   float m = -INFINITY;
-  for (int n = lane; n < parts; n += 64) m = fmaxf(m, p.ml[place(n)].x);
-  m = max4(lane_max<16>(m));
+  if constexpr (FEW) {
+    for (int n = tid & 63; n < parts; n += 64) m = fmaxf(m, p.ml[place(n)].x);
+    m = max4(lane_max<16>(m));
+  } else {
+    for (int n = 0; n < parts; ++n) m = fmaxf(m, p.ml[place(n)].x);
+  }
   const float ref = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
   float4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int n = n0; n < parts; n += N) {
+  for (int n = FEW ? n0 : 0; n < parts; n += STEP) {
     const float2 a = p.ml[place(n)];
     const float f = __builtin_amdgcn_exp2f(a.x - ref);
     l = fmaf(a.y, f, l);
     o += *reinterpret_cast<const float4_t*>(p.part + place(n) * D + e) * f;
   }
-  so[n0][tid % L] = o;
-  if (e == 0) sl[n0] = l;
-  lds_barrier();
-  if (n0) return;
+  if constexpr (FEW) {
+    so[n0][tid % L] = o;
+    if (e == 0) sl[n0] = l;
+    lds_barrier();
+    if (n0) return;
 #pragma unroll
-  for (int n = 1; n < N; ++n) {
-    o += so[n][tid % L];
-    l += sl[n];
+    for (int n = 1; n < N; ++n) {
+      o += so[n][tid % L];
+      l += sl[n];
+    }
   }
+  if (!live) return;
   const int t = r.first + row / p.t.G, h = x.kv * p.t.G + row % p.t.G;
   if (e < p.c.d) write_out<T>(p, o, l, t, h, e);
   if (e == 0) write_lse<T>(p, m, l, t, h);
@@ -675,10 +733,14 @@ size_t workspace_bytes(const PagedPlan& x, int d) {
 template <class T, int D, bool FULL>
 int launch(const PagedAttn& p, const PagedPlan& x, hipStream_t st) {
   if constexpr (sizeof(T) == 2 && FULL) {
-    if (x.many) hipLaunchKernelGGL((paged_many_rows<D>), dim3(x.groups), dim3(512), 0, st, p);
+    if (x.many) {
+      hipLaunchKernelGGL((paged_many_rows<D>), dim3(x.groups), dim3(512), 0, st, p);
+      hipLaunchKernelGGL((paged_join<T, D, false>), dim3(x.groups * (x.R / (1024 / D))), dim3(256), 0, st, p);
+      return check_launch("paged attention");
+    }
   }
-  if (!x.many) hipLaunchKernelGGL((paged_few_rows<T, D, FULL>), dim3(x.groups), dim3(256), 0, st, p);
-  hipLaunchKernelGGL((paged_join<T, D>), dim3(x.groups * x.R), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((paged_few_rows<T, D, FULL>), dim3(x.groups), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((paged_join<T, D, true>), dim3(x.groups * x.R), dim3(256), 0, st, p);
   return check_launch("paged attention");
 }
 template <class T>

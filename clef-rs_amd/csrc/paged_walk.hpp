@@ -64,7 +64,14 @@ __device__ __forceinline__ int64_t line_to(const Rows& t, const Request& x, int 
   return fixed * i + rising + (i - max(below, none)) * C;
 }
 
+// Values that are the same in all lanes, held in scalar registers: the kernels that walk
+// need their vector registers for tiles.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(x >> 32)))) << 32 |
+                              static_cast<uint32_t>(uniform(static_cast<int>(x))));
+}
+__device__ __forceinline__ Request uniform(Request x) { return {uniform(x.first), uniform(x.n), uniform(x.len)}; }
 
 struct WalkShared {
   int64_t sums[16];
@@ -80,7 +87,7 @@ struct Stretch {
   int s;
 };
 __device__ __forceinline__ int64_t cut_at(int64_t total, int w, int W) {
-  return w >= W ? total : static_cast<int64_t>(static_cast<double>(w) * static_cast<double>(total) / W);
+  return w >= W ? total : uniform(static_cast<int64_t>(static_cast<double>(w) * static_cast<double>(total) / W));
 }
 
 template <int NT>
@@ -99,7 +106,7 @@ __device__ __forceinline__ bool walk_begin(const Paged& p, const Rows& t, int64_
     return total > 0 && group / 8 < per && out.w < out.W;
   };
   if (p.nseq == 1) {
-    const Request x = request_of(p, 0);
+    const Request x = uniform(request_of(p, 0));
     const int tiles = tiles_of(t, x);
     out.s = 0;
     out.base = 0;
@@ -127,7 +134,7 @@ __device__ __forceinline__ bool walk_begin(const Paged& p, const Rows& t, int64_
     total += sh.sums[i];
   }
   upto += before;
-  if (!dealt(total)) return false;
+  if (!dealt(uniform(total))) return false;
   const int64_t u = out.u;
   if (u >= upto - mine && u < upto) {
     int64_t at = upto - mine;
@@ -143,7 +150,7 @@ __device__ __forceinline__ bool walk_begin(const Paged& p, const Rows& t, int64_
     sh.base = at;
   }
   __syncthreads();
-  out.base = sh.base;
+  out.base = uniform(sh.base);
   out.s = uniform(sh.s);
   return true;
 }
@@ -162,7 +169,7 @@ __device__ __forceinline__ bool next_piece(const Paged& p, const Rows& t, Stretc
   int64_t line;
   for (;; ++x.s) {
     if (x.s >= p.nseq) return false;  // (the line ends with the last request)
-    r = request_of(p, x.s);
+    r = uniform(request_of(p, x.s));
     tiles = tiles_of(t, r);
     if (!tiles) continue;
     line = line_to(t, r, tiles);
@@ -191,7 +198,7 @@ __device__ __forceinline__ bool next_piece(const Paged& p, const Rows& t, Stretc
   v = seen_by(t, r, lo * t.R, min((lo + 1) * t.R, r.n * t.G));
   // blocks in proportion; the same division on both sides of a cut
   const double scale = v.blocks / static_cast<double>(out.to - out.from);
-  auto block = [&](int64_t y) { return min(v.blocks, static_cast<int>((y - out.from) * scale)); };
+  auto block = [&](int64_t y) { return min(v.blocks, uniform(static_cast<int>((y - out.from) * scale))); };
   out.b0 = uniform(out.head ? 0 : block(x.u));
   out.b1 = uniform(out.tail ? v.blocks : block(stop));
   x.u = stop;
