@@ -473,6 +473,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
     for (int e = 0; e < 16; ++e) o[t][e] = 0.0f;
   float m = -INFINITY, l = 0.0f;
   if (x.b0 + 1 < x.b1) pages_at(seen.key0(x.b0 + 1), pages);
+  if (wave < 4) __builtin_amdgcn_s_setprio(2);
 
 #pragma unroll 1
   for (int b = x.b0; b < x.b1; ++b) {
@@ -570,6 +571,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
       }
     }
   }
+  __builtin_amdgcn_s_setprio(0);
   if (idle) return;
   l = halves_sum(l);
   const bool whole = x.head && x.tail, mine = 32 * wave + n < rows;
