@@ -92,7 +92,8 @@ SIGNATURES = {
     "clef_attention_paged_workspace": (_z, [_i] * 8),
     "clef_attention_gated_paged": (_i, [_p, _p, _i, _p, _p, _i, _i, _p, _l, _i, _p, _l, _l, _i, _i, _p, _l, _p, _p, _z,
                                         _p]),
-    "clef_paged_weights": (_i, [_p, _p, _i, _p, _p, _i, _i, _p, _l, _i, _p, _i, _i, _p, _p, _p]),
+    "clef_paged_weights_workspace": (_z, [_i] * 8),
+    "clef_paged_weights": (_i, [_p, _p, _i, _p, _p, _i, _i, _p, _l, _i, _p, _i, _i, _p, _p, _p, _z, _p]),
     "clef_paged_evict": (_i, [_p, _p, _i, _p, _i, _p, _i, _i, _i, _p, _p, _i, _p, _p, _p, _p]),
     "clef_embed": (_i, [_p, _i, _p, _i, _i, _i, _p, _p]),
     "clef_head_logits": (_i, [_p, _i, _p, _i, _p, _p]),
@@ -901,9 +902,15 @@ class PagedCache:
         self._scores(scores, "scores")
         self._scores(new_scores, "new_scores")
         _here(q, lse, cu_seqlens, key_lens, pages, self.k, self.vt, scores, new_scores)
-        _check(lib().clef_paged_weights(
+        L = lib()
+        n = L.clef_paged_weights_workspace(T, nseq, width, self.page, self.dtype, heads, self.kv_heads, self.d)
+        if n == 0:
+            raise ClefError(-1, last_error())
+        ws = _scratch(n, q.device) if n > 256 else None  # 256: the call keeps nothing there
+        _check(L.clef_paged_weights(
             self._at, pages.data_ptr(), width, cu_seqlens.data_ptr(), key_lens.data_ptr(), nseq, T, q.data_ptr(), T,
-            heads, lse.data_ptr(), int(window), int(sinks), scores.data_ptr(), new_scores.data_ptr(), _stream()))
+            heads, lse.data_ptr(), int(window), int(sinks), scores.data_ptr(), new_scores.data_ptr(), _ptr(ws),
+            n if ws is not None else 0, _stream()))
         return new_scores
 
     def evict(self, scores, key_lens, pages, budget, to, to_pages, to_scores, sinks=0, recent=0):

@@ -17,6 +17,7 @@
 #include "../../include/clef_hip.h"
 #include "attention_parts.hpp"
 #include "common.hpp"
+#include "lds_dma.hpp"
 #include "paged_walk.hpp"
 
 namespace clef {
@@ -278,20 +279,15 @@ template <int NT, class F>
 __device__ __forceinline__ void walk_pieces(const PagedAttn& p, WalkShared& walk, F take) {
   PagedAttn::Split split = {};
   Stretch x;
-  if (walk_begin<NT>(p.c, p.t, p.least, blockIdx.x, p.groups, walk, x)) {
+  if (walk_begin<NT>(
+          p.c, [&](const Request& r) { return line_of(p.c, p.t, r); }, p.least, blockIdx.x, p.groups, walk, x)) {
     Piece piece;
     Request r;
     Seen seen;
     while (next_piece(p.c, p.t, x, piece, r, seen)) {
       take(r, seen, piece, x.w);
       if (piece.head && !piece.tail) {
-        int lo = x.w + 1, hi = x.W - 1;  // the first work-group that ends at or behind the tile's end
-        while (lo < hi) {
-          const int mid = (lo + hi) / 2;
-          if (cut_at(x.total, mid + 1, x.W) >= piece.to) hi = mid;
-          else lo = mid + 1;
-        }
-        split = {piece.s, piece.kv, piece.tile, x.w, lo - x.w + 1};
+        split = {piece.s, piece.kv, piece.tile, x.w, last_of(x, piece.to) - x.w + 1};
       }
     }
   }
@@ -317,22 +313,6 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows(PagedAttn p) {
 // the time of the products.)  16-byte slots are permuted by their row (XOR) against
 // bank conflicts; key row r of LDS holds key r with bits 2 and 3 exchanged, so that the
 // 16 weights that a lane holds of 32 keys are operands of the next product as they stand.
-__device__ __forceinline__ void dma16(const void* src, void* lds_block) {
-  // global_load_lds_dwordx4: lane l writes 16 bytes at M0 + 16 l; awaited by vm_wait_all
-  const uint32_t m0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_block));
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
-}
-__device__ __forceinline__ void dma16s(const void* base, uint32_t off, void* lds_block) {
-  // the same from a base that is uniform; the wait states cover M0 and the readfirstlane
-  const uint32_t m0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_block));
-  const uint64_t b = reinterpret_cast<uint64_t>(base);
-  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(b >> 32)));
-  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(b)));
-  const uint64_t sb = (static_cast<uint64_t>(hi) << 32) | lo;
-  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(sb), "{m0}"(m0) : "memory");
-}
-__device__ __forceinline__ void vm_wait_all() { __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8)); }
-
 __device__ __forceinline__ float halves_max(float x) {  // of lanes l and l ^ 32
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -787,7 +767,7 @@ extern "C" int clef_attention_gated_paged(const clef_paged_cache* cache, const i
                    !(reinterpret_cast<uintptr_t>(workspace) & 255),
                "paged attention: workspace too small or not 256-byte aligned");
   p.c.cu = cu_seqlens; p.c.len = key_lens; p.c.nseq = nseq; p.c.T = T;
-  p.t.G = heads / p.c.kvh; p.t.R = x.R; p.t.window = window; p.t.sinks = sinks;
+  p.t = clef::rows_of(heads / p.c.kvh, x.R, window, sinks);
   p.q = q; p.gate = gate; p.y = y; p.lse = lse;
   p.ldq = ldq_tok; p.ldg = ldg; p.hsg = hsg; p.ldy = ldy;
   p.heads = heads;

@@ -14,9 +14,25 @@ constexpr int kTileCost = 32;    // what a tile costs beside its keys, in keys
 
 struct Rows {         // how query rows become tiles
   int G;              // rows of a token: heads of a key head
+  uint32_t over_g;    // 2^32 / G rounded up (0: G = 1)
   int R;              // rows of a tile
   int window, sinks;  // window 0: all keys
 };
+
+// The token of a row: rows are below 2^24, and 2^32 / G is rounded up by less than G <= 2^8 in
+// all, so the product's high word is exact.
+__device__ __forceinline__ int token_of(const Rows& t, int row) {
+  return t.over_g ? static_cast<int>(__umulhi(static_cast<uint32_t>(row), t.over_g)) : row;
+}
+inline Rows rows_of(int G, int R, int window, int sinks) {
+  Rows t;
+  t.G = G;
+  t.over_g = G == 1 ? 0 : static_cast<uint32_t>(((uint64_t(1) << 32) + G - 1) / G);
+  t.R = R;
+  t.window = window;
+  t.sinks = sinks;
+  return t;
+}
 
 // The keys that rows row0 .. row1 - 1 of a request (stacked (token, head)) see,
 // any of them: 0 .. sink - 1 and from .. to - 1, from <= to, in `blocks` blocks of
@@ -73,6 +89,12 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
 }
 __device__ __forceinline__ Request uniform(Request x) { return {uniform(x.first), uniform(x.n), uniform(x.len)}; }
 
+// all tiles of all key heads of a request
+__device__ __forceinline__ int64_t line_of(const Paged& p, const Rows& t, const Request& x) {
+  const int tiles = tiles_of(t, x);
+  return tiles ? p.kvh * line_to(t, x, tiles) : 0;
+}
+
 struct WalkShared {
   int64_t sums[16];
   int64_t total, base;
@@ -90,8 +112,9 @@ __device__ __forceinline__ int64_t cut_at(int64_t total, int w, int W) {
   return w >= W ? total : uniform(static_cast<int64_t>(static_cast<double>(w) * static_cast<double>(total) / W));
 }
 
-template <int NT>
-__device__ __forceinline__ bool walk_begin(const Paged& p, const Rows& t, int64_t least, int group, int groups,
+// length(request): what a request takes on the line.
+template <int NT, class F>
+__device__ __forceinline__ bool walk_begin(const Paged& p, F length, int64_t least, int group, int groups,
                                            WalkShared& sh, Stretch& out) {
   const int tid = threadIdx.x, lane = tid & 63;
   // few keys: fewer work-groups, each with `least` of the line at least
@@ -106,19 +129,13 @@ __device__ __forceinline__ bool walk_begin(const Paged& p, const Rows& t, int64_
     return total > 0 && group / 8 < per && out.w < out.W;
   };
   if (p.nseq == 1) {
-    const Request x = uniform(request_of(p, 0));
-    const int tiles = tiles_of(t, x);
     out.s = 0;
     out.base = 0;
-    return dealt(tiles ? p.kvh * line_to(t, x, tiles) : 0);
+    return dealt(length(uniform(request_of(p, 0))));
   }
   const int each = (p.nseq + NT - 1) / NT, s0 = tid * each, s1 = min(p.nseq, s0 + each);
   int64_t mine = 0;
-  for (int s = s0; s < s1; ++s) {
-    const Request x = request_of(p, s);
-    const int tiles = tiles_of(t, x);
-    if (tiles) mine += p.kvh * line_to(t, x, tiles);
-  }
+  for (int s = s0; s < s1; ++s) mine += length(request_of(p, s));
   int64_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -140,11 +157,9 @@ __device__ __forceinline__ bool walk_begin(const Paged& p, const Rows& t, int64_
     int64_t at = upto - mine;
     int s = s0;
     for (;; ++s) {
-      const Request x = request_of(p, s);
-      const int tiles = tiles_of(t, x);
-      const int64_t length = tiles ? p.kvh * line_to(t, x, tiles) : 0;
-      if (u < at + length || s + 1 >= s1) break;
-      at += length;
+      const int64_t y = length(request_of(p, s));
+      if (u < at + y || s + 1 >= s1) break;
+      at += y;
     }
     sh.s = s;
     sh.base = at;
@@ -153,6 +168,17 @@ __device__ __forceinline__ bool walk_begin(const Paged& p, const Rows& t, int64_
   out.base = uniform(sh.base);
   out.s = uniform(sh.s);
   return true;
+}
+
+// The work-group whose stretch contains the end of what lies before `to` on the line, behind x's own.
+__device__ __forceinline__ int last_of(const Stretch& x, int64_t to) {
+  int lo = x.w + 1, hi = x.W - 1;  // the first that ends at `to` or behind
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (cut_at(x.total, mid + 1, x.W) >= to) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
 }
 
 // One piece of a stretch: blocks b0 .. b1 - 1 of a tile of one key head.

@@ -514,12 +514,17 @@ int clef_attention_gated_paged(const clef_paged_cache* cache, const int32_t* tab
  * (new_scores may be scores itself); the new tokens' own keys start from 0.  Every
  * key of each request is written, all else is left as it was.  lse: as
  * clef_attention_gated_paged gives it for the same window and sinks.  The sum's
- * order is fixed: no atomics.  Requests of one call that share a page each write its
- * scores: that page receives the sums of one of them.
+ * order is fixed: no atomics.  ldq_tok is at most 2^22.  Requests of one call that
+ * share a page each write its scores: that page receives the sums of one of them.
+ * workspace: clef_paged_weights_workspace bytes, 256-byte aligned; where that is 256 (few
+ * rows to a request) nothing is kept there and workspace may be NULL.
  */
+size_t clef_paged_weights_workspace(int T, int nseq, int max_pages, int page, int dtype, int heads, int kv_heads,
+                                    int d);
 int clef_paged_weights(const clef_paged_cache* cache, const int32_t* table, int max_pages, const int32_t* cu_seqlens,
                        const int32_t* key_lens, int nseq, int T, const void* q, int64_t ldq_tok, int heads,
-                       const float* lse, int window, int sinks, const float* scores, float* new_scores, void* stream);
+                       const float* lse, int window, int sinks, const float* scores, float* new_scores, void* workspace,
+                       size_t workspace_bytes, void* stream);
 /*
  * Caches cut to `budget` keys each: of a request's len keys the first `sinks`, the
  * last `recent` and, of those between, the ones of largest score (per key head; NaN

@@ -40,7 +40,7 @@ def args(clef, kind, kw):
                        ldpos=9, axes=3, axis_of=bytes([0, 1, 2, 0] * 4), rot=32, theta=1e7, out=256, ldo=9),
         "attention": dict(q=256, ldq=9, heads=8, gate=256, ldg=512, hsg=64, window=0, sinks=0, y=256, ldy=512,
                           lse=256, ws=256, wsb=1 << 40),
-        "weights": dict(q=256, ldq=9, heads=8, lse=256, window=0, sinks=0, scores=256, new=256)}[kind])
+        "weights": dict(q=256, ldq=9, heads=8, lse=256, window=0, sinks=0, scores=256, new=256, ws=256, wsb=1 << 40)}[kind])
     kw = {k: v for k, v in kw.items() if not k.startswith("cache_")}
     assert set(kw) <= set(a), kw
     a.update(kw)
@@ -56,7 +56,8 @@ OWN = {
                   dict(ldg=511), dict(hsg=63), dict(ldy=511), dict(window=-1), dict(window=(1 << 24) + 1),
                   dict(sinks=-1), dict(sinks=(1 << 24) + 1), dict(q=264)],
     "weights": [dict(q=None), dict(lse=None), dict(scores=None), dict(new=None), dict(ldq=8), dict(window=-1),
-                dict(window=(1 << 24) + 1), dict(sinks=-1), dict(sinks=(1 << 24) + 1), dict(q=264)],
+                dict(window=(1 << 24) + 1), dict(sinks=-1), dict(sinks=(1 << 24) + 1), dict(q=264), dict(ws=264), dict(ldq=(1 << 22) + 1), dict(T=900, ldq=900, ws=None),
+                dict(T=900, ldq=900, wsb=0)],
 }
 NAME = {"append": "clef_paged_append", "attention": "clef_attention_gated_paged", "weights": "clef_paged_weights"}
 
@@ -69,19 +70,21 @@ def test_batches_refuse(clef, kind, bad):
     assert "paged " + kind in clef.last_error()
 
 
-def test_attention_workspace(clef):
+@pytest.mark.parametrize("kind", ["attention", "weights"])
+def test_workspace(clef, kind):
     L = clef.lib()
-    good = (9, 3, 5, 32, 1, 8, 2, 64)
-    n = L.clef_attention_paged_workspace(*good)
+    size = {"attention": L.clef_attention_paged_workspace, "weights": L.clef_paged_weights_workspace}[kind]
+    good = (900, 3, 5, 32, 1, 8, 2, 64)
+    n = size(*good)
     assert n > 256 and n % 256 == 0
-    assert L.clef_attention_gated_paged(*args(clef, "attention", dict(wsb=n - 1))) < 0
+    assert getattr(L, NAME[kind])(*args(clef, kind, dict(T=900, ldq=900, wsb=n - 1))) < 0
     for i, bad in ((0, 0), (0, 65537), (1, 0), (1, 4097), (2, 0), (2, (1 << 19) + 1), (3, 24), (4, 3), (5, 0), (5, 7),
                    (6, 0), (7, 4), (7, 264)):
         a = list(good)
         a[i] = bad
-        assert L.clef_attention_paged_workspace(*a) == 0, (i, bad)
+        assert size(*a) == 0, (i, bad)
     # the largest call that is allowed
-    assert L.clef_attention_paged_workspace(65536, 4096, 1 << 20, 16, 0, 256, 256, 256) > 0
+    assert size(65536, 4096, 1 << 20, 16, 0, 256, 256, 256) > 0
 
 
 def evict(clef, **kw):
