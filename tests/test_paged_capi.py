@@ -51,7 +51,7 @@ OWN = {
     "append": [dict(q=None), dict(k=None), dict(v=None), dict(qn=None), dict(kn=None), dict(out=None), dict(ldq=511),
                dict(hsq=63), dict(ldk=127), dict(ldv=127), dict(ldo=8), dict(rot=33), dict(rot=-2), dict(rot=66),
                dict(theta=0.0), dict(theta=float("nan")), dict(theta=float("inf")), dict(eps=-1.0),
-               dict(eps=float("nan")), dict(axes=0), dict(axes=5), dict(axes=2), dict(ldpos=8), dict(out=258)],
+               dict(eps=float("nan")), dict(axes=0), dict(axes=5), dict(axes=2), dict(ldpos=8), dict(out=264)],
     "attention": [dict(q=None), dict(gate=None), dict(y=None), dict(ws=None), dict(wsb=0), dict(ws=264), dict(ldq=8),
                   dict(ldg=511), dict(hsg=63), dict(ldy=511), dict(window=-1), dict(window=(1 << 24) + 1),
                   dict(sinks=-1), dict(sinks=(1 << 24) + 1), dict(q=264)],
@@ -100,7 +100,7 @@ def evict(clef, **kw):
 
 @pytest.mark.parametrize("bad", [
     dict(cache=None), dict(to=None), dict(table=None), dict(to_table=None), dict(lens=None), dict(scores=None),
-    dict(to_scores=None), dict(new=None), dict(keep=None), dict(width=0), dict(to_width=0), dict(nseq=0),
+    dict(scores=264), dict(to_scores=None), dict(new=None), dict(keep=None), dict(width=0), dict(to_width=0), dict(nseq=0),
     dict(nseq=4097), dict(budget=0), dict(budget=-1), dict(budget=11), dict(budget=97), dict(sinks=-1),
     dict(sinks=71), dict(recent=-1), dict(recent=67), dict(sinks=2 ** 31 - 1), dict(recent=2 ** 31 - 1),
     dict(to_cache_page=16, to_width=6), dict(to_cache_kv_heads=1), dict(to_cache_d=72), dict(to_cache_dtype=0)] +
