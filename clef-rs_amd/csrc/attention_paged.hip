@@ -44,23 +44,27 @@ struct PagedAttn {
   } * split;         // [groups]
 };
 
-// four features of one output: their gate, and the output itself
+// four features of one output from its sums o and 1 / l (no key: 0): their gate, and the output
+// itself.  f16: the hardware's exp2 and reciprocal, off by 2^-20, in a few instructions.
+__device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 template <class T>
-__device__ __forceinline__ void write_out(const PagedAttn& p, float4_t o, float l, int t, int h, int e) {
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+__device__ __forceinline__ void write_out(const PagedAttn& p, float4_t o, float inv, int t, int h, int e, bool vec) {
   const T* gp = static_cast<const T*>(p.gate) + t * p.ldg + h * p.hsg + e;
   T* y = static_cast<T*>(p.y) + t * p.ldy + (int64_t)h * p.c.d + e;
   typedef T vec4 __attribute__((ext_vector_type(4)));
   vec4 g;
-  if (p.vec) {
+  if (vec) {
     g = *reinterpret_cast<const vec4*>(gp);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) g[j] = gp[j];
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) g[j] = cvt_out<T>(o[j] * inv * sigmoid(to_f32(g[j])));
-  if (p.vec) {
+  for (int j = 0; j < 4; ++j) {
+    const float x = to_f32(g[j]);
+    g[j] = cvt_out<T>(o[j] * inv * (sizeof(T) == 2 ? sigmoid_hw(x) : sigmoid(x)));
+  }
+  if (vec) {
     *reinterpret_cast<vec4*>(y) = g;
   } else {
 #pragma unroll
@@ -179,11 +183,11 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Request& r, c
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, grp = lane >> 4, G = p.t.G;
   // the lane's query (rows behind the last: the last again)
-  const int row = row0 + min(lr, rows - 1), at = r.len - r.n + row / G;
+  const int row = row0 + min(lr, rows - 1), tok = token_of(p.t, row), at = r.len - r.n + tok;
   frag fq[D / KB];
   auto load_queries = [&]() {
     const T* src =
-        static_cast<const T*>(p.q) + ((int64_t)(x.kv * G + row % G) * p.ldq + r.first + row / G) * c.d + grp * EL;
+        static_cast<const T*>(p.q) + ((int64_t)(x.kv * G + row - tok * G) * p.ldq + r.first + tok) * c.d + grp * EL;
 #pragma unroll
     for (int kb = 0; kb < D / KB; ++kb) fq[kb] = FULL || kb * KB + grp * EL < c.d ? frag_at(src + kb * KB) : frag{};
   };
@@ -263,8 +267,8 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Request& r, c
     float m, l;
     const float4_t o = sh.parts.take(y, e, m, l);
     if (whole) {
-      const int t = r.first + (row0 + y) / G, h = x.kv * G + (row0 + y) % G;
-      if (e < c.d) write_out<T>(p, o, l, t, h, e);
+      const int tok = token_of(p.t, row0 + y), t = r.first + tok, h = x.kv * G + row0 + y - tok * G;
+      if (e < c.d) write_out<T>(p, o, inverse(l), t, h, e, p.vec);
       if (e == 0) write_lse<T>(p, m, l, t, h);
     } else {
       *reinterpret_cast<float4_t*>(p.part + (to + y) * D + e) = o;
@@ -365,7 +369,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, g = lane >> 5, G = p.t.G, shift = c.shift, in = (1 << shift) - 1;
   const bool idle = 32 * wave >= rows;  // a wave without rows moves tiles for the others
-  const int row = row0 + min(32 * wave + n, rows - 1), at = r.len - r.n + row / G;
+  const int row = row0 + min(32 * wave + n, rows - 1), at = r.len - r.n + token_of(p.t, row);
   const char* K = static_cast<const char*>(c.k) + (((int64_t)x.kv << shift) * D) * 2;
   const char* V = static_cast<const char*>(c.vt) + (((int64_t)x.kv << shift) * D) * 2;
   auto kswz = [](int y) { return D >= 128 ? y & 15 : y >> 1 & 7; };
@@ -440,7 +444,8 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
   constexpr int QL = kQueryLds<D>(), QR = NKB - QL;
   half8 fq[QR];
   {
-    const T* src = static_cast<const T*>(p.q) + ((int64_t)(x.kv * G + row % G) * p.ldq + r.first + row / G) * D + 8 * g;
+    const int tok = token_of(p.t, row);
+    const T* src = static_cast<const T*>(p.q) + ((int64_t)(x.kv * G + row - tok * G) * p.ldq + r.first + tok) * D + 8 * g;
 #pragma unroll
     for (int kb = 0; kb < QR; ++kb) fq[kb] = *reinterpret_cast<const half8*>(src + 16 * kb);
 #pragma unroll
@@ -558,7 +563,10 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
   const bool odd = *odd_flag != 0;
   // (a whole tile needs no part; the second is free until the last piece)
   const int64_t to = ((int64_t)w * 2 + (x.head ? 1 : 0)) * kManyRows + 32 * wave + n;
-  const int tok = r.first + row / G, h = x.kv * G + row % G;
+  const int tok = r.first + token_of(p.t, row), h = x.kv * G + row - token_of(p.t, row) * G;
+  // straight to the output, or through the part (whose loops are short code)
+  const bool direct = whole && !odd && p.vec;
+  const float inv = inverse(l);
   auto feature = [&](int t, int i) { return 32 * t + 8 * i + 4 * g; };  // of o[t][4 i]
   if (mine && g == 0) {
     if (whole) write_lse<T>(p, m, l, tok, h);
@@ -570,16 +578,16 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
     for (int i = 0; i < 4; ++i) {
       const float4_t y = {o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
       if (!mine) continue;
-      if (whole && !odd) write_out<T>(p, y, l, tok, h, feature(t, i));
+      if (direct) write_out<T>(p, y, inv, tok, h, feature(t, i), true);
       else *reinterpret_cast<float4_t*>(p.part + to * D + feature(t, i)) = y;
     }
-  if (!odd) return;
+  if (direct || (!whole && !odd)) return;
   // (rare) the infinite and NaN values, key by key, to the rows that see them; each lane adds
   // to the features that it has written
   const T* qrow = static_cast<const T*>(p.q) + ((int64_t)h * p.ldq + tok) * D;
   const float ref = (m == -INFINITY ? 0.0f : m) - Ops<T>::UP;
 #pragma unroll 1
-  for (int b = x.b0; b < x.b1; ++b) {
+  for (int b = x.b0; b < x.b1 && odd; ++b) {
     const int k0 = seen.key0(b);
 #pragma unroll 1
     for (int j = k0; j < k0 + BK; ++j) {
@@ -614,7 +622,8 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
   if (whole && mine) {
 #pragma unroll 1
     for (int i = 0; i < D / 8; ++i)
-      write_out<T>(p, *reinterpret_cast<const float4_t*>(p.part + to * D + 8 * i + 4 * g), l, tok, h, 8 * i + 4 * g);
+      write_out<T>(p, *reinterpret_cast<const float4_t*>(p.part + to * D + 8 * i + 4 * g), inv, tok, h, 8 * i + 4 * g,
+                   p.vec);
   }
 }
 
@@ -680,8 +689,8 @@ __global__ __launch_bounds__(256) void paged_join(PagedAttn p) {
     }
   }
   if (!live) return;
-  const int t = r.first + row / p.t.G, h = x.kv * p.t.G + row % p.t.G;
-  if (e < p.c.d) write_out<T>(p, o, l, t, h, e);
+  const int tok = token_of(p.t, row), t = r.first + tok, h = x.kv * p.t.G + row - tok * p.t.G;
+  if (e < p.c.d) write_out<T>(p, o, inverse(l), t, h, e, p.vec);
   if (e == 0) write_lse<T>(p, m, l, t, h);
 }
 

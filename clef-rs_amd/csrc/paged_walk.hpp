@@ -12,10 +12,28 @@ namespace {
 constexpr int kWalkBlock = 64;   // keys that stretches are counted in
 constexpr int kTileCost = 32;    // what a tile costs beside its keys, in keys
 
+// Values that are the same in all lanes, held in scalar registers: the kernels that walk
+// need their vector registers for tiles.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(x >> 32)))) << 32 |
+                              static_cast<uint32_t>(uniform(static_cast<int>(x))));
+}
+__device__ __forceinline__ Request uniform(Request x) { return {uniform(x.first), uniform(x.n), uniform(x.len)}; }
+
+// a / b of whole numbers below 2^53, b > 0, through f64 (a 64-bit division takes more than a
+// hundred instructions, and these kernels' time is in part that of fetching theirs)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  int64_t q = uniform(static_cast<int64_t>(static_cast<double>(a) / static_cast<double>(b)));
+  if (q * b > a) --q;
+  if ((q + 1) * b <= a) ++q;
+  return q;
+}
+
 struct Rows {         // how query rows become tiles
   int G;              // rows of a token: heads of a key head
   uint32_t over_g;    // 2^32 / G rounded up (0: G = 1)
-  int R;              // rows of a tile
+  int R, log_r;       // rows of a tile, a power of two
   int window, sinks;  // window 0: all keys
 };
 
@@ -29,6 +47,7 @@ inline Rows rows_of(int G, int R, int window, int sinks) {
   t.G = G;
   t.over_g = G == 1 ? 0 : static_cast<uint32_t>(((uint64_t(1) << 32) + G - 1) / G);
   t.R = R;
+  t.log_r = __builtin_ctz(R);
   t.window = window;
   t.sinks = sinks;
   return t;
@@ -48,8 +67,8 @@ struct Seen {
 };
 __device__ __forceinline__ Seen seen_by(const Rows& t, const Request& x, int row0, int row1) {
   Seen v;
-  v.low = x.len - x.n + row0 / t.G;
-  v.high = x.len - x.n + (row1 - 1) / t.G;
+  v.low = x.len - x.n + uniform(token_of(t, row0));
+  v.high = x.len - x.n + uniform(token_of(t, row1 - 1));
   v.to = max(v.high + 1, 0);
   v.from = t.window ? min(max(v.low - t.window + 1, 0), v.to) : 0;
   v.sink = t.window ? min(t.sinks, v.from) : 0;
@@ -62,7 +81,7 @@ __device__ __forceinline__ bool sees(const Rows& t, int p, int j) {
   return j <= p && (t.window == 0 || j > p - t.window || j < t.sinks);
 }
 
-__device__ __forceinline__ int tiles_of(const Rows& t, const Request& x) { return (x.n * t.G + t.R - 1) / t.R; }
+__device__ __forceinline__ int tiles_of(const Rows& t, const Request& x) { return (x.n * t.G + t.R - 1) >> t.log_r; }
 
 // The line's length up to tile i of one key head of a request, in keys times G: tile
 // j = 1, 2, .. adds a constant and clamp(A + R j, 0, C), about the keys that its last
@@ -70,24 +89,15 @@ __device__ __forceinline__ int tiles_of(const Rows& t, const Request& x) { retur
 __device__ __forceinline__ int64_t line_to(const Rows& t, const Request& x, int i) {
   const int64_t A = (int64_t)(x.len - x.n) * t.G;
   int64_t C = (int64_t)x.len * t.G;
-  if (t.window) C = min(C, ((int64_t)t.window + t.sinks + t.R / t.G + 1) * t.G);
+  if (t.window) C = min(C, ((int64_t)t.window + t.sinks + 1) * t.G + t.R);
   const int64_t fixed = (int64_t)kTileCost * t.G;
   if (i == 1) return fixed + min(max(A + t.R, (int64_t)0), C);
   // tiles of nothing, and tiles below the bound
-  const int64_t none = A < 0 ? min((int64_t)i, -A / t.R) : 0;
-  const int64_t below = C > A ? min((int64_t)i, (C - A - 1) / t.R) : 0;
+  const int64_t none = A < 0 ? min((int64_t)i, -A >> t.log_r) : 0;
+  const int64_t below = C > A ? min((int64_t)i, (C - A - 1) >> t.log_r) : 0;
   const int64_t rising = below > none ? A * (below - none) + t.R * (below * (below + 1) - none * (none + 1)) / 2 : 0;
   return fixed * i + rising + (i - max(below, none)) * C;
 }
-
-// Values that are the same in all lanes, held in scalar registers: the kernels that walk
-// need their vector registers for tiles.
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(x >> 32)))) << 32 |
-                              static_cast<uint32_t>(uniform(static_cast<int>(x))));
-}
-__device__ __forceinline__ Request uniform(Request x) { return {uniform(x.first), uniform(x.n), uniform(x.len)}; }
 
 // all tiles of all key heads of a request
 __device__ __forceinline__ int64_t line_of(const Paged& p, const Rows& t, const Request& x) {
@@ -120,7 +130,7 @@ __device__ __forceinline__ bool walk_begin(const Paged& p, F length, int64_t lea
   // few keys: fewer work-groups, each with `least` of the line at least
   auto dealt = [&](int64_t total) {
     out.total = total;
-    out.W = static_cast<int>(min((int64_t)groups, max((int64_t)1, total / least)));
+    out.W = static_cast<int>(min((int64_t)groups, max((int64_t)1, quotient(total, least))));
     // neighbours on the line share keys: one XCD (work-groups go round them) takes neighbours
     const int per = (out.W + 7) / 8;
     out.w = group % 8 * per + group / 8;
@@ -203,9 +213,10 @@ __device__ __forceinline__ bool next_piece(const Paged& p, const Rows& t, Stretc
     x.base += p.kvh * line;
   }
   int64_t at = x.u - x.base;
-  const int kv = p.kvh == 1 ? 0 : static_cast<int>(at / line);
+  const int kv = p.kvh == 1 ? 0 : static_cast<int>(quotient(at, line));
   at -= kv * line;
   int lo = 0, hi = tiles;  // the last tile that begins at or before `at`
+#pragma unroll 1
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
     if (line_to(t, r, mid) <= at) lo = mid;

@@ -114,12 +114,12 @@ __global__ __launch_bounds__(256) void weights_few_rows(WeightParams p) {
     if (!r.len) continue;
     const int64_t cost = each(r);
     const int blocks = blocks_of(r);
-    const int64_t count = (int64_t)c.kvh * blocks;
+    const int count = c.kvh * blocks;  // (below 2^28)
     // blocks that begin in the stretch
-    const int64_t b0 = x.u <= x.base ? 0 : min(count, (x.u - x.base + cost - 1) / cost);
-    const int64_t b1 = min(count, (x.end - x.base + cost - 1) / cost);
-    for (int64_t b = b0 + wave; b < b1; b += NW) {
-      const int kv = uniform(static_cast<int>(b / blocks)), key0 = uniform(static_cast<int>(b % blocks)) * BK;
+    const int b0 = x.u <= x.base ? 0 : static_cast<int>(min((int64_t)count, quotient(x.u - x.base + cost - 1, cost)));
+    const int b1 = static_cast<int>(min((int64_t)count, quotient(x.end - x.base + cost - 1, cost)));
+    for (int b = b0 + wave; b < b1; b += NW) {
+      const int kv = b / blocks, key0 = b % blocks * BK;
       float sum[NT][4] = {};
       int from, to;
       rows_seeing(p.t, r, key0, BK, from, to);
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256) void weights_few_rows(WeightParams p) {
       if (lane < BK) write_sum(p, r, s, kv, key0 + lane, part[wave][lane]);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    x.base += count * cost;
+    x.base += (int64_t)count * cost;
   }
 }
 
@@ -206,9 +206,10 @@ __global__ __launch_bounds__(512, 2) void weights_many_rows(WeightParams p) {
     const int blocks = blocks_of(r), first = r.len - r.n;
     const int64_t next = x.base + c.kvh * (blocks * cost);
     while (x.u < min(next, x.end)) {
-      const int64_t b = (x.u - x.base) / cost, start = x.base + b * cost, stop = min(start + cost, x.end);
+      const int b = static_cast<int>(quotient(x.u - x.base, cost));
+      const int64_t start = x.base + b * cost, stop = min(start + cost, x.end);
       const bool head = x.u == start, tail = stop == start + cost;
-      const int kv = uniform(static_cast<int>(b / blocks)), key0 = uniform(static_cast<int>(b % blocks)) * kManyKeys;
+      const int kv = b / blocks, key0 = b % blocks * kManyKeys;
       int from, to;
       rows_seeing(p.t, r, key0, kManyKeys, from, to);
       const int tiles = max(to - from + kManyTile - 1, 0) / kManyTile;
