@@ -33,7 +33,7 @@ struct PagedAttn {
   int64_t ldq, ldg, hsg, ldy;
   int heads, vec;    // vec: gate and y in pieces of four
   float scale;       // log2(e) / sqrt(d): scores in log2 units
-  int64_t least;     // shortest stretch of a work-group, on the line
+  float over_least;  // 1 / the shortest stretch of a work-group, on the line
   int groups;        // work-groups of the first launch
   // each work-group's two parts (0: of the tile that it begins in the middle of, 1: of
   // the one that it ends in the middle of), and the tile whose first part it holds
@@ -284,7 +284,7 @@ __device__ __forceinline__ void walk_pieces(const PagedAttn& p, WalkShared& walk
   PagedAttn::Split split = {};
   Stretch x;
   if (walk_begin<NT>(
-          p.c, [&](const Request& r) { return line_of(p.c, p.t, r); }, p.least, blockIdx.x, p.groups, walk, x)) {
+          p.c, [&](const Request& r) { return line_of(p.c, p.t, r); }, p.over_least, blockIdx.x, p.groups, walk, x)) {
     Piece piece;
     Request r;
     Seen seen;
@@ -334,6 +334,8 @@ __device__ __forceinline__ int fresh_lane() {
 }
 
 constexpr int kManyRows = 256;
+constexpr int kStagePitch = 68;                  // floats of a row of 64 features on their way out
+constexpr int kStage = 32 * kStagePitch + 32;    // of a wave's 32 rows, and 1 / l of each
 
 // Query operands of a wave that stand in LDS: at D = 256 registers hold 13 of the 16 beside
 // the outputs (128 registers) and what a tile needs.
@@ -357,6 +359,47 @@ struct TilePages {
   }
 };
 
+// (rare) The infinite and NaN values of the tiles that not all rows see, key by key, to the rows
+// that see them: features f0 .. + 63 of the lane's row, half of them each of lanes n and n + 32,
+// at `out` in LDS.
+template <int D>
+__device__ __forceinline__ void add_odd(const PagedAttn& p, const Request& r, const Seen& seen, const Piece& x, int row,
+                                        int at, int f0, float m, float* out, bool mine) {
+  typedef half_t T;
+  const Paged& c = p.c;
+  const int lane = threadIdx.x & 63, g = lane >> 5, in = (1 << c.shift) - 1, G = p.t.G;
+  const int tok = token_of(p.t, row);
+  const T* K = static_cast<const T*>(c.k) + (((int64_t)x.kv << c.shift) * D);
+  const T* V = static_cast<const T*>(c.vt) + (((int64_t)x.kv << c.shift) * D);
+  const T* q = static_cast<const T*>(p.q) + ((int64_t)(x.kv * G + row - tok * G) * p.ldq + r.first + tok) * D;
+  const float ref = (m == -INFINITY ? 0.0f : m) - Ops<T>::UP;
+#pragma unroll 1
+  for (int b = x.b0; b < x.b1; ++b) {
+    const int k0 = seen.key0(b);
+    if (k0 + 63 <= seen.low && (p.t.window == 0 || k0 > seen.high - p.t.window || k0 + 64 <= p.t.sinks))
+      continue;  // all rows see it: its products have such values
+#pragma unroll 1
+    for (int j = k0; j < k0 + 64; ++j) {
+      if (!seen.any(j)) continue;
+      const int page = page_of(c, x.s, j);
+      const T* v = V + page * c.vs + (j & in) + ((int64_t)f0 << c.shift);
+      if (!__any(!(fabsf(to_f32(v[lane << c.shift])) < INFINITY))) continue;
+      const T* key = K + page * c.ks + (j & in) * D;
+      float s = 0.0f;
+#pragma unroll 1
+      for (int e = g; e < D; e += 2) s = fmaf(to_f32(q[e]), to_f32(key[e]), s);
+      s = halves_sum(s);
+      if (!mine || !sees(p.t, at, j)) continue;
+      const float f = __builtin_amdgcn_exp2f(fmaf(s, p.scale, -ref));
+#pragma unroll 1
+      for (int e = g; e < 64; e += 2) {
+        const float y = to_f32(v[e << c.shift]);
+        if (!(fabsf(y) < INFINITY)) out[e] += f * y;
+      }
+    }
+  }
+}
+
 template <int D>
 __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, const Seen& seen, const Piece& x,
                                           int row0, int rows, Tiles<D>& sh, int* odd_flag, int w) {
@@ -366,10 +409,12 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
   constexpr float kLow = -1e30f;         // stands for a maximum of -inf where one is subtracted
   constexpr int PD = 4;                  // operands read ahead
   const Paged& c = p.c;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = lane & 31, g = lane >> 5, G = p.t.G, shift = c.shift, in = (1 << shift) - 1;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = p.t.G, shift = c.shift, in = (1 << shift) - 1;
   const bool idle = 32 * wave >= rows;  // a wave without rows moves tiles for the others
-  const int row = row0 + min(32 * wave + n, rows - 1), at = r.len - r.n + token_of(p.t, row);
+  // (what follows from the lane alone is formed where it is used: kept for the loop it would cost the
+  // registers of a query operand)
+  auto row_of = [&]() { return row0 + min(32 * wave + (fresh_lane() & 31), rows - 1); };
   const char* K = static_cast<const char*>(c.k) + (((int64_t)x.kv << shift) * D) * 2;
   const char* V = static_cast<const char*>(c.vt) + (((int64_t)x.kv << shift) * D) * 2;
   auto kswz = [](int y) { return D >= 128 ? y & 15 : y >> 1 & 7; };
@@ -421,36 +466,63 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
   };
 
   // operands: key rows 32 kh + n, 16-byte chunk 2 kb + g; feature rows 32 t + n, chunk 2 y + g
-  // (each read's variant is formed where it is used, in one instruction that the compiler
-  // neither shares nor moves: kept for the loop they cost the registers of three Q operands)
-  const int koff = n * 2 * D + 16 * (g ^ kswz(n)), voff = n * 128 + 16 * (g ^ (n >> 1 & 7));
+  // (each read's variant is formed where it is used, in one instruction that the compiler neither
+  // shares nor moves: kept for the loop they cost the registers of three query operands)
+  auto key_offset = [&]() {
+    const int lane = fresh_lane(), n = lane & 31;
+    return n * 2 * D + 16 * (lane >> 5 ^ kswz(n));
+  };
+  auto value_offset = [&]() {
+    const int lane = fresh_lane(), n = lane & 31;
+    return n * 128 + 16 * (lane >> 5 ^ (n >> 1 & 7));
+  };
   auto variant = [](int off, int bits) {
     int y;
     asm volatile("v_xor_b32 %0, %1, %2" : "=v"(y) : "i"(bits), "v"(off));
     return y;
   };
-  auto key_at = [&](const char* base, int kh, int kb) {
+  auto key_at = [&](const char* base, int koff, int kh, int kb) {
     return *reinterpret_cast<const half8*>(base + variant(koff, 32 * (kb % PER)) + kh * 64 * D + kb / PER * 32 * PER);
   };
-  auto value_at = [&](const char* base, int y, int t) {
+  auto value_at = [&](const char* base, int voff, int y, int t) {
     return *reinterpret_cast<const half8*>(base + variant(voff, 32 * y) + t * 32 * 128);
   };
 
   lds_barrier();  // the piece before is done with the tiles
   if (tid == 0) *odd_flag = 0;
-  TilePages pages;
-  pages_at(seen.key0(x.b0), pages);
-  if (x.b0 < x.b1) issue(0, seen.key0(x.b0), pages);
+  // The wave's queries, whole rows at a time through its eighth of the tiles' LDS (operands straight
+  // from memory take 32 bytes of 32 rows to a load).
   constexpr int QL = kQueryLds<D>(), QR = NKB - QL;
   half8 fq[QR];
-  {
-    const int tok = token_of(p.t, row);
-    const T* src = static_cast<const T*>(p.q) + ((int64_t)(x.kv * G + row - tok * G) * p.ldq + r.first + tok) * D + 8 * g;
-#pragma unroll
-    for (int kb = 0; kb < QR; ++kb) fq[kb] = *reinterpret_cast<const half8*>(src + 16 * kb);
-#pragma unroll
-    for (int kb = 0; kb < QL; ++kb) sh.q[wave][kb][lane] = *reinterpret_cast<const half8*>(src + 16 * (QR + kb));
+  T* const stage = &sh.k[0][0] + wave * 32 * D;
+  if (!idle) {
+    const char* const q0 =
+        static_cast<const char*>(p.q) + ((int64_t)x.kv * G * p.ldq + r.first) * (2 * D);
+    const uint32_t ldq = static_cast<uint32_t>(p.ldq);
+#pragma unroll 2
+    for (int i = 0; i < 32 / KROWS; ++i) {
+      const int lane = fresh_lane(), y = i * KROWS + lane / KS;
+      const int at = row0 + min(32 * wave + y, rows - 1), tok = token_of(p.t, at);
+      dma16(q0 + static_cast<uint64_t>(static_cast<uint32_t>(at - tok * G) * ldq + tok) * (2 * D) +
+                16 * ((lane % KS) ^ kswz(y)),
+            stage + i * KROWS * D);
+    }
   }
+  TilePages pages;
+  pages_at(seen.key0(x.b0), pages);
+  if (!idle) {
+    vm_wait_all();
+    const char* const mine = reinterpret_cast<const char*>(stage);
+    const int koff = key_offset();
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) {
+      const half8 y = *reinterpret_cast<const half8*>(mine + variant(koff, 32 * (kb % PER)) + kb / PER * 32 * PER);
+      if (kb < QR) fq[kb < QR ? kb : 0] = y;
+      else sh.q[wave][kb < QR ? 0 : kb - QR][fresh_lane()] = y;
+    }
+  }
+  lds_barrier();
+  if (x.b0 < x.b1) issue(0, seen.key0(x.b0), pages);
   float16_t o[NDT];
 #pragma unroll
   for (int t = 0; t < NDT; ++t)
@@ -497,19 +569,20 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
     const char* vbase = reinterpret_cast<const char*>(sh.v[buf]);
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh) {
+      const int koff = key_offset();
       float16_t S;
 #pragma unroll
       for (int e = 0; e < 16; ++e) S[e] = 0.0f;
       half8 f[PD], lq = {};
 #pragma unroll
-      for (int i = 0; i < PD; ++i) f[i] = key_at(kbase, kh, i);
+      for (int i = 0; i < PD; ++i) f[i] = key_at(kbase, koff, kh, i);
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
         S = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[kb % PD], kb < QR ? fq[kb < QR ? kb : 0] : lq, S, 0, 0, 0);
         if constexpr (QL > 0) {
           if (kb + 1 >= QR && kb + 1 < NKB) lq = sh.q[wave][kb + 1 - QR][fresh_lane()];
         }
-        if (kb + PD < NKB) f[kb % PD] = key_at(kbase, kh, kb + PD);
+        if (kb + PD < NKB) f[kb % PD] = key_at(kbase, koff, kh, kb + PD);
         __builtin_amdgcn_sched_barrier(0);
       }
       // element e of lane group g: key k0 + 32 kh + 16 (e / 8) + 8 g + e % 8
@@ -517,7 +590,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
         const int first = k0 + 32 * kh + 8 * (fresh_lane() >> 5);
         float hidden;
         asm volatile("v_mov_b32 %0, 0xff800000" : "=v"(hidden));  // -inf
-        const int last = at - first, left = p.t.window ? last - p.t.window : -1, sink = p.t.sinks - first;
+        const int last = r.len - r.n + token_of(p.t, row_of()) - first, left = p.t.window ? last - p.t.window : -1, sink = p.t.sinks - first;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int key = 16 * (e >> 3) + (e & 7);
@@ -546,84 +619,62 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
         wt[e >> 3][e & 7] = static_cast<T>(y);
       }
       __builtin_amdgcn_sched_barrier(0);
+      const int voff = value_offset();
 #pragma unroll
-      for (int i = 0; i < PD; ++i) f[i] = value_at(vbase, 2 * kh + i / NDT, i % NDT);
+      for (int i = 0; i < PD; ++i) f[i] = value_at(vbase, voff, 2 * kh + i / NDT, i % NDT);
 #pragma unroll
       for (int i = 0; i < 2 * NDT; ++i) {
         o[i % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % PD], wt[i / NDT], o[i % NDT], 0, 0, 0);
-        if (i + PD < 2 * NDT) f[i % PD] = value_at(vbase, 2 * kh + (i + PD) / NDT, (i + PD) % NDT);
+        if (i + PD < 2 * NDT) f[i % PD] = value_at(vbase, voff, 2 * kh + (i + PD) / NDT, (i + PD) % NDT);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
   __builtin_amdgcn_s_setprio(0);
+  lds_barrier();  // all are done with the tiles
   if (idle) return;
   l = halves_sum(l);
-  const bool whole = x.head && x.tail, mine = 32 * wave + n < rows;
-  const bool odd = *odd_flag != 0;
-  // (a whole tile needs no part; the second is free until the last piece)
-  const int64_t to = ((int64_t)w * 2 + (x.head ? 1 : 0)) * kManyRows + 32 * wave + n;
-  const int tok = r.first + token_of(p.t, row), h = x.kv * G + row - token_of(p.t, row) * G;
-  // straight to the output, or through the part (whose loops are short code)
-  const bool direct = whole && !odd && p.vec;
-  const float inv = inverse(l);
-  auto feature = [&](int t, int i) { return 32 * t + 8 * i + 4 * g; };  // of o[t][4 i]
-  if (mine && g == 0) {
-    if (whole) write_lse<T>(p, m, l, tok, h);
-    else p.ml[to] = float2{m, l};
-  }
-#pragma unroll
-  for (int t = 0; t < NDT; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4_t y = {o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
-      if (!mine) continue;
-      if (direct) write_out<T>(p, y, inv, tok, h, feature(t, i), true);
-      else *reinterpret_cast<float4_t*>(p.part + to * D + feature(t, i)) = y;
+  const int n = fresh_lane() & 31, g = fresh_lane() >> 5, row = row_of(), at = r.len - r.n + token_of(p.t, row);
+  const bool whole = x.head && x.tail, odd = *odd_flag != 0;
+  const int64_t to = ((int64_t)w * 2 + (x.head ? 1 : 0)) * kManyRows + 32 * wave;
+  const int left = rows - 32 * wave;  // rows of the wave
+  if (n < left && g == 0) {
+    if (whole) {
+      const int tok = token_of(p.t, row);
+      write_lse<T>(p, m, l, r.first + tok, x.kv * G + row - tok * G);
+    } else {
+      p.ml[to + n] = float2{m, l};
     }
-  if (direct || (!whole && !odd)) return;
-  // (rare) the infinite and NaN values, key by key, to the rows that see them; each lane adds
-  // to the features that it has written
-  const T* qrow = static_cast<const T*>(p.q) + ((int64_t)h * p.ldq + tok) * D;
-  const float ref = (m == -INFINITY ? 0.0f : m) - Ops<T>::UP;
+  }
+  // Outputs leave through the wave's share of LDS, 64 features of its 32 rows at a time, in whole pieces
+  // of rows (straight from the registers they are 8 bytes of 32 rows to a store).
+  constexpr int P = kStagePitch;
+  float* const out = reinterpret_cast<float*>(&sh.k[0][0]) + wave * kStage;
+  if (g == 0) out[32 * P + n] = inverse(l);
+#pragma unroll
+  for (int f0 = 0; f0 < D; f0 += 64) {
+#pragma unroll
+    for (int t = f0 / 32; t < f0 / 32 + 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4_t*>(out + n * P + 32 * t - f0 + 8 * i + 4 * g) =
+            float4_t{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+    lds_done();
+    if (odd) add_odd<D>(p, r, seen, x, row, at, f0, m, out + n * P, n < left);
+    lds_done();
 #pragma unroll 1
-  for (int b = x.b0; b < x.b1 && odd; ++b) {
-    const int k0 = seen.key0(b);
-#pragma unroll 1
-    for (int j = k0; j < k0 + BK; ++j) {
-      if (!seen.any(j)) continue;
-      const int page = page_of(c, x.s, j);
-      const T* v = reinterpret_cast<const T*>(V) + page * c.vs + (j & in);
-      bool any = false;
-#pragma unroll 1
-      for (int e = lane; e < D; e += 64) any |= !(fabsf(to_f32(v[e << shift])) < INFINITY);
-      if (!__any(any)) continue;
-      const T* key = reinterpret_cast<const T*>(K) + page * c.ks + (j & in) * D;
-      float s = 0.0f;
-#pragma unroll 1
-      for (int e = g; e < D; e += 2) s = fmaf(to_f32(qrow[e]), to_f32(key[e]), s);
-      s = halves_sum(s);
-      // where all rows see a tile its products have them already
-      const int t0 = j / BK * BK;
-      const bool all = t0 + BK - 1 <= seen.low &&
-                       (p.t.window == 0 || t0 > seen.high - p.t.window || t0 + BK <= p.t.sinks);
-      if (all || !mine || !sees(p.t, at, j)) continue;
-      const float f = __builtin_amdgcn_exp2f(fmaf(s, p.scale, -ref));
-#pragma unroll 1
-      for (int i = 0; i < D / 8; ++i) {
-#pragma unroll 1
-        for (int e = 8 * i + 4 * g; e < 8 * i + 4 * g + 4; ++e) {
-          const float y = to_f32(v[e << shift]);
-          if (!(fabsf(y) < INFINITY)) p.part[to * D + e] += f * y;
-        }
+    for (int y = fresh_lane() >> 4; y < min(32, left); y += 4) {
+      const int lane = fresh_lane();
+      const int e = f0 + (lane & 15) * 4;
+      const float4_t z = *reinterpret_cast<const float4_t*>(out + y * P + (lane & 15) * 4);
+      if (whole) {
+        const int at = row0 + 32 * wave + y, tok = token_of(p.t, at);
+        write_out<T>(p, z, out[32 * P + y], r.first + tok, x.kv * G + at - tok * G, e, p.vec);
+      } else {
+        *reinterpret_cast<float4_t*>(p.part + (to + y) * D + e) = z;
       }
     }
-  }
-  if (whole && mine) {
-#pragma unroll 1
-    for (int i = 0; i < D / 8; ++i)
-      write_out<T>(p, *reinterpret_cast<const float4_t*>(p.part + to * D + 8 * i + 4 * g), inv, tok, h, 8 * i + 4 * g,
-                   p.vec);
+    lds_done();
   }
 }
 
@@ -631,8 +682,8 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
 template <int D>
 __global__ __launch_bounds__(512, 2) void paged_many_rows(PagedAttn p) {
   typedef half_t T;
-  constexpr size_t TILES = sizeof(Tiles<D>), FEW = sizeof(FewRows<T, D, 8>);
-  __shared__ __attribute__((aligned(1024))) char lds[TILES > FEW ? TILES : FEW];
+  constexpr size_t TILES = std::max(sizeof(Tiles<D>), 8 * kStage * sizeof(float));
+  __shared__ __attribute__((aligned(1024))) char lds[std::max(TILES, sizeof(FewRows<T, D, 8>))];
   __shared__ WalkShared walk;
   __shared__ int odd;
   walk_pieces<512>(p, walk, [&](const Request& r, const Seen& seen, const Piece& piece, int w) {
@@ -764,7 +815,7 @@ extern "C" int clef_attention_gated_paged(const clef_paged_cache* cache, const i
   if (int rc = clef::paged_view("paged attention", cache, table, max_pages, p.c)) return rc;
   if (int rc = clef::paged_batch("paged attention", nseq, T, heads, cache->kv_heads)) return rc;
   CLEF_REQUIRE(q && gate && y && cu_seqlens && key_lens, "paged attention: null pointer");
-  CLEF_REQUIRE(ldq_tok >= T, "paged attention: query stride");
+  CLEF_REQUIRE(ldq_tok >= T && ldq_tok <= clef::kMaxQueryStride, "paged attention: query stride (T to 2^22)");
   const int d = cache->d;
   CLEF_REQUIRE(hsg >= d && ldg >= (int64_t)(heads - 1) * hsg + d && ldy >= (int64_t)heads * d,
                "paged attention: gate or output strides");
@@ -784,7 +835,7 @@ extern "C" int clef_attention_gated_paged(const clef_paged_cache* cache, const i
   p.vec = !(reinterpret_cast<uintptr_t>(gate) % four || reinterpret_cast<uintptr_t>(y) % four || ldg % 4 || hsg % 4 ||
             ldy % 4);
   p.scale = static_cast<float>(1.44269504088896340736 / std::sqrt(static_cast<double>(d)));
-  p.least = (int64_t)clef::kWalkBlock * p.t.G;
+  p.over_least = 1.0f / (clef::kWalkBlock * p.t.G);
   p.groups = x.groups;
   p.part = static_cast<float*>(workspace);
   p.ml = reinterpret_cast<float2*>(p.part + (size_t)x.groups * 2 * x.R * clef::padded(d));

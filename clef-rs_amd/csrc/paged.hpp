@@ -12,6 +12,7 @@ namespace {
 constexpr int kPagedSeqs = 4096;
 constexpr int kPagedTokens = 1 << 16;
 constexpr int kPagedKeys = 1 << 24;
+constexpr int64_t kMaxQueryStride = 1 << 22;  // rows of a key head are numbered with 32 bits
 
 struct Paged {
   void *k, *vt;             // [num][kvh][1 << shift][d], [num][kvh][d][1 << shift]

@@ -15,18 +15,20 @@ constexpr int kTileCost = 32;    // what a tile costs beside its keys, in keys
 // Values that are the same in all lanes, held in scalar registers: the kernels that walk
 // need their vector registers for tiles.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(x >> 32)))) << 32 |
-                              static_cast<uint32_t>(uniform(static_cast<int>(x))));
+__device__ __forceinline__ double uniform(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(b >> 32)))) << 32 |
+                                        static_cast<uint32_t>(uniform(static_cast<int>(b))));
 }
 __device__ __forceinline__ Request uniform(Request x) { return {uniform(x.first), uniform(x.n), uniform(x.len)}; }
 
-// a / b of whole numbers below 2^53, b > 0, through f64 (a 64-bit division takes more than a
-// hundred instructions, and these kernels' time is in part that of fetching theirs)
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-  int64_t q = uniform(static_cast<int64_t>(static_cast<double>(a) / static_cast<double>(b)));
-  if (q * b > a) --q;
-  if ((q + 1) * b <= a) ++q;
+// Lengths on the line are whole numbers below 2^53 held in f64, exactly: a 64-bit integer product or
+// division takes tens to hundreds of instructions, and a short call spends its time on such.
+// floor(a / b):
+__device__ __forceinline__ double quotient(double a, double b) {
+  double q = floor(a / b);
+  if (q * b > a) q -= 1.0;
+  if ((q + 1.0) * b <= a) q += 1.0;
   return q;
 }
 
@@ -86,88 +88,90 @@ __device__ __forceinline__ int tiles_of(const Rows& t, const Request& x) { retur
 // The line's length up to tile i of one key head of a request, in keys times G: tile
 // j = 1, 2, .. adds a constant and clamp(A + R j, 0, C), about the keys that its last
 // token sees.  It only balances: any increasing line gives right results.
-__device__ __forceinline__ int64_t line_to(const Rows& t, const Request& x, int i) {
-  const int64_t A = (int64_t)(x.len - x.n) * t.G;
-  int64_t C = (int64_t)x.len * t.G;
-  if (t.window) C = min(C, ((int64_t)t.window + t.sinks + 1) * t.G + t.R);
-  const int64_t fixed = (int64_t)kTileCost * t.G;
-  if (i == 1) return fixed + min(max(A + t.R, (int64_t)0), C);
+__device__ __forceinline__ double line_to(const Rows& t, const Request& x, int i) {
+  const double A = static_cast<double>(x.len - x.n) * t.G, R = t.R;
+  double C = static_cast<double>(x.len) * t.G;
+  if (t.window) C = fmin(C, (static_cast<double>(t.window) + t.sinks + 1) * t.G + R);
+  const double fixed = kTileCost * t.G;
+  if (i == 1) return fixed + fmin(fmax(A + R, 0.0), C);
   // tiles of nothing, and tiles below the bound
-  const int64_t none = A < 0 ? min((int64_t)i, -A >> t.log_r) : 0;
-  const int64_t below = C > A ? min((int64_t)i, (C - A - 1) >> t.log_r) : 0;
-  const int64_t rising = below > none ? A * (below - none) + t.R * (below * (below + 1) - none * (none + 1)) / 2 : 0;
-  return fixed * i + rising + (i - max(below, none)) * C;
+  const double over_r = 1.0 / (1 << t.log_r), n = i;
+  const double none = fmin(n, floor(fmax(-A, 0.0) * over_r));
+  const double below = fmax(none, fmin(n, floor(fmax(C - A - 1.0, 0.0) * over_r)));
+  const double rising = A * (below - none) + R * (below * (below + 1.0) - none * (none + 1.0)) * 0.5;
+  return fixed * n + rising + (n - below) * C;
 }
 
 // all tiles of all key heads of a request
-__device__ __forceinline__ int64_t line_of(const Paged& p, const Rows& t, const Request& x) {
+__device__ __forceinline__ double line_of(const Paged& p, const Rows& t, const Request& x) {
   const int tiles = tiles_of(t, x);
-  return tiles ? p.kvh * line_to(t, x, tiles) : 0;
+  return tiles ? p.kvh * line_to(t, x, tiles) : 0.0;
 }
 
 struct WalkShared {
-  int64_t sums[16];
-  int64_t total, base;
+  double sums[16];
+  double base;
   int s;
 };
 
-// The stretch of work-group `group` of `groups` (both of the launch): [u, end), whose
-// first unit lies in request s, which begins at base; W of the groups take part.
+// The stretch of a work-group: [u, end), whose first unit lies in request s, which begins
+// at base; W work-groups take part, this is number w, and number y begins at floor(y step).
 struct Stretch {
-  int w, W;
-  int64_t total, u, end, base;
-  int s;
+  int w, W, s;
+  double total, step, u, end, base;
+  Request r;  // request s
+  __device__ __forceinline__ double cut(int y) const { return y >= W ? total : floor(y * step); }
 };
-__device__ __forceinline__ int64_t cut_at(int64_t total, int w, int W) {
-  return w >= W ? total : uniform(static_cast<int64_t>(static_cast<double>(w) * static_cast<double>(total) / W));
-}
 
-// length(request): what a request takes on the line.
+// length(request): what a request takes on the line.  over_least: 1 / the shortest stretch.
 template <int NT, class F>
-__device__ __forceinline__ bool walk_begin(const Paged& p, F length, int64_t least, int group, int groups,
+__device__ __forceinline__ bool walk_begin(const Paged& p, F length, float over_least, int group, int groups,
                                            WalkShared& sh, Stretch& out) {
   const int tid = threadIdx.x, lane = tid & 63;
-  // few keys: fewer work-groups, each with `least` of the line at least
-  auto dealt = [&](int64_t total) {
-    out.total = total;
-    out.W = static_cast<int>(min((int64_t)groups, max((int64_t)1, quotient(total, least))));
+  // few keys: fewer work-groups
+  auto dealt = [&](double total) {
+    out.total = uniform(total);
+    out.W = uniform(static_cast<int>(fmin(static_cast<float>(total) * over_least, static_cast<float>(groups))));
+    out.W = max(out.W, 1);
+    out.step = uniform(total / out.W);
     // neighbours on the line share keys: one XCD (work-groups go round them) takes neighbours
     const int per = (out.W + 7) / 8;
     out.w = group % 8 * per + group / 8;
-    out.u = cut_at(total, out.w, out.W);
-    out.end = cut_at(total, out.w + 1, out.W);
+    out.u = uniform(out.cut(out.w));
+    out.end = uniform(out.cut(out.w + 1));
     return total > 0 && group / 8 < per && out.w < out.W;
   };
   if (p.nseq == 1) {
     out.s = 0;
-    out.base = 0;
-    return dealt(length(uniform(request_of(p, 0))));
+    out.base = 0.0;
+    out.r = uniform(request_of(p, 0));
+    return dealt(length(out.r));
   }
   const int each = (p.nseq + NT - 1) / NT, s0 = tid * each, s1 = min(p.nseq, s0 + each);
-  int64_t mine = 0;
+  double mine = 0.0;
   for (int s = s0; s < s1; ++s) mine += length(request_of(p, s));
-  int64_t upto = mine;
+  double upto = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int64_t y = __shfl_up(upto, o, 64);
+    const double y = __shfl_up(upto, o, 64);
     if (lane >= o) upto += y;
   }
   if (lane == 63) sh.sums[tid >> 6] = upto;
   __syncthreads();
-  int64_t before = 0, total = 0;
+  double before = 0.0, total = 0.0;
 #pragma unroll
   for (int i = 0; i < NT / 64; ++i) {
     if (i < (tid >> 6)) before += sh.sums[i];
     total += sh.sums[i];
   }
   upto += before;
-  if (!dealt(uniform(total))) return false;
-  const int64_t u = out.u;
+  if (!dealt(total)) return false;
+  const double u = out.u;
   if (u >= upto - mine && u < upto) {
-    int64_t at = upto - mine;
+    double at = upto - mine;
     int s = s0;
     for (;; ++s) {
-      const int64_t y = length(request_of(p, s));
+      const double y = length(request_of(p, s));
       if (u < at + y || s + 1 >= s1) break;
       at += y;
     }
@@ -177,68 +181,77 @@ __device__ __forceinline__ bool walk_begin(const Paged& p, F length, int64_t lea
   __syncthreads();
   out.base = uniform(sh.base);
   out.s = uniform(sh.s);
+  out.r = uniform(request_of(p, out.s));
   return true;
 }
 
-// The work-group whose stretch contains the end of what lies before `to` on the line, behind x's own.
-__device__ __forceinline__ int last_of(const Stretch& x, int64_t to) {
-  int lo = x.w + 1, hi = x.W - 1;  // the first that ends at `to` or behind
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (cut_at(x.total, mid + 1, x.W) >= to) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
+// The last of the work-groups that take what lies before `to`, behind x's own.
+__device__ __forceinline__ int last_of(const Stretch& x, double to) {
+  // about: to / step, and the neighbours of that
+  int y = max(x.w + 1, min(x.W - 1, uniform(static_cast<int>(to / x.step))));
+  while (y > x.w + 1 && uniform(x.cut(y)) >= to) --y;
+  while (y < x.W - 1 && uniform(x.cut(y + 1)) < to) ++y;
+  return y;
 }
 
 // One piece of a stretch: blocks b0 .. b1 - 1 of a tile of one key head.
 struct Piece {
   int s, kv, tile, b0, b1;
   bool head, tail;  // it begins, ends its tile
-  int64_t from, to; // the tile on the line
+  double from, to;  // the tile on the line
 };
 
 // The piece at x.u, and the stretch behind it; false at the end.
 __device__ __forceinline__ bool next_piece(const Paged& p, const Rows& t, Stretch& x, Piece& out, Request& r, Seen& v) {
   if (x.u >= x.end) return false;
   int tiles;
-  int64_t line;
-  for (;; ++x.s) {
-    if (x.s >= p.nseq) return false;  // (the line ends with the last request)
-    r = uniform(request_of(p, x.s));
+  double line;
+  for (;;) {
+    r = x.r;
     tiles = tiles_of(t, r);
-    if (!tiles) continue;
-    line = line_to(t, r, tiles);
-    if (x.u < x.base + p.kvh * line) break;
-    x.base += p.kvh * line;
+    line = tiles ? line_to(t, r, tiles) : 0.0;
+    if (x.u < uniform(x.base + p.kvh * line)) break;
+    x.base = uniform(x.base + p.kvh * line);
+    if (++x.s >= p.nseq) return false;  // (the line ends with the last request)
+    x.r = uniform(request_of(p, x.s));
   }
-  int64_t at = x.u - x.base;
-  const int kv = p.kvh == 1 ? 0 : static_cast<int>(quotient(at, line));
+  double at = x.u - x.base;
+  const double kv = p.kvh == 1 ? 0.0 : quotient(at, line);
   at -= kv * line;
-  int lo = 0, hi = tiles;  // the last tile that begins at or before `at`
+  const double start = x.base + kv * line;
+  int lo = 0;  // the last tile that begins at or before `at`
+  double from = 0.0, to = line;
+  if (tiles > 1) {
+    int hi = tiles;
 #pragma unroll 1
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (line_to(t, r, mid) <= at) lo = mid;
-    else hi = mid;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      const double y = line_to(t, r, mid);
+      if (uniform(static_cast<int>(y <= at))) {
+        lo = mid;
+        from = y;
+      } else {
+        hi = mid;
+        to = y;
+      }
+    }
   }
-  out.s = uniform(x.s);
-  out.kv = uniform(kv);
-  out.tile = uniform(lo);
-  const int64_t start = x.base + kv * line;
-  out.from = start + (lo ? line_to(t, r, lo) : 0);
-  out.to = start + line_to(t, r, lo + 1);
-  const int64_t stop = min(out.to, x.end);
+  out.s = x.s;
+  out.kv = uniform(static_cast<int>(kv));
+  out.tile = lo;
+  out.from = uniform(start + from);
+  out.to = uniform(start + to);
+  const double stop = fmin(out.to, x.end);
   if (stop <= x.u) return false;  // only where tables do not fit (requests that overlap)
   out.head = x.u == out.from;
   out.tail = stop == out.to;
   v = seen_by(t, r, lo * t.R, min((lo + 1) * t.R, r.n * t.G));
   // blocks in proportion; the same division on both sides of a cut
-  const double scale = v.blocks / static_cast<double>(out.to - out.from);
-  auto block = [&](int64_t y) { return min(v.blocks, uniform(static_cast<int>((y - out.from) * scale))); };
+  const double scale = v.blocks / (out.to - out.from);
+  auto block = [&](double y) { return min(v.blocks, uniform(static_cast<int>((y - out.from) * scale))); };
   out.b0 = uniform(out.head ? 0 : block(x.u));
   out.b1 = uniform(out.tail ? v.blocks : block(stop));
-  x.u = stop;
+  x.u = uniform(stop);
   return true;
 }
 

@@ -27,7 +27,6 @@ namespace {
 constexpr int kBlockCost = 32;   // what a block costs beside its rows, in rows
 constexpr int kManyKeys = 128;   // of a work-group's block
 constexpr int kManyTile = 64;    // rows that pass at a time
-constexpr int64_t kMaxQueryStride = 1 << 22;  // rows of a key head are numbered with 32 bits
 
 struct WeightParams {
   Paged c;
@@ -36,8 +35,9 @@ struct WeightParams {
   const float* lse;     // [T][heads]
   const float* scores;  // [num][kvh][1 << shift]
   float* sums;
-  int64_t ldq, least;
+  int64_t ldq;
   int heads, groups;
+  float over_least;     // 1 / the shortest stretch of a work-group
   float scale;          // log2(e) / sqrt(d)
   // each work-group's sums of the block that it begins, and that it ends in the middle of,
   // and the block whose first part it holds
@@ -104,20 +104,20 @@ __global__ __launch_bounds__(256) void weights_few_rows(WeightParams p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, grp = lane >> 4, G = p.t.G, d = c.d;
   auto blocks_of = [&](const Request& r) { return (r.len + BK - 1) / BK; };
-  auto each = [&](const Request& r) { return (int64_t)r.n * G + kBlockCost; };
+  auto each = [&](const Request& r) { return static_cast<double>(r.n) * G + kBlockCost; };
   Stretch x;
   if (!walk_begin<64 * NW>(
-          c, [&](const Request& r) { return c.kvh * (blocks_of(r) * each(r)); }, p.least, blockIdx.x, p.groups, walk, x))
+          c, [&](const Request& r) { return c.kvh * (blocks_of(r) * each(r)); }, p.over_least, blockIdx.x, p.groups, walk, x))
     return;
   for (int s = x.s; s < c.nseq && x.base < x.end; ++s) {
     const Request r = uniform(request_of(c, s));
     if (!r.len) continue;
-    const int64_t cost = each(r);
+    const double cost = each(r);
     const int blocks = blocks_of(r);
     const int count = c.kvh * blocks;  // (below 2^28)
     // blocks that begin in the stretch
-    const int b0 = x.u <= x.base ? 0 : static_cast<int>(min((int64_t)count, quotient(x.u - x.base + cost - 1, cost)));
-    const int b1 = static_cast<int>(min((int64_t)count, quotient(x.end - x.base + cost - 1, cost)));
+    const int b0 = x.u <= x.base ? 0 : min(count, uniform(static_cast<int>(quotient(x.u - x.base + cost - 1, cost))));
+    const int b1 = uniform(static_cast<int>(fmin(count, quotient(x.end - x.base + cost - 1, cost))));
     for (int b = b0 + wave; b < b1; b += NW) {
       const int kv = b / blocks, key0 = b % blocks * BK;
       float sum[NT][4] = {};
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256) void weights_few_rows(WeightParams p) {
       if (lane < BK) write_sum(p, r, s, kv, key0 + lane, part[wave][lane]);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    x.base += (int64_t)count * cost;
+    x.base += count * cost;
   }
 }
 
@@ -194,28 +194,28 @@ __global__ __launch_bounds__(512, 2) void weights_many_rows(WeightParams p) {
   const int rg = wave & 1, kg = wave >> 1;
   auto slot = [](int row) { return CHUNKS >= 16 ? row & 15 : row >> 1 & 7; };
   auto blocks_of = [&](const Request& r) { return (r.len + kManyKeys - 1) / kManyKeys; };
-  auto each = [&](const Request& r) { return (int64_t)r.n * G + kBlockCost; };
+  auto each = [&](const Request& r) { return static_cast<double>(r.n) * G + kBlockCost; };
   Stretch x;
   WeightParams::Split split = {};
   const bool work = walk_begin<512>(
-      c, [&](const Request& r) { return c.kvh * (blocks_of(r) * each(r)); }, p.least, blockIdx.x, p.groups, walk, x);
+      c, [&](const Request& r) { return c.kvh * (blocks_of(r) * each(r)); }, p.over_least, blockIdx.x, p.groups, walk, x);
   for (int s = x.s; work && s < c.nseq && x.u < x.end; ++s) {
     const Request r = uniform(request_of(c, s));
     if (!r.len) continue;
-    const int64_t cost = each(r);
+    const double cost = each(r);
     const int blocks = blocks_of(r), first = r.len - r.n;
-    const int64_t next = x.base + c.kvh * (blocks * cost);
-    while (x.u < min(next, x.end)) {
-      const int b = static_cast<int>(quotient(x.u - x.base, cost));
-      const int64_t start = x.base + b * cost, stop = min(start + cost, x.end);
+    const double next = uniform(x.base + c.kvh * (blocks * cost));
+    while (x.u < fmin(next, x.end)) {
+      const int b = uniform(static_cast<int>(quotient(x.u - x.base, cost)));
+      const double start = uniform(x.base + b * cost), stop = uniform(fmin(start + cost, x.end));
       const bool head = x.u == start, tail = stop == start + cost;
       const int kv = b / blocks, key0 = b % blocks * kManyKeys;
       int from, to;
       rows_seeing(p.t, r, key0, kManyKeys, from, to);
       const int tiles = max(to - from + kManyTile - 1, 0) / kManyTile;
       // the piece's tiles, in proportion; the same division on both sides of a cut
-      const double scale = tiles / static_cast<double>(cost);
-      auto tile_at = [&](int64_t u) { return min(tiles, uniform(static_cast<int>((u - start) * scale))); };
+      const double scale = tiles / cost;
+      auto tile_at = [&](double u) { return min(tiles, uniform(static_cast<int>((u - start) * scale))); };
       const int t0 = head ? 0 : tile_at(x.u), t1 = tail ? tiles : tile_at(stop);
       x.u = stop;
 
@@ -382,7 +382,7 @@ extern "C" int clef_paged_weights(const clef_paged_cache* cache, const int32_t* 
   p.c.cu = cu_seqlens; p.c.len = key_lens; p.c.nseq = nseq; p.c.T = T;
   p.t = clef::rows_of(heads / p.c.kvh, 16, window, sinks);
   p.q = q; p.lse = lse; p.scores = scores; p.sums = new_scores; p.ldq = ldq_tok; p.heads = heads;
-  p.least = x.many ? 2 * clef::kManyTile : 1;
+  p.over_least = x.many ? 0.5f / clef::kManyTile : 1.0f;
   p.groups = x.groups;
   p.scale = static_cast<float>(1.44269504088896340736 / std::sqrt(static_cast<double>(cache->d)));
   p.part = static_cast<float*>(workspace);

@@ -52,7 +52,7 @@ OWN = {
                dict(hsq=63), dict(ldk=127), dict(ldv=127), dict(ldo=8), dict(rot=33), dict(rot=-2), dict(rot=66),
                dict(theta=0.0), dict(theta=float("nan")), dict(theta=float("inf")), dict(eps=-1.0),
                dict(eps=float("nan")), dict(axes=0), dict(axes=5), dict(axes=2), dict(ldpos=8), dict(out=264)],
-    "attention": [dict(q=None), dict(gate=None), dict(y=None), dict(ws=None), dict(wsb=0), dict(ws=264), dict(ldq=8),
+    "attention": [dict(q=None), dict(gate=None), dict(y=None), dict(ws=None), dict(wsb=0), dict(ws=264), dict(ldq=8), dict(ldq=(1 << 22) + 1),
                   dict(ldg=511), dict(hsg=63), dict(ldy=511), dict(window=-1), dict(window=(1 << 24) + 1),
                   dict(sinks=-1), dict(sinks=(1 << 24) + 1), dict(q=264)],
     "weights": [dict(q=None), dict(lse=None), dict(scores=None), dict(new=None), dict(ldq=8), dict(window=-1),
