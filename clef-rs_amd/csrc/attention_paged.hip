@@ -662,16 +662,41 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
     lds_done();
     if (odd) add_odd<D>(p, r, seen, x, row, at, f0, m, out + n * P, n < left);
     lds_done();
-#pragma unroll 1
-    for (int y = fresh_lane() >> 4; y < min(32, left); y += 4) {
-      const int lane = fresh_lane();
-      const int e = f0 + (lane & 15) * 4;
-      const float4_t z = *reinterpret_cast<const float4_t*>(out + y * P + (lane & 15) * 4);
-      if (whole) {
+    // lane i: features f0 + 4 (i % 16) .. of rows i / 16, + 4, ..; gates are requested together
+    const int i0 = fresh_lane() >> 4, e = (fresh_lane() & 15) * 4;
+    if (whole && p.vec) {
+      half4 gate[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int at = row0 + 32 * wave + min(i0 + 4 * k, left - 1), tok = token_of(p.t, at);
+        gate[k] = *reinterpret_cast<const half4*>(static_cast<const T*>(p.gate) + (int64_t)(r.first + tok) * p.ldg +
+                                                  (int64_t)(x.kv * G + at - tok * G) * p.hsg + f0 + e);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int y = i0 + 4 * k;
+        if (y >= left) break;
         const int at = row0 + 32 * wave + y, tok = token_of(p.t, at);
-        write_out<T>(p, z, out[32 * P + y], r.first + tok, x.kv * G + at - tok * G, e, p.vec);
-      } else {
-        *reinterpret_cast<float4_t*>(p.part + (to + y) * D + e) = z;
+        const float4_t z = *reinterpret_cast<const float4_t*>(out + y * P + e) * out[32 * P + y];
+        half4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = cvt_out<T>(z[j] * sigmoid_hw(to_f32(gate[k][j])));
+        *reinterpret_cast<half4*>(static_cast<T*>(p.y) + (int64_t)(r.first + tok) * p.ldy +
+                                  (int64_t)(x.kv * G + at - tok * G) * D + f0 + e) = v;
+      }
+    } else if (whole) {
+#pragma unroll 1
+      for (int y = i0; y < min(32, left); y += 4) {
+        const int at = row0 + 32 * wave + y, tok = token_of(p.t, at);
+        write_out<T>(p, *reinterpret_cast<const float4_t*>(out + y * P + e), out[32 * P + y], r.first + tok,
+                     x.kv * G + at - tok * G, f0 + e, false);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int y = i0 + 4 * k;
+        if (y < left)
+          *reinterpret_cast<float4_t*>(p.part + (to + y) * D + f0 + e) = *reinterpret_cast<const float4_t*>(out + y * P + e);
       }
     }
     lds_done();
@@ -751,6 +776,7 @@ int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 struct PagedPlan {
   bool many;   // tiles of 256 rows, else of 16
   int R;       // rows of a tile
+  int tile_cost;
   int groups;  // work-groups, a multiple of 8
 };
 PagedPlan plan_of(int T, int nseq, int max_keys, int dtype, int heads, int kvh, int d) {
@@ -758,9 +784,10 @@ PagedPlan plan_of(int T, int nseq, int max_keys, int dtype, int heads, int kvh, 
   const int64_t rows = (int64_t)T * (heads / kvh);
   x.many = dtype == CLEF_F16 && d == padded(d) && rows > 16 * (int64_t)nseq;
   x.R = x.many ? kManyRows : 16;
+  x.tile_cost = x.many ? 512 : 64;
   // no more than blocks of keys that there can be
   const int64_t tiles = (rows / x.R + std::min(T, nseq)) * kvh;
-  const int64_t blocks = tiles * ((max_keys + kTileCost) / kWalkBlock + 1);
+  const int64_t blocks = tiles * ((max_keys + x.tile_cost) / kWalkBlock + 1);
   // as many as run at once: one to a CU by the LDS, or two
   x.groups = static_cast<int>(std::min<int64_t>((x.many ? 1 : 2) * device_cus(), blocks) + 7) / 8 * 8;
   return x;
@@ -827,7 +854,7 @@ extern "C" int clef_attention_gated_paged(const clef_paged_cache* cache, const i
                    !(reinterpret_cast<uintptr_t>(workspace) & 255),
                "paged attention: workspace too small or not 256-byte aligned");
   p.c.cu = cu_seqlens; p.c.len = key_lens; p.c.nseq = nseq; p.c.T = T;
-  p.t = clef::rows_of(heads / p.c.kvh, x.R, window, sinks);
+  p.t = clef::rows_of(heads / p.c.kvh, x.R, x.tile_cost, window, sinks);
   p.q = q; p.gate = gate; p.y = y; p.lse = lse;
   p.ldq = ldq_tok; p.ldg = ldg; p.hsg = hsg; p.ldy = ldy;
   p.heads = heads;

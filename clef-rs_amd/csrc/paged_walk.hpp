@@ -10,7 +10,6 @@ namespace clef {
 namespace {
 
 constexpr int kWalkBlock = 64;   // keys that stretches are counted in
-constexpr int kTileCost = 32;    // what a tile costs beside its keys, in keys
 
 // Values that are the same in all lanes, held in scalar registers: the kernels that walk
 // need their vector registers for tiles.
@@ -36,6 +35,7 @@ struct Rows {         // how query rows become tiles
   int G;              // rows of a token: heads of a key head
   uint32_t over_g;    // 2^32 / G rounded up (0: G = 1)
   int R, log_r;       // rows of a tile, a power of two
+  int tile_cost;      // what a tile costs beside its keys, in keys
   int window, sinks;  // window 0: all keys
 };
 
@@ -44,11 +44,12 @@ struct Rows {         // how query rows become tiles
 __device__ __forceinline__ int token_of(const Rows& t, int row) {
   return t.over_g ? static_cast<int>(__umulhi(static_cast<uint32_t>(row), t.over_g)) : row;
 }
-inline Rows rows_of(int G, int R, int window, int sinks) {
+inline Rows rows_of(int G, int R, int tile_cost, int window, int sinks) {
   Rows t;
   t.G = G;
   t.over_g = G == 1 ? 0 : static_cast<uint32_t>(((uint64_t(1) << 32) + G - 1) / G);
   t.R = R;
+  t.tile_cost = tile_cost;
   t.log_r = __builtin_ctz(R);
   t.window = window;
   t.sinks = sinks;
@@ -92,7 +93,7 @@ __device__ __forceinline__ double line_to(const Rows& t, const Request& x, int i
   const double A = static_cast<double>(x.len - x.n) * t.G, R = t.R;
   double C = static_cast<double>(x.len) * t.G;
   if (t.window) C = fmin(C, (static_cast<double>(t.window) + t.sinks + 1) * t.G + R);
-  const double fixed = kTileCost * t.G;
+  const double fixed = t.tile_cost * t.G;
   if (i == 1) return fixed + fmin(fmax(A + R, 0.0), C);
   // tiles of nothing, and tiles below the bound
   const double over_r = 1.0 / (1 << t.log_r), n = i;
@@ -119,7 +120,9 @@ struct WalkShared {
 struct Stretch {
   int w, W, s;
   double total, step, u, end, base;
-  Request r;  // request s
+  Request r;          // request s
+  int kv, tile;       // of the piece before, which ended its tile at tile_end; tile -1: none in request s
+  double start, tile_end;
   __device__ __forceinline__ double cut(int y) const { return y >= W ? total : floor(y * step); }
 };
 
@@ -129,6 +132,7 @@ __device__ __forceinline__ bool walk_begin(const Paged& p, F length, float over_
                                            WalkShared& sh, Stretch& out) {
   const int tid = threadIdx.x, lane = tid & 63;
   // few keys: fewer work-groups
+  out.tile = -1;
   auto dealt = [&](double total) {
     out.total = uniform(total);
     out.W = uniform(static_cast<int>(fmin(static_cast<float>(total) * over_least, static_cast<float>(groups))));
@@ -212,35 +216,46 @@ __device__ __forceinline__ bool next_piece(const Paged& p, const Rows& t, Stretc
     line = tiles ? line_to(t, r, tiles) : 0.0;
     if (x.u < uniform(x.base + p.kvh * line)) break;
     x.base = uniform(x.base + p.kvh * line);
+    x.tile = -1;
     if (++x.s >= p.nseq) return false;  // (the line ends with the last request)
     x.r = uniform(request_of(p, x.s));
   }
-  double at = x.u - x.base;
-  const double kv = p.kvh == 1 ? 0.0 : quotient(at, line);
-  at -= kv * line;
-  const double start = x.base + kv * line;
-  int lo = 0;  // the last tile that begins at or before `at`
-  double from = 0.0, to = line;
-  if (tiles > 1) {
-    int hi = tiles;
+  if (x.tile >= 0 && x.tile + 1 < tiles && x.u == x.tile_end) {  // the next tile of the same key head
+    ++x.tile;
+    out.from = x.tile_end;
+    out.to = uniform(x.start + line_to(t, r, x.tile + 1));
+  } else {
+    double at = x.u - x.base;
+    const double kv = p.kvh == 1 ? 0.0 : quotient(at, line);
+    at -= kv * line;
+    x.start = uniform(x.base + kv * line);
+    x.kv = uniform(static_cast<int>(kv));
+    int lo = 0;  // the last tile that begins at or before `at`
+    double from = 0.0, to = line;
+    if (tiles > 1) {
+      int hi = tiles;
 #pragma unroll 1
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      const double y = line_to(t, r, mid);
-      if (uniform(static_cast<int>(y <= at))) {
-        lo = mid;
-        from = y;
-      } else {
-        hi = mid;
-        to = y;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        const double y = line_to(t, r, mid);
+        if (uniform(static_cast<int>(y <= at))) {
+          lo = mid;
+          from = y;
+        } else {
+          hi = mid;
+          to = y;
+        }
       }
     }
+    x.tile = lo;
+    out.from = uniform(x.start + from);
+    out.to = uniform(x.start + to);
   }
+  const int lo = x.tile;
   out.s = x.s;
-  out.kv = uniform(static_cast<int>(kv));
+  out.kv = x.kv;
   out.tile = lo;
-  out.from = uniform(start + from);
-  out.to = uniform(start + to);
+  x.tile_end = out.to;
   const double stop = fmin(out.to, x.end);
   if (stop <= x.u) return false;  // only where tables do not fit (requests that overlap)
   out.head = x.u == out.from;

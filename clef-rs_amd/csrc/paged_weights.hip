@@ -380,7 +380,7 @@ extern "C" int clef_paged_weights(const clef_paged_cache* cache, const int32_t* 
                    !(reinterpret_cast<uintptr_t>(workspace) & 255),
                "paged weights: workspace too small or not 256-byte aligned");
   p.c.cu = cu_seqlens; p.c.len = key_lens; p.c.nseq = nseq; p.c.T = T;
-  p.t = clef::rows_of(heads / p.c.kvh, 16, window, sinks);
+  p.t = clef::rows_of(heads / p.c.kvh, 16, 0, window, sinks);
   p.q = q; p.lse = lse; p.scores = scores; p.sums = new_scores; p.ldq = ldq_tok; p.heads = heads;
   p.over_least = x.many ? 0.5f / clef::kManyTile : 1.0f;
   p.groups = x.groups;
