@@ -781,15 +781,22 @@ struct PagedPlan {
 };
 PagedPlan plan_of(int T, int nseq, int max_keys, int dtype, int heads, int kvh, int d) {
   PagedPlan x;
-  const int64_t rows = (int64_t)T * (heads / kvh);
-  x.many = dtype == CLEF_F16 && d == padded(d) && rows > 16 * (int64_t)nseq;
+  const int64_t rows = (int64_t)T * (heads / kvh), cus = device_cus();
+  // Requests of more than 64 rows, or of more than 16 with many keys in all, go on wide tiles.  (Few, many:
+  // 16 requests of 24 rows behind 4,096 keys 36, 55 us; of 32 41, 57; of 64 59, 60; 32 of 32 behind 16,384
+  // 194, 165; of 64 360, 176; one of 64 behind 4,096 24, 36.)
+  const int64_t units = (rows / 16 + nseq) * kvh * (max_keys / kWalkBlock + 1);
+  x.many = dtype == CLEF_F16 && d == padded(d) && rows > 16 * (int64_t)nseq &&
+           (rows > 64 * (int64_t)nseq || units > 32 * cus);
   x.R = x.many ? kManyRows : 16;
-  x.tile_cost = x.many ? 512 : 64;
-  // no more than blocks of keys that there can be
+  // (a wide tile's queries, fill and outputs take as long as about four blocks of keys: a prompt of
+  // 4,096 tokens with 32, 128, 256 and 512 keys for them 416, 317, 273 and 226 us when they took more)
+  x.tile_cost = x.many ? 256 : 64;
+  // no more work-groups than blocks of keys that there can be
   const int64_t tiles = (rows / x.R + std::min(T, nseq)) * kvh;
   const int64_t blocks = tiles * ((max_keys + x.tile_cost) / kWalkBlock + 1);
   // as many as run at once: one to a CU by the LDS, or two
-  x.groups = static_cast<int>(std::min<int64_t>((x.many ? 1 : 2) * device_cus(), blocks) + 7) / 8 * 8;
+  x.groups = static_cast<int>(std::min<int64_t>((x.many ? 1 : 2) * cus, blocks) + 7) / 8 * 8;
   return x;
 }
 size_t parts_bytes(const PagedPlan& x, int d) {
@@ -862,7 +869,7 @@ extern "C" int clef_attention_gated_paged(const clef_paged_cache* cache, const i
   p.vec = !(reinterpret_cast<uintptr_t>(gate) % four || reinterpret_cast<uintptr_t>(y) % four || ldg % 4 || hsg % 4 ||
             ldy % 4);
   p.scale = static_cast<float>(1.44269504088896340736 / std::sqrt(static_cast<double>(d)));
-  p.over_least = 1.0f / (clef::kWalkBlock * p.t.G);
+  p.over_least = 1.0f / ((x.many ? 2 : 1) * clef::kWalkBlock * p.t.G);
   p.groups = x.groups;
   p.part = static_cast<float*>(workspace);
   p.ml = reinterpret_cast<float2*>(p.part + (size_t)x.groups * 2 * x.R * clef::padded(d));
