@@ -468,24 +468,25 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
   // operands: key rows 32 kh + n, 16-byte chunk 2 kb + g; feature rows 32 t + n, chunk 2 y + g
   // (each read's variant is formed where it is used, in one instruction that the compiler neither
   // shares nor moves: kept for the loop they cost the registers of three query operands)
-  auto key_offset = [&]() {
+  auto key_offset = [&](int buf) {
     const int lane = fresh_lane(), n = lane & 31;
-    return n * 2 * D + 16 * (lane >> 5 ^ kswz(n));
+    return n * 2 * D + 16 * (lane >> 5 ^ kswz(n)) + buf * (128 * D);
   };
-  auto value_offset = [&]() {
+  auto value_offset = [&](int buf) {
     const int lane = fresh_lane(), n = lane & 31;
-    return n * 128 + 16 * (lane >> 5 ^ (n >> 1 & 7));
+    return n * 128 + 16 * (lane >> 5 ^ (n >> 1 & 7)) + buf * (128 * D);
   };
   auto variant = [](int off, int bits) {
     int y;
     asm volatile("v_xor_b32 %0, %1, %2" : "=v"(y) : "i"(bits), "v"(off));
     return y;
   };
-  auto key_at = [&](const char* base, int koff, int kh, int kb) {
-    return *reinterpret_cast<const half8*>(base + variant(koff, 32 * (kb % PER)) + kh * 64 * D + kb / PER * 32 * PER);
+  auto key_at = [&](int koff, int kh, int kb) {
+    return *reinterpret_cast<const half8*>(reinterpret_cast<const char*>(sh.k) + variant(koff, 32 * (kb % PER)) +
+                                           (kh * 64 * D + kb / PER * 32 * PER));
   };
-  auto value_at = [&](const char* base, int voff, int y, int t) {
-    return *reinterpret_cast<const half8*>(base + variant(voff, 32 * y) + t * 32 * 128);
+  auto value_at = [&](int voff, int t) {
+    return *reinterpret_cast<const half8*>(reinterpret_cast<const char*>(sh.v) + voff + t * 32 * 128);
   };
 
   lds_barrier();  // the piece before is done with the tiles
@@ -513,7 +514,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
   if (!idle) {
     vm_wait_all();
     const char* const mine = reinterpret_cast<const char*>(stage);
-    const int koff = key_offset();
+    const int koff = key_offset(0);
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb) {
       const half8 y = *reinterpret_cast<const half8*>(mine + variant(koff, 32 * (kb % PER)) + kb / PER * 32 * PER);
@@ -565,24 +566,22 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
       lds_barrier();
     }
     if (idle) continue;
-    const char* kbase = reinterpret_cast<const char*>(sh.k[buf]);
-    const char* vbase = reinterpret_cast<const char*>(sh.v[buf]);
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh) {
-      const int koff = key_offset();
+      const int koff = key_offset(buf);
       float16_t S;
 #pragma unroll
       for (int e = 0; e < 16; ++e) S[e] = 0.0f;
       half8 f[PD], lq = {};
 #pragma unroll
-      for (int i = 0; i < PD; ++i) f[i] = key_at(kbase, koff, kh, i);
+      for (int i = 0; i < PD; ++i) f[i] = key_at(koff, kh, i);
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
         S = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[kb % PD], kb < QR ? fq[kb < QR ? kb : 0] : lq, S, 0, 0, 0);
         if constexpr (QL > 0) {
           if (kb + 1 >= QR && kb + 1 < NKB) lq = sh.q[wave][kb + 1 - QR][fresh_lane()];
         }
-        if (kb + PD < NKB) f[kb % PD] = key_at(kbase, koff, kh, kb + PD);
+        if (kb + PD < NKB) f[kb % PD] = key_at(koff, kh, kb + PD);
         __builtin_amdgcn_sched_barrier(0);
       }
       // element e of lane group g: key k0 + 32 kh + 16 (e / 8) + 8 g + e % 8
@@ -619,13 +618,14 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Request& r, 
         wt[e >> 3][e & 7] = static_cast<T>(y);
       }
       __builtin_amdgcn_sched_barrier(0);
-      const int voff = value_offset();
+      const int voff = value_offset(buf);
+      const int vo[2] = {variant(voff, 64 * kh), variant(voff, 64 * kh + 32)};
 #pragma unroll
-      for (int i = 0; i < PD; ++i) f[i] = value_at(vbase, voff, 2 * kh + i / NDT, i % NDT);
+      for (int i = 0; i < PD; ++i) f[i] = value_at(vo[i / NDT], i % NDT);
 #pragma unroll
       for (int i = 0; i < 2 * NDT; ++i) {
         o[i % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % PD], wt[i / NDT], o[i % NDT], 0, 0, 0);
-        if (i + PD < 2 * NDT) f[i % PD] = value_at(vbase, voff, 2 * kh + (i + PD) / NDT, (i + PD) % NDT);
+        if (i + PD < 2 * NDT) f[i % PD] = value_at(vo[(i + PD) / NDT], (i + PD) % NDT);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -789,9 +789,9 @@ PagedPlan plan_of(int T, int nseq, int max_keys, int dtype, int heads, int kvh, 
   x.many = dtype == CLEF_F16 && d == padded(d) && rows > 16 * (int64_t)nseq &&
            (rows > 64 * (int64_t)nseq || units > 32 * cus);
   x.R = x.many ? kManyRows : 16;
-  // (a wide tile's queries, fill and outputs take as long as about four blocks of keys: a prompt of
-  // 4,096 tokens with 32, 128, 256 and 512 keys for them 416, 317, 273 and 226 us when they took more)
-  x.tile_cost = x.many ? 256 : 64;
+  // (a wide tile's queries, fill, outputs and joining take as long as eight blocks of keys: a prompt of
+  // 4,096 tokens with 256 and 512 keys for them 240, 208 us; with 32, when they took more, twice as long)
+  x.tile_cost = x.many ? 512 : 64;
   // no more work-groups than blocks of keys that there can be
   const int64_t tiles = (rows / x.R + std::min(T, nseq)) * kvh;
   const int64_t blocks = tiles * ((max_keys + x.tile_cost) / kWalkBlock + 1);
