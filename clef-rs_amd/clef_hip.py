@@ -846,9 +846,12 @@ class PagedCache:
                 raise ClefError(-1, "positions must be a contiguous int32 device tensor [axes, T]")
             axes = positions.shape[0] if positions.dim() == 2 else 1
         if axis_of is not None:
-            if len(axis_of) != rot_dim // 2 or not all(0 <= a < axes for a in axis_of):
+            try:
+                axis_of = bytes(tuple(axis_of))  # (the call checks that each is one of the axes)
+            except (TypeError, ValueError):
+                axis_of = None
+            if axis_of is None or len(axis_of) != rot_dim // 2:
                 raise ClefError(-1, "axis_of must name the axis of each of the rot_dim / 2 rotary pairs")
-            axis_of = bytes(axis_of)
         hsq = q.stride(1) if heads > 1 else d
         ldq = q.stride(0) if T > 1 else (heads - 1) * hsq + d
         if hsq < d or ldq < (heads - 1) * hsq + d:
@@ -924,12 +927,13 @@ class PagedCache:
         self._scores(scores, "scores")
         to._scores(to_scores, "to_scores")
         _here(scores, key_lens, pages, self.k, self.vt, to.k, to.vt, to_pages, to_scores)
+        budget = int(budget)
         if budget < 1:
             raise ClefError(-1, "the budget must be at least 1")
         lens = key_lens.new_empty(nseq)
         keep = key_lens.new_empty((nseq, self.kv_heads, budget))
         _check(lib().clef_paged_evict(
-            self._at, pages.data_ptr(), width, key_lens.data_ptr(), nseq, scores.data_ptr(), int(budget), int(sinks),
+            self._at, pages.data_ptr(), width, key_lens.data_ptr(), nseq, scores.data_ptr(), budget, int(sinks),
             int(recent), to._at, to_pages.data_ptr(), to_width, to_scores.data_ptr(), lens.data_ptr(), keep.data_ptr(),
             _stream()))
         return lens, keep

@@ -355,6 +355,56 @@ def test_append(clef, axes, far, dtype, page, kvh, rep, d, rot):
         assert torch.equal(b.vt.nan_to_num(5.0), v0.nan_to_num(5.0)), "a slot of nobody's token was written"
 
 
+@gpu
+@pytest.mark.parametrize("tokens", [1, 3])
+@pytest.mark.parametrize("requests", [64, 65, 200])
+def test_append_many_requests(clef, tokens, requests):
+    """Fewer and more requests than a wave has lanes, few tokens and many, empty ones among them."""
+    shape = [((s + 1) % (tokens + 1), (s + 1) % (tokens + 1) + s * 5 % 37) for s in range(requests)]
+    b = Batch(shape, 16, 2, 64, F16, seed=requests, tail=1)
+    x, k, v = (b.randn(b.T, h, 64) for h in (4, 2, 2))
+    w = torch.ones(64, device="cuda")
+    out = torch.full((4, b.T, 64), 7.0, dtype=F16, device="cuda")
+    clef.PagedCache(b.k, b.vt).append(x, k, v, w, w, b.cu, b.len, b.table, 32, 1e4, out=out)
+    torch.cuda.synchronize()
+    index = torch.cat([torch.arange(m - n, m) for n, m in shape] + [torch.zeros(1)]).cuda().int()[None]
+    axis = torch.zeros(16, dtype=torch.long, device="cuda")
+    t = sum(b.new)
+    y, bound = turned(x, w, index, axis, 32, 1e4, 1e-6)
+    close(out.transpose(0, 1)[:t], y[:t], (bound + HALF[F16] * y.abs() + 2.0 ** -25)[:t], "q")
+    assert (out[:, t:] == 7.0).all()
+    y, bound = turned(k, w, index, axis, 32, 1e4, 1e-6)
+    bound = bound + HALF[F16] * y.abs() + 2.0 ** -25
+    t = 0
+    for s, (n, m) in enumerate(shape):
+        if n:
+            close(b.read(b.k, s, m)[:, m - n:].transpose(0, 1), y[t:t + n], bound[t:t + n], "k")
+            assert torch.equal(b.read(b.vt.transpose(2, 3), s, m)[:, m - n:].transpose(0, 1), v[t:t + n])
+            if m > n:
+                assert torch.equal(b.read(b.k, s, m)[:, :m - n], b.keys[s][:, :m - n])
+                assert torch.equal(b.read(b.vt.transpose(2, 3), s, m)[:, :m - n], b.values[s][:, :m - n])
+        t += n
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32], ids=str)
+@pytest.mark.parametrize("new", [1, 70])
+def test_shared_pages(clef, dtype, new):
+    """Requests whose tables begin with the same pages: each as it would be with its own."""
+    shared, page = 96, 32
+    b = Batch([(new, shared + new + 5 * s) for s in range(3)], page, 2, 64, dtype, seed=new)
+    for s in (1, 2):
+        b.keys[s][:, :shared], b.values[s][:, :shared] = b.keys[0][:, :shared], b.values[0][:, :shared]
+        b.fill(b.k, s, b.keys[s])
+        b.fill(b.vt.transpose(2, 3), s, b.values[s])
+    q, gate = b.randn(8, b.T, 64), b.randn(b.T, 8, 64)
+    cache = clef.PagedCache(b.k, b.vt)
+    want = cache.attention_gated(q, gate, b.cu, b.len, b.table)
+    table = b.table.clone()
+    table[1:, :shared // page] = table[0, :shared // page]
+    assert torch.equal(cache.attention_gated(q, gate, b.cu, b.len, table), want)
+
+
 # --------------------------------------------------------------------------- weights
 @gpu
 @pytest.mark.parametrize("window,sinks", [(0, 0), (50, 4), (1, 0), (70, 200)])
