@@ -1,5 +1,5 @@
 // How the work of a batch over a paged cache is dealt to work-groups: it is laid
-// out on one line, tile after tile of RT query rows, and each of W work-groups
+// out on one line, tile after tile of R query rows, and each of W work-groups
 // takes an equal stretch of it.  A stretch ends inside a tile where it must, so
 // requests of any lengths load the chip evenly without a table from the host or
 // a launch that builds one; the parts of a tile are joined afterwards.

