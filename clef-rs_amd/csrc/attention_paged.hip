@@ -11,7 +11,7 @@
 // attention_parts.hpp, and outputs too, on values stored by feature.
 //
 // Two shapes of work: tiles of 16 rows for single tokens and short chunks, bound by the
-// keys' bytes, and tiles of 256 rows for chunks, bound by MFMA.  Weights are rounded
+// keys' bytes, and tiles of 256 (f16) or 64 rows (f32) for chunks, bound by MFMA.  Weights are rounded
 // once, to the operands' type; scores, maxima, sums and outputs are f32.
 #include <hip/hip_runtime.h>
 
@@ -182,16 +182,20 @@ struct FewRows {
 // 1.20 GB in 220 us, 5.5 TB/s, more than a large copy's 5.2.  A short call is bound by
 // latency: one token behind 700 keys takes 11 us and the joining 4, most of it the chain
 // of table, page and key loads and the fetching of 19 KB of code.
-template <class T, int D, bool FULL, int NW>
+//
+// EACH (f32): a tile of 16 NW rows, 16 to a wave; every wave takes all blocks, which pass through LDS.
+template <class T, int D, bool FULL, int NW, bool EACH = false>
 __device__ __forceinline__ void few_rows(const PagedAttn& p, const Request& r, const Seen& seen, const Piece& x,
-                                         int row0, int rows, FewRows<T, D, NW>& sh, int w) {
+                                         int tile0, int tile_rows, FewRows<T, D, NW>& sh, int w) {
   constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL, PER = kWalkBlock / KB;
   typedef typename Ops<T>::frag frag;
   const Paged& c = p.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, grp = lane >> 4, G = p.t.G;
+  const int row0 = EACH ? tile0 + 16 * wave : tile0, rows = EACH ? min(max(tile_rows - 16 * wave, 0), 16) : tile_rows;
+  const int begin = x.b0 * PER + (EACH ? 0 : wave), step = EACH ? 1 : NW;  // blocks of the wave
   // the lane's query (rows behind the last: the last again)
-  const int row = row0 + min(lr, rows - 1), tok = token_of(p.t, row), at = r.len - r.n + tok;
+  const int row = min(row0 + lr, tile0 + tile_rows - 1), tok = token_of(p.t, row), at = r.len - r.n + tok;
   frag fq[D / KB];
   auto load_queries = [&]() {
     const T* src =
@@ -211,8 +215,66 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Request& r, c
   Soft<T, D, 1> st;
   st.clear();
   bool odd = false;
+  if constexpr (EACH) {
+    // K: 16 rows of D / 4 slots of 16 bytes, V: D rows of 4; slots permuted by their row (XOR)
+    constexpr int S = D / 4, NDMA = D / 16 / NW;  // slots of a key, transfers of a wave for each of K and V
+    frag* const tiles = reinterpret_cast<frag*>(&sh);
+    static_assert(NDMA >= 1 && sizeof(sh) >= 4 * 16 * D * sizeof(T), "two buffers of keys and values");
+    const int in = (1 << c.shift) - 1, end = x.b1 * PER;
+    auto issue = [&](int buf, int c0) {
+      const int page = page_of(c, x.s, c0);
+      const T* const k = K + page * c.ks + (c0 & in) * c.d;
+      const T* const v = V + page * c.vs + (c0 & in);
+      frag* const to = tiles + buf * 32 * S;
+#pragma unroll
+      for (int i = 0; i < NDMA; ++i) {
+        const int slot = (wave * NDMA + i) * 64 + lane, y = slot / S, e = (slot % S ^ y) * 4, f = slot / 4;
+        // (features behind the last: others of the same key, times queries that are 0)
+        dma16(k + y * c.d + (FULL || e < c.d ? e : 0), to + (wave * NDMA + i) * 64);
+        dma16(v + ((FULL ? f : min(f, c.d - 1)) << c.shift) + ((slot ^ f >> 2) & 3) * 4,
+              to + S * 16 + (wave * NDMA + i) * 64);
+      }
+    };
+    auto seen_from = [&](int b) {
+      while (b < end && none(key0(b))) ++b;
+      return b;
+    };
+    int b = seen_from(begin), buf = 0;
+    if (b < end) issue(0, key0(b));
 #pragma unroll 1
-  for (int b = x.b0 * PER + wave; b < x.b1 * PER; b += NW) {
+    while (b < end) {
+      const int next = seen_from(b + 1), c0 = key0(b);
+      if (next < end) {
+        issue(buf ^ 1, key0(next));
+        vm_wait<2 * NDMA>();
+      } else {
+        vm_wait_all();
+      }
+      lds_barrier();
+      const frag *const tk = tiles + buf * 32 * S + lr * S, *const tv = tiles + buf * 32 * S + 16 * S;
+      float4_t sc[1][1] = {};
+#pragma unroll
+      for (int kb = 0; kb < D / KB; ++kb) {
+        const frag y = tk[(kb * 4 + grp) ^ lr];
+        Mma<T>::mma(sc[0][0], FULL || kb * KB + grp * EL < c.d ? y : frag{}, fq[kb]);
+      }
+      PageBlock<T, D, FULL> blk;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) blk.v[e] = tv[e * 64 + lr * 4 + (grp ^ lr >> 2)];
+      if (!all(c0)) {
+        blk.hide(sc, p.t, at, c0, lane);
+        odd |= blk.clean(seen, c0, lane);
+      }
+      frag wt[1][1];
+      st.template weights<1>(sc, wt, p.scale);
+      blk.values(st, wt);
+      lds_barrier();  // the tile is read before others replace it
+      b = next;
+      buf ^= 1;
+    }
+  } else
+#pragma unroll 1
+  for (int b = begin; b < x.b1 * PER; b += step) {
     const int c0 = key0(b);
     if (none(c0)) continue;
     const int first = page_of(c, x.s, c0), second = KB > 16 ? page_of(c, x.s, c0 + 16) : first;
@@ -237,7 +299,7 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Request& r, c
     const float m = lr < rows ? sh.parts.ml[wave][lr].x : 0.0f, ref = (m == -INFINITY ? 0.0f : m) - Ops<T>::UP;
     load_queries();
 #pragma unroll 1
-    for (int b = x.b0 * PER + wave; b < x.b1 * PER; b += NW) {
+    for (int b = begin; b < x.b1 * PER; b += step) {
       const int c0 = key0(b);
       if (none(c0) || all(c0)) continue;
       const int first = page_of(c, x.s, c0), second = KB > 16 ? page_of(c, x.s, c0 + 16) : first;
@@ -267,13 +329,21 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Request& r, c
       lds_done();
     }
   }
-  lds_barrier();
+  if (EACH) lds_done();
+  else lds_barrier();
   const bool whole = x.head && x.tail;
-  const int64_t to = ((int64_t)w * 2 + (x.head ? 1 : 0)) * p.t.R;
-  for (int i = tid; i < rows * (D / 4); i += 64 * NW) {
+  const int64_t to = ((int64_t)w * 2 + (x.head ? 1 : 0)) * p.t.R + row0 - tile0;
+  for (int i = EACH ? lane : tid; i < rows * (D / 4); i += EACH ? 64 : 64 * NW) {
     const int y = i / (D / 4), e = i % (D / 4) * 4;
     float m, l;
-    const float4_t o = sh.parts.take(y, e, m, l);
+    float4_t o;
+    if constexpr (EACH) {
+      m = sh.parts.ml[wave][y].x;
+      l = sh.parts.ml[wave][y].y;
+      o = *reinterpret_cast<const float4_t*>(&sh.parts.o[wave][y][e]);
+    } else {
+      o = sh.parts.take(y, e, m, l);
+    }
     if (whole) {
       const int tok = token_of(p.t, row0 + y), t = r.first + tok, h = x.kv * G + row0 + y - tok * G;
       if (e < c.d) write_out<T>(p, o, inverse(l), t, h, e, p.vec);
@@ -304,6 +374,25 @@ __device__ __forceinline__ void walk_pieces(const PagedAttn& p, WalkShared& walk
     }
   }
   if (threadIdx.x == 0) p.split[blockIdx.x] = split;
+}
+
+// Tiles of 64 rows, for chunks in f32: 16 rows to a wave, and blocks of 16 keys through LDS by DMA,
+// double-buffered, for all four.  Straight into operands every 16 bytes are an access of their own
+// (neighbouring lanes hold different rows), 64 to a load, and the first cache bounds the products at
+// 55 TFLOP/s, whoever shares the keys and however early they are requested.  300 tokens of 16 heads
+// x 256 behind 4,000 keys 370 -> 251 us, 81 TFLOP/s (a library product of 8192^3: 154); 1,024 from
+// nothing 231 -> 141.
+template <int D, bool FULL>
+__global__ __launch_bounds__(256, 2) void paged_some_rows(PagedAttn p) {
+  typedef float T;
+  __shared__ __attribute__((aligned(1024))) FewRows<T, D, 4> sh;
+  __shared__ WalkShared walk;
+  walk_pieces<256>(p, walk, [&](const Request& r, const Seen& seen, const Piece& piece, int w) {
+    const int row0 = piece.tile * 64, rows = min(64, r.n * p.t.G - row0);
+    if (r.n * p.t.G <= 16) few_rows<T, D, FULL, 4>(p, r, seen, piece, row0, rows, sh, w);
+    else few_rows<T, D, FULL, 4, true>(p, r, seen, piece, row0, rows, sh, w);
+    lds_barrier();
+  });
 }
 
 template <class T, int D, bool FULL>
@@ -787,8 +876,8 @@ int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 // How a call is launched, from the shapes alone (the workspace follows from it).
 struct PagedPlan {
-  bool many;   // tiles of 256 rows, else of 16
-  int R;       // rows of a tile
+  bool many;   // tiles of 256 rows, in f16
+  int R;       // rows of a tile: 256, 64 (f32) or 16
   int tile_cost;
   int groups;  // work-groups, a multiple of 8
 };
@@ -801,7 +890,11 @@ PagedPlan plan_of(int T, int nseq, int max_keys, int dtype, int heads, int kvh, 
   const int64_t units = (rows / 16 + nseq) * kvh * (max_keys / kWalkBlock + 1);
   x.many = dtype == CLEF_F16 && d == padded(d) && rows > 16 * (int64_t)nseq &&
            (rows > 64 * (int64_t)nseq || units > 32 * cus);
-  x.R = x.many ? kManyRows : 16;
+  // The same in f32 on tiles of 64 rows.  (16 rows, 64: one request of 32 tokens of 8 heads a key head behind
+  // 4,000 keys 59, 77 us; of 64 94, 82; of 128 162, 121; 16 of 5 86, 93; of 8 109, 97; of 16 178, 133)
+  const int64_t blocks64 = (rows / 64 + nseq) * kvh * (max_keys / kWalkBlock + 1);
+  const bool some = dtype == CLEF_F32 && rows > 48 * (int64_t)nseq && blocks64 > 4 * cus;
+  x.R = x.many ? kManyRows : some ? 64 : 16;
   // (a wide tile's queries, fill, outputs and joining take as long as eight blocks of keys: a prompt of
   // 4,096 tokens with 256 and 512 keys for them 240, 208 us; with 32, when they took more, twice as long)
   x.tile_cost = x.many ? 512 : 64;
@@ -824,6 +917,13 @@ int launch(const PagedAttn& p, const PagedPlan& x, hipStream_t st) {
   if constexpr (sizeof(T) == 2 && FULL) {
     if (x.many) {
       hipLaunchKernelGGL((paged_many_rows<D>), dim3(x.groups), dim3(512), 0, st, p);
+      hipLaunchKernelGGL((paged_join<T, D, false>), dim3(x.groups * (x.R / (1024 / D))), dim3(256), 0, st, p);
+      return check_launch("paged attention");
+    }
+  }
+  if constexpr (sizeof(T) == 4) {
+    if (x.R == 64) {
+      hipLaunchKernelGGL((paged_some_rows<D, FULL>), dim3(x.groups), dim3(256), 0, st, p);
       hipLaunchKernelGGL((paged_join<T, D, false>), dim3(x.groups * (x.R / (1024 / D))), dim3(256), 0, st, p);
       return check_launch("paged attention");
     }

@@ -606,3 +606,65 @@ def test_bad_tables_stay_inside(clef, dtype):
         step(clef, b, to, heads, x, state)
         torch.cuda.synchronize()
         assert torch.equal(b.k.nan_to_num(5.0), k0.nan_to_num(5.0)) and torch.equal(b.vt.nan_to_num(5.0), v0.nan_to_num(5.0))
+
+
+# --- chunks in f32: tables wide enough for tiles of 64 rows
+def widened(monkeypatch, page):
+    import functools
+    import sys
+    monkeypatch.setattr(sys.modules[__name__], "Batch", functools.partial(Batch, spare=(1 << 16) // page))
+
+
+@gpu
+@pytest.mark.parametrize("name", ["chunk", "prompt", "behind", "mixed", "early"])
+@pytest.mark.parametrize("page,kvh,rep,d", [(16, 2, 8, 256), (32, 1, 4, 64), (256, 2, 3, 128), (64, 3, 24, 40),
+                                            (16, 2, 5, 72), (64, 1, 16, 200), (32, 4, 2, 8)])
+def test_attention_wide_f32(clef, monkeypatch, name, page, kvh, rep, d):
+    widened(monkeypatch, page)
+    test_attention(clef, name, F32, page, kvh, rep, d)
+
+
+@gpu
+@pytest.mark.parametrize("window,sinks", [(1, 0), (5, 4), (64, 70), (100, 1000), (2000, 4)])
+@pytest.mark.parametrize("page,d", [(16, 256), (32, 64), (64, 104)])
+def test_window_and_sinks_wide_f32(clef, monkeypatch, window, sinks, page, d):
+    widened(monkeypatch, page)
+    test_window_and_sinks(clef, window, sinks, F32, page, d)
+
+
+@gpu
+@pytest.mark.parametrize("window,sinks", [(0, 0), (30, 4)])
+@pytest.mark.parametrize("page,d", [(16, 128), (32, 72), (64, 256)])
+def test_infinite_and_nan_values_wide_f32(clef, monkeypatch, window, sinks, page, d):
+    widened(monkeypatch, page)
+    test_infinite_and_nan_values(clef, window, sinks, F32, page, d, [(100, 230), (3, 70), (60, 60)])
+
+
+@gpu
+@pytest.mark.parametrize("requests", [[(300, 3000)], [(700, 700)], [(200, 1000), (90, 2500), (1, 4000)]], ids=str)
+def test_long_chunks_f32(clef, requests):
+    attend(clef, Batch(requests, 64, 2, 128, F32, seed=len(requests), spare=1000), 16)
+
+
+@gpu
+def test_captured_chunk_f32(clef):
+    """A chunk in f32 in a captured launch whose lengths change between replays."""
+    b = Batch([(80, 900), (64, 300)], 64, 2, 256, F32, seed=4, spare=1000)
+    q, gate = b.randn(16, b.T, 256), b.randn(b.T, 16, 256)
+    cache = clef.PagedCache(b.k, b.vt)
+    lens = b.len.clone()
+    out = torch.zeros((b.T, 16 * 256), device="cuda")
+    run = lambda: cache.attention_gated(q, gate, b.cu, lens, b.table, out=out)  # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for less in (0, 100, 200, 0, 170):
+        lens.copy_(b.len - less)
+        out.fill_(9.0)
+        graph.replay()
+        got = out.clone()
+        run()
+        torch.cuda.synchronize()
+        assert torch.equal(got, out)
