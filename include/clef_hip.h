@@ -535,7 +535,8 @@ int clef_paged_weights(const clef_paged_cache* cache, const int32_t* table, int 
  * than budget keys are copied whole.  new_lens (device int32 [nseq]) receives min(len,
  * budget), keep (device int32 [nseq][kv_heads][budget]) the kept indices, -1 behind
  * them.  The pages written must not be pages that this call reads.  sinks + recent <=
- * budget <= to_max_pages * page; scores 16-byte aligned.
+ * budget <= to_max_pages * page; scores 16-byte aligned.  One call moves at most 2^23
+ * pieces: ceil(min(budget, max_pages * page) / 64) * (1 + ceil(d / 64)) * kv_heads * nseq.
  */
 int clef_paged_evict(const clef_paged_cache* cache, const int32_t* table, int max_pages, const int32_t* key_lens,
                      int nseq, const float* scores, int budget, int sinks, int recent, const clef_paged_cache* to,
