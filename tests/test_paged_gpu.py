@@ -668,3 +668,20 @@ def test_captured_chunk_f32(clef):
         run()
         torch.cuda.synchronize()
         assert torch.equal(got, out)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32], ids=str)
+@pytest.mark.parametrize("requests", [[(1, 700), (3, 90)], [(120, 2000), (1, 30)]], ids=str)
+def test_odd_addresses(clef, dtype, requests):
+    """Gates and outputs that begin at any element, rows any distance apart."""
+    heads, d = 8, 128
+    b = Batch(requests, 64, 2, d, dtype, seed=3, spare=1000)
+    q, wide = b.randn(heads, b.T, d), b.randn(b.T, heads * (d + 1) + 2)
+    gate = wide[:, 1:1 + heads * (d + 1)].view(b.T, heads, d + 1)[:, :, :d]
+    cache = clef.PagedCache(b.k, b.vt)
+    want = cache.attention_gated(q, gate.contiguous(), b.cu, b.len, b.table)
+    out = torch.full((b.T, heads * d + 7), 7.0, dtype=dtype, device="cuda")
+    cache.attention_gated(q, gate, b.cu, b.len, b.table, out=out[:, 3:3 + heads * d])
+    assert torch.equal(out[:, 3:3 + heads * d], want)
+    assert (out[:, :3] == 7.0).all() and (out[:, 3 + heads * d:] == 7.0).all()
