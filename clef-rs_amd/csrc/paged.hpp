@@ -23,14 +23,15 @@ struct Paged {
 };
 
 // The tokens and keys of a request, inside the buffers whatever the tables hold:
-// tokens first .. first + n - 1, the last of them at key len - 1.
+// tokens first .. first + n - 1, the last of them at key len - 1.  (An end is bounded on both sides before
+// first is taken from it: the least whole number less first is a large one.)
 struct Request {
   int first, n, len;
 };
 __device__ __forceinline__ Request request_of(const Paged& p, int s) {
   Request x;
   x.first = min(max(p.cu[s], 0), p.T);
-  x.n = max(min(p.cu[s + 1], p.T) - x.first, 0);
+  x.n = min(max(p.cu[s + 1], x.first), p.T) - x.first;
   x.len = min(max(p.len[s], 0), p.max_keys);
   return x;
 }
@@ -71,7 +72,7 @@ __device__ __forceinline__ int request_at(const Paged& p, int t, int lane, Reque
   const int begin = s ? __builtin_amdgcn_readlane(end, s - 1) : zero;
   if (begin > t) return -1;
   r.first = min(max(begin, 0), p.T);
-  r.n = max(min(__builtin_amdgcn_readlane(end, s), p.T) - r.first, 0);
+  r.n = min(max(__builtin_amdgcn_readlane(end, s), r.first), p.T) - r.first;
   r.len = min(max(__builtin_amdgcn_readlane(len, s), 0), p.max_keys);
   return s;
 }

@@ -1,0 +1,95 @@
+"""The device code of a paged cache's calls that finds requests and deals out work from
+device tables (paged.hpp, paged_walk.hpp), compiled for the host with the threads of a
+work-group as fibers (host_wave/): over tables that fit, every token and every block of
+keys is found once, and over tables that do not, no index leaves its buffer."""
+import ctypes as C
+import pathlib
+import subprocess
+
+import numpy as np
+import pytest
+
+HERE = pathlib.Path(__file__).resolve().parent
+CLANG = "/opt/rocm/llvm/bin/clang++"
+INT_MIN, INT_MAX = -2 ** 31, 2 ** 31 - 1
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    out = tmp_path_factory.mktemp("host_wave") / "paged_tables.so"
+    subprocess.run([CLANG, "-O1", "-std=c++17", "-fPIC", "-shared", "-I", str(HERE / "host_wave"), "-o", str(out),
+                    str(HERE / "host_wave" / "paged_tables.cpp")], check=True)
+    return C.CDLL(str(out))
+
+
+def ints(x):
+    return np.ascontiguousarray(np.clip(x, INT_MIN, INT_MAX).astype(np.int32))
+
+
+def at(x):
+    return x.ctypes.data_as(C.c_void_p)
+
+
+def fitting(rng, nseq, T):
+    """Offsets from 0, some requests empty, up to a few rows behind the last one."""
+    total = int(rng.integers(0, T + 1))
+    return np.concatenate([[0], np.sort(rng.integers(0, total + 1, nseq - 1)), [total]])
+
+
+def bad(rng, nseq, T):
+    kind = rng.integers(0, 5)
+    if kind == 0:
+        return rng.integers(INT_MIN, INT_MAX, nseq + 1, endpoint=True)
+    if kind == 1:
+        return rng.integers(-T, 2 * T + 1, nseq + 1)
+    if kind == 2:
+        return rng.integers(0, T + 1, nseq + 1)
+    table = fitting(rng, nseq, T)
+    if kind == 3:  # a fitting one with a few entries replaced
+        table[rng.integers(0, nseq + 1, 3)] = rng.choice([INT_MIN, -1, 0, T // 2, T, T + 1, INT_MAX], 3)
+        return table
+    return table[::-1]
+
+
+def requests(host, cu, lens, T, page, width, tokens):
+    out = np.zeros((len(tokens), 4), np.int32)
+    for i, t in enumerate(tokens):
+        host.requests_at(at(cu), at(lens), len(lens), T, page, width, int(t), int(t) + 1, at(out[i:i + 1]))
+    return out
+
+
+# ---------------------------------------------------------------------------- requests
+@pytest.mark.parametrize("nseq", [1, 2, 65, 4096])
+def test_requests_stay_inside(host, nseq):
+    """A request's tokens lie in the batch and its keys in its table, whatever the tables hold."""
+    rng = np.random.default_rng(nseq)
+    for i in range(30):
+        T = int(rng.integers(1, 65537))
+        cu, lens = bad(rng, nseq, T), rng.choice([INT_MIN, -1, 0, 1, 239, 240, 241, INT_MAX], nseq)
+        if i == 0:
+            cu[0], cu[1] = 1, INT_MIN
+        cu, lens = ints(cu), ints(lens)
+        out = np.zeros((nseq, 3), np.int32)
+        host.requests_of(at(cu), at(lens), nseq, T, 16, 15, at(out))
+        first, n, length = out.astype(np.int64).T
+        assert (first == np.clip(cu[:-1], 0, T)).all()
+        assert (n == np.maximum(np.clip(cu[1:], 0, T) - first, 0)).all()
+        assert (length == np.clip(lens, 0, 240)).all()
+
+
+# ---------------------------------------------------------------------------- the request of a token
+@pytest.mark.parametrize("nseq", [1, 2, 63, 64, 65, 130, 4096])
+def test_tokens_find_their_request(host, nseq):
+    rng = np.random.default_rng(nseq)
+    for _ in range(4):
+        T = int(rng.integers(1, min(3 * nseq, 60000) + 2))
+        cu = ints(fitting(rng, nseq, T))
+        lens = ints(cu[1:] - cu[:-1] + rng.integers(0, 50, nseq))
+        tokens = rng.integers(0, T, 40)
+        for t, (s, first, n, length) in zip(tokens, requests(host, cu, lens, T, 16, 8192, tokens)):
+            want = int(np.searchsorted(cu[1:], t, side="right"))
+            assert s == (want if want < nseq else -1)
+            if s >= 0:
+                assert (first, n, length) == (cu[s], cu[s + 1] - cu[s], lens[s]) and first <= t < first + n
+
+
