@@ -57,24 +57,27 @@ __device__ __forceinline__ int request_at(const Paged& p, int t, int lane) {
   return lo < p.nseq && p.cu[lo] <= t ? lo : -1;
 }
 
-// The same with its tokens and keys; of up to 64 requests in one round of loads.
+// The same with its tokens and keys, first <= t < first + n: offsets that do not ascend can lead
+// the search to a request that ends before t, which then has none (its key would be behind the
+// table's last).  Of up to 64 requests in one round of loads.
 __device__ __forceinline__ int request_at(const Paged& p, int t, int lane, Request& r) {
   if (p.nseq > 64) {
     const int s = __builtin_amdgcn_readfirstlane(request_at(p, t, lane));
-    if (s >= 0) r = request_of(p, s);
-    return s;
+    if (s < 0) return -1;
+    r = request_of(p, s);
+    return t - r.first < r.n ? s : -1;
   }
   const int i = min(lane, p.nseq - 1);
   const int end = p.cu[i + 1], len = p.len[i], zero = p.cu[0];
   const int s = __popcll(__ballot(lane < p.nseq && end <= t) & (p.nseq == 64 ? ~0ull : (1ull << p.nseq) - 1));
-  // (as the search above: requests that end at or before t, counted; tables that do not fit may skip one)
+  // (as the search above: requests that end at or before t, counted)
   if (s >= p.nseq) return -1;
   const int begin = s ? __builtin_amdgcn_readlane(end, s - 1) : zero;
   if (begin > t) return -1;
   r.first = min(max(begin, 0), p.T);
   r.n = min(max(__builtin_amdgcn_readlane(end, s), r.first), p.T) - r.first;
   r.len = min(max(__builtin_amdgcn_readlane(len, s), 0), p.max_keys);
-  return s;
+  return t - r.first < r.n ? s : -1;
 }
 
 inline bool misaligned(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) != 0; }

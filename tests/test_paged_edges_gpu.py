@@ -1,0 +1,78 @@
+"""The paged cache's calls at their edges: tables that do not fit beside pages of others,
+lengths updated in place, requests that share pages."""
+import pytest
+import torch
+
+import test_paged_gpu as base
+
+gpu = pytest.mark.gpu
+F16, F32 = torch.float16, torch.float32
+MIN, MAX = -2 ** 31, 2 ** 31 - 1
+ints = base.ints
+
+
+@pytest.fixture(scope="module")
+def clef():
+    import clef_hip
+    clef_hip.lib()
+    return clef_hip
+
+
+def same(a, b):
+    return torch.equal(a.nan_to_num(5.0), b.nan_to_num(5.0))
+
+
+# Device tables that do not fit, of three requests with at most 15 pages of 16 keys and 22 tokens
+BAD = [([0, 20, 3, 5], [5, 6, 240]), ([22, 22, 0, 0], [1, 2, MAX]), ([0, 9, 2, 4], [MAX, MAX, MAX]),
+       ([0, 5, MIN, 22], [200, 240, 33]), ([MIN, MIN, MIN, MIN], [MAX, 0, 7]), ([0, MAX, MIN, MAX], [MIN, MAX, 241]),
+       ([0, 22, 0, 22], [240, 240, 240]), ([-5, 3, 40, 2], [1, 500, MIN])]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32], ids=str)
+@pytest.mark.parametrize("rep", [1, 4])
+@pytest.mark.parametrize("requests", [3, 70])
+def test_bad_tables_beside_others(clef, dtype, rep, requests):
+    """Page tables lie between rows that name pages of others: an index that left a request's table would
+    find such a page.  Nothing of others changes, nor a row before or behind the batch's."""
+    T, width, page, kvh, d, heads = 22, 15, 16, 2, 64, 2 * rep
+    g = torch.Generator(device="cuda").manual_seed(rep)
+    randn = lambda *s: torch.randn(s, generator=g, device="cuda").to(dtype)  # noqa: E731
+    mine, others = requests * width, 40
+    around = torch.randint(mine, mine + others, (requests + 20, width), generator=g, device="cuda").int()
+    around[10:10 + requests] = torch.randperm(mine, generator=g, device="cuda").int().view(requests, width)
+    table = around[10:10 + requests]
+    to_around = torch.randint(mine, mine + others, (requests + 20, 3), generator=g, device="cuda").int()
+    to_around[10:10 + requests] = torch.arange(requests * 3, device="cuda").int().view(requests, 3)
+    total = mine + others
+    w = torch.ones(d, device="cuda")
+    for cu, lens in BAD:
+        k, vt = randn(total, kvh, page, d), randn(total, kvh, d, page)
+        to_k, to_vt = k.clone(), vt.clone()
+        scores = torch.rand((total, kvh, page), generator=g, device="cuda")
+        new, to_scores = torch.full_like(scores, 7.0), torch.full_like(scores, 7.0)
+        before = [x.clone() for x in (k, vt, to_k, to_vt)]
+        cu = ints((cu[:-1] + [22, 0, 9] * 30)[:requests] + cu[-1:])
+        lens = ints((lens + [240, MAX, MIN] * 30)[:requests])
+        cache, to = clef.PagedCache(k, vt), clef.PagedCache(to_k, to_vt)
+        # each output between rows of its own
+        q_all = torch.full((heads + 2, T, d), 7.0, dtype=dtype, device="cuda")
+        y_all = torch.full((T + 40, heads * d), 7.0, dtype=dtype, device="cuda")
+        lse_all = torch.full((T + 40, heads), 7.0, device="cuda")
+        q = cache.append(randn(T, heads, d), randn(T, kvh, d), randn(T, kvh, d), w, w, cu, lens, table, 32, 1e4,
+                         out=q_all[1:1 + heads])
+        q.copy_(randn(heads, T, d))
+        lse = lse_all[20:20 + T]
+        for window, sinks in ((0, 0), (30, 4)):
+            cache.attention_gated(q, randn(T, heads, d), cu, lens, table, window=window, sinks=sinks, lse=lse,
+                                  out=y_all[20:20 + T])
+            cache.add_weights(q, torch.zeros_like(lse), cu, lens, table, scores, new_scores=new, window=window, sinks=sinks)
+        cache.evict(scores, lens, table, 40, to, to_around[10:10 + requests], to_scores, sinks=4, recent=8)
+        torch.cuda.synchronize()
+        for now, was in zip((k, vt, to_k, to_vt), before):
+            assert same(now[mine:], was[mine:]), (cu.tolist()[:4], "a page of others")
+        assert same(to_k[requests * 3:], before[2][requests * 3:]) and same(to_vt[requests * 3:], before[3][requests * 3:])
+        assert (new[mine:] == 7.0).all() and (to_scores[requests * 3:] == 7.0).all()
+        assert (q_all[0] == 7.0).all() and (q_all[-1] == 7.0).all()
+        for x in (y_all, lse_all):
+            assert (x[:20] == 7.0).all() and (x[20 + T:] == 7.0).all()

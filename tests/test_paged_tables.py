@@ -93,3 +93,24 @@ def test_tokens_find_their_request(host, nseq):
                 assert (first, n, length) == (cu[s], cu[s + 1] - cu[s], lens[s]) and first <= t < first + n
 
 
+
+
+@pytest.mark.parametrize("nseq", [1, 2, 3, 63, 64, 65, 200, 4096])
+def test_bad_tables_find_tokens_inside_a_request(host, nseq):
+    """What a token's page is found by: its index among the request's keys is below their number,
+    so the table's column is one of the request's."""
+    rng = np.random.default_rng(nseq)
+    special = [([0, 20, 3, 5], [5, 6, 240], 22), ([22, 22, 0, 0], [1, 2, INT_MAX], 22), ([0, 9, 2, 4], [9, 9, 240], 9)]
+    for i in range(40):
+        if nseq == 3 and i < len(special):
+            cu, lens, T = special[i]
+        else:
+            T = int(rng.integers(1, 65537 if i % 2 else 300))
+            cu, lens = bad(rng, nseq, T), rng.choice([INT_MIN, -1, 0, 1, 239, 240, 241, INT_MAX], nseq)
+        cu, lens = ints(cu), ints(lens)
+        tokens = range(T) if T <= 22 else rng.integers(0, T, 30)
+        for t, (s, first, n, length) in zip(tokens, requests(host, cu, lens, T, 16, 15, tokens)):
+            assert -1 <= s < nseq
+            if s >= 0:
+                assert 0 <= first <= t < first + int(n) <= T and 0 <= length <= 240
+                assert length - n + (t - first) < 240  # max_pages * page
