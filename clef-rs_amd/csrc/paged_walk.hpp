@@ -21,9 +21,9 @@ __device__ __forceinline__ double uniform(double x) {
 }
 __device__ __forceinline__ Request uniform(Request x) { return {uniform(x.first), uniform(x.n), uniform(x.len)}; }
 
-// Lengths on the line are whole numbers below 2^53 held in f64, exactly: a 64-bit integer product or
-// division takes tens to hundreds of instructions, and a short call spends its time on such.
-// floor(a / b):
+// Lengths on the line are whole numbers below 2^53 held in f64, exactly (where requests do not
+// overlap): a 64-bit integer product or division takes tens to hundreds of instructions, and a
+// short call spends its time on such.  floor(a / b):
 __device__ __forceinline__ double quotient(double a, double b) {
   double q = floor(a / b);
   if (q * b > a) q -= 1.0;
@@ -161,6 +161,7 @@ __device__ __forceinline__ bool walk_begin(const Paged& p, F length, float over_
     if (lane >= o) upto += y;
   }
   if (lane == 63) sh.sums[tid >> 6] = upto;
+  if (tid == 0) sh.s = -1;
   __syncthreads();
   double before = 0.0, total = 0.0;
 #pragma unroll
@@ -183,6 +184,9 @@ __device__ __forceinline__ bool walk_begin(const Paged& p, F length, float over_
     sh.base = at;
   }
   __syncthreads();
+  // Requests that overlap can be so long together that sums are rounded, and u lies between two threads':
+  // nobody's, and the work-group has none.
+  if (uniform(sh.s) < 0) return false;
   out.base = uniform(sh.base);
   out.s = uniform(sh.s);
   out.r = uniform(request_of(p, out.s));
@@ -261,9 +265,10 @@ __device__ __forceinline__ bool next_piece(const Paged& p, const Rows& t, Stretc
   out.head = x.u == out.from;
   out.tail = stop == out.to;
   v = seen_by(t, r, lo * t.R, min((lo + 1) * t.R, r.n * t.G));
-  // blocks in proportion; the same division on both sides of a cut
+  // blocks in proportion; the same division on both sides of a cut (rounded sums, as above, may place y
+  // before the tile)
   const double scale = v.blocks / (out.to - out.from);
-  auto block = [&](double y) { return min(v.blocks, uniform(static_cast<int>((y - out.from) * scale))); };
+  auto block = [&](double y) { return max(0, min(v.blocks, uniform(static_cast<int>((y - out.from) * scale)))); };
   out.b0 = uniform(out.head ? 0 : block(x.u));
   out.b1 = uniform(out.tail ? v.blocks : block(stop));
   x.u = uniform(stop);

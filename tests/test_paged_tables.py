@@ -114,3 +114,74 @@ def test_bad_tables_find_tokens_inside_a_request(host, nseq):
             if s >= 0:
                 assert 0 <= first <= t < first + int(n) <= T and 0 <= length <= 240
                 assert length - n + (t - first) < 240  # max_pages * page
+
+
+# ---------------------------------------------------------------------------- the line
+PIECE = ("s", "kv", "tile", "b0", "b1", "head", "tail", "blocks", "rows", "first", "n", "last")
+
+
+def pieces(host, cu, lens, T, page, width, kvh, G, R, cost, window, sinks, least, groups, threads, which=None, most=4000):
+    """The pieces of each work-group, as dicts with its number on the line's order of groups."""
+    out = np.zeros((most, len(PIECE)), np.int32)
+    got = []
+    for group in range(groups) if which is None else which:
+        n = host.walk(at(cu), at(lens), len(lens), T, page, width, kvh, G, R, cost, window, sinks,
+                      C.c_float(1.0 / (least * 64 * G)), group, groups, threads, at(out), most)
+        assert n >= 0, "a request that there is not"
+        got += [dict(zip(PIECE, row), group=group) for row in out[:n].tolist()]
+    return got
+
+
+def inside(y, nseq, T, kvh, groups):
+    assert 0 <= y["s"] < nseq and 0 <= y["kv"] < kvh and y["tile"] >= 0 and y["rows"] > 0, y
+    assert 0 <= y["b0"] <= y["b1"] <= y["blocks"], y
+    assert 0 <= y["first"] and y["first"] + y["n"] <= T and y["last"] <= groups, y
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 4)])
+@pytest.mark.parametrize("nseq,kvh,G,R,cost,threads", [(1, 2, 8, 256, 512, 512), (5, 2, 8, 16, 64, 256),
+                                                       (70, 1, 3, 64, 64, 256), (600, 3, 1, 16, 64, 256)])
+def test_every_block_is_dealt_once(host, nseq, kvh, G, R, cost, threads, window, sinks):
+    rng = np.random.default_rng(nseq + window)
+    groups, T = 64, 4 * nseq + 90
+    cu = ints(fitting(rng, nseq, T))
+    n = cu[1:] - cu[:-1]
+    lens = ints(n + rng.integers(0, 700, nseq))
+    got = pieces(host, cu, lens, T, 16, 400, kvh, G, R, cost, window, sinks, 2, groups, threads)
+    tiles = {}
+    for y in got:
+        inside(y, nseq, T, kvh, groups)
+        assert (y["first"], y["n"]) == (cu[y["s"]], n[y["s"]])
+        tiles.setdefault((y["s"], y["kv"], y["tile"]), []).append(y)
+    assert set(tiles) == {(s, kv, i) for s in range(nseq) for kv in range(kvh) for i in range(-(-int(n[s]) * G // R))}
+    for parts in tiles.values():
+        parts.sort(key=lambda y: (not y["head"], y["b0"]))
+        assert parts[0]["head"] and parts[-1]["tail"]
+        assert sum(y["head"] for y in parts) == sum(y["tail"] for y in parts) == 1
+        assert parts[0]["b0"] == 0 and parts[-1]["b1"] == parts[-1]["blocks"]
+        assert all(a["b1"] == b["b0"] for a, b in zip(parts, parts[1:]))
+
+
+@pytest.mark.parametrize("nseq", [1, 2, 3, 65, 1000])
+def test_bad_tables_are_dealt_inside(host, nseq):
+    rng = np.random.default_rng(nseq)
+    for i in range(12):
+        T, groups, kvh = int(rng.integers(1, 300)), 32, int(rng.integers(1, 4))
+        cu = ints(bad(rng, nseq, T))
+        lens = ints(rng.choice([INT_MIN, -1, 0, 1, 239, 240, 241, INT_MAX], nseq))
+        window, sinks = ((0, 0), (30, 4))[i % 2]
+        for y in pieces(host, cu, lens, T, 16, 15, kvh, 1 + i % 3, 16, 64, window, sinks, 1, groups, 256):
+            inside(y, nseq, T, kvh, groups)
+
+
+@pytest.mark.parametrize("nseq", [512, 1024, 4096])
+@pytest.mark.parametrize("kvh", [1, 3, 5])
+def test_overlapping_requests_are_dealt_inside(host, nseq, kvh):
+    """Every second request has all tokens behind 2^24 keys: the line is longer than f64 counts exactly, and cuts
+    fall on the borders between threads."""
+    rng = np.random.default_rng(nseq + kvh)
+    T, groups = 65536 - int(rng.integers(0, 50)), 512
+    cu = ints(np.where(np.arange(nseq + 1) % 2 == 0, 0, T))
+    lens = ints(np.full(nseq, (1 << 24) - int(rng.integers(0, 100000))))
+    for y in pieces(host, cu, lens, T, 16, 1 << 20, kvh, 256 // kvh, 16, 64, 0, 0, 1, groups, 256, most=2):
+        inside(y, nseq, T, kvh, groups)
