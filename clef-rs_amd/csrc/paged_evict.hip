@@ -72,7 +72,6 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select(EvictParams p) {
   const int tid = threadIdx.x, s = blockIdx.x / c.kvh, kv = blockIdx.x % c.kvh;
   const int len = min(max(c.len[s], 0), c.max_keys), count = min(len, p.budget);
   int* keep = p.keep + ((int64_t)s * c.kvh + kv) * p.budget;
-  if (kv == 0 && tid == 0) p.new_lens[s] = count;
   for (int i = count + tid; i < p.budget; i += kSelectThreads) keep[i] = -1;
   if (len <= p.budget) {
     for (int i = tid; i < count; i += kSelectThreads) keep[i] = i;
@@ -179,6 +178,9 @@ __global__ __launch_bounds__(256) void evict_move(EvictParams p, int tiles) {
   const int slice = blockIdx.x % slices, tile = blockIdx.x / slices % tiles, at = blockIdx.x / slices / tiles;
   const int kv = at % c.kvh, s = at / c.kvh;
   const int len = min(max(c.len[s], 0), c.max_keys), count = min(len, p.budget);
+  // here, where the selection has read the lengths of all heads: they may be the same array (a
+  // work-group that reads the new one finds the same count)
+  if (kv == 0 && slice == 0 && tile == 0 && tid == 0) p.new_lens[s] = count;
   const int i0 = tile * kMoved;
   if (i0 >= count) return;
   __shared__ int from_page[kMoved], from_slot[kMoved], to_page[kMoved];
@@ -254,6 +256,8 @@ extern "C" int clef_paged_evict(const clef_paged_cache* cache, const int32_t* ta
   if (int rc = clef::paged_batch("paged evict", nseq, 1, cache->kv_heads, cache->kv_heads)) return rc;
   CLEF_REQUIRE(key_lens && scores && to_scores && new_lens && keep, "paged evict: null pointer");
   CLEF_REQUIRE(!clef::misaligned(scores), "paged evict: scores must be 16-byte aligned");
+  CLEF_REQUIRE(new_lens == key_lens || new_lens + nseq <= key_lens || key_lens + nseq <= new_lens,
+               "paged evict: new_lens must be key_lens itself or apart from it");
   CLEF_REQUIRE(to->page == cache->page && to->kv_heads == cache->kv_heads && to->d == cache->d &&
                    to->dtype == cache->dtype,
                "paged evict: both caches must have the same page, heads, width and dtype");

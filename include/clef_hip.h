@@ -532,9 +532,9 @@ int clef_paged_weights(const clef_paged_cache* cache, const int32_t* table, int 
  * counts as lowest, ties go to the lowest index) stay, in their order, and are copied
  * with their scores into the pages that to_table [nseq][to_max_pages] names in `to`
  * (the same geometry; slots behind them are left as they were).  Requests of no more
- * than budget keys are copied whole.  new_lens (device int32 [nseq]) receives min(len,
- * budget), keep (device int32 [nseq][kv_heads][budget]) the kept indices, -1 behind
- * them.  The pages written must not be pages that this call reads.  sinks + recent <=
+ * than budget keys are copied whole.  new_lens (device int32 [nseq], key_lens itself or
+ * apart from it) receives min(len, budget), keep (device int32
+ * [nseq][kv_heads][budget]) the kept indices, -1 behind them.  The pages written must not be pages that this call reads.  sinks + recent <=
  * budget <= to_max_pages * page; scores 16-byte aligned.  One call moves at most 2^23
  * pieces: ceil(min(budget, max_pages * page) / 64) * (1 + ceil(d / 64)) * kv_heads * nseq.
  */

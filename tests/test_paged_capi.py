@@ -147,3 +147,9 @@ def test_binding_refuses_host_tensors_and_shapes(clef):
         for a in several:
             with pytest.raises(clef.ClefError):
                 call(*a)
+
+
+def test_evict_refuses_lengths_that_overlap(clef):
+    for lens, new in ((256, 260), (260, 256), (256, 264), (264, 256)):
+        assert clef.lib().clef_paged_evict(*evict(clef, lens=lens, new=new)) < 0
+        assert "new_lens" in clef.last_error()

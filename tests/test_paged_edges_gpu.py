@@ -76,3 +76,31 @@ def test_bad_tables_beside_others(clef, dtype, rep, requests):
         assert (q_all[0] == 7.0).all() and (q_all[-1] == 7.0).all()
         for x in (y_all, lse_all):
             assert (x[:20] == 7.0).all() and (x[20 + T:] == 7.0).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32], ids=str)
+def test_evict_lengths_in_place(clef, dtype):
+    """Lengths updated where they stand: every key head still cuts from the old ones."""
+    requests, budget, sinks, recent, kvh, page, d = 70, 48, 4, 8, 8, 16, 16
+    lens = [budget // 2 + 13 * s for s in range(requests)]
+    b = base.Batch([(0, m) for m in lens], page, kvh, d, dtype, seed=1)
+    to = base.Batch([(0, min(m, budget)) for m in lens], page, kvh, d, dtype, seed=2)
+    scores = torch.rand((b.total, kvh, page), generator=b.g, device="cuda")
+    to_scores = torch.zeros((to.total, kvh, page), device="cuda")
+    cache, target = clef.PagedCache(b.k, b.vt), clef.PagedCache(to.k, to.vt)
+    want_lens, want = cache.evict(scores, b.len, b.table, budget, target, to.table, to_scores, sinks=sinks, recent=recent)
+    pools = [x.clone() for x in (to.k, to.vt, to_scores)]
+    for _ in range(5):
+        length, keep = b.len.clone(), torch.empty_like(want)
+        for x in (to.k, to.vt, to_scores):
+            x.zero_()
+        rc = clef.lib().clef_paged_evict(
+            cache._at, b.table.data_ptr(), b.table.shape[1], length.data_ptr(), requests, scores.data_ptr(), budget, sinks,
+            recent, target._at, to.table.data_ptr(), to.table.shape[1], to_scores.data_ptr(), length.data_ptr(),
+            keep.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, clef.last_error()
+        assert torch.equal(length, want_lens) and torch.equal(keep, want)
+        for s, m in enumerate(lens):
+            for x, y in zip((to.k, to.vt.transpose(2, 3), to_scores), (pools[0], pools[1].transpose(2, 3), pools[2])):
+                assert same(to.read(x, s, min(m, budget)), to.read(y, s, min(m, budget)))
