@@ -894,8 +894,9 @@ class PagedCache:
     def add_weights(self, q, lse, cu_seqlens, key_lens, pages, scores, new_scores=None, window=0, sinks=0):
         """Adds to each cached key's score [pages, kvh, page] (f32) the attention weights
         that the new tokens' rows give it (lse from attention_gated, for the same window and
-        sinks); the new tokens' own keys start from 0.  Writes new_scores (default: in place)
-        and returns it."""
+        sinks); the new tokens' own keys start from 0.  Of requests that share a page, at the
+        same place of their tables, the first that has a key gives its sum.  Writes new_scores
+        (default: in place) and returns it."""
         nseq, width = self._batch(cu_seqlens, key_lens, pages)
         heads, T = self._queries(q)
         if lse.shape != (T, heads) or lse.dtype != torch.float32 or not lse.is_contiguous():

@@ -44,13 +44,57 @@ struct WeightParams {
   float* part;          // [groups][2][kManyKeys]
   struct Split {
     int s, kv, key0, w, parts;  // of the work-groups w, w + 1, ..; parts 0: no block
+    int shared;                 // whether pages of the block may be those of requests before s
   } * split;            // [groups]
 };
 
-// The key that a sum belongs to: its old score and the sum, where the table has a page.
-__device__ __forceinline__ void write_sum(const WeightParams& p, const Request& r, int s, int kv, int key, float y) {
+// Requests may share pages, at the same place of their tables.  A key's score is written by the first
+// of them that has the key: by whichever came last it would differ from run to run, and in place
+// hold the sums of some.
+//
+// Whether any page of blocks b0 .. b1 - 1 (BK keys each, `blocks` to a key head) of request s is one of a
+// request before it; for all threads of the work-group, and most often false.
+template <int NT>
+__device__ __forceinline__ bool shares_pages(const Paged& c, const Request& r, int s, int b0, int b1, int blocks, int BK) {
+  if (s == 0 || b0 >= b1) return false;
+  const int per = max(BK >> c.shift, 1), columns = min(b1 - b0, blocks) * per;
+  // neighbouring threads take neighbouring columns, and groups of threads each their requests
+  const int wide = columns >= NT ? NT : 1 << (32 - __clz((columns - 1) | 1));
+  int any = 0;
+  for (int i = threadIdx.x % wide; i < columns; i += wide) {
+    const int at = ((b0 + i / per) % blocks * BK >> c.shift) + i % per;
+    if (at << c.shift >= r.len) continue;
+    const int page = c.table[(int64_t)s * c.max_pages + at];
+#pragma unroll 4
+    for (int x = threadIdx.x / wide; x < s; x += NT / wide) any |= c.table[(int64_t)x * c.max_pages + at] == page;
+  }
+  return __syncthreads_or(any) != 0;
+}
+// Lane i: the first of the keys in the page of key key0 + i of request s that no request before s has
+// there.  The lanes look at 64 requests at a time, a page after the other.
+__device__ __forceinline__ int first_own(const Paged& c, int s, int key0, int lane) {
+  const int mine = (key0 + lane) >> c.shift;
+  int first = 0;
+#pragma unroll 1
+  for (int at = key0 >> c.shift; at <= (key0 + 63) >> c.shift && at < c.max_pages; ++at) {
+    const int page = c.table[(int64_t)s * c.max_pages + at];
+    int most = 0;
+#pragma unroll 1
+    for (int x = lane; x < s; x += 64)
+      if (c.table[(int64_t)x * c.max_pages + at] == page) most = max(most, min(c.len[x], c.max_keys));
+#pragma unroll
+    for (int o = 32; o; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+    if (at == mine) first = most;
+  }
+  return first;
+}
+
+// The key that a sum belongs to: its old score and the sum, where the table has a page and the request
+// writes it (from key `first` on).
+__device__ __forceinline__ void write_sum(const WeightParams& p, const Request& r, int s, int kv, int key, int first,
+                                          float y) {
   const Paged& c = p.c;
-  if (key >= r.len) return;
+  if (key >= r.len || key < first) return;
   const int page = c.table[(int64_t)s * c.max_pages + (key >> c.shift)];
   if (page < 0 || page >= c.num) return;
   const int64_t at = (((int64_t)page * c.kvh + kv) << c.shift) + (key & ((1 << c.shift) - 1));
@@ -119,6 +163,7 @@ __global__ __launch_bounds__(256) void weights_few_rows(WeightParams p) {
     // blocks that begin in the stretch
     const int b0 = x.u <= x.base ? 0 : min(count, uniform(static_cast<int>(quotient(x.u - x.base + cost - 1, cost))));
     const int b1 = uniform(static_cast<int>(fmin(count, quotient(x.end - x.base + cost - 1, cost))));
+    const bool shared = shares_pages<64 * NW>(c, r, s, b0, b1, blocks, BK);
     for (int b = b0 + wave; b < b1; b += NW) {
       const int kv = b / blocks, key0 = b % blocks * BK;
       float sum[NT][4] = {};
@@ -162,7 +207,8 @@ __global__ __launch_bounds__(256) void weights_few_rows(WeightParams p) {
           if (lr == 0) part[wave][16 * y + 4 * grp + i] = z;
         }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (lane < BK) write_sum(p, r, s, kv, key0 + lane, part[wave][lane]);
+      const int first = shared ? first_own(c, s, key0, lane) : 0;
+      if (lane < BK) write_sum(p, r, s, kv, key0 + lane, first, part[wave][lane]);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     x.base += count * cost;
@@ -208,6 +254,9 @@ __global__ __launch_bounds__(512, 2) void weights_many_rows(WeightParams p) {
     const double cost = each(r);
     const int blocks = blocks_of(r), first = r.len - r.n;
     const double next = uniform(x.base + c.kvh * (blocks * cost));
+    const bool shared = shares_pages<512>(
+        c, r, s, uniform(static_cast<int>(quotient(x.u - x.base, cost))),
+        uniform(static_cast<int>(quotient(fmin(next, x.end) - x.base + cost - 1, cost))), blocks, kManyKeys);
     while (x.u < fmin(next, x.end)) {
       const int b = uniform(static_cast<int>(quotient(x.u - x.base, cost)));
       const double start = uniform(x.base + b * cost), stop = uniform(fmin(start + cost, x.end));
@@ -292,10 +341,10 @@ __global__ __launch_bounds__(512, 2) void weights_many_rows(WeightParams p) {
       lds_barrier();
       if (tid < kManyKeys) {
         const float y = sh.part[2 * (tid >> 5)][tid & 31] + sh.part[2 * (tid >> 5) + 1][tid & 31];
-        if (head && tail) write_sum(p, r, s, kv, key0 + tid, y);
+        if (head && tail) write_sum(p, r, s, kv, key0 + tid, shared ? first_own(c, s, key0 + tid - lane, lane) : 0, y);
         else p.part[((int64_t)x.w * 2 + (head ? 1 : 0)) * kManyKeys + tid] = y;
       }
-      if (head && !tail) split = {s, kv, key0, x.w, last_of(x, start + cost) - x.w + 1};
+      if (head && !tail) split = {s, kv, key0, x.w, last_of(x, start + cost) - x.w + 1, shared};
     }
     x.base = next;
   }
@@ -309,7 +358,8 @@ __global__ __launch_bounds__(kManyKeys) void weights_join(WeightParams p) {
 #pragma unroll 4
   for (int n = 0; n < x.parts; ++n)
     y += p.part[((int64_t)(x.w + n) * 2 + (n == 0 ? 1 : 0)) * kManyKeys + threadIdx.x];
-  write_sum(p, request_of(p.c, x.s), x.s, x.kv, x.key0 + static_cast<int>(threadIdx.x), y);
+  const int lane = threadIdx.x & 63, key = x.key0 + static_cast<int>(threadIdx.x);
+  write_sum(p, request_of(p.c, x.s), x.s, x.kv, key, x.shared ? first_own(p.c, x.s, key - lane, lane) : 0, y);
 }
 
 // How a call is launched, from the shapes alone (the workspace follows from it).

@@ -515,8 +515,9 @@ int clef_attention_gated_paged(const clef_paged_cache* cache, const int32_t* tab
  * (new_scores may be scores itself); the new tokens' own keys start from 0.  Every
  * key of each request is written, all else is left as it was.  lse: as
  * clef_attention_gated_paged gives it for the same window and sinks.  The sum's
- * order is fixed: no atomics.  ldq_tok is at most 2^22.  Requests of one call that
- * share a page each write its scores: that page receives the sums of one of them.
+ * order is fixed: no atomics.  ldq_tok is at most 2^22.  Requests of one call may share
+ * pages, at the same place of their tables: a key's score takes the sum of the first of
+ * them that has the key, in place or not (one call per request adds up all of them).
  * workspace: clef_paged_weights_workspace bytes, 256-byte aligned; where that is 256 (few
  * rows to a request) nothing is kept there and workspace may be NULL.
  */

@@ -104,3 +104,66 @@ def test_evict_lengths_in_place(clef, dtype):
         for s, m in enumerate(lens):
             for x, y in zip((to.k, to.vt.transpose(2, 3), to_scores), (pools[0], pools[1].transpose(2, 3), pools[2])):
                 assert same(to.read(x, s, min(m, budget)), to.read(y, s, min(m, budget)))
+
+
+# (keys behind the shared ones, whose pages, how many pages of 32 keys, from which column)
+SHARED = {
+    "family": [(200, None, 0, 0), (130, 0, 3, 0), (70, None, 0, 0), (90, 2, 3, 0), (110, 2, 2, 1), (97, 0, 3, 0), (40, 3, 1, 0)],
+    "all": [(96 + 7 * s, 0 if s else None, 3, 0) for s in range(9)],
+    "hundred": [(65 + s % 40, s % 3 if s > 2 else None, 2, 0) for s in range(130)],
+}
+
+
+@gpu
+@pytest.mark.parametrize("name", SHARED, ids=str)
+@pytest.mark.parametrize("dtype,new,rep,d", [(F16, 1, 4, 64), (F16, 20, 8, 64), (F16, 33, 8, 256), (F32, 1, 3, 72),
+                                             (F32, 20, 8, 128)], ids=str)
+def test_weights_of_shared_pages(clef, name, dtype, new, rep, d):
+    """Requests that share pages: each key's score is what the first request that has it gives with pages of
+    its own, in place or not; the same in every run."""
+    page, kvh = 32, 2
+    shape = SHARED[name]
+    new = min(new, 3) if len(shape) > 100 else new
+    b = base.Batch([(min(new, 1 + 5 * s), m) for s, (m, *_) in enumerate(shape)], page, kvh, d, dtype, seed=d)
+    heads = kvh * rep
+    before = [torch.rand((kvh, m), generator=b.g, device="cuda") for m, *_ in shape]
+    rows = [list(x) for x in b.rows]
+    for s, (m, of, count, at) in enumerate(shape):
+        if of is not None:
+            rows[s][at:at + count] = rows[of][at:at + count]
+        for j in range(m):  # a shared key is the same in all requests that have it
+            first = next(i for i in range(s + 1) if shape[i][0] > j and rows[i][j // page] == rows[s][j // page])
+            if first < s:
+                for x in (b.keys, b.values, before):
+                    x[s][:, j] = x[first][:, j]
+    scores = torch.full((b.total, kvh, page), float("nan"), device="cuda")
+
+    def fill():
+        for s in range(len(shape)):
+            b.fill(b.k, s, b.keys[s])
+            b.fill(b.vt.transpose(2, 3), s, b.values[s])
+            b.fill(scores, s, before[s])
+
+    fill()
+    cache = clef.PagedCache(b.k, b.vt)
+    q, gate = b.randn(heads, b.T, d), b.randn(b.T, heads, d)
+    lse = torch.zeros((b.T, heads), device="cuda")
+    cache.attention_gated(q, gate, b.cu, b.len, b.table, lse=lse)
+    own = cache.add_weights(q, lse, b.cu, b.len, b.table, scores, new_scores=torch.full_like(scores, 7.0))
+    own = [b.read(own, s, m) for s, (m, *_) in enumerate(shape)]
+    b.rows = rows
+    for s, x in enumerate(rows):
+        b.table[s, :len(x)] = ints(x)
+    for x in (b.k, b.vt, scores):
+        x.fill_(float("nan"))
+    fill()
+    want, held = torch.full_like(scores, 7.0), scores.clone()
+    for s in reversed(range(len(shape))):  # the first request last: it stays
+        b.fill(want, s, own[s])
+        b.fill(held, s, own[s])
+    for _ in range(4):
+        got = cache.add_weights(q, lse, b.cu, b.len, b.table, scores, new_scores=torch.full_like(scores, 7.0))
+        assert torch.equal(got, want)
+        assert same(cache.add_weights(q, lse, b.cu, b.len, b.table, scores), held), "in place"
+        for s in range(len(shape)):
+            b.fill(scores, s, before[s])
