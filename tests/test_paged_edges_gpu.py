@@ -167,3 +167,75 @@ def test_weights_of_shared_pages(clef, name, dtype, new, rep, d):
         assert same(cache.add_weights(q, lse, b.cu, b.len, b.table, scores), held), "in place"
         for s in range(len(shape)):
             b.fill(scores, s, before[s])
+
+
+@gpu
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 4)])
+@pytest.mark.parametrize("dtype,page,kvh,rep,d", [(F16, 64, 2, 8, 64), (F16, 32, 1, 16, 128), (F16, 256, 3, 5, 24),
+                                                  (F32, 64, 2, 8, 256), (F32, 16, 1, 10, 200), (F32, 128, 2, 3, 8)],
+                         ids=str)
+def test_weights_widths(clef, window, sinks, dtype, page, kvh, rep, d):
+    """Accumulated weights in every instance: the bounds are those of test_paged_gpu.py."""
+    base.test_weights(clef, window, sinks, dtype, page, kvh, rep, d)
+
+
+def spread(b, gap):
+    """b's pools as views of one buffer, with NaN between the pages: (keys, values)."""
+    pool = torch.full((b.total, 2, b.k[0].numel() + gap), float("nan"), dtype=b.dtype, device="cuda")
+    n = b.k[0].numel()
+    pool[:, 0, :n], pool[:, 1, :n] = b.k.flatten(1), b.vt.flatten(1)
+    return pool[:, 0, :n].unflatten(1, b.k.shape[1:]), pool[:, 1, :n].unflatten(1, b.vt.shape[1:])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, F32], ids=str)
+@pytest.mark.parametrize("requests", [[(1, 300), (2, 90)], [(40, 300), (20, 90), (0, 500)]], ids=str)
+def test_weights_and_evict_of_spread_pools(clef, dtype, requests):
+    b = base.Batch(requests, 16, 2, 64, dtype, seed=2)
+    heads, budget = 8, 60
+    q, gate, lse = b.randn(heads, b.T, 64), b.randn(b.T, heads, 64), torch.zeros((b.T, heads), device="cuda")
+    scores = torch.rand((b.total, 2, 16), generator=b.g, device="cuda")
+    to = base.Batch([(0, min(m, budget)) for _, m in requests], 16, 2, 64, dtype, seed=3)
+    results = []
+    for far in (False, True):
+        cache = clef.PagedCache(*(spread(b, 24) if far else (b.k, b.vt)))
+        target = clef.PagedCache(*(spread(to, 8) if far else (to.k.clone(), to.vt.clone())))
+        cache.attention_gated(q, gate, b.cu, b.len, b.table, lse=lse)
+        new = cache.add_weights(q, lse, b.cu, b.len, b.table, scores, new_scores=torch.zeros_like(scores))
+        to_scores = torch.zeros((to.total, 2, 16), device="cuda")
+        kept = cache.evict(new, b.len, b.table, budget, target, to.table, to_scores, sinks=4, recent=8)
+        results.append((lse.clone(), new, to_scores, *kept, target.k.contiguous(), target.vt.contiguous()))
+    for near, far in zip(*results):
+        assert same(near, far)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,d,kvh,bits", [(F16, 256, 4, 32), (F32, 256, 4, 32), (F16, 8, 4, 34)], ids=str)
+def test_weights_and_evict_of_far_pages(clef, dtype, d, kvh, bits):
+    """Pages whose keys, and at d = 8 scores (2^31 of them), lie behind what 32 bits count."""
+    page, heads, budget = 64, 8, 100
+    near = base.Batch([(1, 500), (20, 200)], page, kvh, d, dtype, seed=11)
+    q, gate = near.randn(heads, near.T, d), near.randn(near.T, heads, d)
+    scores = torch.rand((near.total, kvh, page), generator=near.g, device="cuda")
+    to = ints([[0, 1], [2, 3]])
+    more = (1 << bits) // (page * kvh * d) + 40
+    results = []
+    for shift in (4, more):  # the pages that evictions fill, then those of the requests
+        k = torch.empty((shift + near.total, kvh, page, d), dtype=dtype, device="cuda")
+        vt = torch.empty((shift + near.total, kvh, d, page), dtype=dtype, device="cuda")
+        pool = torch.empty((shift + near.total, kvh, page), device="cuda")
+        k[:4], vt[:4], pool[:4] = 9.0, 9.0, 9.0
+        k[shift:], vt[shift:], pool[shift:] = near.k, near.vt, scores
+        table = torch.where((near.table >= 0) & (near.table < near.total), near.table + shift, near.table)
+        cache, lse = clef.PagedCache(k, vt), torch.zeros((near.T, heads), device="cuda")
+        y = cache.attention_gated(q, gate, near.cu, near.len, table, lse=lse)
+        cache.add_weights(q, lse, near.cu, near.len, table, pool)
+        kept = cache.evict(pool, near.len, table, budget, cache, to, pool, sinks=4, recent=8)
+        # and back, to far pages
+        far = ints([[shift, shift + 1], [shift + 2, shift + 3]])
+        again = cache.evict(pool, kept[0], to, 50, cache, far, pool, sinks=4, recent=8)
+        torch.cuda.synchronize()
+        results.append([x.clone() for x in (y, lse, *kept, *again, k[:4], vt[:4], pool[:4], k[shift:], vt[shift:], pool[shift:])])
+        del k, vt, pool, cache
+    for a, b in zip(*results):
+        assert same(a, b)
