@@ -178,11 +178,13 @@ __global__ __launch_bounds__(256) void evict_move(EvictParams p, int tiles) {
   const int slice = blockIdx.x % slices, tile = blockIdx.x / slices % tiles, at = blockIdx.x / slices / tiles;
   const int kv = at % c.kvh, s = at / c.kvh;
   const int len = min(max(c.len[s], 0), c.max_keys), count = min(len, p.budget);
+  const int i0 = tile * kMoved;
   // here, where the selection has read the lengths of all heads: they may be the same array (a
   // work-group that reads the new one finds the same count)
-  if (kv == 0 && slice == 0 && tile == 0 && tid == 0) p.new_lens[s] = count;
-  const int i0 = tile * kMoved;
-  if (i0 >= count) return;
+  auto store_length = [&]() {
+    if (kv == 0 && slice == 0 && tile == 0 && tid == 0) p.new_lens[s] = count;
+  };
+  if (i0 >= count) return store_length();
   __shared__ int from_page[kMoved], from_slot[kMoved], to_page[kMoved];
   if (tid < kMoved) {
     const int i = i0 + tid;
@@ -204,6 +206,7 @@ __global__ __launch_bounds__(256) void evict_move(EvictParams p, int tiles) {
     to_page[tid] = b;
   }
   __syncthreads();
+  store_length();
   if (slice == 0) {
     const int chunks = d / EL;
 #pragma unroll 1
