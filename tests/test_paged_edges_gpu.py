@@ -239,3 +239,47 @@ def test_weights_and_evict_of_far_pages(clef, dtype, d, kvh, bits):
         del k, vt, pool, cache
     for a, b in zip(*results):
         assert same(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,d", [(F16, 64), (F16, 8), (F32, 16)], ids=str)
+def test_most_rows(clef, dtype, d):
+    """The most rows of a request that a call takes, 65,536 tokens of 256 heads on one key head, behind a window
+    of 64: sampled tokens, and the weights of sampled keys, against 64 bits (bounds as in test_paged_gpu.py)."""
+    T, heads, page, window = 65536, 256, 64, 64
+    b = base.Batch([(T, T)], page, 1, d, dtype, seed=d)
+    cache = clef.PagedCache(b.k, b.vt)
+    q, gate = b.randn(heads, T, d), b.randn(T, heads, d)
+    lse = torch.zeros((T, heads), device="cuda")
+    y = cache.attention_gated(q, gate, b.cu, b.len, b.table, window=window, lse=lse).view(T, heads, d)
+    new = cache.add_weights(q, lse, b.cu, b.len, b.table, torch.zeros((b.total, 1, page), device="cuda"), window=window)
+    new = b.read(new, 0, T)[0]
+    keys, values = b.keys[0][0].double(), b.values[0][0].double()
+
+    def rows(t):  # scores [tokens, heads, window] of tokens t, and their bounds
+        j = t[:, None] - torch.arange(window - 1, -1, -1, device="cuda")
+        at = j.clamp(min=0)
+        x = q[:, t].double().transpose(0, 1)
+        z = torch.bmm(x, keys[at].transpose(1, 2).contiguous()) / d ** 0.5
+        ds = (d + 2) * base.E * torch.bmm(x.abs(), keys[at].abs().transpose(1, 2).contiguous()) / d ** 0.5
+        return j, at, torch.where((j >= 0)[:, None], z, -torch.inf), ds
+
+    t = torch.tensor([0, 1, 62, 63, 64, 65, 4095, 32767, 32768, 40000, T - 65, T - 2, T - 1], device="cuda")
+    j, at, z, ds = rows(t)
+    ds = ds.amax(2)
+    w = torch.softmax(z, 2)
+    sig = torch.sigmoid(gate[t].double())
+    want, most = torch.bmm(w, values[at]) * sig, torch.bmm(w, values[at].abs()) * sig
+    rel = 2 * ds + 2.0 ** -14 + (window + 16) * base.E + (2.0 ** -11 if dtype == F16 else 0.0)
+    base.close(y[t], want, most * rel[..., None] + base.HALF[dtype] * want.abs() + 2.0 ** -24 * (dtype == F16), "y")
+    total = torch.logsumexp(z, 2)
+    base.close(lse[t], total, ds + 2.0 ** -15 + (window + 16) * base.E + total.abs() * 2 * base.E, "lse")
+    for key in (0, 1, 63, 64, 40000, T - 64, T - 1):
+        t = torch.arange(key, min(key + window, T), device="cuda")
+        j, _, z, ds = rows(t)
+        z = z[j[:, None].expand_as(z) == key].view(len(t), heads)
+        ds = ds[j[:, None].expand_as(ds) == key].view(len(t), heads)
+        w = torch.exp(z - lse[t].double())
+        want = w.sum()
+        tol = (w * (2 * ds + 2.0 ** -14)).sum() + want * (heads * window + 8) * base.E
+        base.close(new[key], want, tol, f"weight of key {key}")
