@@ -11,8 +11,10 @@
 // attention_parts.hpp, and outputs too, on values stored by feature.
 //
 // Two shapes of work: tiles of 16 rows for single tokens and short chunks, bound by the
-// keys' bytes, and tiles of 256 (f16) or 64 rows (f32) for chunks, bound by MFMA.  Weights are rounded
-// once, to the operands' type; scores, maxima, sums and outputs are f32.
+// keys' bytes, and tiles of 256 (f16) or 64 rows (f32) for chunks, bound by MFMA.  Weights are
+// rounded once, to the operands' type, so that their product with the values runs at its rate (f32
+// products: a seventh of f16's).  In f16 outputs are off by 2.5e-4 .. 2.9e-4 of their size, of which
+// their own rounding is 2.1e-4.  Scores, maxima, sums and outputs are f32.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -83,9 +85,6 @@ __device__ __forceinline__ void write_lse(const PagedAttn& p, float m, float l, 
         l == 0.0f ? -INFINITY : (m - Ops<T>::UP + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
 }
 
-// One block of KB keys, c0 .. + KB - 1 (c0 a multiple of KB), straight from the
-// pages into operands.  The pages hold at least 16 keys each, so a block lies in
-// one or in two.  FULL: d = D.
 // a wave's own writes to LDS are done, and none of its accesses moves across
 __device__ __forceinline__ void lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
@@ -96,6 +95,9 @@ __device__ __forceinline__ uint32_t odd_bits(uint32_t x) {
   return ((x & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((x & 0x7c000000u) == 0x7c000000u ? ~0xffffu : 0u);
 }
 
+// One block of KB keys, c0 .. + KB - 1 (c0 a multiple of KB), straight from the
+// pages into operands.  The pages hold at least 16 keys each, so a block lies in
+// one or in two.  FULL: d = D.
 template <class T, int D, bool FULL>
 struct PageBlock {
   static constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL, TPB = Ops<T>::TPB;
@@ -179,7 +181,7 @@ struct FewRows {
 // Single tokens and short chunks: the waves of a work-group take blocks of a piece in
 // turn, straight from the pages into operands (no other wave would use the same keys),
 // and their parts are joined in LDS.  64 requests of up to 16,384 keys, 2 x 256, f16:
-// 1.20 GB in 220 us, 5.5 TB/s, more than a large copy's 5.2.  A short call is bound by
+// 1.20 GB in 220 us, 5.5 TB/s (1.40 GB cross the memory bus, counted).  A short call is bound by
 // latency: one token behind 700 keys takes 11 us and the joining 4, most of it the chain
 // of table, page and key loads and the fetching of 19 KB of code.
 //
@@ -884,7 +886,8 @@ struct PagedPlan {
 PagedPlan plan_of(int T, int nseq, int max_keys, int dtype, int heads, int kvh, int d) {
   PagedPlan x;
   const int64_t rows = (int64_t)T * (heads / kvh), cus = device_cus();
-  // Requests of more than 64 rows, or of more than 16 with many keys in all, go on wide tiles.  (Few, many:
+  // Requests of more than 64 rows, or of more than 16 with many keys in all, go on wide tiles, by the batch's
+  // average: the lengths are on the device.  A chunk among many single tokens can go on narrow ones.  (Few, many:
   // 16 requests of 24 rows behind 4,096 keys 36, 55 us; of 32 41, 57; of 64 59, 60; 32 of 32 behind 16,384
   // 194, 165; of 64 360, 176; one of 64 behind 4,096 24, 36.)
   const int64_t units = (rows / 16 + nseq) * kvh * (max_keys / kWalkBlock + 1);

@@ -8,7 +8,8 @@
 // 2 heads, 19 us, a chain of passes on 32 work-groups.  move: the listed keys, values and
 // scores are copied; 16 x 4,096 of 2 x 256, f16, kept of twice to four times as many, in 88
 // us.  What stays is read and written once, but values lie in rows of a page's keys, and the
-// rows' cache lines come whole: 350 MB instead of 270, at 4.0 TB/s.
+// rows' cache lines come whole: 326 MB read and 135 written, counted, instead of 270 in all, at
+// 5.2 TB/s, a large copy's rate.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

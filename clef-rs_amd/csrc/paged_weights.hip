@@ -8,7 +8,8 @@
 // bound by the keys' bytes: a wave takes a block for itself, and its rows straight
 // from memory.  With more rows a work-group of eight waves takes 128 keys, and the
 // rows pass through LDS by DMA for all of them.  Blocks lie on a line that is dealt to
-// work-groups in equal stretches (paged_walk.hpp); the sums of a block that a cut goes
+// work-groups in equal stretches (paged_walk.hpp), each priced at all rows of its request
+// (behind a window, too, where the keys that it has left cost less); the sums of a block that a cut goes
 // through are added by a second launch.  No atomics: the order of a sum is fixed.
 #include <hip/hip_runtime.h>
 
@@ -24,7 +25,9 @@
 namespace clef {
 namespace {
 
-constexpr int kBlockCost = 32;   // what a block costs beside its rows, in rows
+// What a block costs beside its rows, in rows.  (8, 32, 128: 16 requests of 16 tokens of 8 heads a key
+// head behind 4,096 keys 41, 41, 41 us; one of 32 tokens 19, 19, 15; 16 of one 26, 24, 24.)
+constexpr int kBlockCost = 32;
 constexpr int kManyKeys = 128;   // of a work-group's block
 constexpr int kManyTile = 64;    // rows that pass at a time
 
@@ -155,7 +158,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 // ---------------------------------------------------------------------------
 // A block to a wave, its rows straight from memory (64 keys, f32 32).  32 requests of one
-// token behind up to 8,192 keys, 2 x 256, f16: 141 MB in 35 us, 4.0 TB/s.
+// token behind up to 8,192 keys, 2 x 256, f16: 141 MB in 38 us, 3.7 TB/s; three of them go into the
+// look for shared pages, which a work-group begins with.
 template <class T, int D, bool FULL>
 __global__ __launch_bounds__(256) void weights_few_rows(WeightParams p) {
   constexpr int KB = Ops<T>::KB, EL = Ops<T>::EL, NT = sizeof(T) == 2 ? 4 : 2, BK = 16 * NT, NW = 4;
@@ -386,6 +390,10 @@ struct WeightPlan {
 };
 WeightPlan plan_of(int T, int nseq, int max_keys, int dtype, int heads, int kvh) {
   WeightPlan x;
+  // (Few, many, 8 heads a key head behind 4,096 keys: 16 requests of 4 tokens 27, 36 us, of 8 32, 35, of 16
+  // 41, 41, of 32 58, 51; one of 8 13, 19, of 16 16, 19, of 32 23, 19; f32, 16 of 8 74, 77, of 16 123, 110.
+  // By the batch's average, since the lengths are on the device: a chunk of 1,024 tokens with 199 single
+  // ones behind 2,000 keys each goes the first way, 510, 385.)
   x.many = (int64_t)T * (heads / kvh) > 64 * (int64_t)nseq;
   const int keys = x.many ? kManyKeys : dtype == CLEF_F16 ? 64 : 32;
   const int64_t blocks = (int64_t)(max_keys / keys + 1) * kvh * nseq;

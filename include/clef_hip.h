@@ -496,8 +496,10 @@ int clef_paged_append(const clef_paged_cache* cache, const int32_t* table, int m
  * row over the keys it sees.  A query that sees no key gives zeros and an lse of
  * -inf; keys that no query of its request sees may hold anything.  Rows behind the
  * last request leave y and lse as they were.  q [heads, ldq_tok, d] (rows 0..T-1,
- * 16-byte aligned, ldq_tok at most 2^22), gate as in clef_attention_gated_shared; f32
- * sums and softmax.
+ * 16-byte aligned, ldq_tok at most 2^22), gate as in clef_attention_gated_shared.  f32
+ * scores, sums and softmax; with CLEF_F16 each weight is rounded once to f16 for its
+ * product with the values (by 2^-11 of itself, or 2^-32 of the largest where that is
+ * more), as in the other attention calls.
  * workspace: clef_attention_paged_workspace bytes, 256-byte aligned.
  */
 size_t clef_attention_paged_workspace(int T, int nseq, int max_pages, int page, int dtype, int heads, int kv_heads,
